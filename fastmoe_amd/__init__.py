@@ -5,10 +5,11 @@ interface; `fmoe_cuda` is the operator module that stands in for the
 reference's compiled extension of the same name.
 """
 from . import fmoe_cuda
-from .gates import BaseGate, GShardGate, NaiveGate, SwitchGate
+from .gates import BaseGate, GShardGate, NaiveGate, ScoreGate, SwitchGate
 from .layers import FMoE
 from .linear import FMoELinear
 from .transformer import FMoETransformerMLP
+from . import mx
 
 
 def install_as_fmoe_cuda(compiled: bool = True) -> None:
@@ -43,4 +44,4 @@ def graphed(layer, sample_input, num_warmup_iters: int = 3):
 
 
 __all__ = ["FMoE", "FMoELinear", "FMoETransformerMLP", "BaseGate", "NaiveGate",
-           "GShardGate", "SwitchGate", "fmoe_cuda", "install_as_fmoe_cuda", "graphed"]
+           "GShardGate", "ScoreGate", "SwitchGate", "fmoe_cuda", "mx", "install_as_fmoe_cuda", "graphed"]

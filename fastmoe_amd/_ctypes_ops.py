@@ -642,6 +642,210 @@ def topk_softmax_bwd(dscore: torch.Tensor, score: torch.Tensor, idx: torch.Tenso
     return dlogits
 
 
+def score_topk_fwd(logits: torch.Tensor, bias: Optional[torch.Tensor], top_k: int,
+                   n_group: int = 1, top_group: int = 1, group_best: int = 2, score: int = 0,
+                   renormalize: bool = True, scale: float = 1.0
+                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(idx int64 [T, k], weight [T, k]) of scored routing: sigmoid (score 0) or softmax (1)
+    scores, chosen by score + bias among the best groups (fmoe_score_topk_fwd)."""
+    _dev(logits, "logits")
+    _need(logits.dim() == 2, "logits must be [tokens, experts]")
+    t, e = logits.shape
+    if bias is not None:
+        _dev(bias, "bias", torch.float32)
+        _need(bias.numel() == e and bias.device == logits.device,
+              "bias must have one float per expert, on the logits' device")
+    _need(1 <= top_k <= e, "top_k must lie between 1 and the number of experts")
+    idx = torch.empty((t, top_k), dtype=torch.int64, device=logits.device)
+    weight = torch.empty((t, top_k), dtype=logits.dtype, device=logits.device)
+    with _launch(logits, "score_topk_fwd"):
+        _lib.check(
+            _L.fmoe_score_topk_fwd(logits.data_ptr(), _ptr(bias), t, e, top_k, n_group, top_group,
+                                   group_best, score, bool(renormalize), scale, idx.data_ptr(),
+                                   weight.data_ptr(), _dt(logits, "logits"), _stream(logits)),
+            "score_topk_fwd")
+    return idx, weight
+
+
+def score_topk_bwd(dweight: torch.Tensor, logits: torch.Tensor, idx: torch.Tensor,
+                   score: int = 0, renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """dlogits [T, E] of score_topk_fwd."""
+    _dev(logits, "logits")
+    _dev(dweight, "dweight", logits.dtype)
+    _dev(idx, "idx", torch.int64)
+    _need(logits.dim() == 2 and idx.dim() == 2 and idx.shape[0] == logits.shape[0]
+          and dweight.shape == idx.shape,
+          "logits must be [tokens, experts], dweight and idx [tokens, top_k]")
+    dlogits = torch.empty_like(logits)
+    with _launch(logits, "score_topk_bwd"):
+        _lib.check(
+            _L.fmoe_score_topk_bwd(dweight.data_ptr(), logits.data_ptr(), idx.data_ptr(),
+                                   logits.shape[0], logits.shape[1], idx.shape[1], score,
+                                   bool(renormalize), scale, dlogits.data_ptr(),
+                                   _dt(logits, "logits"), _stream(logits)),
+            "score_topk_bwd")
+    return dlogits
+
+
+# --------------------------------------------------------------------------
+# Rows in microscaled 4-bit floating point
+# --------------------------------------------------------------------------
+def _mx_bytes(features: int) -> Tuple[int, int]:
+    """Code and scale bytes of a row of `features` values."""
+    sizes = _L.fmoe_mx_code_bytes(features), _L.fmoe_mx_scale_bytes(features)
+    for n in sizes:
+        _lib.check(min(n, 0), "mx row size")
+    return sizes
+
+
+def _mx_empty(rows: int, features: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    return tuple(torch.empty((rows, n), dtype=torch.uint8, device=device)
+                 for n in _mx_bytes(features))
+
+
+def _mx_check(codes: torch.Tensor, scales: torch.Tensor, features: int, name: str) -> None:
+    _dev(codes, name, torch.uint8)
+    _dev(scales, name, torch.uint8)
+    _need(features >= 1, f"{name}: features must be positive")
+    _need(codes.dim() >= 2 and scales.dim() == codes.dim()
+          and codes.shape[:-1] == scales.shape[:-1]
+          and (codes.shape[-1], scales.shape[-1]) == _mx_bytes(features)
+          and codes.device == scales.device,
+          f"{name}: codes and scales do not hold rows of that many features")
+
+
+def mx_quantize(x: torch.Tensor, n_rows_dev: Optional[torch.Tensor] = None
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of the rows of x [rows, features] in MXFP4 (fmoe_mx_quantize)."""
+    _dev(x, "x")
+    _need(x.dim() == 2 and x.shape[1] >= 1, "x must be [rows, features]")
+    if n_rows_dev is not None:
+        _dev(n_rows_dev, "n_rows_dev", torch.int32)
+    codes, scales = _mx_empty(x.shape[0], x.shape[1], x.device)
+    with _launch(x, "mx_quantize"):
+        _lib.check(
+            _L.fmoe_mx_quantize(x.data_ptr(), x.shape[0], x.shape[1], _ptr(n_rows_dev),
+                                codes.data_ptr(), scales.data_ptr(), _dt(x, "x"), _stream(x)),
+            "mx_quantize")
+    return codes, scales
+
+
+def mx_quantize_tokens(x: torch.Tensor, inv: torch.Tensor, top_k: int
+                       ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """mx_quantize of token rows, written to their places in expert order: rows
+    inv[t * top_k + j] (-1: dropped) of [tokens * top_k] rows."""
+    _dev(x, "x")
+    _dev(inv, "inv", torch.int32)
+    _need(x.dim() == 2 and x.shape[1] >= 1, "x must be [tokens, features]")
+    _need(top_k >= 1 and inv.numel() == x.shape[0] * top_k,
+          "inv must have tokens * top_k entries")
+    codes, scales = _mx_empty(x.shape[0] * top_k, x.shape[1], x.device)
+    with _launch(x, "mx_quantize_tokens"):
+        _lib.check(
+            _L.fmoe_mx_quantize_tokens(x.data_ptr(), inv.data_ptr(), x.shape[0], top_k,
+                                       x.shape[1], codes.data_ptr(), scales.data_ptr(),
+                                       _dt(x, "x"), _stream(x)),
+            "mx_quantize_tokens")
+    return codes, scales
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """Writes the values of MXFP4 rows into out [rows, features] and returns it."""
+    _dev(out, "out")
+    _need(out.dim() == 2 and out.shape[1] >= 1, "out must be [rows, features]")
+    _mx_check(codes, scales, out.shape[1], "mx_dequantize")
+    _need(codes.dim() == 2 and codes.shape[0] == out.shape[0],
+          "mx_dequantize: out has other rows")
+    with _launch(out, "mx_dequantize"):
+        _lib.check(
+            _L.fmoe_mx_dequantize(codes.data_ptr(), scales.data_ptr(), out.shape[0], out.shape[1],
+                                  out.data_ptr(), _dt(out, "out"), _stream(out)),
+            "mx_dequantize")
+    return out
+
+
+def _mx_product_check(xc, xs, wc, ws, in_feat, bias, seg_off) -> None:
+    _mx_check(xc, xs, in_feat, "x")
+    _mx_check(wc, ws, in_feat, "weight")
+    _dev(seg_off, "seg_off", torch.int32)
+    _need(xc.dim() == 2 and wc.dim() == 3, "x must be 2-d and weight 3-d")
+    _need(xc.device == wc.device == seg_off.device, "x, weight and seg_off must share a device")
+    _need(seg_off.numel() == wc.shape[0] + 1, "seg_off must have E+1 entries")
+    if bias is not None:
+        _dev(bias, "bias")
+        _need(bias.dim() == 2 and bias.shape == wc.shape[:2], "bias must be [E, out]")
+
+
+def mx_linear_fwd(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.Tensor,
+                  w_scales: torch.Tensor, in_feat: int, bias: Optional[torch.Tensor],
+                  seg_off: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """out[seg_e] = x[seg_e] @ w[e].T + bias[e] on MXFP4 rows and weights; returns out."""
+    _mx_product_check(x_codes, x_scales, w_codes, w_scales, in_feat, bias, seg_off)
+    _dev(out, "out")
+    _need(out.dim() == 2 and out.shape == (x_codes.shape[0], w_codes.shape[1]),
+          "out must be [rows, out]")
+    if bias is not None:
+        _dev(bias, "bias", out.dtype)
+    with _launch(out, "mx_linear_fwd"):
+        _lib.check(
+            _L.fmoe_mx_linear_fwd(x_codes.data_ptr(), x_scales.data_ptr(), w_codes.data_ptr(),
+                                  w_scales.data_ptr(), _ptr(bias), seg_off.data_ptr(), 0,
+                                  out.data_ptr(), None, None, x_codes.shape[0], in_feat,
+                                  w_codes.shape[1], w_codes.shape[0], _dt(out, "out"),
+                                  _stream(out)),
+            "mx_linear_fwd")
+    return out
+
+
+def mx_linear_act_fwd(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.Tensor,
+                      w_scales: torch.Tensor, in_feat: int, bias: Optional[torch.Tensor],
+                      seg_off: torch.Tensor, act: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """act(x @ w.T + bias) in MXFP4 again (codes, scales): one launch."""
+    _mx_product_check(x_codes, x_scales, w_codes, w_scales, in_feat, bias, seg_off)
+    codes, scales = _mx_empty(x_codes.shape[0], w_codes.shape[1], x_codes.device)
+    with _launch(x_codes, "mx_linear_act_fwd"):
+        _lib.check(
+            _L.fmoe_mx_linear_fwd(x_codes.data_ptr(), x_scales.data_ptr(), w_codes.data_ptr(),
+                                  w_scales.data_ptr(), _ptr(bias), seg_off.data_ptr(), act,
+                                  None, codes.data_ptr(), scales.data_ptr(), x_codes.shape[0],
+                                  in_feat, w_codes.shape[1], w_codes.shape[0],
+                                  0 if bias is None else _dt(bias, "bias"), _stream(x_codes)),
+            "mx_linear_act_fwd")
+    return codes, scales
+
+
+def mx_linear_bwd(dy: torch.Tensor, seg_off: torch.Tensor, w_codes: torch.Tensor,
+                  w_scales: torch.Tensor, in_feat: int, need_dx: bool = True,
+                  need_bias: bool = False
+                  ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dbias) in front of frozen MXFP4 weights: dx[seg_e] = dy[seg_e] @ w[e]."""
+    _dev(dy, "dy")
+    _mx_check(w_codes, w_scales, in_feat, "weight")
+    _dev(seg_off, "seg_off", torch.int32)
+    _need(dy.dim() == 2 and w_codes.dim() == 3 and dy.shape[1] == w_codes.shape[1],
+          "dy must be [rows, out]")
+    _need(dy.device == w_codes.device == seg_off.device,
+          "dy, weight and seg_off must share a device")
+    _need(seg_off.numel() == w_codes.shape[0] + 1, "seg_off must have E+1 entries")
+    e, out_f = w_codes.shape[:2]
+    dx = db = w = None
+    if need_dx:
+        w = dy.new_empty((e * out_f, in_feat))
+        mx_dequantize(w_codes.view(e * out_f, -1), w_scales.view(e * out_f, -1), w)
+        dx = dy.new_empty((dy.shape[0], in_feat))
+    if need_bias:
+        db = dy.new_empty((e, out_f))
+    if need_dx or need_bias:
+        with _launch(dy, "mx_linear_bwd"):
+            _lib.check(
+                _L.fmoe_grouped_linear_bwd(dy.data_ptr(), dy.data_ptr(), _ptr(w),
+                                           seg_off.data_ptr(), _ptr(dx), None, _ptr(db),
+                                           dy.shape[0], in_feat, out_f, e, _dt(dy, "dy"),
+                                           _stream(dy)),
+                "mx_linear_bwd")
+    return dx, db
+
+
 def _row_len(x: torch.Tensor) -> int:
     return x.shape[-1] if x.dim() >= 1 and x.numel() else 0
 

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int32, c_int64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libfmoe_hip.so")
@@ -90,6 +90,20 @@ SIGNATURES = {
                                                        c_int64, c_int, c_void_p]),
     "fmoe_topk_softmax_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32,
                                       c_int32, c_int, c_void_p]),
+    "fmoe_score_topk_fwd": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                    c_int32, c_int, c_int, c_float, c_void_p, c_void_p, c_int,
+                                    c_void_p]),
+    "fmoe_score_topk_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int,
+                                    c_int, c_float, c_void_p, c_int, c_void_p]),
+    "fmoe_mx_code_bytes": (c_int64, [c_int64]),
+    "fmoe_mx_scale_bytes": (c_int64, [c_int64]),
+    "fmoe_mx_quantize": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int,
+                                 c_void_p]),
+    "fmoe_mx_quantize_tokens": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                                        c_void_p, c_int, c_void_p]),
+    "fmoe_mx_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "fmoe_mx_linear_fwd": (c_int, [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int64] * 4
+                           + [c_int, c_void_p]),
     "fmoe_scatter_tokens": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                     c_int, c_void_p]),
     "fmoe_gelu_fwd": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),

@@ -514,6 +514,189 @@ Tensor topk_softmax_bwd(Tensor dscore, Tensor score, Tensor idx, int64_t n_exper
   return dlogits;
 }
 
+std::tuple<Tensor, Tensor> score_topk_fwd(Tensor logits, OptTensor bias, int64_t top_k,
+                                          int64_t n_group, int64_t top_group, int64_t group_best,
+                                          int64_t score, bool renormalize, double scale) {
+  dev(logits, "logits");
+  need(logits.dim() == 2, "logits must be [tokens, experts]");
+  const int64_t t = logits.size(0), e = logits.size(1);
+  if (bias.has_value() && bias->defined()) {
+    dev(*bias, "bias", at::kFloat);
+    need(bias->numel() == e && bias->device() == logits.device(),
+         "bias must have one float per expert, on the logits' device");
+  }
+  need(top_k >= 1 && top_k <= e, "top_k must lie between 1 and the number of experts");
+  c10::DeviceGuard guard(logits.device());
+  Tensor idx = torch::empty({t, top_k}, logits.options().dtype(at::kLong));
+  Tensor weight = torch::empty({t, top_k}, logits.options());
+  check(fmoe_score_topk_fwd(logits.data_ptr(), (const float*)ptr(bias), t, (int32_t)e,
+                            (int32_t)top_k, (int32_t)n_group, (int32_t)top_group,
+                            (int32_t)group_best, (int)score, renormalize, (float)scale,
+                            idx.data_ptr<int64_t>(), weight.data_ptr(), dt(logits, "logits"),
+                            stream_of(logits)),
+        "score_topk_fwd");
+  return {idx, weight};
+}
+
+Tensor score_topk_bwd(Tensor dweight, Tensor logits, Tensor idx, int64_t score, bool renormalize,
+                      double scale) {
+  dev(logits, "logits");
+  dev(dweight, "dweight", logits.scalar_type());
+  dev(idx, "idx", at::kLong);
+  need(logits.dim() == 2 && idx.dim() == 2 && idx.size(0) == logits.size(0) &&
+           dweight.sizes() == idx.sizes(),
+       "logits must be [tokens, experts], dweight and idx [tokens, top_k]");
+  c10::DeviceGuard guard(logits.device());
+  Tensor dlogits = torch::empty_like(logits);
+  check(fmoe_score_topk_bwd(dweight.data_ptr(), logits.data_ptr(), idx.data_ptr<int64_t>(),
+                            logits.size(0), (int32_t)logits.size(1), (int32_t)idx.size(1),
+                            (int)score, renormalize, (float)scale, dlogits.data_ptr(),
+                            dt(logits, "logits"), stream_of(logits)),
+        "score_topk_bwd");
+  return dlogits;
+}
+
+// ---------------------------------------------------------------- 4-bit operators
+int64_t mx_bytes(int64_t n, const char* what) {
+  check(n < 0 ? (int)n : 0, what);
+  return n;
+}
+
+// codes [rows, code bytes] and scales [rows, scale bytes] of rows of `features` values
+std::tuple<Tensor, Tensor> mx_empty(int64_t rows, int64_t features, const Tensor& like) {
+  const auto opts = like.options().dtype(at::kByte);
+  return {torch::empty({rows, mx_bytes(fmoe_mx_code_bytes(features), "mx_code_bytes")}, opts),
+          torch::empty({rows, mx_bytes(fmoe_mx_scale_bytes(features), "mx_scale_bytes")}, opts)};
+}
+
+void mx_check(const Tensor& codes, const Tensor& scales, int64_t features, const char* name) {
+  dev(codes, name, at::kByte);
+  dev(scales, name, at::kByte);
+  need(features >= 1, std::string(name) + ": features must be positive");
+  need(codes.dim() >= 2 && scales.dim() == codes.dim() &&
+           codes.sizes().slice(0, codes.dim() - 1) == scales.sizes().slice(0, codes.dim() - 1) &&
+           codes.size(-1) == fmoe_mx_code_bytes(features) &&
+           scales.size(-1) == fmoe_mx_scale_bytes(features) && codes.device() == scales.device(),
+       std::string(name) + ": codes and scales do not hold rows of that many features");
+}
+
+std::tuple<Tensor, Tensor> mx_quantize(Tensor x, OptTensor n_rows_dev) {
+  dev(x, "x");
+  need(x.dim() == 2 && x.size(1) >= 1, "x must be [rows, features]");
+  if (n_rows_dev.has_value() && n_rows_dev->defined()) dev(*n_rows_dev, "n_rows_dev", at::kInt);
+  c10::DeviceGuard guard(x.device());
+  auto q = mx_empty(x.size(0), x.size(1), x);
+  check(fmoe_mx_quantize(x.data_ptr(), x.size(0), x.size(1), (const int32_t*)ptr(n_rows_dev),
+                         std::get<0>(q).data_ptr(), std::get<1>(q).data_ptr(), dt(x, "x"),
+                         stream_of(x)),
+        "mx_quantize");
+  return q;
+}
+
+std::tuple<Tensor, Tensor> mx_quantize_tokens(Tensor x, Tensor inv, int64_t top_k) {
+  dev(x, "x");
+  dev(inv, "inv", at::kInt);
+  need(x.dim() == 2 && x.size(1) >= 1, "x must be [tokens, features]");
+  need(top_k >= 1 && inv.numel() == x.size(0) * top_k, "inv must have tokens * top_k entries");
+  c10::DeviceGuard guard(x.device());
+  auto q = mx_empty(x.size(0) * top_k, x.size(1), x);
+  check(fmoe_mx_quantize_tokens(x.data_ptr(), inv.data_ptr<int32_t>(), x.size(0), top_k, x.size(1),
+                                std::get<0>(q).data_ptr(), std::get<1>(q).data_ptr(), dt(x, "x"),
+                                stream_of(x)),
+        "mx_quantize_tokens");
+  return q;
+}
+
+Tensor mx_dequantize(Tensor codes, Tensor scales, Tensor out) {
+  dev(out, "out");
+  need(out.dim() == 2 && out.size(1) >= 1, "out must be [rows, features]");
+  mx_check(codes, scales, out.size(1), "mx_dequantize");
+  need(codes.dim() == 2 && codes.size(0) == out.size(0), "mx_dequantize: out has other rows");
+  c10::DeviceGuard guard(out.device());
+  check(fmoe_mx_dequantize(codes.data_ptr(), scales.data_ptr(), out.size(0), out.size(1),
+                           out.data_ptr(), dt(out, "out"), stream_of(out)),
+        "mx_dequantize");
+  return out;
+}
+
+// What the two products share: x [rows, in], w [E, out, in] in MXFP4, seg_off [E + 1].
+void mx_product_check(const Tensor& xc, const Tensor& xs, const Tensor& wc, const Tensor& ws,
+                      int64_t in_f, const OptTensor& bias, const Tensor& seg_off) {
+  mx_check(xc, xs, in_f, "x");
+  mx_check(wc, ws, in_f, "weight");
+  dev(seg_off, "seg_off", at::kInt);
+  need(xc.dim() == 2 && wc.dim() == 3, "x must be 2-d and weight 3-d");
+  need(xc.device() == wc.device() && xc.device() == seg_off.device(),
+       "x, weight and seg_off must share a device");
+  need(seg_off.numel() == wc.size(0) + 1, "seg_off must have E+1 entries");
+  if (bias.has_value() && bias->defined()) {
+    dev(*bias, "bias");
+    need(bias->dim() == 2 && bias->size(0) == wc.size(0) && bias->size(1) == wc.size(1),
+         "bias must be [E, out]");
+  }
+}
+
+Tensor mx_linear_fwd(Tensor xc, Tensor xs, Tensor wc, Tensor ws, int64_t in_f, OptTensor bias,
+                     Tensor seg_off, Tensor out) {
+  mx_product_check(xc, xs, wc, ws, in_f, bias, seg_off);
+  dev(out, "out");
+  need(out.dim() == 2 && out.size(0) == xc.size(0) && out.size(1) == wc.size(1),
+       "out must be [rows, out]");
+  if (bias.has_value() && bias->defined()) dev(*bias, "bias", out.scalar_type());
+  c10::DeviceGuard guard(out.device());
+  check(fmoe_mx_linear_fwd(xc.data_ptr(), xs.data_ptr(), wc.data_ptr(), ws.data_ptr(), ptr(bias),
+                           seg_off.data_ptr<int32_t>(), FMOE_ACT_NONE, out.data_ptr(), nullptr,
+                           nullptr, xc.size(0), in_f, wc.size(1), wc.size(0), dt(out, "out"),
+                           stream_of(out)),
+        "mx_linear_fwd");
+  return out;
+}
+
+std::tuple<Tensor, Tensor> mx_linear_act_fwd(Tensor xc, Tensor xs, Tensor wc, Tensor ws,
+                                             int64_t in_f, OptTensor bias, Tensor seg_off,
+                                             int64_t act) {
+  mx_product_check(xc, xs, wc, ws, in_f, bias, seg_off);
+  c10::DeviceGuard guard(xc.device());
+  auto q = mx_empty(xc.size(0), wc.size(1), xc);
+  const bool has_bias = bias.has_value() && bias->defined();
+  check(fmoe_mx_linear_fwd(xc.data_ptr(), xs.data_ptr(), wc.data_ptr(), ws.data_ptr(), ptr(bias),
+                           seg_off.data_ptr<int32_t>(), (int)act, nullptr,
+                           std::get<0>(q).data_ptr(), std::get<1>(q).data_ptr(), xc.size(0), in_f,
+                           wc.size(1), wc.size(0), has_bias ? dt(*bias, "bias") : FMOE_F32,
+                           stream_of(xc)),
+        "mx_linear_act_fwd");
+  return q;
+}
+
+// Gradients of the rows and of the bias in front of frozen 4-bit weights: the weights' values in
+// dy's dtype, then the grouped product of the other weights.
+std::tuple<OptTensor, OptTensor> mx_linear_bwd(Tensor dy, Tensor seg_off, Tensor wc, Tensor ws,
+                                               int64_t in_f, bool need_dx, bool need_bias) {
+  dev(dy, "dy");
+  mx_check(wc, ws, in_f, "weight");
+  dev(seg_off, "seg_off", at::kInt);
+  need(dy.dim() == 2 && wc.dim() == 3 && dy.size(1) == wc.size(1), "dy must be [rows, out]");
+  need(dy.device() == wc.device() && dy.device() == seg_off.device(),
+       "dy, weight and seg_off must share a device");
+  need(seg_off.numel() == wc.size(0) + 1, "seg_off must have E+1 entries");
+  c10::DeviceGuard guard(dy.device());
+  const int64_t e = wc.size(0), out_f = wc.size(1);
+  OptTensor dx, db;
+  Tensor w;
+  if (need_dx) {
+    w = torch::empty({e * out_f, in_f}, dy.options());
+    mx_dequantize(wc.view({e * out_f, -1}), ws.view({e * out_f, -1}), w);
+    dx = torch::empty({dy.size(0), in_f}, dy.options());
+  }
+  if (need_bias) db = torch::empty({e, out_f}, dy.options());
+  if (need_dx || need_bias)   // (the layer's input takes part in the weight gradient alone)
+    check(fmoe_grouped_linear_bwd(dy.data_ptr(), dy.data_ptr(), need_dx ? w.data_ptr() : nullptr,
+                                  seg_off.data_ptr<int32_t>(), ptr(dx), nullptr, ptr(db),
+                                  dy.size(0), in_f, out_f, e, dt(dy, "dy"), stream_of(dy)),
+          "mx_linear_bwd");
+  return {dx, db};
+}
+
 int64_t row_len(const Tensor& x) { return x.dim() >= 1 && x.numel() ? x.size(-1) : 0; }
 
 Tensor gelu_fwd(Tensor x, OptTensor n_rows_dev) {
@@ -587,6 +770,25 @@ PYBIND11_MODULE(fmoe_cuda, m) {
   m.def("scatter_reduce", &scatter_reduce);
   m.def("topk_softmax_fwd", &topk_softmax_fwd);
   m.def("topk_softmax_bwd", &topk_softmax_bwd);
+  m.def("score_topk_fwd", &score_topk_fwd, py::arg("logits"), py::arg("bias"), py::arg("top_k"),
+        py::arg("n_group") = 1, py::arg("top_group") = 1, py::arg("group_best") = 2,
+        py::arg("score") = (int)FMOE_SCORE_SIGMOID, py::arg("renormalize") = true,
+        py::arg("scale") = 1.0);
+  m.def("score_topk_bwd", &score_topk_bwd, py::arg("dweight"), py::arg("logits"), py::arg("idx"),
+        py::arg("score") = (int)FMOE_SCORE_SIGMOID, py::arg("renormalize") = true,
+        py::arg("scale") = 1.0);
+  m.def("mx_quantize", &mx_quantize, py::arg("x"), py::arg("n_rows_dev") = py::none());
+  m.def("mx_quantize_tokens", &mx_quantize_tokens, py::arg("x"), py::arg("inv"), py::arg("top_k"));
+  m.def("mx_dequantize", &mx_dequantize, py::arg("codes"), py::arg("scales"), py::arg("out"));
+  m.def("mx_linear_fwd", &mx_linear_fwd, py::arg("x_codes"), py::arg("x_scales"),
+        py::arg("w_codes"), py::arg("w_scales"), py::arg("in_feat"), py::arg("bias"),
+        py::arg("seg_off"), py::arg("out"));
+  m.def("mx_linear_act_fwd", &mx_linear_act_fwd, py::arg("x_codes"), py::arg("x_scales"),
+        py::arg("w_codes"), py::arg("w_scales"), py::arg("in_feat"), py::arg("bias"),
+        py::arg("seg_off"), py::arg("act"));
+  m.def("mx_linear_bwd", &mx_linear_bwd, py::arg("dy"), py::arg("seg_off"), py::arg("w_codes"),
+        py::arg("w_scales"), py::arg("in_feat"), py::arg("need_dx") = true,
+        py::arg("need_bias") = false);
   m.def("gelu_fwd", &gelu_fwd, py::arg("x"), py::arg("n_rows_dev") = py::none());
   m.def("gelu_bwd", &gelu_bwd, py::arg("dy"), py::arg("x"), py::arg("n_rows_dev") = py::none());
   py::class_<ParamTables>(m, "ParamTables").def(py::init<>());

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import fmoe_cuda
 
@@ -216,6 +217,55 @@ class TopKSoftmax(Function):
         idx, score = ctx.saved_tensors
         return fmoe_cuda.topk_softmax_bwd(grad_score.contiguous(), score, idx,
                                           ctx.n_expert), None
+
+
+SCORES = {"sigmoid": 0, "softmax": 1}      # FMOE_SCORE_* of the C ABI
+
+
+class ScoreTopK(Function):
+    r"""(idx, weight) of scored routing, one kernel each way; idx carries no gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, n_group, top_group, group_best, score, renormalize,
+                scale):
+        logits = logits.contiguous()
+        idx, weight = fmoe_cuda.score_topk_fwd(logits, bias, top_k, n_group, top_group,
+                                               group_best, score, renormalize, scale)
+        ctx.args = score, renormalize, scale
+        ctx.save_for_backward(logits, idx)
+        ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)
+        return idx, weight
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _grad_idx, grad_weight):
+        if grad_weight is None:
+            return (None,) * 9
+        logits, idx = ctx.saved_tensors
+        return (fmoe_cuda.score_topk_bwd(grad_weight.contiguous(), logits, idx, *ctx.args),
+                ) + (None,) * 8
+
+
+def score_topk(logits, top_k: int, bias=None, score: str = "sigmoid", n_group: int = 1,
+               top_group: int = 1, group_best: int = 2, renormalize: bool = True,
+               scale: float = 1.0):
+    r"""Scored routing of logits [..., E] on the GPU: `(idx [T, k] int64, weight [T, k])`.
+
+    The scores s are the sigmoid or the softmax of the logits.  Experts are chosen by
+    v = s + bias (`bias`: float32 [E], e.g. a load-balancing bias; it takes no part in the
+    weights and gets no gradient) among the `top_group` best of `n_group` equal groups of
+    consecutive experts, a group counting the sum of its `group_best` (1 or 2) largest v;
+    ties go to the lower index.  The weights are the chosen scores, divided by their sum if
+    `renormalize`, times `scale`.  An expert whose logit or bias is -inf is never chosen; a
+    slot for which nobody is left is -1 (a dropped slot) with weight 0."""
+    if score not in SCORES:
+        raise ValueError(f"score must be one of {sorted(SCORES)}, not {score!r}")
+    flat = logits.reshape(-1, logits.shape[-1])
+    if bias is not None:
+        bias = bias.detach().to(torch.float32).contiguous()
+    return ScoreTopK.apply(flat, bias, top_k, n_group, top_group, group_best, SCORES[score],
+                           renormalize, scale)
 
 
 class Gelu(Function):

@@ -4,7 +4,9 @@ ops or define the default behaviour)."""
 from .base_gate import BaseGate
 from .naive_gate import NaiveGate
 from .gshard_gate import GShardGate
+from .score_gate import ScoreGate
 from .switch_gate import SwitchGate
 from .utils import limit_by_capacity
 
-__all__ = ["BaseGate", "NaiveGate", "GShardGate", "SwitchGate", "limit_by_capacity"]
+__all__ = ["BaseGate", "NaiveGate", "GShardGate", "ScoreGate", "SwitchGate",
+           "limit_by_capacity"]

@@ -1,0 +1,227 @@
+r"""Experts with 4-bit weights: rows in microscaled floating point (MXFP4 of the OCP
+Microscaling Formats specification), their products on the matrix cores, and an expert
+module for `FMoE` layers that holds nothing else.
+
+A block of 32 features shares a power of two (one byte, exponent + 127; 255 is NaN), every
+value is a 4-bit E2M1 code (0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign).  Weights are quantised
+once and stay frozen; rows of activations are quantised on the way into a product, their
+gradient passes straight through that rounding.
+
+The reference has no such experts; they stand in the place of the fused `_Expert` of
+fmoe/transformer.py:11-31.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import fmoe_cuda
+from .functions import (FusedGatherCombine, FusedScatter, RoutePlan, SegmentTable,
+                        apply_activation)
+from .linear import _segments, native_act
+
+BLOCK = 32      # features that share a scale
+
+
+class MXTensor:
+    r"""Rows of `features` values in MXFP4: `codes` uint8 [..., rows, 64 ceil(features / 128)],
+    the even feature of a pair in the low half of its byte, and `scales` uint8
+    [..., rows, 16 ceil(features / 512)].  Codes behind the last feature are zero."""
+
+    __slots__ = ("codes", "scales", "features")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int):
+        self.codes, self.scales, self.features = codes, scales, int(features)
+
+    @property
+    def shape(self):
+        return torch.Size((*self.codes.shape[:-1], self.features))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def to(self, device) -> "MXTensor":
+        return MXTensor(self.codes.to(device), self.scales.to(device), self.features)
+
+    def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
+        r"""The values [..., rows, features] as `dtype` (float32, float16 or bfloat16)."""
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        if out.numel():
+            fmoe_cuda.mx_dequantize(
+                self.codes.reshape(-1, self.codes.shape[-1]),
+                self.scales.reshape(-1, self.scales.shape[-1]), out.view(-1, self.features))
+        return out
+
+    @classmethod
+    def from_blocks(cls, codes: torch.Tensor, scales: torch.Tensor) -> "MXTensor":
+        r"""From the tight layout of MXFP4 checkpoints: codes uint8 [..., rows, K / 2] and
+        scales uint8 [..., rows, K / 32], K a multiple of 32."""
+        k = 2 * codes.shape[-1]
+        if (k % BLOCK or k == 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8
+                or scales.shape != (*codes.shape[:-1], k // BLOCK)):
+            raise ValueError("codes must be uint8 [..., K / 2] and scales uint8 [..., K / 32]")
+        pad = nn.functional.pad
+        return cls(pad(codes, (0, -(-k // 128) * 64 - codes.shape[-1])),
+                   pad(scales, (0, -(-k // 512) * 16 - scales.shape[-1])), k)
+
+
+def quantize(x: torch.Tensor) -> MXTensor:
+    r"""x [..., features] (float32, float16 or bfloat16, on the GPU) in MXFP4.  The scale of a
+    block is 2^(floor(log2(max |x|)) - 2); values are rounded to nearest, ties to the even
+    code, and saturate at 6 times the scale.  A block with an infinity or a NaN is NaN."""
+    x = x.detach()
+    k = x.shape[-1]
+    codes, scales = fmoe_cuda.mx_quantize(x.reshape(-1, k).contiguous())
+    return MXTensor(codes.view(*x.shape[:-1], codes.shape[-1]),
+                    scales.view(*x.shape[:-1], scales.shape[-1]), k)
+
+
+class MXLinear(Function):
+    r"""All experts' linear maps on 4-bit weights in one grouped product; the gradient of the
+    rows is that of the weights' values, straight through the rounding of the rows."""
+
+    @staticmethod
+    def forward(ctx, x, seg_off, w_codes, w_scales, bias):
+        in_feat = x.shape[1]
+        codes, scales = fmoe_cuda.mx_quantize(x.contiguous())
+        out = torch.empty((x.shape[0], w_codes.shape[1]), dtype=x.dtype, device=x.device)
+        fmoe_cuda.mx_linear_fwd(codes, scales, w_codes, w_scales, in_feat, bias, seg_off, out)
+        ctx.in_feat = in_feat
+        ctx.save_for_backward(seg_off, w_codes, w_scales)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        seg_off, w_codes, w_scales = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, db = fmoe_cuda.mx_linear_bwd(grad_out.contiguous(), seg_off, w_codes, w_scales,
+                                         ctx.in_feat, need[0], need[4])
+        return dx, None, None, None, db
+
+
+def linear(x: torch.Tensor, fwd_expert_count, weight: MXTensor, bias=None) -> torch.Tensor:
+    r"""y[rows of e] = x[rows of e] @ weight[e].T + bias[e]: the grouped linear layer of
+    `FMoELinear` with 4-bit weights [E, out, in].  x [rows, in] holds the rows in expert
+    order and is quantised on the way; `fwd_expert_count` is an int64 tensor of row counts
+    (host or device) or a SegmentTable; bias [E, out] has x's dtype, as has the result."""
+    if x.dim() != 2 or x.shape[1] != weight.features:
+        raise RuntimeError(f"x must be [rows, {weight.features}], got {tuple(x.shape)}")
+    if not x.is_cuda:
+        raise RuntimeError("x must be a CUDA tensor")
+    if isinstance(fwd_expert_count, torch.Tensor) and not fwd_expert_count.is_cuda and (
+            bool((fwd_expert_count < 0).any()) or int(fwd_expert_count.sum()) > x.shape[0]):
+        raise RuntimeError("expert counts are negative or claim more rows than x holds")
+    return MXLinear.apply(x, _segments(fwd_expert_count, x.device), weight.codes, weight.scales,
+                          None if bias is None else bias.contiguous())
+
+
+def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w1: MXTensor, b1,
+                 w2: MXTensor, b2, activation) -> torch.Tensor:
+    r"""sum_j score[t, j] * expert_{gate_idx[t, j]}(x[t]) over the live slots (index >= 0), the
+    experts being `linear -> activation -> linear` with 4-bit weights w1 [E, hidden, in] and
+    w2 [E, out, hidden].  Without gradients and for GELU and ReLU: routing, one pass that
+    quantises the tokens into expert order, the first product with bias, activation and
+    quantisation in its epilogue, the second product, the weighted combine.  Otherwise the
+    chain of single operators, in which the hidden layer is rounded to x's dtype on its way."""
+    top_k = gate_idx.shape[-1] if gate_idx.dim() >= 2 else 1
+    if x.dim() != 2 or x.shape[1] != w1.features or w1.codes.shape[-2] != w2.features:
+        raise RuntimeError("x [tokens, in], w1 [E, hidden, in] and w2 [E, out, hidden] disagree")
+    n_expert = w1.codes.shape[0]
+    act = native_act(activation, x)
+    grads = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, score, b1, b2))
+    if grads or not act or x.dtype == torch.float64:
+        plan = RoutePlan(gate_idx.reshape(-1, top_k), n_expert)
+        h = linear(FusedScatter.apply(x, plan), plan.segments, w1, b1)
+        h = apply_activation(activation, h, plan.n_rows_dev)
+        y = linear(h, plan.segments, w2, b2)
+        return FusedGatherCombine.apply(y, score.reshape(-1, top_k), plan)
+    x = x.contiguous()
+    n_tokens = x.shape[0]
+    _pos, _counts, seg_off, inv = fmoe_cuda.route(gate_idx.reshape(-1, top_k).contiguous(),
+                                                  n_expert)
+    codes, scales = fmoe_cuda.mx_quantize_tokens(x, inv, top_k)
+    codes, scales = fmoe_cuda.mx_linear_act_fwd(codes, scales, w1.codes, w1.scales, w1.features,
+                                                b1, seg_off, act)
+    out = torch.empty((n_tokens * top_k, w2.codes.shape[1]), dtype=x.dtype, device=x.device)
+    fmoe_cuda.mx_linear_fwd(codes, scales, w2.codes, w2.scales, w2.features, b2, seg_off, out)
+    score = score.reshape(n_tokens, top_k).contiguous().to(x.dtype)
+    return fmoe_cuda.gather_combine_fwd(out, inv, score, n_tokens, top_k)
+
+
+class MXExpert(nn.Module):
+    r"""The experts of a layer (`linear -> activation -> linear`) with 4-bit weights, in the
+    place of the fused `_Expert`: `layer.experts = MXExpert.from_expert(layer.experts)`, or
+    `quantize_experts(layer)`.  Weights are uint8 buffers and frozen; the biases stay
+    parameters.  Accepts host counts or a device-side SegmentTable, as `_Expert` does."""
+
+    accepts_segment_table = True
+
+    def __init__(self, w1: MXTensor, b1, w2: MXTensor, b2, activation):
+        super().__init__()
+        if w1.codes.dim() != 3 or w2.codes.dim() != 3 or w1.shape[0] != w2.shape[0] or \
+                w1.shape[1] != w2.features:
+            raise ValueError(f"w1 [E, hidden, in] and w2 [E, out, hidden] disagree: "
+                             f"{tuple(w1.shape)}, {tuple(w2.shape)}")
+        for name, w in (("w1", w1), ("w2", w2)):
+            self.register_buffer(name + "_codes", w.codes.contiguous())
+            self.register_buffer(name + "_scales", w.scales.contiguous())
+        self.in_features, self.hidden_features = w1.features, w2.features
+        self.num_expert = w1.shape[0]
+        for name, b in (("b1", b1), ("b2", b2)):
+            b = None if b is None else nn.Parameter(b.detach().clone(),
+                                                    requires_grad=b.requires_grad)
+            self.register_parameter(name, b)
+        self.activation = activation
+
+    @classmethod
+    def from_expert(cls, expert) -> "MXExpert":
+        r"""From a fused `_Expert` on the GPU, its weights quantised."""
+        l1, l2 = expert.htoh4, expert.h4toh
+        return cls(quantize(l1.weight), l1.bias, quantize(l2.weight), l2.bias, expert.activation)
+
+    @property
+    def w1(self) -> MXTensor:
+        return MXTensor(self.w1_codes, self.w1_scales, self.in_features)
+
+    @property
+    def w2(self) -> MXTensor:
+        return MXTensor(self.w2_codes, self.w2_scales, self.hidden_features)
+
+    def forward(self, inp, fwd_expert_count):
+        x = linear(inp, fwd_expert_count, self.w1, self.b1)
+        live = fwd_expert_count.seg_off[-1:] if isinstance(fwd_expert_count, SegmentTable) else None
+        x = apply_activation(self.activation, x, live)
+        return linear(x, fwd_expert_count, self.w2, self.b2)
+
+    # what FMoE.forward asks of a module that can run the whole dispatch
+    def can_run_layer(self, inp, top_k) -> bool:
+        return (torch.is_tensor(inp) and inp.dim() == 2 and inp.is_cuda and 1 <= top_k <= 64
+                and "forward" not in self.__dict__ and type(self).forward is MXExpert.forward
+                and not (self._forward_hooks or self._forward_pre_hooks or self._backward_hooks
+                         or self._backward_pre_hooks))
+
+    def run_layer(self, inp, gate_idx, score):
+        return expert_layer(inp, gate_idx, score, self.w1, self.b1, self.w2, self.b2,
+                            self.activation)
+
+    def run_gated_layer(self, gate, inp):
+        return None      # (the gate always runs as the module it is)
+
+    def __len__(self):
+        return self.num_expert
+
+
+def quantize_experts(layer):
+    r"""Puts the fused experts of an `FMoE` layer on the GPU into 4 bits, in place; returns the
+    layer.  Its state dict then holds `experts.w1_codes` and so on; gate and hooks stay."""
+    from .transformer import _Expert
+
+    if not isinstance(layer.experts, _Expert):
+        raise TypeError("only a layer whose experts are one fused module can be quantised")
+    layer.experts = MXExpert.from_expert(layer.experts)
+    return layer

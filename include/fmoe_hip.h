@@ -62,6 +62,14 @@ typedef enum fmoe_balance_gate {
   FMOE_GATE_SWITCH = 1  /* top-1, fmoe/gates/switch_gate.py:24-60 */
 } fmoe_balance_gate;
 
+/* The scores of fmoe_score_topk_fwd. */
+typedef enum fmoe_score {
+  FMOE_SCORE_SIGMOID = 0,
+  FMOE_SCORE_SOFTMAX = 1
+} fmoe_score;
+
+/* Largest feature size of a row in MXFP4. */
+#define FMOE_MX_MAX_FEATURES (1 << 22)
 /* Largest number of experts the routing kernels keep in LDS. */
 #define FMOE_MAX_EXPERTS 4096
 /* Largest top_k of the fused gate kernels. */
@@ -465,6 +473,76 @@ int fmoe_gate_linear_grad(const void* x, const int64_t* pos, const int32_t* seg_
                           const void* dslot, void* dwg, void* dbg, int64_t n_tokens, int64_t top_k,
                           int64_t d, int32_t n_expert, void* workspace, int64_t workspace_bytes,
                           int dtype, void* stream);
+
+/*
+ * Scored top-k routing: with logits l [n_tokens, n_expert] (f32, f16 or bf16) and
+ *   s = sigmoid(l) or softmax(l) over the experts (`score`, an fmoe_score), in f32
+ *   v = s + bias                       (bias float[n_expert] or NULL)
+ * the experts of the top_group best of n_group equal groups of consecutive experts stay (the
+ * value of a group: the sum of its group_best = 1 or 2 largest v), and
+ *   idx[t][j]    = the expert with the j-th largest v among them (equal v: lower index first)
+ *   weight[t][j] = scale * s / (sum of the chosen s + 1e-20) with renormalize, else scale * s
+ * An expert whose logit or bias is -inf is never chosen; where fewer than top_k experts are
+ * left, the last slots are -1 (dropped, as everywhere in this library) with weight 0.  A NaN
+ * ranks above every number, as in fmoe_topk_softmax_fwd.  n_expert <= 512, n_group <= 64,
+ * top_k <= FMOE_MAX_GATE_TOP_K.
+ * The reference has no such gate; it stands beside fmoe/gates/naive_gate.py:31-38.
+ */
+int fmoe_score_topk_fwd(const void* logits, const float* bias, int64_t n_tokens, int32_t n_expert,
+                        int32_t top_k, int32_t n_group, int32_t top_group, int32_t group_best,
+                        int score, int renormalize, float scale, int64_t* idx, void* weight,
+                        int dtype, void* stream);
+/*
+ * Its gradient with respect to the logits (all n_tokens * n_expert entries are written); the
+ * choice and the bias have none.  With S = sum of the chosen s + 1e-20:
+ *   ds_j = scale / S * (dweight_j - sum_i dweight_i s_i / S)   (renormalize),  or scale * dweight_j
+ *   sigmoid: dl = ds s (1 - s), zero for experts not chosen
+ *   softmax: dl_e = s_e (ds_e - sum_i ds_i s_i) for every expert
+ */
+int fmoe_score_topk_bwd(const void* dweight, const void* logits, const int64_t* idx,
+                        int64_t n_tokens, int32_t n_expert, int32_t top_k, int score,
+                        int renormalize, float scale, void* dlogits, int dtype, void* stream);
+
+/*
+ * Rows in MXFP4 (OCP Microscaling Formats): blocks of 32 features, each value a 4-bit E2M1 code
+ * (0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign bit), each block a power of two held as the byte
+ * exponent + 127 (255: the whole block is NaN).  A row of `features` values takes
+ * fmoe_mx_code_bytes() = 64 ceil(features / 128) bytes of codes, the even feature of a pair in
+ * the low half of its byte, and fmoe_mx_scale_bytes() = 16 ceil(features / 512) scale bytes.
+ * Behind the last feature, codes are zero and the scale bytes up to the next multiple of 128
+ * features are not 255; later ones are never used.  Both arrays are 16-byte aligned.
+ *
+ *   _quantize         per block e = floor(log2(max |x|)) - 2, not below -127; codes are x / 2^e
+ *                     rounded to nearest (ties to the even code) and saturated at 6.  A block
+ *                     with an infinity or a NaN becomes NaN.  The first *n_rows_dev rows only, if
+ *                     n_rows_dev (DEVICE int32) is not NULL.
+ *   _quantize_tokens  row t goes to the rows inv[t * top_k + j] that are not -1 (inv of
+ *                     fmoe_route): the dispatch of fmoe_scatter_tokens in the same pass.
+ *   _dequantize       the values, rounded to dtype where that is too narrow for them.
+ * dtype: f32, f16 or bf16.  The reference has no such format.
+ */
+int64_t fmoe_mx_code_bytes(int64_t features);
+int64_t fmoe_mx_scale_bytes(int64_t features);
+int fmoe_mx_quantize(const void* x, int64_t n_rows, int64_t features, const int32_t* n_rows_dev,
+                     void* codes, void* scales, int dtype, void* stream);
+int fmoe_mx_quantize_tokens(const void* x, const int32_t* inv, int64_t n_tokens, int64_t top_k,
+                            int64_t features, void* codes, void* scales, int dtype, void* stream);
+int fmoe_mx_dequantize(const void* codes, const void* scales, int64_t n_rows, int64_t features,
+                       void* out, int dtype, void* stream);
+
+/*
+ * The grouped linear layer (fmoe_grouped_linear_fwd) on MXFP4 operands:
+ *   y[seg_e] = act(x[seg_e] * w_e^T + b_e),  f32 products and sums on the matrix cores
+ * x: n_rows rows of in_feat features; w: n_expert * out_feat rows of in_feat features; bias
+ * [n_expert, out_feat] of `dtype` or NULL.  The result is either y [n_rows, out_feat] of `dtype`
+ * (f32, f16 or bf16), or, with y_codes and y_scales, MXFP4 rows of out_feat features: the
+ * f32 values quantised as fmoe_mx_quantize does (y is NULL then).  Rows at or behind
+ * seg_off[n_expert] are not written.
+ */
+int fmoe_mx_linear_fwd(const void* x_codes, const void* x_scales, const void* w_codes,
+                       const void* w_scales, const void* bias, const int32_t* seg_off, int act,
+                       void* y, void* y_codes, void* y_scales, int64_t n_rows, int64_t in_feat,
+                       int64_t out_feat, int64_t n_expert, int dtype, void* stream);
 
 /*
  * y[i] = gelu(x[i]) = 0.5 x (1 + erf(x / sqrt 2)) over n elements, and
