@@ -69,7 +69,7 @@ typedef enum fmoe_score {
 } fmoe_score;
 
 /* Largest feature size of a row in MXFP4. */
-#define FMOE_MX_MAX_FEATURES (1 << 22)
+#define FMOE_MX_MAX_FEATURES (1 << 20)
 /* Largest number of experts the routing kernels keep in LDS. */
 #define FMOE_MAX_EXPERTS 4096
 /* Largest top_k of the fused gate kernels. */
