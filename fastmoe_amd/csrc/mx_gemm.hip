@@ -54,79 +54,133 @@ __device__ __forceinline__ i32x4 mx_descriptor(const void* p, int64_t bytes) {
   return r;
 }
 
-// What a tile writes: descriptors that end with its last valid row, so that rows past the end
-// need no branch, and the bias of its expert.
-template <typename T, bool QUANT> struct MxOutput {
-  __amdgpu_buffer_rsrc_t y, yc, ys, bias;
-  int n, size, bias_dtype, act;
-  bool packed, has_bias;
+// gelu(x) = x Phi(x) with Phi(x) = 1/2 + x P(x^2) on |x| <= 5.2 and constant outside: P of
+// degree 13 in t = 2 x^2 / 5.2^2 - 1 (a least-squares fit on Chebyshev nodes), within 1e-6 of
+// gelu for |x| < 7, which is what rounding to f32 on the way costs as well.  18 full-rate
+// instructions where erff takes about 60, with branches: with one wave on a SIMD nothing hides
+// them (a 256 x 256 tile of 4096 features: 27 us of matrix instructions, 26 us of erff).
+__device__ __forceinline__ float mx_gelu(float x) {
+  const float c = __builtin_amdgcn_fmed3f(x, -5.2f, 5.2f);
+  const float t = fmaf(c * (2.f / (5.2f * 5.2f)), c, -1.f);
+  float r = -0.000377040647f;
+  r = fmaf(r, t, 0.00118033495f);
+  r = fmaf(r, t, -0.00150067825f);
+  r = fmaf(r, t, 0.00202824641f);
+  r = fmaf(r, t, -0.00450842502f);
+  r = fmaf(r, t, 0.00834169798f);
+  r = fmaf(r, t, -0.012636275f);
+  r = fmaf(r, t, 0.0180494618f);
+  r = fmaf(r, t, -0.0246950798f);
+  r = fmaf(r, t, 0.0319717675f);
+  r = fmaf(r, t, -0.0399323255f);
+  r = fmaf(r, t, 0.0500257686f);
+  r = fmaf(r, t, -0.0677436069f);
+  r = fmaf(r, t, 0.135949984f);
+  return x * fmaf(c, r, 0.5f);          // (the clamp takes a NaN for a number, the product not)
+}
 
-  // rows x0 .. x0 + rows - 1 of the output, of expert e
-  __device__ __forceinline__ MxOutput(const MxGemmArgs& a, int e, int64_t x0, int rows) {
+// How a product leaves: y where rows are whole 16-byte packs, any other y, or MXFP4 again behind
+// one of the activations.
+enum MxMode { kMxPacked, kMxAny, kMxQuant, kMxQuantGelu, kMxQuantRelu };
+constexpr bool mx_quantises(int mode) { return mode >= kMxQuant; }
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_resource(const void* p, int64_t bytes) {
+  const uint64_t u = (uint64_t)p;
+  void* q = (void*)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) |
+                    (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u));
+  return __builtin_amdgcn_make_buffer_rsrc(
+      q, 0, __builtin_amdgcn_readfirstlane(dma_num_records(bytes)), 0x00020000);
+}
+
+// The bias of expert e, as its rows are read: nothing behind the last feature, nothing at all
+// without a bias.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_bias_rows(const MxGemmArgs& a, int e) {
+  const int64_t bytes = (int64_t)a.out_feat * (a.dtype == FMOE_F32 ? 4 : 2);
+  return mx_resource((const char*)a.bias + e * bytes, a.bias ? bytes : 0);
+}
+// The bias of 8 consecutive features from n0 on (zeros where there is none).
+__device__ __forceinline__ void mx_load_bias(const MxGemmArgs& a, __amdgpu_buffer_rsrc_t rows,
+                                             int n0, float (&b)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (a.dtype == FMOE_F32) {
+      b[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, (n0 + i) * 4, 0, 0));
+    } else {
+      const uint16_t u = __builtin_amdgcn_raw_buffer_load_b16(rows, (n0 + i) * 2, 0, 0);
+      b[i] = a.dtype == FMOE_BF16 ? __uint_as_float((uint32_t)u << 16)
+                                  : __half2float(__builtin_bit_cast(__half, u));
+    }
+  }
+}
+
+// What a tile writes: descriptors that end with its last valid row, so that rows past the end
+// need no branch.
+template <typename T, int MODE> struct MxOutput {
+  static constexpr bool QUANT = mx_quantises(MODE);
+  __amdgpu_buffer_rsrc_t y, yc, ys;
+  T* y_row;                 // row 0 of the tile
+  int n, rows;
+
+  // rows x0 .. x0 + rows - 1 of the output
+  __device__ __forceinline__ MxOutput(const MxGemmArgs& a, int64_t x0, int rows_) {
     n = a.out_feat;
-    act = a.act;
-    bias_dtype = a.dtype;
-    has_bias = a.bias != nullptr;
-    const int bsize = a.dtype == FMOE_F32 ? 4 : 2;
-    bias = resource((const char*)a.bias + (int64_t)e * n * bsize, (int64_t)n * bsize);
+    rows = rows_;
     if (QUANT) {
       const int64_t cr = mx_code_bytes(n), sr = mx_scale_bytes(n);
-      yc = resource(a.yc + x0 * cr, rows * cr);
-      ys = resource(a.ys + x0 * sr, rows * sr);
+      yc = mx_resource(a.yc + x0 * cr, rows * cr);
+      ys = mx_resource(a.ys + x0 * sr, rows * sr);
     } else {
-      y = resource((T*)a.y + x0 * n, (int64_t)rows * n * sizeof(T));
-      packed = n % 8 == 0 && (uintptr_t)a.y % 16 == 0;
+      y_row = (T*)a.y + x0 * n;
+      y = mx_resource(y_row, (int64_t)rows * n * sizeof(T));
     }
-  }
-  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_t bytes) {
-    const uint64_t u = (uint64_t)p;
-    void* q = (void*)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) |
-                      (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u));
-    return __builtin_amdgcn_make_buffer_rsrc(
-        q, 0, __builtin_amdgcn_readfirstlane(dma_num_records(bytes)), 0x00020000);
   }
 
-  // The bias of features n0 .. n0 + 7 (zero behind the last one, and without a bias).
-  __device__ __forceinline__ void load_bias(int n0, float (&b)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = 0.f;
-    if (!has_bias) return;
-    if (bias_dtype == FMOE_F32) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        b[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(bias, (n0 + i) * 4, 0, 0));
-      return;
-    }
+  static __device__ __forceinline__ void activate(float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint16_t u = __builtin_amdgcn_raw_buffer_load_b16(bias, (n0 + i) * 2, 0, 0);
-      b[i] = bias_dtype == FMOE_BF16 ? __uint_as_float((uint32_t)u << 16)
-                                     : __half2float(__builtin_bit_cast(__half, u));
+      if (MODE == kMxQuantGelu) v[i] = mx_gelu(v[i]);
+      if (MODE == kMxQuantRelu) v[i] = v[i] < 0.f ? 0.f : v[i];     // (a NaN stays)
     }
   }
 
-  // Activation and output of features n0 .. n0 + 7 of the tile's row `row`.  All lanes of a wave
-  // come here together; lanes l, l ^ 16, l ^ 32 and l ^ 48 hold one block of 32 features.
-  __device__ __forceinline__ void store(int row, int n0, float (&v)[8]) const {
-    if (act == FMOE_ACT_GELU) {
+  // The word of codes and the scale byte of features n0 .. n0 + 7.  All lanes of a wave come here
+  // together; lanes l, l ^ 16, l ^ 32 and l ^ 48 hold one block of 32 features.
+  __device__ __forceinline__ uint32_t quantised(int n0, float (&v)[8], int& byte) const {
+    uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = gelu_direct(v[i]);
-    } else if (act == FMOE_ACT_RELU) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];   // (a NaN stays)
+    for (int i = 0; i < 8; ++i) {
+      v[i] = n0 + i < n ? v[i] : 0.f;
+      m = max(m, magnitude_bits(v[i]));
     }
-    if constexpr (!QUANT) {
-      const uint32_t at = ((uint32_t)row * n + n0) * (uint32_t)sizeof(T);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16, kWave));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
+    byte = mx_scale_byte(m);
+    return mx_codes(v, byte);
+  }
+
+  // Activation and output of features n0 .. n0 + 7 of the tile's row `row`, from the registers.
+  __device__ __forceinline__ void store(int row, int n0, float (&v)[8]) const {
+    activate(v);
+    if constexpr (QUANT) {
+      int byte;
+      const uint32_t word = quantised(n0, v, byte);
+      const int cr = (int)mx_code_bytes(n), sr = (int)mx_scale_bytes(n);
+      const bool in = n0 < cr * 2;
+      __builtin_amdgcn_raw_buffer_store_b32(word, yc, in ? row * cr + n0 / 2 : kDmaOutOfRange, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b8(
+          (uint8_t)byte, ys, in && (n0 & 31) == 0 ? row * sr + n0 / kMxBlock : kDmaOutOfRange, 0, 0);
+    } else {
       T o[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = Elem<T>::from_acc(v[i]);
-      if (packed) {
-        const uint32_t to = n0 < n ? at : kDmaOutOfRange;
+      const uint32_t at = ((uint32_t)row * n + n0) * (uint32_t)sizeof(T);
+      if constexpr (MODE == kMxPacked) {
 #pragma unroll
         for (int p = 0; p < (int)sizeof(T) / 2; ++p) {
           i32x4 w;
           __builtin_memcpy(&w, (const char*)o + p * 16, 16);
-          __builtin_amdgcn_raw_buffer_store_b128(w, y, to, p * 16, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(
+              w, y, n0 + p * Pack16<T>::kN < n ? at + p * 16 : kDmaOutOfRange, 0, 0);
         }
       } else {
 #pragma unroll
@@ -138,24 +192,85 @@ template <typename T, bool QUANT> struct MxOutput {
             __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, o[i]), y, to, 0, 0);
         }
       }
-    } else {
-      uint32_t m = 0;
+    }
+  }
+
+  // Stores of a wave for 16 rows of P groups of 32 features, `times` over, where their number is
+  // known (and the counter takes it).
+  template <int P, int ROW> static constexpr int stores(int times) {
+    const int n = times * (QUANT ? 2 : P * 32 * (int)sizeof(T) / 64);
+    return n < 63 ? n : 63;
+  }
+
+  // Activation and output of 16 rows from row `row0` of the tile on: lane (m, g) holds features
+  // 8 g .. 8 g + 7 of each of P groups of 32, from feature `col` on, of row m.  They change places
+  // in `stage` (16 rows of ROW bytes, the wave's own) so that a store covers whole pieces of rows.
+  template <int P, int ROW>
+  __device__ __forceinline__ void store_rows(char* stage, int lane, int row0, int col,
+                                             float (&v)[P][8]) const {
+    const int m = lane & 15, g = lane >> 4;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = n0 + i < n ? v[i] : 0.f;
-        m = max(m, magnitude_bits(v[i]));
-      }
-      m = max(m, (uint32_t)__shfl_xor((int)m, 16, kWave));
-      m = max(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
-      const int byte = mx_scale_byte(m);
+    for (int p = 0; p < P; ++p) activate(v[p]);
+    if constexpr (QUANT) {
+      static_assert(P == 2 || P == 4, "a wave's features are 64 or 128");
       const int cr = (int)mx_code_bytes(n), sr = (int)mx_scale_bytes(n);
-      const bool in = n0 < cr * 2;
-      __builtin_amdgcn_raw_buffer_store_b32(mx_codes(v, byte), yc,
-                                            in ? row * cr + n0 / 2 : kDmaOutOfRange, 0, 0);
-      // (the row's scales reach at least as far as its codes)
-      const bool first = in && (n0 & 31) == 0;
-      __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, ys,
-                                           first ? row * sr + n0 / kMxBlock : kDmaOutOfRange, 0, 0);
+      uint32_t bytes = 0;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        int byte;
+        const uint32_t word = quantised(col + p * 32 + 8 * g, v[p], byte);
+        bytes |= (uint32_t)byte << (8 * p);
+        *(uint32_t*)(stage + m * (P * 16) + ((p * 16 + g * 4) ^ ((m & 4) * 4))) = word;
+      }
+      // (columns end on 128 features, and the row's scales reach at least as far as its codes)
+      const int r = lane / P, c = lane % P, n0 = col + c * 32;
+      const bool in = r < 16 && n0 < cr * 2;
+      const i32x4 w = *(const i32x4*)(stage + (r & 15) * (P * 16) + ((c * 16) ^ ((r & 4) * 4)));
+      __builtin_amdgcn_raw_buffer_store_b128(w, yc, in ? (row0 + r) * cr + n0 / 2 : kDmaOutOfRange, 0, 0);
+      const int to = g == 0 && col < cr * 2 ? (row0 + m) * sr + col / kMxBlock : (int)kDmaOutOfRange;
+      if constexpr (P == 4) __builtin_amdgcn_raw_buffer_store_b32(bytes, ys, to, 0, 0);
+      else __builtin_amdgcn_raw_buffer_store_b16((uint16_t)bytes, ys, to, 0, 0);
+    } else {
+      constexpr int kPass = ROW / (32 * (int)sizeof(T)) < P ? ROW / (32 * (int)sizeof(T)) : P;
+      constexpr int kBytes = kPass * 32 * (int)sizeof(T);       // of a row, in a pass
+      constexpr int kPacks = kBytes / 16, kN = 16 / (int)sizeof(T);
+      static_assert(P % kPass == 0 && (kPacks == 8 || kPacks == 16), "whole passes");
+#pragma unroll
+      for (int q = 0; q < P; q += kPass) {
+#pragma unroll
+        for (int p = 0; p < kPass; ++p)
+#pragma unroll
+          for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+            T o[kN];
+#pragma unroll
+            for (int i = 0; i < kN; ++i) o[i] = Elem<T>::from_acc(v[q + p][h * kN + i]);
+            i32x4 w;
+            __builtin_memcpy(&w, o, 16);
+            const int pack = (p * 4 + g) * ((int)sizeof(T) / 2) + h;
+            *(i32x4*)(stage + m * kBytes + ((pack ^ m) & (kPacks - 1)) * 16) = w;
+          }
+        const int c = lane % kPacks, n0 = col + q * 32 + c * kN;
+#pragma unroll
+        for (int u = 0; u < kPacks / 4; ++u) {
+          const int r = u * (64 / kPacks) + lane / kPacks, row = row0 + r;
+          const i32x4 w = *(const i32x4*)(stage + r * kBytes + ((c ^ r) & (kPacks - 1)) * 16);
+          if constexpr (MODE == kMxPacked) {
+            __builtin_amdgcn_raw_buffer_store_b128(
+                w, y, n0 < n ? ((uint32_t)row * n + n0) * (uint32_t)sizeof(T) : kDmaOutOfRange, 0, 2);
+          } else if (row < rows) {
+            T* to = y_row + (int64_t)row * n + n0;
+            if (n0 + kN <= n) {
+              __builtin_memcpy(to, &w, 16);
+            } else {
+              T o[kN];
+              __builtin_memcpy(o, &w, 16);
+#pragma unroll
+              for (int i = 0; i < kN; ++i)
+                if (n0 + i < n) to[i] = o[i];
+            }
+          }
+        }
+      }
     }
   }
 };
@@ -163,7 +278,7 @@ template <typename T, bool QUANT> struct MxOutput {
 // ------------------------------------------------------------------------- few rows
 // Weights straight from memory into registers: a workgroup's 4 waves take 16 NT rows of an expert and
 // 32 features each (KS == 1), or the same 32 features and a quarter of K each (KS == 4).
-template <typename T, int NT, int KS, bool QUANT>
+template <typename T, int NT, int KS, int MODE>
 __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
   constexpr int kWaves = 4, kCols = 32 * (kWaves / KS);
   __shared__ int s_sum[2 * kWaves], s_out[4];
@@ -171,7 +286,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   RowTiles<16 * NT, kOneHeight, kWaves> tiles;
   tiles.scan(a.seg_off, a.n_expert, s_sum);
-  const int n_pad = QUANT ? (int)mx_code_bytes(a.out_feat) * 2 : a.out_feat;
+  const int n_pad = mx_quantises(MODE) ? (int)mx_code_bytes(a.out_feat) * 2 : a.out_feat;
   const int n_cols = (n_pad + kCols - 1) / kCols;
   if (tiles.rows_f == 0) return;
   const int col = blockIdx.x / tiles.rows_f, v = blockIdx.x - col * tiles.rows_f;
@@ -242,14 +357,14 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
         for (int j = 0; j < 8; ++j)
           acc[i][j >> 2][j & 3] += part[((w2 * NT + i) * 8 + j) * kWave + lane];
   }
-  const MxOutput<T, QUANT> out(a, t.e, (int64_t)t.row0 + t.m0, min(16 * NT, t.cnt - t.m0));
-  float bias[8];
-  out.load_bias(base + 8 * g, bias);
+  const MxOutput<T, MODE> out(a, (int64_t)t.row0 + t.m0, min(16 * NT, t.cnt - t.m0));
+  float b[8];
+  mx_load_bias(a, mx_bias_rows(a, t.e), base + 8 * g, b);
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     float r[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = acc[i][j >> 2][j & 3] + bias[j];
+    for (int j = 0; j < 8; ++j) r[j] = acc[i][j >> 2][j & 3] + b[j];
     out.store(i * 16 + m, base + 8 * g, r);
   }
 }
@@ -265,9 +380,13 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
 //
 // A stage is two matrix steps of FW * TW instructions per wave.  While the first multiplies, the
 // second's fragments are read, and a barrier behind those reads releases the stage's buffer: the
-// copies of the stage after next follow, dealt out over the rest of both steps.  In the middle of
-// the second step a wait and a barrier publish the next stage, whose first fragments are read in
-// the shadow of the remaining instructions.
+// copies of the stage after next follow, dealt out over the rest of both steps.  In the second
+// step a wait and a barrier publish the next stage, whose first fragments are read in the shadow
+// of the remaining instructions.
+//
+// One workgroup fills a CU (all its registers, nearly all its LDS) and runs tile after tile: the
+// next tile's first two stages are on their way while this one's results leave through a corner
+// of LDS, which turns the lanes' 16 bytes of 16 rows into pieces of 256 bytes of a row.
 typedef __attribute__((address_space(3))) char lds_char;
 
 template <int I, int N, typename F> __device__ __forceinline__ void unroll(F&& f) {
@@ -291,91 +410,130 @@ __device__ __forceinline__ void mx_mfma_at(i32x4 a, int sa, i32x4 b, int sb, f32
   if constexpr (BYTE == 3) FMOE_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
 #undef FMOE_MFMA
 }
+// An accumulator's value.  (Read like this, accumulators have no use in which they would have to
+// be ordinary registers, so that they stay where the matrix instructions want them.)
+__device__ __forceinline__ float mx_read(float c) {
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(c));
+  return v;
+}
 // The 18 wait states between the last matrix instruction and a read of its result.
 __device__ __forceinline__ void mx_mfma_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 template <int TN, int TM> struct MxTile {
-  static constexpr int kRows = TN + TM;
-  static constexpr int kStageBytes = kRows * 128;
+  static constexpr int kStageBytes = (TN + TM) * 128;
   static constexpr int kLoadsW = TN / 32, kLoadsX = TM / 32;       // copies of a wave per stage
   static constexpr int kLoads = kLoadsW + kLoadsX;
-  static constexpr int kScaleLoads = 2;                            // and per group of scales
-  static constexpr int kScaleBytes = 8192;                         // 4 KiB for either operand
-  static constexpr int kLdsBytes = 2 * (kStageBytes + kScaleBytes);
+  static constexpr int kScaleLoads = ((TN + TM) / 64 + 3) / 4;     // and per group of scales
+  static constexpr int kScaleBytes = kScaleLoads * 4096;
+  static constexpr int kOutRow = TN <= 128 ? 128 : 256;            // bytes of a row on its way out
+  static constexpr int kOutBytes = 4 * 16 * kOutRow;
+  static constexpr int kLdsBytes = 2 * (kStageBytes + kScaleBytes) + kOutBytes;
   static constexpr int kGroups = kLdsBytes > 81920 ? 1 : 2;        // workgroups on a CU
-  static_assert(TN % 64 == 0 && TM % 64 == 0 && TN <= 256 && TM <= 256, "even copies per wave");
+  static_assert(TN % 128 == 0 && TM % 64 == 0 && TN <= 256 && TM <= 256, "even copies per wave");
 };
 
-template <typename T, int TN, int TM, bool QUANT>
+// `v`, as a value that the compiler has to derive things from anew: what it could compute once
+// for all tiles would be kept in scratch memory through the K loop, and reading it back waits for
+// the copies under way.
+__device__ __forceinline__ int mx_fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// Where a tile lies.
+struct MxPlace {
+  int e, base, rows;      // expert, first feature, valid rows
+  int64_t x0;             // first row
+};
+
+template <typename T, int TN, int TM, int MODE>
 __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel(MxGemmArgs a) {
   using S = MxTile<TN, TM>;
   constexpr int FW = TN / 32, TW = TM / 32;         // fragments of a wave
   constexpr int kMma = FW * TW;
   extern __shared__ __align__(16) char lds[];
-  __shared__ int s_sum[8], s_out[4];
+  int* const s_find = (int*)(lds + 2 * S::kStageBytes + S::kScaleBytes);   // (idle between tiles)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   RowTiles<TM, kOneHeight, 4> tiles;
-  tiles.scan(a.seg_off, a.n_expert, s_sum);
-  const int n_pad = QUANT ? (int)mx_code_bytes(a.out_feat) * 2 : a.out_feat;
-  const int n_cols = (n_pad + TN - 1) / TN, live = tiles.rows_f * n_cols;
-  const int number = tile_number(blockIdx.x, live);
-  if (number >= live) return;
-  int v, col;
-  tile_order(number, tiles.rows_f, n_cols, v, col);
-  const TileRows t = tiles.find(a.seg_off, v, false, s_out);
-
+  tiles.scan(a.seg_off, a.n_expert, s_find);
+  const int n_pad = mx_quantises(MODE) ? (int)mx_code_bytes(a.out_feat) * 2 : a.out_feat;
+  const int n_cols = (n_pad + TN - 1) / TN;
+  const int live = __builtin_amdgcn_readfirstlane(tiles.rows_f * n_cols);
   const int code_row = (int)mx_code_bytes(a.in_feat), scale_row = (int)mx_scale_bytes(a.in_feat);
-  const int base = col * TN;                        // (below out_feat: columns end on 128)
   const int steps = __builtin_amdgcn_readfirstlane((a.in_feat + kMxStep - 1) / kMxStep);
   const int stages = (steps + 1) / 2;
-  const int64_t w0 = (int64_t)t.e * a.out_feat + base, x0 = (int64_t)t.row0 + t.m0;
-  const int w_rows = min(TN, a.out_feat - base), x_rows = min(TM, t.cnt - t.m0);
-  // every descriptor ends with its last valid row: rows past the end read as zeros
-  const i32x4 w_rsrc = mx_descriptor(a.wc + w0 * code_row, (int64_t)w_rows * code_row);
-  const i32x4 x_rsrc = mx_descriptor(a.xc + x0 * code_row, (int64_t)x_rows * code_row);
-  const i32x4 ws_rsrc = mx_descriptor(a.ws + w0 * scale_row, (int64_t)w_rows * scale_row);
-  const i32x4 xs_rsrc = mx_descriptor(a.xs + x0 * scale_row, (int64_t)x_rows * scale_row);
+
   // A lane's part of the offset of a copy, by the parity of the KiB (8 rows of a fragment's 16):
   // its row within the 8 and its pack.  Rows of a fragment are features 8 (m / 4) + m % 4 of 32.
-  uint32_t w_lane[2], x_lane[2];
-  const int r8 = lane >> 3;
+  uint32_t w_lane[2], x_lane[2], s_lane[S::kScaleLoads];
+  i32x4 w_rsrc, x_rsrc, s_rsrc[S::kScaleLoads];
+  auto pack_of = [](int lane, int p) { return (lane & 7) ^ ((4 * p + (lane >> 4)) & 7); };
+  auto place = [&](int number) {
+    int v, col;
+    tile_order(number, tiles.rows_f, n_cols, v, col);
+    const TileRows t = tiles.find(a.seg_off, v, false, s_find);
+    MxPlace at;
+    at.e = t.e;
+    at.base = col * TN;                             // (below out_feat: columns end on 128)
+    at.x0 = (int64_t)t.row0 + t.m0;
+    at.rows = min(TM, t.cnt - t.m0);
+    return at;
+  };
+  auto aim = [&](const MxPlace& at) {
+    const int lane = mx_fresh(threadIdx.x & 63), r8 = lane >> 3;
+    const int64_t w0 = (int64_t)at.e * a.out_feat + at.base;
+    const int w_rows = min(TN, a.out_feat - at.base);
+    // every descriptor ends with its last valid row: rows past the end read as zeros
+    w_rsrc = mx_descriptor(a.wc + w0 * code_row, (int64_t)w_rows * code_row);
+    x_rsrc = mx_descriptor(a.xc + at.x0 * code_row, (int64_t)at.rows * code_row);
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    const int pack = (lane & 7) ^ ((4 * p + (r8 >> 1)) & 7);
-    w_lane[p] = (uint32_t)((8 * (r8 >> 2) + (r8 & 3)) * code_row + pack * 16);
-    x_lane[p] = (uint32_t)(r8 * code_row + pack * 16);
-  }
-  uint32_t ws_lane = (uint32_t)(((lane & 32) + mx_feature((lane >> 4) & 1, lane & 15)) * scale_row);
-  uint32_t xs_lane = (uint32_t)(lane * scale_row);
+    for (int p = 0; p < 2; ++p) {
+      w_lane[p] = (uint32_t)((8 * (r8 >> 2) + (r8 & 3)) * code_row + pack_of(lane, p) * 16);
+      x_lane[p] = (uint32_t)(r8 * code_row + pack_of(lane, p) * 16);
+    }
+    // the scales of 64 rows of one operand (past both: zeros)
+#pragma unroll
+    for (int i = 0; i < S::kScaleLoads; ++i) {
+      const int kib = wave * S::kScaleLoads + i;
+      const bool w = kib < TN / 64;
+      const i32x4 rw = mx_descriptor(a.ws + w0 * scale_row, (int64_t)w_rows * scale_row);
+      const i32x4 rx = mx_descriptor(a.xs + at.x0 * scale_row, (int64_t)at.rows * scale_row);
+      const int row = w ? kib * 64 + (lane & 32) + mx_feature((lane >> 4) & 1, lane & 15)
+                        : (kib - TN / 64) * 64 + lane;
+      s_rsrc[i] = w ? rw : rx;
+      s_lane[i] = row * 64 < TM * 64 || w ? (uint32_t)(row * scale_row) : kDmaOutOfRange;
+    }
+  };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds;
   auto dma = [&](uint32_t dst, uint32_t offset, i32x4 rsrc) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(offset), "s"(rsrc)
                  : "memory", "m0");
   };
+  auto dma4 = [&](uint32_t dst, uint32_t offset, i32x4 rsrc) {      // a word per lane
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :: "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(offset), "s"(rsrc)
+                 : "memory", "m0");
+  };
   // Copy i of stage `st` into the buffer of its parity: every wave has its share of either
   // operand, so that nothing here depends on the wave but numbers.
-  auto copy = [&](auto ic, int st) {
+  auto copy = [&](auto ic, int st, int row_bytes) {
     constexpr int i = decltype(ic)::value;
     const uint32_t buf = lds0 + (st & 1) * S::kStageBytes;
     if constexpr (i < S::kLoadsW) {
-      constexpr int in4 = 16 * (i & 1) + 4 * ((i >> 1) & 1);
       const int kib = wave * S::kLoadsW + i;
-      const int row = S::kLoadsW % 4 ? 32 * (kib >> 2) + 16 * (kib & 1) + 4 * ((kib >> 1) & 1)
-                                     : wave * (TN / 4) + 32 * (i >> 2) + in4;
-      dma(buf + kib * 1024, w_lane[i & 1] + (uint32_t)(row * code_row + st * 128), w_rsrc);
+      const int row = wave * (TN / 4) + 32 * (i >> 2) + 16 * (i & 1) + 4 * ((i >> 1) & 1);
+      dma(buf + kib * 1024, w_lane[i & 1] + (uint32_t)(row * row_bytes + st * 128), w_rsrc);
     } else {
       const int kib = wave * S::kLoadsX + i - S::kLoadsW;
       dma(buf + TN * 128 + kib * 1024,
-          x_lane[(i - S::kLoadsW) & 1] + (uint32_t)(kib * 8 * code_row + st * 128), x_rsrc);
+          x_lane[(i - S::kLoadsW) & 1] + (uint32_t)(kib * 8 * row_bytes + st * 128), x_rsrc);
     }
   };
-  // The scales of 64 rows of either operand (past the tile: zeros).
   auto copy_scales = [&](int i, int group) {
-    const uint32_t dst = lds0 + 2 * S::kStageBytes + (group & 1) * S::kScaleBytes + i * 4096 + wave * 1024;
-    const uint32_t off = (uint32_t)(wave * 64 * scale_row + group * 16);
-    if (i == 0) dma(dst, ws_lane + off, ws_rsrc);
-    else dma(dst, xs_lane + off, xs_rsrc);
+    dma(lds0 + 2 * S::kStageBytes + (group & 1) * S::kScaleBytes + (wave * S::kScaleLoads + i) * 1024,
+        s_lane[i] + (uint32_t)(group * 16), s_rsrc[i]);
   };
   // Before the copies of stage `st`: past the end of K nothing is read any more, and of a last
   // stage of one step only the first four packs of a row.
@@ -383,13 +541,20 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
     const bool past = st >= stages, half = st * 2 + 1 >= steps;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int pack = (lane & 7) ^ ((4 * p + (r8 >> 1)) & 7);
-      const bool off = past | (half & (pack >= 4));
+      const bool off = past | (half & (pack_of(lane, p) >= 4));
       w_lane[p] = off ? kDmaOutOfRange : w_lane[p];
       x_lane[p] = off ? kDmaOutOfRange : x_lane[p];
     }
-    ws_lane = past ? kDmaOutOfRange : ws_lane;
-    xs_lane = past ? kDmaOutOfRange : xs_lane;
+#pragma unroll
+    for (int i = 0; i < S::kScaleLoads; ++i) s_lane[i] = past ? kDmaOutOfRange : s_lane[i];
+  };
+  auto start = [&] {                                // the copies that a tile begins with
+    bound(0);
+#pragma unroll
+    for (int i = 0; i < S::kScaleLoads; ++i) copy_scales(i, 0);
+    unroll<0, S::kLoads>([&](auto i) { copy(i, 0, code_row); });
+    bound(1);
+    unroll<0, S::kLoads>([&](auto i) { copy(i, 1, code_row); });
   };
 
   const int m = lane & 15, g = lane >> 4, wn = wave >> 1, wm = wave & 1;
@@ -409,44 +574,38 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   // byte g of each of a row's four words (the steps of a group)
   const uint32_t pick = (uint32_t)g | (uint32_t)(4 + g) << 8 | 0x0c0c0000u;
   const uint32_t last_mask = (steps & 3) ? (1u << (8 * (steps & 3))) - 1 : ~0u;
+  // Scales are read kLag ahead of their use, so that nobody waits where they are read: call j
+  // reads fragment j's and finishes fragment j - kLag's.
+  constexpr int kLag = 4;
+  i32x4 sraw[kLag];
   auto read_scale = [&](auto jc, int group) {
     constexpr int j = decltype(jc)::value;
-    const int row = j < FW ? wn * (TN / 2) + j * 16 : 256 + wm * (TM / 2) + (j - FW) * 16;
-    const i32x4 b = *(const i32x4*)(lds + 2 * S::kStageBytes + (group & 1) * S::kScaleBytes +
-                                    (row + m) * 16);
-    const uint32_t lo = __builtin_amdgcn_perm((uint32_t)b[1], (uint32_t)b[0], pick);
-    const uint32_t hi = __builtin_amdgcn_perm((uint32_t)b[3], (uint32_t)b[2], pick);
-    // bytes behind the last step of K may hold anything, and 255 would make a NaN of a zero
-    const int all = (int)(__builtin_amdgcn_perm(hi, lo, 0x05040100u) &
-                          (group * 4 + 4 <= steps ? ~0u : last_mask));
-    if constexpr (j < FW) wsn[j] = all;
-    else xsn[j - FW] = all;
+    if constexpr (j >= kLag) {
+      constexpr int d = j - kLag;
+      const i32x4 b = sraw[d % kLag];
+      const uint32_t lo = __builtin_amdgcn_perm((uint32_t)b[1], (uint32_t)b[0], pick);
+      const uint32_t hi = __builtin_amdgcn_perm((uint32_t)b[3], (uint32_t)b[2], pick);
+      // bytes behind the last step of K may hold anything, and 255 would make a NaN of a zero
+      const int all = (int)(__builtin_amdgcn_perm(hi, lo, 0x05040100u) &
+                            (group * 4 + 4 <= steps ? ~0u : last_mask));
+      if constexpr (d < FW) wsn[d] = all;
+      else xsn[d - FW] = all;
+    }
+    if constexpr (j < FW + TW) {
+      const int row = j < FW ? wn * (TN / 2) + j * 16 : TN + wm * (TM / 2) + (j - FW) * 16;
+      sraw[j % kLag] = *(const i32x4*)(lds + 2 * S::kStageBytes + (group & 1) * S::kScaleBytes +
+                                       (row + m) * 16);
+    }
   };
-  f32x4 acc[TW][FW];
-#pragma unroll
-  for (int i = 0; i < TW; ++i)
-#pragma unroll
-    for (int f = 0; f < FW; ++f) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  using C0 = std::integral_constant<int, 0>;
-  using C1 = std::integral_constant<int, 1>;
   auto next_scales = [&] {
 #pragma unroll
     for (int j = 0; j < FW; ++j) wsc[j] = wsn[j];
 #pragma unroll
     for (int j = 0; j < TW; ++j) xsc[j] = xsn[j];
   };
-  bound(0);
-#pragma unroll
-  for (int i = 0; i < S::kScaleLoads; ++i) copy_scales(i, 0);
-  unroll<0, S::kLoads>([&](auto i) { copy(i, 0); });
-  bound(1);
-  unroll<0, S::kLoads>([&](auto i) { copy(i, 1); });
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
-  __builtin_amdgcn_s_barrier();
-  unroll<0, FW + TW>([&](auto j) { read(j, C0{}, 0); });
-  unroll<0, FW + TW>([&](auto j) { read_scale(j, 0); });
-  next_scales();
+  f32x4 acc[TW][FW];
+  using C0 = std::integral_constant<int, 0>;
+  using C1 = std::integral_constant<int, 1>;
 
   // Where things happen among the 2 * kMma instructions of a stage: the second step's fragments
   // are read behind the first ones, the buffer is released behind kRelease, the next stage is
@@ -455,10 +614,14 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   constexpr int kWindow = kReads < kMma / 2 ? kReads : kMma / 2;
   constexpr int kRelease = kWindow + kMma / 8;
   constexpr int kPublish = kMma + kMma / 4;
-  static_assert(kRelease < kMma && kPublish + kWindow + kWindow / 2 < 2 * kMma, "room for the reads");
+  static_assert(kRelease < kMma && kPublish + kWindow < 2 * kMma, "room for the reads");
   auto one_stage = [&](auto odd_c, int st) {
     constexpr int odd = decltype(odd_c)::value;
     constexpr int kCopies = S::kLoads + (odd ? 0 : S::kScaleLoads);
+    // (the multiples of the row size in the copies' offsets are made where they are used: kept,
+    // they would take more scalar registers than there are)
+    int row_bytes = code_row;
+    asm volatile("" : "+s"(row_bytes));
     // of `count` things dealt over the instructions from .. from + len - 1, those out behind k
     constexpr auto dealt = [](int k, int from, int len, int count) {
       const int n = k < from ? 0 : (k - from + 1) * count / len;
@@ -471,7 +634,7 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
       constexpr int k = decltype(kc)::value;
       unroll<copied(k - 1), copied(k)>([&](auto c) {
         constexpr int i = decltype(c)::value;
-        if constexpr (i < S::kLoads) copy(c, st + 2);
+        if constexpr (i < S::kLoads) copy(c, st + 2, row_bytes);
         else copy_scales(i - S::kLoads, (st + 2) >> 1);
       });
     };
@@ -493,73 +656,160 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
       mx_mfma_at<2 * odd + 1>(wf[1][f], wsc[f], xf[1][i], xsc[i], acc[i][f]);
       if constexpr (k == kPublish) {
         static_assert(copied(kPublish - 1) < 64, "vmcnt is a 6-bit counter");
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(copied(kPublish - 1)) : "memory");
+        // (a tile's first two stages are in LDS from the start, and a wait for what came behind
+        // them would be one for the last tile's results)
+        if (odd || st > 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(copied(kPublish - 1)) : "memory");
         __builtin_amdgcn_s_barrier();
       }
       constexpr int r0 = kPublish + 1, r1 = r0 + kWindow / 2;
       unroll<dealt(k - 1, r0, kWindow, kReads), dealt(k, r0, kWindow, kReads)>(
           [&](auto j) { read(j, C0{}, (st + 1) & 1); });
+      constexpr int len = kWindow * 5 / 4 < 2 * kMma - r1 ? kWindow * 5 / 4 : 2 * kMma - r1;
       if constexpr (odd)
-        unroll<dealt(k - 1, r1, kWindow, kReads), dealt(k, r1, kWindow, kReads)>(
+        unroll<dealt(k - 1, r1, len, kReads + kLag), dealt(k, r1, len, kReads + kLag)>(
             [&](auto j) { read_scale(j, (st + 1) >> 1); });
       issue(kc);
       __builtin_amdgcn_sched_barrier(0);
     });
     if constexpr (odd) next_scales();
   };
-  // (the last group's missing steps, if any, multiply zeros)
-  const int groups = (steps + 3) >> 2;
-  for (int q = 0; q < groups; ++q) {
-    one_stage(C0{}, 2 * q);
-    one_stage(C1{}, 2 * q + 1);
-  }
-  mx_mfma_done();
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS after the end
 
-  const MxOutput<T, QUANT> out(a, t.e, x0, x_rows);
+  char* const stage = lds + 2 * (S::kStageBytes + S::kScaleBytes) + wave * (16 * S::kOutRow);
+  // by LDS where it is words throughout
+  const bool wide = a.dtype == FMOE_F32;
+  const bool bias_by_lds = a.bias != nullptr &&
+                           (wide || (a.out_feat % 2 == 0 && (uintptr_t)a.bias % 4 == 0));
+  int pid = blockIdx.x;
+  int number = tile_number(pid, live);
+  if (number >= live) return;
+  MxPlace at = place(number);
+  __syncthreads();                                    // s_find has been read by everyone
+  aim(at);
+  start();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  for (;;) {
+    __builtin_amdgcn_s_barrier();
+    unroll<0, FW + TW>([&](auto j) { read(j, C0{}, 0); });
+    unroll<0, FW + TW + kLag>([&](auto j) { read_scale(j, 0); });
+    next_scales();
+    // the bias waits out the K loop where the results will pass
+    if (bias_by_lds) {
+      const int64_t row = (int64_t)a.out_feat * (wide ? 4 : 2);
+      const i32x4 rsrc = mx_descriptor((const char*)a.bias + at.e * row, row);
+      const uint32_t dst = lds0 + (uint32_t)(stage - lds);
+      const uint32_t off = (uint32_t)((at.base + wn * (TN / 2)) * (wide ? 4 : 2) + lane * 4);
+      dma4(dst, off, rsrc);
+      if (wide) dma4(dst + 256, off + 256, rsrc);
+    }
 #pragma unroll
-  for (int p = 0; p < FW / 2; ++p) {
-    const int n0 = base + wn * (TN / 2) + p * 32 + 8 * g;
-    float bias[8];
-    out.load_bias(n0, bias);
+    for (int i = 0; i < TW; ++i)
+#pragma unroll
+      for (int f = 0; f < FW; ++f) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // (the last group's missing steps, if any, multiply zeros)
+    const int groups = (steps + 3) >> 2;
+    int q = 0;
+    do {
+      one_stage(C0{}, 2 * q);
+      one_stage(C1{}, 2 * q + 1);
+    } while (++q < groups);
+    mx_mfma_done();
+    // what is still on its way to LDS is zeros from behind the end of K
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    float b[FW / 2][8];
+    if (bias_by_lds) {
+      const char* const at_g = stage + (mx_fresh(lane) >> 4) * (wide ? 32 : 16);
+#pragma unroll
+      for (int p = 0; p < FW / 2; ++p) {
+        if (wide) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b[p][i] = *(const float*)(at_g + p * 128 + i * 4);
+        } else {
+          const i32x4 u = *(const i32x4*)(at_g + p * 64);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t bits = ((uint32_t)u[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+            b[p][i] = a.dtype == FMOE_BF16 ? __uint_as_float(bits << 16)
+                                           : __half2float(__builtin_bit_cast(__half, (uint16_t)bits));
+          }
+        }
+      }
+    } else {
+      const auto rows = mx_bias_rows(a, at.e);
+#pragma unroll
+      for (int p = 0; p < FW / 2; ++p)
+        mx_load_bias(a, rows, at.base + wn * (TN / 2) + p * 32 + 8 * (mx_fresh(lane) >> 4), b[p]);
+#pragma unroll
+      for (int p = 0; p < FW / 2; ++p)      // (waits for them here, before the next tile's copies)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(b[p][i]));
+    }
+    __builtin_amdgcn_s_barrier();
+    pid += gridDim.x;
+    number = tile_number(pid, live);
+    const bool more = number < live;
+    MxPlace next = at;
+    if (more) {
+      next = place(number);
+      aim(next);
+      start();
+    }
+    const MxOutput<T, MODE> out(a, at.x0, at.rows);
+    const int fresh = mx_fresh(lane);
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
-      float r[8];
+      float r[FW / 2][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = acc[i][2 * p + (j >> 2)][j & 3] + bias[j];
-      out.store(wm * (TM / 2) + i * 16 + m, n0, r);
+      for (int p = 0; p < FW / 2; ++p)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[p][j] = mx_read(acc[i][2 * p + (j >> 2)][j & 3]) + b[p][j];
+      out.template store_rows<FW / 2, S::kOutRow>(stage, fresh, wm * (TM / 2) + i * 16,
+                                                  at.base + wn * (TN / 2), r);
     }
+    if (!more) break;
+    // the next tile's first stages are older than the results just sent
+    constexpr int kSent = MODE == kMxAny ? 0
+                              : MxOutput<T, MODE>::template stores<FW / 2, S::kOutRow>(TW);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kSent) : "memory");
+    at = next;
   }
 }
 
-template <typename T, bool QUANT>
+constexpr int kCus = 256;
+
+template <typename T, int MODE>
 static int launch(const MxGemmArgs& a, hipStream_t s) {
-  const int n_pad = QUANT ? (int)mx_code_bytes(a.out_feat) * 2 : a.out_feat;
+  const int n_pad = mx_quantises(MODE) ? (int)mx_code_bytes(a.out_feat) * 2 : a.out_feat;
   const double mean = (double)a.n_rows / a.n_expert;
-#define FMOE_CALL(NT, KS)                                                                        \
+#define FMOE_STREAM(NT, KS)                                                                      \
   do {                                                                                           \
     const int64_t rows = a.n_rows / (16 * NT) + std::min<int64_t>(a.n_expert, a.n_rows);         \
     const int64_t blocks = rows * ceil_div(n_pad, 32 * (4 / KS));                                \
     FMOE_REQUIRE(blocks <= INT32_MAX, FMOE_ERR_UNSUPPORTED, "mx_linear: too many tiles");        \
-    hipLaunchKernelGGL((mx_stream_kernel<T, NT, KS, QUANT>), dim3((unsigned)blocks), dim3(256), 0, \
+    hipLaunchKernelGGL((mx_stream_kernel<T, NT, KS, MODE>), dim3((unsigned)blocks), dim3(256), 0, \
                        s, a);                                                                    \
   } while (0)
 #define FMOE_TILE(TN, TM)                                                                        \
   do {                                                                                           \
     const int64_t rows = a.n_rows / TM + std::min<int64_t>(a.n_expert, a.n_rows);                \
-    const int64_t blocks = (rows * ceil_div(n_pad, TN) + 255) / 256 * 256;                       \
-    FMOE_REQUIRE(blocks <= INT32_MAX, FMOE_ERR_UNSUPPORTED, "mx_linear: too many tiles");        \
-    FMOE_SET_DYNAMIC_LDS_ONCE((mx_tile_kernel<T, TN, TM, QUANT>), (MxTile<TN, TM>::kLdsBytes));  \
-    hipLaunchKernelGGL((mx_tile_kernel<T, TN, TM, QUANT>), dim3((unsigned)blocks), dim3(256),    \
-                       (MxTile<TN, TM>::kLdsBytes), s, a);                                       \
+    FMOE_REQUIRE(rows * ceil_div(n_pad, TN) <= INT32_MAX, FMOE_ERR_UNSUPPORTED,                  \
+                 "mx_linear: too many tiles");                                                   \
+    FMOE_SET_DYNAMIC_LDS_ONCE((mx_tile_kernel<T, TN, TM, MODE>), (MxTile<TN, TM>::kLdsBytes));   \
+    hipLaunchKernelGGL((mx_tile_kernel<T, TN, TM, MODE>), dim3(kCus * MxTile<TN, TM>::kGroups),  \
+                       dim3(256), (MxTile<TN, TM>::kLdsBytes), s, a);                            \
   } while (0)
   if (mean >= 128) FMOE_TILE(256, 256);
-  else if (mean <= 16) FMOE_CALL(1, 4);
-  else FMOE_CALL(4, 1);
-#undef FMOE_CALL
+  else if (mean <= 16) FMOE_STREAM(1, 4);
+  else FMOE_STREAM(4, 1);
+#undef FMOE_STREAM
 #undef FMOE_TILE
   FMOE_LAUNCH_CHECK("mx_linear");
   return FMOE_OK;
+}
+
+template <typename T> static int launch_y(const MxGemmArgs& a, hipStream_t s) {
+  constexpr int kN = Pack16<T>::kN;
+  return a.out_feat % kN == 0 && (uintptr_t)a.y % 16 == 0 ? launch<T, kMxPacked>(a, s)
+                                                          : launch<T, kMxAny>(a, s);
 }
 
 }  // namespace fmoe
@@ -578,6 +828,8 @@ extern "C" int fmoe_mx_linear_fwd(const void* x_codes, const void* x_scales, con
                "mx_linear: unsupported dtype %d", dtype);
   FMOE_REQUIRE(act == FMOE_ACT_NONE || act == FMOE_ACT_GELU || act == FMOE_ACT_RELU,
                FMOE_ERR_INVALID, "mx_linear: unknown activation %d", act);
+  FMOE_REQUIRE(act == FMOE_ACT_NONE || y == nullptr, FMOE_ERR_INVALID,
+               "mx_linear: an activation only in front of y_codes");
   if (n_rows == 0) return FMOE_OK;
   FMOE_REQUIRE(x_codes && x_scales && w_codes && w_scales && seg_off, FMOE_ERR_INVALID,
                "mx_linear: null pointer");
@@ -590,10 +842,13 @@ extern "C" int fmoe_mx_linear_fwd(const void* x_codes, const void* x_scales, con
                      (const uint8_t*)w_scales, bias, seg_off, y, (uint8_t*)y_codes,
                      (uint8_t*)y_scales, n_rows, (int)in_feat, (int)out_feat, (int)n_expert, act, dtype};
   hipStream_t s = (hipStream_t)stream;
-  const bool q = y_codes != nullptr;
+  if (y_codes)      // (the element type then is that of the bias alone, which is read as it comes)
+    return act == FMOE_ACT_GELU   ? launch<float, kMxQuantGelu>(a, s)
+           : act == FMOE_ACT_RELU ? launch<float, kMxQuantRelu>(a, s)
+                                  : launch<float, kMxQuant>(a, s);
   switch (dtype) {
-    case FMOE_F32: return q ? launch<float, true>(a, s) : launch<float, false>(a, s);
-    case FMOE_F16: return q ? launch<__half, true>(a, s) : launch<__half, false>(a, s);
-    default: return q ? launch<__hip_bfloat16, true>(a, s) : launch<__hip_bfloat16, false>(a, s);
+    case FMOE_F32: return launch_y<float>(a, s);
+    case FMOE_F16: return launch_y<__half>(a, s);
+    default: return launch_y<__hip_bfloat16>(a, s);
   }
 }

@@ -535,8 +535,8 @@ int fmoe_mx_dequantize(const void* codes, const void* scales, int64_t n_rows, in
  *   y[seg_e] = act(x[seg_e] * w_e^T + b_e),  f32 products and sums on the matrix cores
  * x: n_rows rows of in_feat features; w: n_expert * out_feat rows of in_feat features; bias
  * [n_expert, out_feat] of `dtype` or NULL.  The result is either y [n_rows, out_feat] of `dtype`
- * (f32, f16 or bf16), or, with y_codes and y_scales, MXFP4 rows of out_feat features: the
- * f32 values quantised as fmoe_mx_quantize does (y is NULL then).  Rows at or behind
+ * (f32, f16 or bf16; act is FMOE_ACT_NONE), or, with y_codes and y_scales, MXFP4 rows of out_feat
+ * features: the f32 values quantised as fmoe_mx_quantize does (y is NULL then).  Rows at or behind
  * seg_off[n_expert] are not written.
  */
 int fmoe_mx_linear_fwd(const void* x_codes, const void* x_scales, const void* w_codes,
