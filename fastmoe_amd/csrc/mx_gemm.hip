@@ -384,9 +384,12 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
 // step a wait and a barrier publish the next stage, whose first fragments are read in the shadow
 // of the remaining instructions.
 //
-// One workgroup fills a CU (all its registers, nearly all its LDS) and runs tile after tile: the
-// next tile's first two stages are on their way while this one's results leave through a corner
-// of LDS, which turns the lanes' 16 bytes of 16 rows into pieces of 256 bytes of a row.
+// One workgroup fills a CU (all its registers, all its LDS) and runs tile after tile in one
+// pipeline: the last group of a tile copies the next tile's first two stages and scales and ends
+// with its first fragments in registers, so that between two tiles there is nothing but the
+// output.  The results leave through a corner of LDS that turns the lanes' 16 bytes of 16 rows
+// into pieces of 256 bytes of a row (stored from the registers, 64 bytes of each of 16 rows at a
+// time, they took 16 us a tile instead of 9).
 typedef __attribute__((address_space(3))) char lds_char;
 
 template <int I, int N, typename F> __device__ __forceinline__ void unroll(F&& f) {
@@ -453,7 +456,8 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   constexpr int FW = TN / 32, TW = TM / 32;         // fragments of a wave
   constexpr int kMma = FW * TW;
   extern __shared__ __align__(16) char lds[];
-  int* const s_find = (int*)(lds + 2 * S::kStageBytes + S::kScaleBytes);   // (idle between tiles)
+  // (the first wave's corner, behind the bias)
+  int* const s_find = (int*)(lds + 2 * (S::kStageBytes + S::kScaleBytes) + 1024);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   RowTiles<TM, kOneHeight, 4> tiles;
   tiles.scan(a.seg_off, a.n_expert, s_find);
@@ -472,7 +476,7 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   auto place = [&](int number) {
     int v, col;
     tile_order(number, tiles.rows_f, n_cols, v, col);
-    const TileRows t = tiles.find(a.seg_off, v, false, s_find);
+    const TileRows t = tiles.find(a.seg_off, v, false, s_find + 16);
     MxPlace at;
     at.e = t.e;
     at.base = col * TN;                             // (below out_feat: columns end on 128)
@@ -516,11 +520,10 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
                  :: "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(offset), "s"(rsrc)
                  : "memory", "m0");
   };
-  // Copy i of stage `st` into the buffer of its parity: every wave has its share of either
-  // operand, so that nothing here depends on the wave but numbers.
-  auto copy = [&](auto ic, int st, int row_bytes) {
+  // Copy i of stage `st`, whose buffer is `par`: every wave has its share of either operand, so that nothing here depends on the wave but numbers.
+  auto copy = [&](auto ic, auto par, int st, int row_bytes) {
     constexpr int i = decltype(ic)::value;
-    const uint32_t buf = lds0 + (st & 1) * S::kStageBytes;
+    const uint32_t buf = lds0 + decltype(par)::value * S::kStageBytes;
     if constexpr (i < S::kLoadsW) {
       const int kib = wave * S::kLoadsW + i;
       const int row = wave * (TN / 4) + 32 * (i >> 2) + 16 * (i & 1) + 4 * ((i >> 1) & 1);
@@ -531,8 +534,8 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
           x_lane[(i - S::kLoadsW) & 1] + (uint32_t)(kib * 8 * row_bytes + st * 128), x_rsrc);
     }
   };
-  auto copy_scales = [&](int i, int group) {
-    dma(lds0 + 2 * S::kStageBytes + (group & 1) * S::kScaleBytes + (wave * S::kScaleLoads + i) * 1024,
+  auto copy_scales = [&](int i, int group, int buf) {
+    dma(lds0 + 2 * S::kStageBytes + buf * S::kScaleBytes + (wave * S::kScaleLoads + i) * 1024,
         s_lane[i] + (uint32_t)(group * 16), s_rsrc[i]);
   };
   // Before the copies of stage `st`: past the end of K nothing is read any more, and of a last
@@ -548,15 +551,6 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
 #pragma unroll
     for (int i = 0; i < S::kScaleLoads; ++i) s_lane[i] = past ? kDmaOutOfRange : s_lane[i];
   };
-  auto start = [&] {                                // the copies that a tile begins with
-    bound(0);
-#pragma unroll
-    for (int i = 0; i < S::kScaleLoads; ++i) copy_scales(i, 0);
-    unroll<0, S::kLoads>([&](auto i) { copy(i, 0, code_row); });
-    bound(1);
-    unroll<0, S::kLoads>([&](auto i) { copy(i, 1, code_row); });
-  };
-
   const int m = lane & 15, g = lane >> 4, wn = wave >> 1, wm = wave & 1;
   const int frag0 = m * 128 + (g ^ ((m >> 1) & 7)) * 16;      // step 0; step 1 has packs 4..7
   const char* const w_lds = lds + wn * (TN / 2) * 128;
@@ -565,9 +559,9 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   int wsc[FW], xsc[TW];            // per fragment, this lane's bytes of the group's 4 steps
   int wsn[FW], xsn[TW];            // the next group's
   // fragment j (features first) of step S of the stage in buffer `buf`
-  auto read = [&](auto jc, auto step, int buf) {
+  auto read = [&](auto jc, auto step, auto buf) {
     constexpr int j = decltype(jc)::value, s = decltype(step)::value;
-    const int at = buf * S::kStageBytes + (s ? frag0 ^ 64 : frag0);
+    const int at = decltype(buf)::value * S::kStageBytes + (s ? frag0 ^ 64 : frag0);
     if constexpr (j < FW) wf[s][j] = *(const i32x4*)(w_lds + at + j * 2048);
     else xf[s][j - FW] = *(const i32x4*)(x_lds + at + (j - FW) * 2048);
   };
@@ -578,7 +572,7 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   // reads fragment j's and finishes fragment j - kLag's.
   constexpr int kLag = 4;
   i32x4 sraw[kLag];
-  auto read_scale = [&](auto jc, int group) {
+  auto read_scale = [&](auto jc, int group, int buf) {
     constexpr int j = decltype(jc)::value;
     if constexpr (j >= kLag) {
       constexpr int d = j - kLag;
@@ -593,15 +587,18 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
     }
     if constexpr (j < FW + TW) {
       const int row = j < FW ? wn * (TN / 2) + j * 16 : TN + wm * (TM / 2) + (j - FW) * 16;
-      sraw[j % kLag] = *(const i32x4*)(lds + 2 * S::kStageBytes + (group & 1) * S::kScaleBytes +
+      sraw[j % kLag] = *(const i32x4*)(lds + 2 * S::kStageBytes + buf * S::kScaleBytes +
                                        (row + m) * 16);
     }
   };
+  // (In assembly so that they stay here: a matrix instruction reads what an ordinary one wrote two
+  // wait states later at the earliest, and the compiler does not know that ours are such.)
   auto next_scales = [&] {
 #pragma unroll
-    for (int j = 0; j < FW; ++j) wsc[j] = wsn[j];
+    for (int j = 0; j < FW; ++j) asm volatile("v_mov_b32 %0, %1" : "=v"(wsc[j]) : "v"(wsn[j]));
 #pragma unroll
-    for (int j = 0; j < TW; ++j) xsc[j] = xsn[j];
+    for (int j = 0; j < TW; ++j) asm volatile("v_mov_b32 %0, %1" : "=v"(xsc[j]) : "v"(xsn[j]));
+    asm volatile("s_nop 1");
   };
   f32x4 acc[TW][FW];
   using C0 = std::integral_constant<int, 0>;
@@ -615,8 +612,15 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   constexpr int kRelease = kWindow + kMma / 8;
   constexpr int kPublish = kMma + kMma / 4;
   static_assert(kRelease < kMma && kPublish + kWindow < 2 * kMma, "room for the reads");
-  auto one_stage = [&](auto odd_c, int st) {
+  // The stage in buffer `odd`; meanwhile the copies of stage `st` (of this tile or the next) into
+  // the same buffer and, in an even stage, of its group's scales into `sbuf`.  `first`: of a tile
+  // behind another one.
+  constexpr int kSent = MODE == kMxAny ? 0
+                            : MxOutput<T, MODE>::template stores<FW / 2, S::kOutRow>(TW);
+  auto one_stage = [&](auto odd_c, int st, int sbuf, bool first) {
     constexpr int odd = decltype(odd_c)::value;
+    using Odd = std::integral_constant<int, odd>;
+    using Other = std::integral_constant<int, 1 - odd>;
     constexpr int kCopies = S::kLoads + (odd ? 0 : S::kScaleLoads);
     // (the multiples of the row size in the copies' offsets are made where they are used: kept,
     // they would take more scalar registers than there are)
@@ -634,16 +638,16 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
       constexpr int k = decltype(kc)::value;
       unroll<copied(k - 1), copied(k)>([&](auto c) {
         constexpr int i = decltype(c)::value;
-        if constexpr (i < S::kLoads) copy(c, st + 2, row_bytes);
-        else copy_scales(i - S::kLoads, (st + 2) >> 1);
+        if constexpr (i < S::kLoads) copy(c, Odd{}, st, row_bytes);
+        else copy_scales(i - S::kLoads, st >> 1, sbuf);
       });
     };
-    bound(st + 2);
+    bound(st);
     unroll<0, kMma>([&](auto kc) {
       constexpr int k = decltype(kc)::value, i = k / FW, f = k % FW;
       mx_mfma_at<2 * odd>(wf[0][f], wsc[f], xf[0][i], xsc[i], acc[i][f]);
       unroll<dealt(k - 1, 0, kWindow, kReads), dealt(k, 0, kWindow, kReads)>(
-          [&](auto j) { read(j, C1{}, st & 1); });
+          [&](auto j) { read(j, C1{}, Odd{}); });
       if constexpr (k == kRelease) {
         __builtin_amdgcn_s_waitcnt(0xc07f);           // lgkmcnt(0): my reads of this stage are done
         __builtin_amdgcn_s_barrier();
@@ -655,19 +659,21 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
       constexpr int k = decltype(kc)::value, i = (k - kMma) / FW, f = (k - kMma) % FW;
       mx_mfma_at<2 * odd + 1>(wf[1][f], wsc[f], xf[1][i], xsc[i], acc[i][f]);
       if constexpr (k == kPublish) {
-        static_assert(copied(kPublish - 1) < 64, "vmcnt is a 6-bit counter");
-        // (a tile's first two stages are in LDS from the start, and a wait for what came behind
-        // them would be one for the last tile's results)
-        if (odd || st > 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(copied(kPublish - 1)) : "memory");
+        // everything but this stage's own copies has landed; the last tile's results, which lie
+        // between a tile's second stage and its third, may still be on their way
+        constexpr int own = copied(kPublish - 1), sent = own + kSent < 63 ? own + kSent : 63;
+        static_assert(own < 64, "vmcnt is a 6-bit counter");
+        if (!odd && first) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(sent) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(own) : "memory");
         __builtin_amdgcn_s_barrier();
       }
       constexpr int r0 = kPublish + 1, r1 = r0 + kWindow / 2;
       unroll<dealt(k - 1, r0, kWindow, kReads), dealt(k, r0, kWindow, kReads)>(
-          [&](auto j) { read(j, C0{}, (st + 1) & 1); });
+          [&](auto j) { read(j, C0{}, Other{}); });
       constexpr int len = kWindow * 5 / 4 < 2 * kMma - r1 ? kWindow * 5 / 4 : 2 * kMma - r1;
       if constexpr (odd)
         unroll<dealt(k - 1, r1, len, kReads + kLag), dealt(k, r1, len, kReads + kLag)>(
-            [&](auto j) { read_scale(j, (st + 1) >> 1); });
+            [&](auto j) { read_scale(j, st >> 1, sbuf); });
       issue(kc);
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -679,19 +685,27 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   const bool wide = a.dtype == FMOE_F32;
   const bool bias_by_lds = a.bias != nullptr &&
                            (wide || (a.out_feat % 2 == 0 && (uintptr_t)a.bias % 4 == 0));
+  // (the last group's missing steps, if any, multiply zeros)
+  const int groups = (steps + 3) >> 2;
   int pid = blockIdx.x;
   int number = tile_number(pid, live);
   if (number >= live) return;
-  MxPlace at = place(number);
-  __syncthreads();                                    // s_find has been read by everyone
+  MxPlace at = place(number), next = at;
+  bool first = false;
+  int sbuf = 0;                                       // buffer of the current group's scales
   aim(at);
-  start();
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  bound(0);
+#pragma unroll
+  for (int i = 0; i < S::kScaleLoads; ++i) copy_scales(i, 0, 0);
+  unroll<0, S::kLoads>([&](auto i) { copy(i, C0{}, 0, code_row); });
+  bound(1);
+  unroll<0, S::kLoads>([&](auto i) { copy(i, C1{}, 1, code_row); });
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
+  __builtin_amdgcn_s_barrier();
+  unroll<0, FW + TW>([&](auto j) { read(j, C0{}, C0{}); });
+  unroll<0, FW + TW + kLag>([&](auto j) { read_scale(j, 0, 0); });
+  next_scales();
   for (;;) {
-    __builtin_amdgcn_s_barrier();
-    unroll<0, FW + TW>([&](auto j) { read(j, C0{}, 0); });
-    unroll<0, FW + TW + kLag>([&](auto j) { read_scale(j, 0); });
-    next_scales();
     // the bias waits out the K loop where the results will pass
     if (bias_by_lds) {
       const int64_t row = (int64_t)a.out_feat * (wide ? 4 : 2);
@@ -705,19 +719,32 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
     for (int i = 0; i < TW; ++i)
 #pragma unroll
       for (int f = 0; f < FW; ++f) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // (the last group's missing steps, if any, multiply zeros)
-    const int groups = (steps + 3) >> 2;
+    bool more = true;
     int q = 0;
     do {
-      one_stage(C0{}, 2 * q);
-      one_stage(C1{}, 2 * q + 1);
+      int st = 2 * q + 2;                             // the stages copied meanwhile
+      if (q + 1 == groups) {
+        st = 0;
+        pid += gridDim.x;
+        number = tile_number(pid, live);
+        more = number < live;
+        if (more) {
+          next = place(number);
+          aim(next);
+        } else {
+          bound(stages);                              // nothing any more
+        }
+      }
+      one_stage(C0{}, st, sbuf ^ 1, first);
+      one_stage(C1{}, st + 1, sbuf ^ 1, false);
+      sbuf ^= 1;
+      first = false;
     } while (++q < groups);
     mx_mfma_done();
-    // what is still on its way to LDS is zeros from behind the end of K
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     float b[FW / 2][8];
+    const int fresh = mx_fresh(lane);
     if (bias_by_lds) {
-      const char* const at_g = stage + (mx_fresh(lane) >> 4) * (wide ? 32 : 16);
+      const char* const at_g = stage + (fresh >> 4) * (wide ? 32 : 16);
 #pragma unroll
       for (int p = 0; p < FW / 2; ++p) {
         if (wide) {
@@ -737,24 +764,9 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
       const auto rows = mx_bias_rows(a, at.e);
 #pragma unroll
       for (int p = 0; p < FW / 2; ++p)
-        mx_load_bias(a, rows, at.base + wn * (TN / 2) + p * 32 + 8 * (mx_fresh(lane) >> 4), b[p]);
-#pragma unroll
-      for (int p = 0; p < FW / 2; ++p)      // (waits for them here, before the next tile's copies)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(b[p][i]));
-    }
-    __builtin_amdgcn_s_barrier();
-    pid += gridDim.x;
-    number = tile_number(pid, live);
-    const bool more = number < live;
-    MxPlace next = at;
-    if (more) {
-      next = place(number);
-      aim(next);
-      start();
+        mx_load_bias(a, rows, at.base + wn * (TN / 2) + p * 32 + 8 * (fresh >> 4), b[p]);
     }
     const MxOutput<T, MODE> out(a, at.x0, at.rows);
-    const int fresh = mx_fresh(lane);
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
       float r[FW / 2][8];
@@ -766,12 +778,12 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
                                                   at.base + wn * (TN / 2), r);
     }
     if (!more) break;
-    // the next tile's first stages are older than the results just sent
-    constexpr int kSent = MODE == kMxAny ? 0
-                              : MxOutput<T, MODE>::template stores<FW / 2, S::kOutRow>(TW);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kSent) : "memory");
     at = next;
+    first = true;
+    // (the corner is read out before the next bias lands there)
+    __builtin_amdgcn_s_waitcnt(0xc07f);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS after the end
 }
 
 constexpr int kCus = 256;

@@ -193,6 +193,28 @@ def test_product_against_64_bits(dt, counts):
         assert torch.equal(y, again)
 
 
+@pytest.mark.parametrize("dt,n", [("bf16", 6016), ("f32", 6016), ("f16", 6011)])
+def test_many_tiles(dt, n):
+    """More tiles than there are compute units, so that a workgroup runs several."""
+    from fastmoe_amd import mx
+
+    counts, k = [3001, 0, 700, 2500], 200
+    x, w, b = _problem(counts, k, n, dt, 12)
+    wq, xd, bd = mx.quantize(w.view(4, n, k).cuda()), x.cuda(), b.cuda()
+    y = mx.linear(xd, torch.tensor(counts), wq, bd)
+    again = mx.linear(xd, torch.tensor(counts), wq, bd)
+    assert torch.equal(y, again)
+    xv, wv = mx.quantize(xd).dequantize(torch.float32).double(), wq.dequantize(torch.float32).double()
+    at = 0
+    for e, c in enumerate(counts):
+        rows = xv[at:at + c]
+        want = rows @ wv[e].T + bd[e].double()
+        mag = rows.abs() @ wv[e].abs().T + bd[e].double().abs()
+        tol = UNIT[dt] * want.abs() + 2.0 ** -23 * (k / 128 + 4) * mag
+        assert ((y[at:at + c].double() - want).abs() <= tol).all(), e
+        at += c
+
+
 @pytest.mark.parametrize("act", [0, 1, 2])
 @pytest.mark.parametrize("counts", [[5, 0, 1], [70, 33], [300, 129, 0]], ids=lambda c: str(sum(c)))
 def test_product_with_activation_comes_out_quantised(act, counts):
@@ -218,6 +240,27 @@ def test_product_with_activation_comes_out_quantised(act, counts):
         assert not codes.cpu().numpy()[:, -(-n // 2):].any()
         pad = scales.cpu().numpy()[:, :-(-n // 128) * 4]
         assert (pad != 255).all()
+
+
+def test_many_tiles_come_out_quantised():
+    from fastmoe_amd import fmoe_cuda, mx
+
+    counts, k, n = [3001, 0, 700, 2500], 200, 6020
+    x, w, b = _problem(counts, k, n, "bf16", 13)
+    wq, xq, bd = mx.quantize(w.view(4, n, k).cuda()), mx.quantize(x.cuda()), b.cuda()
+    seg = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32).cuda()
+    y = fmoe_cuda.mx_linear_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k, bd.float(), seg,
+                                torch.empty(sum(counts), n).cuda())
+    for act in (0, 1, 2):
+        codes, scales = fmoe_cuda.mx_linear_act_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k,
+                                                    bd, seg, act)
+        got = mx.MXTensor(codes, scales, n).dequantize(torch.float32)
+        h = [y, torch.nn.functional.gelu(y.double()).float(), y.relu()][act]
+        want = mx.quantize(h).dequantize(torch.float32)
+        if act != 1:
+            assert torch.equal(got, want)
+        else:                    # the two GELUs differ by up to 1e-6
+            assert (got != want).float().mean() < 1e-4
 
 
 def test_rows_without_an_expert_stay_as_they_are():
