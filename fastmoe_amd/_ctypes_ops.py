@@ -730,6 +730,27 @@ def mx_quantize(x: torch.Tensor, n_rows_dev: Optional[torch.Tensor] = None
     return codes, scales
 
 
+def mx_quantize_counted(x: torch.Tensor, expert_count: torch.Tensor
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """mx_quantize of expert-ordered rows and, in the same launch, the seg_off (device
+    int32[E+1]) of their device int64 counts."""
+    _dev(x, "x")
+    _dev(expert_count, "expert_count", torch.int64)
+    _need(x.dim() == 2 and x.shape[1] >= 1, "x must be [rows, features]")
+    _need(expert_count.numel() >= 1 and expert_count.device == x.device,
+          "expert_count must lie on x's device")
+    codes, scales = _mx_empty(x.shape[0], x.shape[1], x.device)
+    seg = torch.empty(expert_count.numel() + 1, dtype=torch.int32, device=x.device)
+    with _launch(x, "mx_quantize_counted"):
+        _lib.check(
+            _L.fmoe_mx_quantize_counted(x.data_ptr(), x.shape[0], x.shape[1],
+                                        expert_count.data_ptr(), expert_count.numel(),
+                                        seg.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                                        _dt(x, "x"), _stream(x)),
+            "mx_quantize_counted")
+    return codes, scales, seg
+
+
 def mx_quantize_tokens(x: torch.Tensor, inv: torch.Tensor, top_k: int
                        ) -> Tuple[torch.Tensor, torch.Tensor]:
     """mx_quantize of token rows, written to their places in expert order: rows

@@ -99,6 +99,8 @@ SIGNATURES = {
     "fmoe_mx_scale_bytes": (c_int64, [c_int64]),
     "fmoe_mx_quantize": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int,
                                  c_void_p]),
+    "fmoe_mx_quantize_counted": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                         c_void_p, c_void_p, c_int, c_void_p]),
     "fmoe_mx_quantize_tokens": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
                                         c_void_p, c_int, c_void_p]),
     "fmoe_mx_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),

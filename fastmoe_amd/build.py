@@ -119,7 +119,7 @@ def ext_source_hash() -> str:
     import hashlib
 
     h = hashlib.sha256()
-    for path in (EXT_SRC, os.path.join(CSRC, "moe_layer.h"),
+    for path in (EXT_SRC, os.path.join(CSRC, "moe_layer.h"), os.path.join(CSRC, "mx_layer.h"),
                  os.path.join(PKG_DIR, "..", "include", "fmoe_hip.h")):
         with open(path, "rb") as f:
             h.update(f.read() + b"\0")

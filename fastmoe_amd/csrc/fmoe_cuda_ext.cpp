@@ -593,6 +593,24 @@ std::tuple<Tensor, Tensor> mx_quantize(Tensor x, OptTensor n_rows_dev) {
   return q;
 }
 
+// mx_quantize and, in the same launch, the segment table of the rows' device counts
+std::tuple<Tensor, Tensor, Tensor> mx_quantize_counted(Tensor x, Tensor expert_count) {
+  dev(x, "x");
+  dev(expert_count, "expert_count", at::kLong);
+  need(x.dim() == 2 && x.size(1) >= 1, "x must be [rows, features]");
+  need(expert_count.numel() >= 1 && expert_count.device() == x.device(),
+       "expert_count must lie on x's device");
+  c10::DeviceGuard guard(x.device());
+  auto q = mx_empty(x.size(0), x.size(1), x);
+  Tensor seg = torch::empty({expert_count.numel() + 1}, x.options().dtype(at::kInt));
+  check(fmoe_mx_quantize_counted(x.data_ptr(), x.size(0), x.size(1),
+                                 expert_count.data_ptr<int64_t>(), expert_count.numel(),
+                                 seg.data_ptr<int32_t>(), std::get<0>(q).data_ptr(),
+                                 std::get<1>(q).data_ptr(), dt(x, "x"), stream_of(x)),
+        "mx_quantize_counted");
+  return {std::get<0>(q), std::get<1>(q), seg};
+}
+
 std::tuple<Tensor, Tensor> mx_quantize_tokens(Tensor x, Tensor inv, int64_t top_k) {
   dev(x, "x");
   dev(inv, "inv", at::kInt);
@@ -724,6 +742,7 @@ Tensor gelu_bwd(Tensor dy, Tensor x, OptTensor n_rows_dev) {
 }  // namespace
 
 #include "moe_layer.h"   // the whole layer as one native autograd node
+#include "mx_layer.h"    // scored routing and 4-bit experts
 
 namespace {
 
@@ -778,6 +797,10 @@ PYBIND11_MODULE(fmoe_cuda, m) {
         py::arg("score") = (int)FMOE_SCORE_SIGMOID, py::arg("renormalize") = true,
         py::arg("scale") = 1.0);
   m.def("mx_quantize", &mx_quantize, py::arg("x"), py::arg("n_rows_dev") = py::none());
+  m.def("mx_quantize_counted", &mx_quantize_counted, py::arg("x"), py::arg("expert_count"));
+  m.def("score_topk", &score_topk);
+  m.def("mx_linear", &mx_linear);
+  m.def("mx_expert_layer", &mx_expert_layer);
   m.def("mx_quantize_tokens", &mx_quantize_tokens, py::arg("x"), py::arg("inv"), py::arg("top_k"));
   m.def("mx_dequantize", &mx_dequantize, py::arg("codes"), py::arg("scales"), py::arg("out"));
   m.def("mx_linear_fwd", &mx_linear_fwd, py::arg("x_codes"), py::arg("x_scales"),

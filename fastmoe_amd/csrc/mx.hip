@@ -66,6 +66,30 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   return v;
 }
 
+// Row counts of experts as segment bounds, for the call's first workgroup to leave behind.
+struct MxSegments {
+  const int64_t* count = nullptr;
+  int n_expert = 0;
+  int32_t* seg_off = nullptr;
+};
+
+// seg_off = exclusive prefix of the counts, by one wave.  Counts on the device nobody has looked
+// at: negative ones count as zero, and what lies beyond the rows there are is cut off.
+__device__ __forceinline__ void write_segments(const MxSegments& sg, int64_t n_rows, int lane) {
+  int64_t carry = 0;
+  for (int e0 = 0; e0 < sg.n_expert; e0 += kWave) {
+    const int64_t c = e0 + lane < sg.n_expert ? min(max(sg.count[e0 + lane], (int64_t)0), n_rows) : 0;
+    int64_t sum = c;
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int64_t o = __shfl_up(sum, d, kWave);
+      if (lane >= d) sum += o;
+    }
+    if (e0 + lane < sg.n_expert) sg.seg_off[e0 + lane] = (int32_t)min(carry + sum - c, n_rows);
+    carry += __shfl(sum, kWave - 1, kWave);
+  }
+  if (lane == 0) sg.seg_off[sg.n_expert] = (int32_t)min(carry, n_rows);
+}
+
 // One wave takes `U` chunks of a row at a time.  inv == nullptr: row r goes to row r, and rows
 // from *n_rows_dev on (if given) are skipped; else row t goes to the rows inv[t * top_k + j]
 // that are not -1.
@@ -73,8 +97,9 @@ template <typename T, bool VEC, int U>
 __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(
     const T* __restrict__ x, int64_t n_rows, int k, const int32_t* __restrict__ n_rows_dev,
     const int32_t* __restrict__ inv, int top_k, uint8_t* __restrict__ codes,
-    uint8_t* __restrict__ scales) {
+    uint8_t* __restrict__ scales, MxSegments segments) {
   const int lane = threadIdx.x & (kWave - 1);
+  if (segments.seg_off && blockIdx.x == 0 && threadIdx.x < kWave) write_segments(segments, n_rows, lane);
   const int chunks = (k + kMxChunk - 1) / kMxChunk, runs = (chunks + U - 1) / U;
   const int64_t code_row = mx_code_bytes(k), scale_row = mx_scale_bytes(k);
   int64_t rows = n_rows;
@@ -152,15 +177,15 @@ constexpr int kMxManyItems = 256 * 32;
 template <typename T>
 static int launch_quantize(const void* x, int64_t n_rows, int k, const int32_t* n_rows_dev,
                            const int32_t* inv, int top_k, uint8_t* codes, uint8_t* scales,
-                           hipStream_t s) {
+                           const MxSegments& segments, hipStream_t s) {
   const bool vec = k % Pack16<T>::kN == 0 && (uintptr_t)x % 16 == 0;
   const int64_t chunks = ceil_div(k, kMxChunk);
   const bool many = chunks >= 4 && n_rows * (chunks / 4) >= kMxManyItems;
   const int64_t items = n_rows * (many ? (chunks + 3) / 4 : chunks);
-  const dim3 grid((unsigned)std::min<int64_t>((items + kMxWaves - 1) / kMxWaves, 256 * 64));
+  const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>((items + kMxWaves - 1) / kMxWaves, 1), 256 * 64));
 #define FMOE_CALL(VEC, U)                                                                        \
   hipLaunchKernelGGL((mx_quantize_kernel<T, VEC, U>), grid, dim3(kMxThreads), 0, s, (const T*)x, \
-                     n_rows, k, n_rows_dev, inv, top_k, codes, scales)
+                     n_rows, k, n_rows_dev, inv, top_k, codes, scales, segments)
   if (vec && many) FMOE_CALL(true, 4);
   else if (vec) FMOE_CALL(true, 1);
   else FMOE_CALL(false, 1);
@@ -190,23 +215,23 @@ static int launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64_
 
 static int quantize(const void* x, int64_t n_rows, int64_t k, const int32_t* n_rows_dev,
                     const int32_t* inv, int64_t top_k, void* codes, void* scales, int dtype,
-                    hipStream_t s) {
+                    hipStream_t s, const MxSegments& segments = {}) {
   FMOE_REQUIRE(n_rows >= 0 && k >= 1 && k <= FMOE_MX_MAX_FEATURES, FMOE_ERR_INVALID,
                "mx_quantize: bad sizes");
   FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_F16 || dtype == FMOE_BF16, FMOE_ERR_UNSUPPORTED,
                "mx_quantize: unsupported dtype %d", dtype);
-  if (n_rows == 0) return FMOE_OK;
-  FMOE_REQUIRE(x && codes && scales, FMOE_ERR_INVALID, "mx_quantize: null pointer");
+  if (n_rows == 0 && !segments.seg_off) return FMOE_OK;
+  FMOE_REQUIRE((x && codes && scales) || n_rows == 0, FMOE_ERR_INVALID, "mx_quantize: null pointer");
   FMOE_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, FMOE_ERR_INVALID,
                "mx_quantize: codes and scales must be 16-byte aligned");
   uint8_t *c = (uint8_t*)codes, *sc = (uint8_t*)scales;
   switch (dtype) {
     case FMOE_F32:
-      return launch_quantize<float>(x, n_rows, (int)k, n_rows_dev, inv, (int)top_k, c, sc, s);
+      return launch_quantize<float>(x, n_rows, (int)k, n_rows_dev, inv, (int)top_k, c, sc, segments, s);
     case FMOE_F16:
-      return launch_quantize<__half>(x, n_rows, (int)k, n_rows_dev, inv, (int)top_k, c, sc, s);
+      return launch_quantize<__half>(x, n_rows, (int)k, n_rows_dev, inv, (int)top_k, c, sc, segments, s);
     default:
-      return launch_quantize<__hip_bfloat16>(x, n_rows, (int)k, n_rows_dev, inv, (int)top_k, c, sc, s);
+      return launch_quantize<__hip_bfloat16>(x, n_rows, (int)k, n_rows_dev, inv, (int)top_k, c, sc, segments, s);
   }
 }
 
@@ -229,6 +254,16 @@ extern "C" int fmoe_mx_quantize(const void* x, int64_t n_rows, int64_t features,
                                 void* stream) {
   return fmoe::quantize(x, n_rows, features, n_rows_dev, nullptr, 1, codes, scales, dtype,
                         (hipStream_t)stream);
+}
+
+extern "C" int fmoe_mx_quantize_counted(const void* x, int64_t n_rows, int64_t features,
+                                        const int64_t* expert_count, int64_t n_expert,
+                                        int32_t* seg_off, void* codes, void* scales, int dtype,
+                                        void* stream) {
+  FMOE_REQUIRE(expert_count && seg_off && n_expert >= 1 && n_expert < INT32_MAX, FMOE_ERR_INVALID,
+               "mx_quantize_counted: bad counts");
+  return fmoe::quantize(x, n_rows, features, nullptr, nullptr, 1, codes, scales, dtype,
+                        (hipStream_t)stream, {expert_count, (int)n_expert, seg_off});
 }
 
 extern "C" int fmoe_mx_quantize_tokens(const void* x, const int32_t* inv, int64_t n_tokens,

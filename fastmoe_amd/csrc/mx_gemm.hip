@@ -152,8 +152,11 @@ template <typename T, int MODE> struct MxOutput {
       v[i] = n0 + i < n ? v[i] : 0.f;
       m = max(m, magnitude_bits(v[i]));
     }
-    m = max(m, (uint32_t)__shfl_xor((int)m, 16, kWave));
-    m = max(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
+    // (rows of 16 lanes, then halves of the wave, swap places: either result holds one of the two)
+    const auto r16 = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max(r16[0], r16[1]);
+    const auto r32 = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    m = max(r32[0], r32[1]);
     byte = mx_scale_byte(m);
     return mx_codes(v, byte);
   }
@@ -276,15 +279,15 @@ template <typename T, int MODE> struct MxOutput {
 };
 
 // ------------------------------------------------------------------------- few rows
-// Weights straight from memory into registers: a workgroup's 4 waves take 16 NT rows of an expert and
-// 32 features each (KS == 1), or the same 32 features and a quarter of K each (KS == 4).
-template <typename T, int NT, int KS, int MODE>
+// Weights straight from memory into registers: a workgroup's 4 waves take 16 rows of an expert,
+// 32 features, and a quarter of K each.
+template <typename T, int MODE>
 __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
-  constexpr int kWaves = 4, kCols = 32 * (kWaves / KS);
+  constexpr int kWaves = 4, kCols = 32;
   __shared__ int s_sum[2 * kWaves], s_out[4];
-  __shared__ float part[KS > 1 ? (KS - 1) * NT * 8 * kWave : 1];
+  __shared__ float part[(kWaves - 1) * 8 * kWave];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  RowTiles<16 * NT, kOneHeight, kWaves> tiles;
+  RowTiles<16, kOneHeight, kWaves> tiles;
   tiles.scan(a.seg_off, a.n_expert, s_sum);
   const int n_pad = mx_quantises(MODE) ? (int)mx_code_bytes(a.out_feat) * 2 : a.out_feat;
   const int n_cols = (n_pad + kCols - 1) / kCols;
@@ -293,80 +296,55 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
   if (col >= n_cols) return;
   const TileRows t = tiles.find(a.seg_off, v, false, s_out);
 
-  const int m = lane & 15, g = lane >> 4;
-  const int base = col * kCols + (KS == 1 ? wave * 32 : 0);
+  const int m = lane & 15, g = lane >> 4, base = col * kCols;
   const int64_t code_row = mx_code_bytes(a.in_feat), scale_row = mx_scale_bytes(a.in_feat);
   // rows and features past the end repeat the last one; their results are not stored
-  const uint8_t *wc[2], *ws[2], *xc[NT], *xs[NT];
+  const uint8_t *wc[2], *ws[2];
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
     const int64_t n = (int64_t)t.e * a.out_feat + min(base + mx_feature(f, m), a.out_feat - 1);
     wc[f] = a.wc + n * code_row + g * 16;
     ws[f] = a.ws + n * scale_row;
   }
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int64_t r = t.row0 + min(t.m0 + i * 16 + m, t.cnt - 1);
-    xc[i] = a.xc + r * code_row + g * 16;
-    xs[i] = a.xs + r * scale_row;
-  }
+  const int64_t r = (int64_t)t.row0 + min(t.m0 + m, t.cnt - 1);
+  const uint8_t *const xc = a.xc + r * code_row + g * 16, *const xs = a.xs + r * scale_row;
   const int steps = (a.in_feat + kMxStep - 1) / kMxStep, groups = (steps + 3) / 4;
-  const int g0 = KS == 1 ? 0 : wave * groups / KS, g1 = KS == 1 ? groups : (wave + 1) * groups / KS;
-  f32x4 acc[NT][2];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int q = g0; q < g1; ++q) {
-    i32x4 wsv[2], xsv[NT];
+  const int g1 = (wave + 1) * groups / kWaves;
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  for (int q = wave * groups / kWaves; q < g1; ++q) {
+    const i32x4 xsv = *(const i32x4*)(xs + q * 16);
+    i32x4 wsv[2];
 #pragma unroll
     for (int f = 0; f < 2; ++f) wsv[f] = *(const i32x4*)(ws[f] + q * 16);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) xsv[i] = *(const i32x4*)(xs[i] + q * 16);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       if (q * 4 + s >= steps) break;
       const int64_t off = (int64_t)(q * 4 + s) * 64;
-      i32x4 w[2], x[NT];
+      const i32x4 x = *(const i32x4*)(xc + off);
 #pragma unroll
-      for (int f = 0; f < 2; ++f) w[f] = *(const i32x4*)(wc[f] + off);
-#pragma unroll
-      for (int i = 0; i < NT; ++i) x[i] = *(const i32x4*)(xc[i] + off);
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int f = 0; f < 2; ++f)
-          acc[i][f] = mx_mfma(w[f], (int)((uint32_t)wsv[f][s] >> (8 * g)), x[i],
-                              (int)((uint32_t)xsv[i][s] >> (8 * g)), acc[i][f]);
+      for (int f = 0; f < 2; ++f)
+        acc[f] = mx_mfma(*(const i32x4*)(wc[f] + off), (int)((uint32_t)wsv[f][s] >> (8 * g)), x,
+                         (int)((uint32_t)xsv[s] >> (8 * g)), acc[f]);
     }
   }
-  if (KS > 1) {
-    // the quarters meet in the first wave, always in the same order
-    if (wave > 0) {
+  // the quarters meet in the first wave, always in the same order
+  if (wave > 0) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          part[(((wave - 1) * NT + i) * 8 + j) * kWave + lane] = acc[i][j >> 2][j & 3];
-    }
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int w2 = 0; w2 < KS - 1; ++w2)
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          acc[i][j >> 2][j & 3] += part[((w2 * NT + i) * 8 + j) * kWave + lane];
+    for (int j = 0; j < 8; ++j) part[((wave - 1) * 8 + j) * kWave + lane] = acc[j >> 2][j & 3];
   }
-  const MxOutput<T, MODE> out(a, (int64_t)t.row0 + t.m0, min(16 * NT, t.cnt - t.m0));
-  float b[8];
+  __syncthreads();
+  if (wave > 0) return;
+  float b[8], y[8];
   mx_load_bias(a, mx_bias_rows(a, t.e), base + 8 * g, b);
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    float r[8];
+  for (int j = 0; j < 8; ++j) {
+    y[j] = acc[j >> 2][j & 3];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = acc[i][j >> 2][j & 3] + b[j];
-    out.store(i * 16 + m, base + 8 * g, r);
+    for (int w = 0; w < kWaves - 1; ++w) y[j] += part[(w * 8 + j) * kWave + lane];
+    y[j] += b[j];
   }
+  const MxOutput<T, MODE> out(a, (int64_t)t.row0 + t.m0, min(16, t.cnt - t.m0));
+  out.store(m, base + 8 * g, y);
 }
 
 // ------------------------------------------------------------------------- many rows
@@ -788,18 +766,38 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
 
 constexpr int kCus = 256;
 
+// Which kernel: by the mean number of rows per expert, the features and the number of tiles this
+// makes.  Measured (us; a row of a table is one shape, weights from the last-level cache or HBM):
+//   rows  experts  in -> out     stream   128x64  128x128  256x128  256x256
+//     64    8    4096 -> 14336     47       45       48       47       60
+//    128   16    4096 -> 1024      10       13       15       19       29
+//    512   16    1024 -> 4096      24        9       11       12       16
+//   2048   16    1024 -> 4096      69       17       15       20       17
+//   1024    8   14336 -> 4096     585       90       87       67       80
+//   4096   16    1024 -> 4096     124       26       21       26       27
+//  65536  128    2048 -> 1408    1129      207      147      156      139
+//   4096    8    4096 -> 14336   1515      220      154      156      134
+// Few rows and few tiles: the kernel that splits K.  Large tiles move the least through L2 and
+// win where there are rounds enough of them; 128-row ones share a CU by two, so that one's
+// beginning and end are the other's middle, and win where tiles are short.
+enum MxKernel { kStream, kTile128x64, kTile128x128, kTile256x128, kTile256x256 };
+static MxKernel choose_kernel(const MxGemmArgs& a) {
+  const double live = (double)std::min<int64_t>(a.n_expert, a.n_rows);
+  const double mean = (double)a.n_rows / a.n_expert;
+  // (an expert's last tile is half empty on average)
+  auto tiles = [&](int tn, int tm) {
+    return std::max((double)a.n_rows / tm + live / 2, live) * ceil_div(a.out_feat, tn);
+  };
+  if (mean <= 16 && tiles(128, 64) <= kCus) return kStream;
+  if (mean < 56) return kTile128x64;
+  if (mean >= 192 && tiles(256, 256) >= 600) return kTile256x256;
+  if (mean >= 96 && a.in_feat >= 4096 && tiles(128, 128) > kCus) return kTile256x128;
+  return kTile128x128;
+}
+
 template <typename T, int MODE>
 static int launch(const MxGemmArgs& a, hipStream_t s) {
   const int n_pad = mx_quantises(MODE) ? (int)mx_code_bytes(a.out_feat) * 2 : a.out_feat;
-  const double mean = (double)a.n_rows / a.n_expert;
-#define FMOE_STREAM(NT, KS)                                                                      \
-  do {                                                                                           \
-    const int64_t rows = a.n_rows / (16 * NT) + std::min<int64_t>(a.n_expert, a.n_rows);         \
-    const int64_t blocks = rows * ceil_div(n_pad, 32 * (4 / KS));                                \
-    FMOE_REQUIRE(blocks <= INT32_MAX, FMOE_ERR_UNSUPPORTED, "mx_linear: too many tiles");        \
-    hipLaunchKernelGGL((mx_stream_kernel<T, NT, KS, MODE>), dim3((unsigned)blocks), dim3(256), 0, \
-                       s, a);                                                                    \
-  } while (0)
 #define FMOE_TILE(TN, TM)                                                                        \
   do {                                                                                           \
     const int64_t rows = a.n_rows / TM + std::min<int64_t>(a.n_expert, a.n_rows);                \
@@ -809,10 +807,18 @@ static int launch(const MxGemmArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((mx_tile_kernel<T, TN, TM, MODE>), dim3(kCus * MxTile<TN, TM>::kGroups),  \
                        dim3(256), (MxTile<TN, TM>::kLdsBytes), s, a);                            \
   } while (0)
-  if (mean >= 128) FMOE_TILE(256, 256);
-  else if (mean <= 16) FMOE_STREAM(1, 4);
-  else FMOE_STREAM(4, 1);
-#undef FMOE_STREAM
+  switch (choose_kernel(a)) {
+    case kStream: {
+      const int64_t rows = a.n_rows / 16 + std::min<int64_t>(a.n_expert, a.n_rows);
+      hipLaunchKernelGGL((mx_stream_kernel<T, MODE>), dim3((unsigned)(rows * ceil_div(n_pad, 32))),
+                         dim3(256), 0, s, a);      // (few tiles, or this kernel is not chosen)
+      break;
+    }
+    case kTile128x64: FMOE_TILE(128, 64); break;
+    case kTile128x128: FMOE_TILE(128, 128); break;
+    case kTile256x128: FMOE_TILE(256, 128); break;
+    case kTile256x256: FMOE_TILE(256, 256); break;
+  }
 #undef FMOE_TILE
   FMOE_LAUNCH_CHECK("mx_linear");
   return FMOE_OK;

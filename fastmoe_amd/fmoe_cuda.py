@@ -48,7 +48,8 @@ OPERATORS = ("expert_count", "assign_pos", "linear_forward", "linear_backward",
              "grouped_linear_bwd", "pointer_table", "grouped_linear_fwd_ptrs",
              "grouped_linear_bwd_ptrs", "gather_combine_fwd", "gather_combine_bwd",
              "scatter_reduce", "topk_softmax_fwd", "topk_softmax_bwd", "score_topk_fwd", "score_topk_bwd",
-             "mx_quantize", "mx_quantize_tokens", "mx_dequantize", "mx_linear_fwd",
+             "mx_quantize", "mx_quantize_counted", "mx_quantize_tokens", "mx_dequantize",
+             "mx_linear_fwd",
              "mx_linear_act_fwd", "mx_linear_bwd", "gelu_fwd", "gelu_bwd", "set_gemm_path", "_seg_off_from_counts")
 
 

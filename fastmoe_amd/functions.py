@@ -259,13 +259,18 @@ def score_topk(logits, top_k: int, bias=None, score: str = "sigmoid", n_group: i
     ties go to the lower index.  The weights are the chosen scores, divided by their sum if
     `renormalize`, times `scale`.  An expert whose logit or bias is -inf is never chosen; a
     slot for which nobody is left is -1 (a dropped slot) with weight 0."""
-    if score not in SCORES:
+    kind = SCORES.get(score)
+    if kind is None:
         raise ValueError(f"score must be one of {sorted(SCORES)}, not {score!r}")
+    native = fmoe_cuda.native()
+    if native is not None:
+        return native.score_topk(logits, bias, top_k, n_group, top_group, group_best, kind,
+                                 renormalize, scale)
     flat = logits.reshape(-1, logits.shape[-1])
     if bias is not None:
         bias = bias.detach().to(torch.float32).contiguous()
-    return ScoreTopK.apply(flat, bias, top_k, n_group, top_group, group_best, SCORES[score],
-                           renormalize, scale)
+    return ScoreTopK.apply(flat, bias, top_k, n_group, top_group, group_best, kind, renormalize,
+                           scale)
 
 
 class Gelu(Function):

@@ -86,7 +86,10 @@ class MXLinear(Function):
     @staticmethod
     def forward(ctx, x, seg_off, w_codes, w_scales, bias):
         in_feat = x.shape[1]
-        codes, scales = fmoe_cuda.mx_quantize(x.contiguous())
+        if seg_off.dtype == torch.int64:      # counts on the device
+            codes, scales, seg_off = fmoe_cuda.mx_quantize_counted(x.contiguous(), seg_off)
+        else:
+            codes, scales = fmoe_cuda.mx_quantize(x.contiguous())
         out = torch.empty((x.shape[0], w_codes.shape[1]), dtype=x.dtype, device=x.device)
         fmoe_cuda.mx_linear_fwd(codes, scales, w_codes, w_scales, in_feat, bias, seg_off, out)
         ctx.in_feat = in_feat
@@ -108,14 +111,19 @@ def linear(x: torch.Tensor, fwd_expert_count, weight: MXTensor, bias=None) -> to
     `FMoELinear` with 4-bit weights [E, out, in].  x [rows, in] holds the rows in expert
     order and is quantised on the way; `fwd_expert_count` is an int64 tensor of row counts
     (host or device) or a SegmentTable; bias [E, out] has x's dtype, as has the result."""
-    if x.dim() != 2 or x.shape[1] != weight.features:
-        raise RuntimeError(f"x must be [rows, {weight.features}], got {tuple(x.shape)}")
-    if not x.is_cuda:
-        raise RuntimeError("x must be a CUDA tensor")
+    native = fmoe_cuda.native()
+    if native is not None:
+        segments = (fwd_expert_count.seg_off if isinstance(fwd_expert_count, SegmentTable)
+                    else fwd_expert_count)
+        return native.mx_linear(x, segments, weight.codes, weight.scales, weight.features, bias)
+    if x.dim() != 2 or x.shape[1] != weight.features or not x.is_cuda:
+        raise RuntimeError(f"x must be a CUDA tensor [rows, {weight.features}]")
     if isinstance(fwd_expert_count, torch.Tensor) and not fwd_expert_count.is_cuda and (
             bool((fwd_expert_count < 0).any()) or int(fwd_expert_count.sum()) > x.shape[0]):
         raise RuntimeError("expert counts are negative or claim more rows than x holds")
-    return MXLinear.apply(x, _segments(fwd_expert_count, x.device), weight.codes, weight.scales,
+    if not isinstance(fwd_expert_count, torch.Tensor) or not fwd_expert_count.is_cuda:
+        fwd_expert_count = _segments(fwd_expert_count, x.device)
+    return MXLinear.apply(x, fwd_expert_count.contiguous(), weight.codes, weight.scales,
                           None if bias is None else bias.contiguous())
 
 
@@ -140,6 +148,10 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
         h = apply_activation(activation, h, plan.n_rows_dev)
         y = linear(h, plan.segments, w2, b2)
         return FusedGatherCombine.apply(y, score.reshape(-1, top_k), plan)
+    native = fmoe_cuda.native()
+    if native is not None:
+        return native.mx_expert_layer(x, gate_idx.reshape(-1, top_k), score, w1.codes, w1.scales,
+                                      w1.features, b1, w2.codes, w2.scales, w2.features, b2, act)
     x = x.contiguous()
     n_tokens = x.shape[0]
     _pos, _counts, seg_off, inv = fmoe_cuda.route(gate_idx.reshape(-1, top_k).contiguous(),

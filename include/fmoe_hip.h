@@ -518,6 +518,9 @@ int fmoe_score_topk_bwd(const void* dweight, const void* logits, const int64_t* 
  *                     n_rows_dev (DEVICE int32) is not NULL.
  *   _quantize_tokens  row t goes to the rows inv[t * top_k + j] that are not -1 (inv of
  *                     fmoe_route): the dispatch of fmoe_scatter_tokens in the same pass.
+ *   _quantize_counted _quantize of rows in expert order that also writes seg_off (int32
+ *                     [n_expert + 1]) from their DEVICE int64 counts: a linear layer that is
+ *                     handed counts then needs no launch of its own for them.
  *   _dequantize       the values, rounded to dtype where that is too narrow for them.
  * dtype: f32, f16 or bf16.  The reference has no such format.
  */
@@ -525,6 +528,9 @@ int64_t fmoe_mx_code_bytes(int64_t features);
 int64_t fmoe_mx_scale_bytes(int64_t features);
 int fmoe_mx_quantize(const void* x, int64_t n_rows, int64_t features, const int32_t* n_rows_dev,
                      void* codes, void* scales, int dtype, void* stream);
+int fmoe_mx_quantize_counted(const void* x, int64_t n_rows, int64_t features,
+                             const int64_t* expert_count, int64_t n_expert, int32_t* seg_off,
+                             void* codes, void* scales, int dtype, void* stream);
 int fmoe_mx_quantize_tokens(const void* x, const int32_t* inv, int64_t n_tokens, int64_t top_k,
                             int64_t features, void* codes, void* scales, int dtype, void* stream);
 int fmoe_mx_dequantize(const void* codes, const void* scales, int64_t n_rows, int64_t features,
