@@ -799,6 +799,8 @@ PYBIND11_MODULE(fmoe_cuda, m) {
   m.def("mx_quantize", &mx_quantize, py::arg("x"), py::arg("n_rows_dev") = py::none());
   m.def("mx_quantize_counted", &mx_quantize_counted, py::arg("x"), py::arg("expert_count"));
   m.def("score_topk", &score_topk);
+  m.def("mx_quantize_rows", &mx_quantize_rows);
+  m.def("mx_dequantize_rows", &mx_dequantize_rows);
   m.def("mx_linear", &mx_linear);
   m.def("mx_expert_layer", &mx_expert_layer);
   m.def("mx_quantize_tokens", &mx_quantize_tokens, py::arg("x"), py::arg("inv"), py::arg("top_k"));

@@ -18,44 +18,32 @@ constexpr int kMxWaves = kMxThreads / kWave;
 constexpr int kMxChunk = kWave * 8;          // values of a row that a wave takes at once
 static_assert(kMxChunk == kMxGroup, "a chunk's scales are one 16-byte pack");
 
-// 8 values of a row from element k on, as f32; zeros from k_total on.  VEC: 16-byte packs.
-template <typename T, bool VEC>
+// N values, moved as one.
+template <typename T, int N> struct alignas(sizeof(T) * N) Run { T v[N]; };
+
+// 8 values of a row from element k on, as f32; zeros from k_total on.  Rows are moved in runs of N
+// values, of which they hold whole ones.
+template <typename T, int N>
 __device__ __forceinline__ void load8(const T* row, int k, int k_total, float (&v)[8]) {
-  if (VEC) {
-    constexpr int kN = Pack16<T>::kN;
 #pragma unroll
-    for (int p = 0; p < 8 / kN; ++p) {
-      if (k + p * kN < k_total) {
-        const Pack16<T> x = *reinterpret_cast<const Pack16<T>*>(row + k + p * kN);
+  for (int p = 0; p < 8; p += N) {
+    Run<T, N> x;
+    const bool in = k + p < k_total;
+    if (in) x = *reinterpret_cast<const Run<T, N>*>(row + k + p);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[p * kN + i] = Elem<T>::to_acc(x.v[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kN; ++i) v[p * kN + i] = 0.f;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < k_total ? Elem<T>::to_acc(row[k + i]) : 0.f;
+    for (int i = 0; i < N; ++i) v[p + i] = in ? Elem<T>::to_acc(x.v[i]) : 0.f;
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, int N>
 __device__ __forceinline__ void store8(T* row, int k, int k_total, const float (&v)[8]) {
-  if (VEC) {
-    constexpr int kN = Pack16<T>::kN;
 #pragma unroll
-    for (int p = 0; p < 8 / kN; ++p) {
-      if (k + p * kN >= k_total) break;
-      Pack16<T> x;
+  for (int p = 0; p < 8; p += N) {
+    if (k + p >= k_total) break;
+    Run<T, N> x;
 #pragma unroll
-      for (int i = 0; i < kN; ++i) x.v[i] = Elem<T>::from_acc(v[p * kN + i]);
-      *reinterpret_cast<Pack16<T>*>(row + k + p * kN) = x;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k + i < k_total) row[k + i] = Elem<T>::from_acc(v[i]);
+    for (int i = 0; i < N; ++i) x.v[i] = Elem<T>::from_acc(v[p + i]);
+    *reinterpret_cast<Run<T, N>*>(row + k + p) = x;
   }
 }
 
@@ -64,6 +52,29 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));  // 1 0 3 2
   v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));  // 2 3 0 1
   return v;
+}
+
+// w[u] of lane i to w[i] of lane u among every four lanes: four words of a block, one in each
+// lane, for four blocks become a block's 16 bytes in one lane, so that four chunks take one store
+// of 1 KiB instead of four of 256 bytes.
+__device__ __forceinline__ void transpose_quad(uint32_t (&w)[4], int lane) {
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    const bool up = lane & d;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (u & d) continue;
+      const uint32_t send = up ? w[u] : w[u | d];
+      const uint32_t got = (uint32_t)(d == 1 ? __builtin_amdgcn_update_dpp(0, (int)send, 0xb1, 0xf, 0xf, false)
+                                             : __builtin_amdgcn_update_dpp(0, (int)send, 0x4e, 0xf, 0xf, false));
+      w[u] = up ? got : w[u];
+      w[u | d] = up ? w[u | d] : got;
+    }
+  }
+}
+
+__device__ __forceinline__ int of_four(const int (&v)[4], int i) {
+  return i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
 }
 
 // Row counts of experts as segment bounds, for the call's first workgroup to leave behind.
@@ -90,105 +101,161 @@ __device__ __forceinline__ void write_segments(const MxSegments& sg, int64_t n_r
   if (lane == 0) sg.seg_off[sg.n_expert] = (int32_t)min(carry, n_rows);
 }
 
-// One wave takes `U` chunks of a row at a time.  inv == nullptr: row r goes to row r, and rows
-// from *n_rows_dev on (if given) are skipped; else row t goes to the rows inv[t * top_k + j]
-// that are not -1.
-template <typename T, bool VEC, int U>
+// The chunks of all rows are numbered row by row; a wave takes U consecutive ones at a time.
+struct MxChunk {
+  int64_t row;
+  int k;                  // first value
+  __device__ __forceinline__ MxChunk(int64_t number, int chunks) {
+    row = number / chunks;
+    k = (int)(number - row * chunks) * kMxChunk;
+  }
+};
+
+// inv == nullptr: row r goes to row r, and rows from *n_rows_dev on (if given) are skipped; else
+// row t goes to the rows inv[t * top_k + j] that are not -1.
+template <typename T, int N, int U>
 __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(
     const T* __restrict__ x, int64_t n_rows, int k, const int32_t* __restrict__ n_rows_dev,
     const int32_t* __restrict__ inv, int top_k, uint8_t* __restrict__ codes,
     uint8_t* __restrict__ scales, MxSegments segments) {
+  static_assert(U == 1 || U == 4, "the lanes of a block share the chunks between them");
   const int lane = threadIdx.x & (kWave - 1);
   if (segments.seg_off && blockIdx.x == 0 && threadIdx.x < kWave) write_segments(segments, n_rows, lane);
-  const int chunks = (k + kMxChunk - 1) / kMxChunk, runs = (chunks + U - 1) / U;
+  const int chunks = (k + kMxChunk - 1) / kMxChunk;
   const int64_t code_row = mx_code_bytes(k), scale_row = mx_scale_bytes(k);
   int64_t rows = n_rows;
   if (n_rows_dev) rows = min(rows, (int64_t)*n_rows_dev);
-  const int64_t items = rows * runs, n_waves = (int64_t)gridDim.x * kMxWaves;
-  for (int64_t it = (int64_t)blockIdx.x * kMxWaves + threadIdx.x / kWave; it < items;
-       it += n_waves) {
-    const int64_t row = it / runs;
-    const int c0 = (int)(it - row * runs) * U;
+  const int64_t items = rows * chunks, stride = (int64_t)gridDim.x * kMxWaves * U;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  for (int64_t it = ((int64_t)blockIdx.x * kMxWaves + wave) * U; it < items; it += stride) {
     float v[U][8];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      load8<T, VEC>(x + row * k, (c0 + u) * kMxChunk + lane * 8, k, v[u]);
+    for (int u = 0; u < U; ++u) {
+      const MxChunk c(min(it + u, items - 1), chunks);
+      load8<T, N>(x + c.row * k, c.k + lane * 8, k, v[u]);
+    }
+    uint32_t word[U];
+    int byte[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (c0 + u >= chunks) break;
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = max(m, magnitude_bits(v[u][i]));
-      const int byte = mx_scale_byte(quad_max(m));
-      const uint32_t word = mx_codes(v[u], byte);
-      const int64_t at = (int64_t)(c0 + u) * (kMxChunk / 2) + lane * 4;
-      const int64_t sat = (int64_t)(c0 + u) * 16 + (lane >> 2);
-      if (inv == nullptr) {
-        if (at < code_row) *reinterpret_cast<uint32_t*>(codes + row * code_row + at) = word;
-        if ((lane & 3) == 0) scales[row * scale_row + sat] = (uint8_t)byte;
-      } else {
-        for (int j = 0; j < top_k; ++j) {
-          const int64_t to = inv[row * top_k + j];
-          if (to < 0) continue;
-          if (at < code_row) *reinterpret_cast<uint32_t*>(codes + to * code_row + at) = word;
-          if ((lane & 3) == 0) scales[to * scale_row + sat] = (uint8_t)byte;
-        }
+      byte[u] = mx_scale_byte(quad_max(m));
+      word[u] = mx_codes(v[u], byte[u]);
+    }
+    if constexpr (U == 4) {
+      // lane j of a block's four lanes gets the whole block of chunk j
+      transpose_quad(word, lane);
+      byte[0] = of_four(byte, lane & 3);
+    }
+    const int64_t mine = it + (U == 4 ? lane & 3 : 0);
+    if (mine >= items) continue;
+    const MxChunk c(mine, chunks);
+    const int at = c.k / 2 + (U == 4 ? (lane >> 2) * 16 : lane * 4);
+    const int sat = c.k / kMxBlock + (lane >> 2);
+    auto put = [&](int64_t to) {
+      uint8_t* const p = codes + to * code_row + at;
+      if (at < code_row) {
+        if constexpr (U == 4) *reinterpret_cast<uint4*>(p) = make_uint4(word[0], word[1], word[2], word[3]);
+        else *reinterpret_cast<uint32_t*>(p) = word[0];
+      }
+      if (U == 4 || (lane & 3) == 0) scales[to * scale_row + sat] = (uint8_t)byte[0];
+    };
+    if (inv == nullptr) {
+      put(c.row);
+    } else {
+      for (int j = 0; j < top_k; ++j) {
+        const int64_t to = inv[c.row * top_k + j];
+        if (to >= 0) put(to);
       }
     }
   }
 }
 
-template <typename T, bool VEC, int U>
+template <typename T, int N, int U>
 __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_rows, int k,
     T* __restrict__ out) {
   const int lane = threadIdx.x & (kWave - 1);
-  const int chunks = (k + kMxChunk - 1) / kMxChunk, runs = (chunks + U - 1) / U;
+  const int chunks = (k + kMxChunk - 1) / kMxChunk;
   const int64_t code_row = mx_code_bytes(k), scale_row = mx_scale_bytes(k);
-  const int64_t items = n_rows * runs, n_waves = (int64_t)gridDim.x * kMxWaves;
-  for (int64_t it = (int64_t)blockIdx.x * kMxWaves + threadIdx.x / kWave; it < items;
-       it += n_waves) {
-    const int64_t row = it / runs;
-    const int c0 = (int)(it - row * runs) * U;
-    uint32_t word[U];
-    int byte[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = (int64_t)(c0 + u) * (kMxChunk / 2) + lane * 4;
-      const bool in = at < code_row;       // (the row's scales reach at least as far)
-      word[u] = in ? *reinterpret_cast<const uint32_t*>(codes + row * code_row + at) : 0;
-      byte[u] = in ? scales[row * scale_row + (int64_t)(c0 + u) * 16 + (lane >> 2)] : 0;
+  const int64_t items = n_rows * chunks, stride = (int64_t)gridDim.x * kMxWaves * U;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  for (int64_t it = ((int64_t)blockIdx.x * kMxWaves + wave) * U; it < items; it += stride) {
+    // the way of mx_quantize_kernel backwards: lane j fetches the block of chunk j
+    const MxChunk c(min(it + (U == 4 ? lane & 3 : 0), items - 1), chunks);
+    const int at = c.k / 2 + (U == 4 ? (lane >> 2) * 16 : lane * 4);
+    const uint8_t* const p = codes + c.row * code_row + at;
+    uint32_t word[U] = {};
+    int byte = 0;
+    if (at < code_row) {                  // (the row's scales reach at least as far)
+      if constexpr (U == 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        word[0] = w.x; word[1] = w.y; word[2] = w.z; word[3] = w.w;
+      } else {
+        word[0] = *reinterpret_cast<const uint32_t*>(p);
+      }
+      byte = scales[c.row * scale_row + c.k / kMxBlock + (lane >> 2)];
     }
+    if constexpr (U == 4) transpose_quad(word, lane);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int at = (c0 + u) * kMxChunk + lane * 8;
-      if (at >= k) break;
+      if (it + u >= items) break;
+      const MxChunk d(it + u, chunks);
+      const int first = d.k + lane * 8;
+      const int b = U == 4 ? __shfl(byte, (lane & ~3) + u, kWave) : byte;
       float v[8];
-      mx_values(word[u], byte[u], v);
-      store8<T, VEC>(out + row * k, at, k, v);
+      mx_values(word[u], b, v);
+      if (first < k) store8<T, N>(out + d.row * k, first, k, v);
     }
   }
 }
 
-// Chunks that a wave takes at once: one where the rows are too few to fill the GPU with waves
-// of four.
-constexpr int kMxManyItems = 256 * 32;
+// Four chunks at a time where that leaves every CU several waves.
+constexpr int64_t kMxManyItems = 256 * 32;
+struct MxGrid {
+  bool many;
+  unsigned blocks;
+  MxGrid(int64_t rows, int k) {
+    const int64_t items = rows * ((k + kMxChunk - 1) / kMxChunk);
+    many = items >= kMxManyItems;
+    const int64_t per_block = kMxWaves * (many ? 4 : 1);
+    blocks = (unsigned)std::max<int64_t>(std::min<int64_t>((items + per_block - 1) / per_block, 256 * 64), 1);
+  }
+};
+
+// The longest run (of at most 16 bytes) that every row holds a whole number of, at its alignment.
+template <typename T> static int run_length(const void* p, int k) {
+  int n = 16 / (int)sizeof(T);
+  while (n > 1 && (k % n || (uintptr_t)p % (n * sizeof(T)))) n /= 2;
+  return n;
+}
+#define FMOE_RUN(CALL, N)          \
+  do {                             \
+    if (g.many) CALL(N, 4);        \
+    else CALL(N, 1);               \
+  } while (0)
+#define FMOE_RUNS(CALL)                                             \
+  do {                                                              \
+    constexpr int kMost = 16 / (int)sizeof(T);                      \
+    if (run == 8) FMOE_RUN(CALL, kMost);                            \
+    else if (run == 4) FMOE_RUN(CALL, 4);                           \
+    else if (run == 2) FMOE_RUN(CALL, 2);                           \
+    else FMOE_RUN(CALL, 1);                                         \
+  } while (0)
 
 template <typename T>
 static int launch_quantize(const void* x, int64_t n_rows, int k, const int32_t* n_rows_dev,
                            const int32_t* inv, int top_k, uint8_t* codes, uint8_t* scales,
                            const MxSegments& segments, hipStream_t s) {
-  const bool vec = k % Pack16<T>::kN == 0 && (uintptr_t)x % 16 == 0;
-  const int64_t chunks = ceil_div(k, kMxChunk);
-  const bool many = chunks >= 4 && n_rows * (chunks / 4) >= kMxManyItems;
-  const int64_t items = n_rows * (many ? (chunks + 3) / 4 : chunks);
-  const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>((items + kMxWaves - 1) / kMxWaves, 1), 256 * 64));
-#define FMOE_CALL(VEC, U)                                                                        \
-  hipLaunchKernelGGL((mx_quantize_kernel<T, VEC, U>), grid, dim3(kMxThreads), 0, s, (const T*)x, \
+  const int run = run_length<T>(x, k);
+  const MxGrid g(n_rows, k);
+  const dim3 grid(g.blocks);
+#define FMOE_CALL(N, U)                                                                          \
+  hipLaunchKernelGGL((mx_quantize_kernel<T, N, U>), grid, dim3(kMxThreads), 0, s, (const T*)x, \
                      n_rows, k, n_rows_dev, inv, top_k, codes, scales, segments)
-  if (vec && many) FMOE_CALL(true, 4);
-  else if (vec) FMOE_CALL(true, 1);
-  else FMOE_CALL(false, 1);
+  FMOE_RUNS(FMOE_CALL);
 #undef FMOE_CALL
   FMOE_LAUNCH_CHECK("mx_quantize");
   return FMOE_OK;
@@ -197,17 +264,13 @@ static int launch_quantize(const void* x, int64_t n_rows, int k, const int32_t* 
 template <typename T>
 static int launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, int k,
                              void* out, hipStream_t s) {
-  const bool vec = k % Pack16<T>::kN == 0 && (uintptr_t)out % 16 == 0;
-  const int64_t chunks = ceil_div(k, kMxChunk);
-  const bool many = chunks >= 4 && n_rows * (chunks / 4) >= kMxManyItems;
-  const int64_t items = n_rows * (many ? (chunks + 3) / 4 : chunks);
-  const dim3 grid((unsigned)std::min<int64_t>((items + kMxWaves - 1) / kMxWaves, 256 * 64));
-#define FMOE_CALL(VEC, U)                                                                      \
-  hipLaunchKernelGGL((mx_dequantize_kernel<T, VEC, U>), grid, dim3(kMxThreads), 0, s, codes,   \
+  const int run = run_length<T>(out, k);
+  const MxGrid g(n_rows, k);
+  const dim3 grid(g.blocks);
+#define FMOE_CALL(N, U)                                                                        \
+  hipLaunchKernelGGL((mx_dequantize_kernel<T, N, U>), grid, dim3(kMxThreads), 0, s, codes,   \
                      scales, n_rows, k, (T*)out)
-  if (vec && many) FMOE_CALL(true, 4);
-  else if (vec) FMOE_CALL(true, 1);
-  else FMOE_CALL(false, 1);
+  FMOE_RUNS(FMOE_CALL);
 #undef FMOE_CALL
   FMOE_LAUNCH_CHECK("mx_dequantize");
   return FMOE_OK;

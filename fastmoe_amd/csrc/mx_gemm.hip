@@ -54,29 +54,26 @@ __device__ __forceinline__ i32x4 mx_descriptor(const void* p, int64_t bytes) {
   return r;
 }
 
-// gelu(x) = x Phi(x) with Phi(x) = 1/2 + x P(x^2) on |x| <= 5.2 and constant outside: P of
-// degree 13 in t = 2 x^2 / 5.2^2 - 1 (a least-squares fit on Chebyshev nodes), within 1e-6 of
-// gelu for |x| < 7, which is what rounding to f32 on the way costs as well.  18 full-rate
-// instructions where erff takes about 60, with branches: with one wave on a SIMD nothing hides
-// them (a 256 x 256 tile of 4096 features: 27 us of matrix instructions, 26 us of erff).
+// gelu(x) = x Phi(x) with Phi(x) = 1 / (1 + 2^z), z = -log2(Phi(x) / Phi(-x)) = x P(x^2) for
+// |x| <= 6 and x P(36) outside: P of degree 9, a reweighted least-squares fit on Chebyshev nodes.
+// Within 0.8e-6 of gelu everywhere and, for |x| <= 6, within 2.6e-5 of its value, so that blocks
+// whose values all lie in the negative tail keep their digits as well.  22 issue slots where erff
+// takes about 60, with branches, and loses the tail: with one wave on a SIMD nothing hides them
+// (a 256 x 256 tile of 4096 features: 27 us of matrix instructions, 26 us of erff).
 __device__ __forceinline__ float mx_gelu(float x) {
-  const float c = __builtin_amdgcn_fmed3f(x, -5.2f, 5.2f);
-  const float t = fmaf(c * (2.f / (5.2f * 5.2f)), c, -1.f);
-  float r = -0.000377040647f;
-  r = fmaf(r, t, 0.00118033495f);
-  r = fmaf(r, t, -0.00150067825f);
-  r = fmaf(r, t, 0.00202824641f);
-  r = fmaf(r, t, -0.00450842502f);
-  r = fmaf(r, t, 0.00834169798f);
-  r = fmaf(r, t, -0.012636275f);
-  r = fmaf(r, t, 0.0180494618f);
-  r = fmaf(r, t, -0.0246950798f);
-  r = fmaf(r, t, 0.0319717675f);
-  r = fmaf(r, t, -0.0399323255f);
-  r = fmaf(r, t, 0.0500257686f);
-  r = fmaf(r, t, -0.0677436069f);
-  r = fmaf(r, t, 0.135949984f);
-  return x * fmaf(c, r, 0.5f);          // (the clamp takes a NaN for a number, the product not)
+  const float u = fminf(x * x, 36.f);
+  float p = 2.19136148e-14f;
+  p = fmaf(p, u, -4.54144361e-12f);
+  p = fmaf(p, u, 4.11870843e-10f);
+  p = fmaf(p, u, -2.14399911e-08f);
+  p = fmaf(p, u, 7.0298131e-07f);
+  p = fmaf(p, u, -1.47544906e-05f);
+  p = fmaf(p, u, 0.000177562615f);
+  p = fmaf(p, u, 4.6205645e-05f);
+  p = fmaf(p, u, -0.104784109f);
+  p = fmaf(p, u, -2.30222034f);
+  // (2^z overflows to infinity far down, its inverse is 0 there)
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * p));
 }
 
 // How a product leaves: y where rows are whole 16-byte packs, any other y, or MXFP4 again behind
@@ -143,15 +140,18 @@ template <typename T, int MODE> struct MxOutput {
     }
   }
 
-  // The word of codes and the scale byte of features n0 .. n0 + 7.  All lanes of a wave come here
-  // together; lanes l, l ^ 16, l ^ 32 and l ^ 48 hold one block of 32 features.
-  __device__ __forceinline__ uint32_t quantised(int n0, float (&v)[8], int& byte) const {
-    uint32_t m = 0;
+  // The word of codes and the scale byte of features n0 .. n0 + 7 (`whole`: none of the wave's is
+  // behind the last).  All lanes of a wave come here together; lanes l, l ^ 16, l ^ 32 and l ^ 48
+  // hold one block of 32 features.
+  __device__ __forceinline__ uint32_t quantised(int n0, bool whole, float (&v)[8], int& byte) const {
+    if (!whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = n0 + i < n ? v[i] : 0.f;
-      m = max(m, magnitude_bits(v[i]));
+      for (int i = 0; i < 8; ++i) v[i] = n0 + i < n ? v[i] : 0.f;
     }
+    float top = 0.f;                         // (this maximum keeps a NaN)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[i]));
+    uint32_t m = magnitude_bits(top);
     // (rows of 16 lanes, then halves of the wave, swap places: either result holds one of the two)
     const auto r16 = __builtin_amdgcn_permlane16_swap(m, m, false, false);
     m = max(r16[0], r16[1]);
@@ -166,7 +166,7 @@ template <typename T, int MODE> struct MxOutput {
     activate(v);
     if constexpr (QUANT) {
       int byte;
-      const uint32_t word = quantised(n0, v, byte);
+      const uint32_t word = quantised(n0, false, v, byte);
       const int cr = (int)mx_code_bytes(n), sr = (int)mx_scale_bytes(n);
       const bool in = n0 < cr * 2;
       __builtin_amdgcn_raw_buffer_store_b32(word, yc, in ? row * cr + n0 / 2 : kDmaOutOfRange, 0, 0);
@@ -221,7 +221,7 @@ template <typename T, int MODE> struct MxOutput {
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         int byte;
-        const uint32_t word = quantised(col + p * 32 + 8 * g, v[p], byte);
+        const uint32_t word = quantised(col + p * 32 + 8 * g, col + 32 * P <= n, v[p], byte);
         bytes |= (uint32_t)byte << (8 * p);
         *(uint32_t*)(stage + m * (P * 16) + ((p * 16 + g * 4) ^ ((m & 4) * 4))) = word;
       }
@@ -767,20 +767,22 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
 constexpr int kCus = 256;
 
 // Which kernel: by the mean number of rows per expert, the features and the number of tiles this
-// makes.  Measured (us; a row of a table is one shape, weights from the last-level cache or HBM):
-//   rows  experts  in -> out     stream   128x64  128x128  256x128  256x256
-//     64    8    4096 -> 14336     47       45       48       47       60
-//    128   16    4096 -> 1024      10       13       15       19       29
-//    512   16    1024 -> 4096      24        9       11       12       16
-//   2048   16    1024 -> 4096      69       17       15       20       17
-//   1024    8   14336 -> 4096     585       90       87       67       80
-//   4096   16    1024 -> 4096     124       26       21       26       27
-//  65536  128    2048 -> 1408    1129      207      147      156      139
-//   4096    8    4096 -> 14336   1515      220      154      156      134
-// Few rows and few tiles: the kernel that splits K.  Large tiles move the least through L2 and
-// win where there are rounds enough of them; 128-row ones share a CU by two, so that one's
-// beginning and end are the other's middle, and win where tiles are short.
-enum MxKernel { kStream, kTile128x64, kTile128x128, kTile256x128, kTile256x256 };
+// makes.  Measured with three sets of operands in turn (us; GELU and quantisation behind the
+// products marked q):
+//   rows  experts  in -> out        stream   128x64  128x128  256x256
+//    128   16    4096 -> 1024           10       13       15       29
+//     64   16    1024 -> 4096           12       10       11       17
+//    128    8    4096 -> 14336 q        90       56       62       99
+//   4096   32    4096 -> 1024          140       29       25       32
+//  15560  128    2048 -> 1408 q        325       83       68      109
+//  30000   16    2048 -> 2048          729      116       89       84
+//  32768    8    4096 -> 14336                           1239      980
+//  16384    4    4096 -> 11008 q                          542      549
+//  32768    8    4096 -> 14336 q                         1376     1311
+// Few rows and few tiles: the kernel that splits K.  The largest tiles move the least through L2
+// and win where K is long and there are rounds enough of them; smaller ones share a CU by two, so
+// that one's beginning and end (with GELU, half its time) are the other's middle.
+enum MxKernel { kStream, kTile128x64, kTile128x128, kTile256x256 };
 static MxKernel choose_kernel(const MxGemmArgs& a) {
   const double live = (double)std::min<int64_t>(a.n_expert, a.n_rows);
   const double mean = (double)a.n_rows / a.n_expert;
@@ -788,10 +790,11 @@ static MxKernel choose_kernel(const MxGemmArgs& a) {
   auto tiles = [&](int tn, int tm) {
     return std::max((double)a.n_rows / tm + live / 2, live) * ceil_div(a.out_feat, tn);
   };
-  if (mean <= 16 && tiles(128, 64) <= kCus) return kStream;
+  if (mean <= 16 && tiles(128, 64) <= kCus / 2) return kStream;
   if (mean < 56) return kTile128x64;
-  if (mean >= 192 && tiles(256, 256) >= 600) return kTile256x256;
-  if (mean >= 96 && a.in_feat >= 4096 && tiles(128, 128) > kCus) return kTile256x128;
+  const bool quant = a.yc != nullptr;
+  if (mean >= 192 && a.in_feat >= (quant ? 4096 : 2048) && tiles(256, 256) >= (quant ? 4000 : 600))
+    return kTile256x256;
   return kTile128x128;
 }
 
@@ -816,7 +819,6 @@ static int launch(const MxGemmArgs& a, hipStream_t s) {
     }
     case kTile128x64: FMOE_TILE(128, 64); break;
     case kTile128x128: FMOE_TILE(128, 128); break;
-    case kTile256x128: FMOE_TILE(256, 128); break;
     case kTile256x256: FMOE_TILE(256, 256); break;
   }
 #undef FMOE_TILE

@@ -61,6 +61,35 @@ std::tuple<Tensor, Tensor> score_topk(const Tensor& logits, const OptTensor& bia
   return {r[0], r[1]};
 }
 
+// mx.quantize: x [..., features], codes and scales with its leading dimensions
+std::tuple<Tensor, Tensor> mx_quantize_rows(const Tensor& x) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  need(x.is_cuda() && x.dim() >= 1 && x.size(-1) >= 1, "x must be a CUDA tensor [..., features]");
+  if (x.dim() == 2) return mx_quantize(x.contiguous(), c10::nullopt);
+  auto q = mx_quantize(x.reshape({-1, x.size(-1)}).contiguous(), c10::nullopt);
+  auto shaped = [&](const Tensor& t) {
+    auto sizes = x.sizes().vec();
+    sizes.back() = t.size(1);
+    return t.view(sizes);
+  };
+  return {shaped(std::get<0>(q)), shaped(std::get<1>(q))};
+}
+
+// MXTensor.dequantize
+Tensor mx_dequantize_rows(const Tensor& codes, const Tensor& scales, int64_t features,
+                          at::ScalarType dtype) {
+  mx_check(codes, scales, features, "mx_dequantize");
+  c10::DeviceGuard guard(codes.device());
+  auto sizes = codes.sizes().vec();
+  sizes.back() = features;
+  Tensor out = torch::empty(sizes, codes.options().dtype(dtype));
+  if (out.numel() == 0) return out;
+  check(fmoe_mx_dequantize(codes.data_ptr(), scales.data_ptr(), out.numel() / features, features,
+                           out.data_ptr(), dt(out, "out"), stream_of(out)),
+        "mx_dequantize");
+  return out;
+}
+
 // x in MXFP4 and the segment table of `counts` (int64 row counts on x's device, or on the host),
 // unless that is at hand.
 struct MxRows {

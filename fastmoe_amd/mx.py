@@ -48,11 +48,15 @@ class MXTensor:
 
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
         r"""The values [..., rows, features] as `dtype` (float32, float16 or bfloat16)."""
+        native = fmoe_cuda.native()
+        if native is not None:
+            return native.mx_dequantize_rows(self.codes.contiguous(), self.scales.contiguous(),
+                                             self.features, dtype)
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         if out.numel():
             fmoe_cuda.mx_dequantize(
-                self.codes.reshape(-1, self.codes.shape[-1]),
-                self.scales.reshape(-1, self.scales.shape[-1]), out.view(-1, self.features))
+                self.codes.reshape(-1, self.codes.shape[-1]).contiguous(),
+                self.scales.reshape(-1, self.scales.shape[-1]).contiguous(), out.view(-1, self.features))
         return out
 
     @classmethod
@@ -72,8 +76,11 @@ def quantize(x: torch.Tensor) -> MXTensor:
     r"""x [..., features] (float32, float16 or bfloat16, on the GPU) in MXFP4.  The scale of a
     block is 2^(floor(log2(max |x|)) - 2); values are rounded to nearest, ties to the even
     code, and saturate at 6 times the scale.  A block with an infinity or a NaN is NaN."""
-    x = x.detach()
     k = x.shape[-1]
+    native = fmoe_cuda.native()
+    if native is not None:
+        return MXTensor(*native.mx_quantize_rows(x), k)
+    x = x.detach()
     codes, scales = fmoe_cuda.mx_quantize(x.reshape(-1, k).contiguous())
     return MXTensor(codes.view(*x.shape[:-1], codes.shape[-1]),
                     scales.view(*x.shape[:-1], scales.shape[-1]), k)
