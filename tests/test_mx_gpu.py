@@ -263,6 +263,107 @@ def test_many_tiles_come_out_quantised():
             assert (got != want).float().mean() < 1e-4
 
 
+# by the rule on rows, features and tiles: tiles of 256 x 256 with fewer and with more experts
+# than lanes, tiles of 128 x 128 with more experts than lanes, many small ones, the split sums
+BY_RULE = {"256": ([3001, 0, 700, 2500], 2100, 8200),
+           "256 odd": ([3001, 0, 700, 2500], 2100, 8203),
+           "256 many": ([300, 210, 0, 393, 255, 0, 257] * 14, 2049, 3000),
+           "128 many": ([60, 0, 200, 1] * 20, 513, 300),
+           "64 many": ([1, 30, 0, 65, 17] * 30, 1100, 260),
+           "split": ([1, 0, 2, 17, 0, 0, 3, 16], 4100, 330)}
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("case", BY_RULE)
+def test_every_tile_shape(case, dt):
+    from fastmoe_amd import mx
+
+    counts, k, n = BY_RULE[case]
+    g = torch.Generator(device="cuda").manual_seed(len(counts))
+    draw = lambda *shape: torch.randn(*shape, device="cuda", generator=g)
+    x = draw(sum(counts), k).to(DTYPES[dt])
+    b = draw(len(counts), n).to(DTYPES[dt])
+    wq = mx.quantize(draw(len(counts), n, k) * 0.05)
+    y = mx.linear(x, torch.tensor(counts), wq, b)
+    assert torch.equal(y, mx.linear(x, torch.tensor(counts).cuda(), wq, b))
+    xv, at = mx.quantize(x).dequantize(torch.float32).double(), 0
+    for e, c in enumerate(counts):
+        rows = xv[at:at + c]
+        we = mx.MXTensor(wq.codes[e], wq.scales[e], k).dequantize(torch.float32).double()
+        want = rows @ we.T + b[e].double()
+        mag = rows.abs() @ we.abs().T + b[e].double().abs()
+        # as above: the instructions' sums and the bias in f32, then the output's rounding
+        tol = UNIT[dt] * want.abs() + 2.0 ** -23 * (k / 128 + 4) * mag
+        assert ((y[at:at + c].double() - want).abs() <= tol).all(), e
+        at += c
+
+
+@pytest.mark.parametrize("k,n,counts", [
+    (4100, 13000, [9000, 0, 4001, 7000]), (1030, 4000, [900, 0, 401, 700]),
+    (1030, 260, [60, 0, 200, 1] * 20), (520, 1500, [1, 30, 0, 65, 17] * 30)])
+def test_every_tile_shape_comes_out_quantised(k, n, counts):
+    from fastmoe_amd import fmoe_cuda, mx
+
+    g = torch.Generator(device="cuda").manual_seed(n)
+    draw = lambda *shape: torch.randn(*shape, device="cuda", generator=g)
+    xq, wq = mx.quantize(draw(sum(counts), k)), mx.quantize(draw(len(counts), n, k) * 0.05)
+    b = draw(len(counts), n)
+    seg = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32).cuda()
+    y = fmoe_cuda.mx_linear_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k, b, seg,
+                                torch.empty(sum(counts), n).cuda())
+    for act in (0, 1, 2):
+        codes, scales = fmoe_cuda.mx_linear_act_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k,
+                                                    b, seg, act)
+        got = mx.MXTensor(codes, scales, n).dequantize(torch.float32)
+        h = [lambda: y, lambda: torch.nn.functional.gelu(y.double()).float(), lambda: y.relu()][act]()
+        want = mx.quantize(h).dequantize(torch.float32)
+        # sums in the same order in every tile shape; the two GELUs differ by up to 1e-6
+        assert torch.equal(got, want) if act != 1 else (got != want).float().mean() < 1e-4
+        tail = codes[:, -(-n // 2):]
+        assert not tail.any()
+
+
+def test_counts_that_do_not_fit_are_cut_off():
+    """On the device nobody looks at them: negative counts are none, rows there are not are left."""
+    from fastmoe_amd import mx
+
+    x = torch.randn(20, 96).cuda()
+    w = mx.quantize(torch.randn(3, 40, 96).cuda())
+    fit = mx.linear(x, torch.tensor([5, 0, 15]), w)
+    for counts in ([5, -3, 15], [5, -3, 10 ** 12], [5, -2 ** 62, 2 ** 62]):
+        assert torch.equal(mx.linear(x, torch.tensor(counts).cuda(), w), fit), counts
+    all_first = mx.linear(x, torch.tensor([20, 0, 0]), w)
+    assert torch.equal(mx.linear(x, torch.tensor([2 ** 62, 2 ** 62, 2 ** 62]).cuda(), w), all_first)
+    assert mx.linear(x, torch.tensor([-1, -1, -1]).cuda(), w).shape == (20, 40)
+
+
+def test_both_bindings_count_alike():
+    from fastmoe_amd import _ext, fmoe_cuda
+
+    py, cx = fmoe_cuda.ctypes_ops, _ext.load()
+    x = torch.randn(130, 72).cuda()
+    counts = torch.tensor([0, 1, 60, 0, 64] + [0] * 70 + [5]).cuda()
+    p, c = py.mx_quantize_counted(x, counts), cx.mx_quantize_counted(x, counts)
+    assert all(torch.equal(a, b) for a, b in zip(p, c))
+    want = torch.cumsum(counts, 0).cpu()
+    assert torch.equal(p[2].cpu(), torch.cat([torch.zeros(1).long(), want]).int())
+    plain = py.mx_quantize(x)
+    assert torch.equal(p[0], plain[0]) and torch.equal(p[1], plain[1])
+
+
+def test_results_beyond_32_bits():
+    """An output of more than 2^32 elements: its last rows."""
+    from fastmoe_amd import mx
+
+    rows, k, n = 66000, 64, 65536
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, k, device="cuda", generator=g).bfloat16()
+    w = mx.quantize(torch.randn(1, n, k, device="cuda", generator=g))
+    y = mx.linear(x, torch.tensor([rows]), w)
+    last = mx.linear(x[-300:], torch.tensor([300]), w)
+    assert torch.equal(y[-300:], last)
+
+
 def test_rows_without_an_expert_stay_as_they_are():
     from fastmoe_amd import fmoe_cuda, mx
 
