@@ -9,11 +9,15 @@
 // from the logit itself) is never chosen; a slot with nobody left is -1 with weight 0.
 //
 // The arrays are a few MiB at most, so what counts is launch latency and the number of
-// instructions per token.  16 lanes share a token (32 above 256 experts), so a wave serves four;
-// they hold all v in registers as 64-bit keys that order first by v, then by index: the f32 v
-// widened to a double, whose 29 free mantissa bits take the index.  One v_max_f64 then is an
-// arg-max with its tie rule, and a round of the selection is one such maximum per register,
-// four rotations within the 16 lanes, and one comparison per register that drops the winner.
+// instructions per token.  16 lanes share a token (32 above 256 experts; all 64 with few tokens,
+// see FMOE_SCORE_SHAPES), so a wave serves four; they hold all v in registers as 64-bit keys that
+// order first by v, then by index: the f32 v widened to a double, whose 29 free mantissa bits
+// take the index.  One v_max_f64 then is an arg-max with its tie rule, and a round of the
+// selection is one such maximum per register, four rotations within the 16 lanes, and one
+// comparison per register that drops the winner.
+// Measured: 16384 tokens of 128 experts in f32, the best 3 of 8 groups, 10.8 us forward (the
+// 10 MB it moves take 1.9; the rest is instructions) and 4.2 us backward; 64 tokens 4.8 and
+// 2.5 us, of which an empty launch is 2.1.
 #include <algorithm>
 
 #include "common.h"
@@ -72,6 +76,26 @@ struct MaxOp {
 struct SumOp {
   template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
 };
+// op of a lane's value and the one 32 (FAR) or 16 lanes away
+template <bool FAR> __device__ __forceinline__ void swap_rows(uint32_t a, uint32_t (&r)[2]) {
+  const auto p = FAR ? __builtin_amdgcn_permlane32_swap(a, a, false, false)
+                     : __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  r[0] = p[0];
+  r[1] = p[1];
+}
+template <bool FAR, typename Op> __device__ __forceinline__ float op_swapped(float v, Op op) {
+  uint32_t r[2];
+  swap_rows<FAR>(__float_as_uint(v), r);
+  return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <bool FAR, typename Op> __device__ __forceinline__ double op_swapped(double v, Op op) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  uint32_t lo[2], hi[2];
+  swap_rows<FAR>((uint32_t)b, lo);
+  swap_rows<FAR>((uint32_t)(b >> 32), hi);
+  return op(__builtin_bit_cast(double, ((uint64_t)hi[0] << 32) | lo[0]),
+            __builtin_bit_cast(double, ((uint64_t)hi[1] << 32) | lo[1]));
+}
 // f(all lanes of the token), in every lane; the same bits in each (rotations by 8, 4, 2, 1 pair
 // the same operands everywhere up to their order)
 template <int LANES, typename V, typename Op>
@@ -80,7 +104,8 @@ __device__ __forceinline__ V over_lanes(V v, Op op) {
   v = op(v, rotate<0x124>(v));
   v = op(v, rotate<0x122>(v));
   v = op(v, rotate<0x121>(v));
-  if (LANES == 32) v = op(v, __shfl_xor(v, 16, kWave));
+  if (LANES >= 32) v = op_swapped<false>(v, op);
+  if (LANES == 64) v = op_swapped<true>(v, op);
   return v;
 }
 
@@ -127,7 +152,8 @@ __device__ __forceinline__ void load_logits(const T* logits, int64_t t, bool liv
   }
 }
 
-// LDS per token: scores [n_expert], with groups also v [n_expert], and the groups' keys
+// LDS per token: scores [n_expert], with groups also v [n_expert], the groups' keys and whether
+// they stay
 template <typename T, int LANES, int C>
 __global__ __launch_bounds__(kScoreThreads) void score_topk_fwd_kernel(
     const T* __restrict__ logits, const float* __restrict__ bias, ScoreArgs a,
@@ -141,6 +167,7 @@ __global__ __launch_bounds__(kScoreThreads) void score_topk_fwd_kernel(
   double* group_keys = score_lds + slot * a.n_group;
   float* s_row = (float*)(score_lds + (grouped ? kTokens * a.n_group : 0)) + slot * a.n_expert;
   float* v_row = s_row + kTokens * a.n_expert;
+  uint8_t* stays = (uint8_t*)(score_lds + kTokens * (a.n_group + a.n_expert)) + slot * a.n_group;
 
   float l[C], s[C], v[C];
   load_logits<T, LANES, C>(logits, t, live, a.n_expert, g, l);
@@ -158,33 +185,43 @@ __global__ __launch_bounds__(kScoreThreads) void score_topk_fwd_kernel(
   __syncthreads();
   if (grouped) {
     const int size = a.n_expert / a.n_group;
-    for (int q = g; q < a.n_group; q += LANES) {
+    // `parts` lanes share a group (one if there are more groups than half the lanes)
+    int parts = 1;
+    while (2 * parts * a.n_group <= LANES) parts *= 2;
+    for (int q = g / parts; q < a.n_group; q += LANES / parts) {
       float best = -INFINITY, second = -INFINITY;
       bool nan = false;
-      for (int i = 0; i < size; ++i) {
-        const float x = v_row[q * size + i];
+      auto take = [&](float x) {
         nan |= x != x;
-        if (x > best) {
-          second = best;
-          best = x;
-        } else if (x > second) {
-          second = x;
-        }
+        second = fmaxf(second, fminf(x, best));        // (a NaN is no part of either)
+        best = fmaxf(best, x);
+      };
+#pragma unroll 4
+      for (int i = g % parts; i < size; i += parts) take(v_row[q * size + i]);
+      for (int d = 1; d < parts; d *= 2) {
+        const float b = __shfl_xor(best, d, kWave), s2 = __shfl_xor(second, d, kWave);
+        nan |= (bool)__shfl_xor((int)nan, d, kWave);
+        take(b);
+        take(s2);
       }
       float value = best;
       if (a.group_best == 2 && second != -INFINITY) value += second;
-      group_keys[q] = order_key(nan ? NAN : value, q);
+      if (g % parts == 0) group_keys[q] = order_key(nan ? NAN : value, q);
+    }
+    __syncthreads();
+    for (int q = g; q < a.n_group; q += LANES) {
+      const double mine = group_keys[q];
+      int better = 0;
+#pragma unroll 4
+      for (int o = 0; o < a.n_group; ++o) better += group_keys[o] > mine;
+      stays[q] = better < a.top_group;
     }
     __syncthreads();
     const float per_size = 1.f / (float)size;
 #pragma unroll
     for (int u = 0; u < C; ++u) {
       const int e = u * LANES + g;
-      if (e >= a.n_expert) continue;
-      const double mine = group_keys[min((int)(((float)e + 0.5f) * per_size), a.n_group - 1)];
-      int better = 0;
-      for (int q = 0; q < a.n_group; ++q) better += group_keys[q] > mine;
-      if (better >= a.top_group) v[u] = -INFINITY;
+      if (!stays[min((int)(((float)e + 0.5f) * per_size), a.n_group - 1)]) v[u] = -INFINITY;
     }
   }
 
@@ -300,15 +337,32 @@ static int check_args(const ScoreArgs& a, int dtype) {
   return FMOE_OK;
 }
 
-// LANES lanes hold a token's n_expert <= LANES * C values: f<T, LANES, C>()
-#define FMOE_SCORE_SHAPES(T, CALL)                    \
-  do {                                                \
-    if (a.n_expert <= 16) CALL(T, 16, 1);             \
-    else if (a.n_expert <= 32) CALL(T, 16, 2);        \
-    else if (a.n_expert <= 64) CALL(T, 16, 4);        \
-    else if (a.n_expert <= 128) CALL(T, 16, 8);       \
-    else if (a.n_expert <= 256) CALL(T, 16, 16);      \
-    else CALL(T, 32, 16);                             \
+// LANES lanes hold a token's n_expert <= LANES * C values: f<T, LANES, C>().  With few tokens
+// what counts is how long one takes, so a wave has one; with many, how many instructions all of
+// them take, and the steps over the lanes are shared by four (two above 256 experts).  Measured
+// (us, a launch alone takes 2.1):
+//   tokens  experts, of groups     16 or 32 lanes   64 lanes
+//       64  256, 4 of 8                  10.8           5.8
+//       64  128                           5.0           3.5
+//     2048  128                           5.3           4.4
+//     2048   64                           3.7           3.6
+//     4096  256, 4 of 8                  11.0           9.1
+//     4096  128                           5.4           6.2
+//     8192  256, 4 of 8                  13.1          14.0
+//    16384  128, 3 of 8                  10.9          20.7
+#define FMOE_SCORE_SHAPES(T, CALL)                                       \
+  do {                                                                   \
+    const bool few = a.n_tokens <= (a.n_expert > 128 ? 4096 : 2048);     \
+    if (a.n_expert <= 16) CALL(T, 16, 1);                                \
+    else if (a.n_expert <= 32) CALL(T, 16, 2);                           \
+    else if (a.n_expert <= 64 && few) CALL(T, 64, 1);                    \
+    else if (a.n_expert <= 64) CALL(T, 16, 4);                           \
+    else if (a.n_expert <= 128 && few) CALL(T, 64, 2);                   \
+    else if (a.n_expert <= 128) CALL(T, 16, 8);                          \
+    else if (a.n_expert <= 256 && few) CALL(T, 64, 4);                   \
+    else if (a.n_expert <= 256) CALL(T, 16, 16);                         \
+    else if (few) CALL(T, 64, 8);                                        \
+    else CALL(T, 32, 16);                                                \
   } while (0)
 
 template <typename T>
@@ -319,7 +373,7 @@ static int launch_fwd(const void* logits, const float* bias, const ScoreArgs& a,
   hipLaunchKernelGGL((score_topk_fwd_kernel<T, LANES, C>),                                      \
                      dim3(ceil_div(a.n_tokens, kScoreThreads / LANES)), dim3(kScoreThreads),    \
                      (kScoreThreads / LANES) *                                                  \
-                         ((grouped ? 2 : 1) * a.n_expert * 4 + (grouped ? a.n_group * 8 : 0)),  \
+                         ((grouped ? 2 : 1) * a.n_expert * 4 + (grouped ? a.n_group * 9 : 0)),  \
                      s, (const T*)logits, bias, a, idx, (T*)weight)
   FMOE_SCORE_SHAPES(T, FMOE_CALL);
 #undef FMOE_CALL

@@ -220,3 +220,31 @@ def test_gate_module_balances_its_load():
     gate.load.zero_()
     layer(x)
     assert not gate.load.any()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("e,n_group,top_group", [(17, 1, 1), (48, 4, 2), (64, 1, 1), (65, 5, 3),
+                                                 (128, 8, 3), (200, 25, 4), (256, 1, 1),
+                                                 (257, 1, 1), (320, 64, 9), (512, 8, 4)])
+def test_many_tokens_route_as_few(e, n_group, top_group, dt):
+    """However many lanes share a token, its slots, weights and gradients have the same bits."""
+    from fastmoe_amd.functions import score_topk
+
+    g = torch.Generator().manual_seed(e)
+    logits = torch.randn(4611, e, generator=g).to(DTYPES[dt]).cuda()
+    logits[5, : e // 2] = float("-inf")
+    logits[4500] = float("-inf")
+    bias = (torch.randn(e, generator=g) * 0.1).cuda()
+    k = min(8, e // n_group * top_group)
+    dw = torch.randn(4611, k, generator=g).to(DTYPES[dt]).cuda()
+    for score in ("sigmoid", "softmax"):
+        def run(rows):
+            x = logits[rows].clone().requires_grad_(True)
+            idx, w = score_topk(x, k, bias=bias, score=score, n_group=n_group, top_group=top_group)
+            w.backward(dw[rows])
+            return idx, w.detach(), x.grad
+
+        many = run(slice(None))
+        for rows in (slice(0, 1), slice(1, 700), slice(700, 2748), slice(2748, 4611)):
+            for whole, part in zip(many, run(rows)):
+                assert torch.equal(whole[rows], part)
