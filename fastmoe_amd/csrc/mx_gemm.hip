@@ -446,9 +446,9 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   const int steps = __builtin_amdgcn_readfirstlane((a.in_feat + kMxStep - 1) / kMxStep);
   const int stages = (steps + 1) / 2;
 
-  // A lane's part of the offset of a copy, by the parity of the KiB (8 rows of a fragment's 16):
-  // its row within the 8 and its pack.  Rows of a fragment are features 8 (m / 4) + m % 4 of 32.
-  uint32_t w_lane[2], x_lane[2], s_lane[S::kScaleLoads];
+  // The offset a lane fetches from in each of its wave's copies, one stage (of the scales: one
+  // group) back: a copy moves its own on.
+  uint32_t c_off[S::kLoads], s_off[S::kScaleLoads];
   i32x4 w_rsrc, x_rsrc, s_rsrc[S::kScaleLoads];
   auto pack_of = [](int lane, int p) { return (lane & 7) ^ ((4 * p + (lane >> 4)) & 7); };
   auto place = [&](int number) {
@@ -469,10 +469,15 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
     // every descriptor ends with its last valid row: rows past the end read as zeros
     w_rsrc = mx_descriptor(a.wc + w0 * code_row, (int64_t)w_rows * code_row);
     x_rsrc = mx_descriptor(a.xc + at.x0 * code_row, (int64_t)at.rows * code_row);
+    // every wave has its share of either operand, so that nothing here depends on the wave but
+    // numbers; rows of a weight fragment are features 8 (m / 4) + m % 4 of 32
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      w_lane[p] = (uint32_t)((8 * (r8 >> 2) + (r8 & 3)) * code_row + pack_of(lane, p) * 16);
-      x_lane[p] = (uint32_t)(r8 * code_row + pack_of(lane, p) * 16);
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int kib = i < S::kLoadsW ? wave * S::kLoadsW + i : wave * S::kLoadsX + i - S::kLoadsW;
+      const int row = i < S::kLoadsW ? wave * (TN / 4) + 32 * (i >> 2) + 16 * (i & 1) +
+                                           4 * ((i >> 1) & 1) + 8 * (r8 >> 2) + (r8 & 3)
+                                     : kib * 8 + r8;
+      c_off[i] = (uint32_t)(row * code_row + pack_of(lane, kib & 1) * 16 - 128);
     }
     // the scales of 64 rows of one operand (past both: zeros)
 #pragma unroll
@@ -484,50 +489,63 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
       const int row = w ? kib * 64 + (lane & 32) + mx_feature((lane >> 4) & 1, lane & 15)
                         : (kib - TN / 64) * 64 + lane;
       s_rsrc[i] = w ? rw : rx;
-      s_lane[i] = row * 64 < TM * 64 || w ? (uint32_t)(row * scale_row) : kDmaOutOfRange;
+      s_off[i] = (w || row < TM ? (uint32_t)(row * scale_row) : kDmaOutOfRange) - 16;
     }
   };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds;
-  auto dma = [&](uint32_t dst, uint32_t offset, i32x4 rsrc) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(offset), "s"(rsrc)
-                 : "memory", "m0");
+  // A copy is two parts that stand behind different matrix instructions (together they would take
+  // longer than one of them): where it goes, and the load.
+  auto dma_to = [&](uint32_t dst) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, %1" : "={m0}"(m0) : "s"(__builtin_amdgcn_readfirstlane(dst)));
+    return m0;
+  };
+  auto dma = [&](uint32_t m0, uint32_t offset, i32x4 rsrc) {
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :: "v"(offset), "s"(rsrc), "{m0}"(m0) : "memory");
   };
   auto dma4 = [&](uint32_t dst, uint32_t offset, i32x4 rsrc) {      // a word per lane
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :: "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(offset), "s"(rsrc)
                  : "memory", "m0");
   };
-  // Copy i of stage `st`, whose buffer is `par`: every wave has its share of either operand, so that nothing here depends on the wave but numbers.
-  auto copy = [&](auto ic, auto par, int st, int row_bytes) {
+  // Copies 0 .. kLoads - 1 are the next stage's, into buffer `par`; those behind them the next
+  // group's scales, into theirs.
+  auto aim_copy = [&](auto ic, auto par, int buf) {
     constexpr int i = decltype(ic)::value;
-    const uint32_t buf = lds0 + decltype(par)::value * S::kStageBytes;
     if constexpr (i < S::kLoadsW) {
-      const int kib = wave * S::kLoadsW + i;
-      const int row = wave * (TN / 4) + 32 * (i >> 2) + 16 * (i & 1) + 4 * ((i >> 1) & 1);
-      dma(buf + kib * 1024, w_lane[i & 1] + (uint32_t)(row * row_bytes + st * 128), w_rsrc);
+      c_off[i] += 128;
+      return dma_to(lds0 + decltype(par)::value * S::kStageBytes + (wave * S::kLoadsW + i) * 1024);
+    } else if constexpr (i < S::kLoads) {
+      c_off[i] += 128;
+      return dma_to(lds0 + decltype(par)::value * S::kStageBytes + TN * 128 +
+                    (wave * S::kLoadsX + i - S::kLoadsW) * 1024);
     } else {
-      const int kib = wave * S::kLoadsX + i - S::kLoadsW;
-      dma(buf + TN * 128 + kib * 1024,
-          x_lane[(i - S::kLoadsW) & 1] + (uint32_t)(kib * 8 * row_bytes + st * 128), x_rsrc);
+      s_off[i - S::kLoads] += 16;
+      return dma_to(lds0 + 2 * S::kStageBytes + buf * S::kScaleBytes +
+                    (wave * S::kScaleLoads + i - S::kLoads) * 1024);
     }
   };
-  auto copy_scales = [&](int i, int group, int buf) {
-    dma(lds0 + 2 * S::kStageBytes + buf * S::kScaleBytes + (wave * S::kScaleLoads + i) * 1024,
-        s_lane[i] + (uint32_t)(group * 16), s_rsrc[i]);
+  auto copy = [&](auto ic, uint32_t m0) {
+    constexpr int i = decltype(ic)::value;
+    if constexpr (i < S::kLoadsW) dma(m0, c_off[i], w_rsrc);
+    else if constexpr (i < S::kLoads) dma(m0, c_off[i], x_rsrc);
+    else dma(m0, s_off[i - S::kLoads], s_rsrc[i - S::kLoads]);
   };
-  // Before the copies of stage `st`: past the end of K nothing is read any more, and of a last
-  // stage of one step only the first four packs of a row.
+  auto copy_now = [&](auto ic, auto par, int buf) {
+    const uint32_t m0 = aim_copy(ic, par, buf);
+    asm volatile("s_nop 0");                           // between the write of m0 and the load
+    copy(ic, m0);
+  };
+  // Before the copies of stage `st`: past the end of K nothing is read any more.  (In a last stage
+  // of one step the packs of the other come from the next row; their scales are 2^-127 on both
+  // sides, which leaves zero.)
   auto bound = [&](int st) {
-    const bool past = st >= stages, half = st * 2 + 1 >= steps;
+    const bool past = st >= stages;
+    w_rsrc[2] = past ? 0 : w_rsrc[2];
+    x_rsrc[2] = past ? 0 : x_rsrc[2];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const bool off = past | (half & (pack_of(lane, p) >= 4));
-      w_lane[p] = off ? kDmaOutOfRange : w_lane[p];
-      x_lane[p] = off ? kDmaOutOfRange : x_lane[p];
-    }
-#pragma unroll
-    for (int i = 0; i < S::kScaleLoads; ++i) s_lane[i] = past ? kDmaOutOfRange : s_lane[i];
+    for (int i = 0; i < S::kScaleLoads; ++i) s_rsrc[i][2] = past ? 0 : s_rsrc[i][2];
   };
   const int m = lane & 15, g = lane >> 4, wn = wave >> 1, wm = wave & 1;
   const int frag0 = m * 128 + (g ^ ((m >> 1) & 7)) * 16;      // step 0; step 1 has packs 4..7
@@ -600,25 +618,25 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
     using Odd = std::integral_constant<int, odd>;
     using Other = std::integral_constant<int, 1 - odd>;
     constexpr int kCopies = S::kLoads + (odd ? 0 : S::kScaleLoads);
-    // (the multiples of the row size in the copies' offsets are made where they are used: kept,
-    // they would take more scalar registers than there are)
-    int row_bytes = code_row;
-    asm volatile("" : "+s"(row_bytes));
     // of `count` things dealt over the instructions from .. from + len - 1, those out behind k
     constexpr auto dealt = [](int k, int from, int len, int count) {
       const int n = k < from ? 0 : (k - from + 1) * count / len;
       return n < count ? n : count;
     };
-    constexpr auto copied = [dealt](int k) {
-      return dealt(k, kRelease + 1, 2 * kMma - kRelease - 1, kCopies);
-    };
+    // copies aimed up to instruction k, and issued: an instruction later where there is room
+    constexpr int kFrom = kRelease + 1, kLen = 2 * kMma - kFrom - 1;
+    constexpr bool kApart = 2 * kCopies <= kLen;
+    constexpr auto aimed = [dealt](int k) { return dealt(k, kFrom, kLen, kCopies); };
+    constexpr auto copied = [aimed](int k) { return aimed(kApart ? k - 1 : k); };
+    uint32_t m0 = 0;
     auto issue = [&](auto kc) {
       constexpr int k = decltype(kc)::value;
-      unroll<copied(k - 1), copied(k)>([&](auto c) {
-        constexpr int i = decltype(c)::value;
-        if constexpr (i < S::kLoads) copy(c, Odd{}, st, row_bytes);
-        else copy_scales(i - S::kLoads, st >> 1, sbuf);
-      });
+      if constexpr (kApart) {
+        unroll<copied(k - 1), copied(k)>([&](auto c) { copy(c, m0); });
+        unroll<aimed(k - 1), aimed(k)>([&](auto c) { m0 = aim_copy(c, Odd{}, sbuf); });
+      } else {
+        unroll<copied(k - 1), copied(k)>([&](auto c) { copy_now(c, Odd{}, sbuf); });
+      }
     };
     bound(st);
     unroll<0, kMma>([&](auto kc) {
@@ -673,11 +691,10 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   int sbuf = 0;                                       // buffer of the current group's scales
   aim(at);
   bound(0);
-#pragma unroll
-  for (int i = 0; i < S::kScaleLoads; ++i) copy_scales(i, 0, 0);
-  unroll<0, S::kLoads>([&](auto i) { copy(i, C0{}, 0, code_row); });
+  unroll<S::kLoads, S::kLoads + S::kScaleLoads>([&](auto i) { copy_now(i, C0{}, 0); });
+  unroll<0, S::kLoads>([&](auto i) { copy_now(i, C0{}, 0); });
   bound(1);
-  unroll<0, S::kLoads>([&](auto i) { copy(i, C1{}, 1, code_row); });
+  unroll<0, S::kLoads>([&](auto i) { copy_now(i, C1{}, 0); });
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
   __builtin_amdgcn_s_barrier();
   unroll<0, FW + TW>([&](auto j) { read(j, C0{}, C0{}); });
