@@ -509,39 +509,43 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
                  :: "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(offset), "s"(rsrc)
                  : "memory", "m0");
   };
-  // Copies 0 .. kLoads - 1 are the next stage's, into buffer `par`; those behind them the next
-  // group's scales, into theirs.
+  // Copies 0 .. kScaleLoads - 1 are the next group's scales, into buffer `buf`; those behind them
+  // the next stage, into buffer `par`.
   auto aim_copy = [&](auto ic, auto par, int buf) {
-    constexpr int i = decltype(ic)::value;
-    if constexpr (i < S::kLoadsW) {
-      c_off[i] += 128;
-      return dma_to(lds0 + decltype(par)::value * S::kStageBytes + (wave * S::kLoadsW + i) * 1024);
-    } else if constexpr (i < S::kLoads) {
-      c_off[i] += 128;
-      return dma_to(lds0 + decltype(par)::value * S::kStageBytes + TN * 128 +
-                    (wave * S::kLoadsX + i - S::kLoadsW) * 1024);
-    } else {
-      s_off[i - S::kLoads] += 16;
+    constexpr int i = decltype(ic)::value, c = i - S::kScaleLoads;
+    const uint32_t stage_at = lds0 + decltype(par)::value * S::kStageBytes;
+    if constexpr (c < 0) {
+      s_off[i] += 16;
       return dma_to(lds0 + 2 * S::kStageBytes + buf * S::kScaleBytes +
-                    (wave * S::kScaleLoads + i - S::kLoads) * 1024);
+                    (wave * S::kScaleLoads + i) * 1024);
+    } else if constexpr (c < S::kLoadsW) {
+      c_off[c] += 128;
+      return dma_to(stage_at + (wave * S::kLoadsW + c) * 1024);
+    } else {
+      c_off[c] += 128;
+      return dma_to(stage_at + TN * 128 + (wave * S::kLoadsX + c - S::kLoadsW) * 1024);
     }
   };
   auto copy = [&](auto ic, uint32_t m0) {
-    constexpr int i = decltype(ic)::value;
-    if constexpr (i < S::kLoadsW) dma(m0, c_off[i], w_rsrc);
-    else if constexpr (i < S::kLoads) dma(m0, c_off[i], x_rsrc);
-    else dma(m0, s_off[i - S::kLoads], s_rsrc[i - S::kLoads]);
+    constexpr int i = decltype(ic)::value, c = i - S::kScaleLoads;
+    if constexpr (c < 0) dma(m0, s_off[i], s_rsrc[i]);
+    else dma(m0, c_off[c], c < S::kLoadsW ? w_rsrc : x_rsrc);
   };
   auto copy_now = [&](auto ic, auto par, int buf) {
     const uint32_t m0 = aim_copy(ic, par, buf);
     asm volatile("s_nop 0");                           // between the write of m0 and the load
     copy(ic, m0);
   };
-  // Before the copies of stage `st`: past the end of K nothing is read any more.  (In a last stage
-  // of one step the packs of the other come from the next row; their scales are 2^-127 on both
-  // sides, which leaves zero.)
+  constexpr int kFirst = S::kScaleLoads, kCopiesAll = S::kScaleLoads + S::kLoads;
+  // Before the copies of stage `st`: past the end of K nothing is read any more, and of a last
+  // stage of one step only the first four packs of a row.
   auto bound = [&](int st) {
     const bool past = st >= stages;
+    if (st * 2 + 1 == steps) {
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i)
+        c_off[i] = pack_of(lane, i & 1) >= 4 ? kDmaOutOfRange : c_off[i];
+    }
     w_rsrc[2] = past ? 0 : w_rsrc[2];
     x_rsrc[2] = past ? 0 : x_rsrc[2];
 #pragma unroll
@@ -617,7 +621,7 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
     constexpr int odd = decltype(odd_c)::value;
     using Odd = std::integral_constant<int, odd>;
     using Other = std::integral_constant<int, 1 - odd>;
-    constexpr int kCopies = S::kLoads + (odd ? 0 : S::kScaleLoads);
+    constexpr int kSkip = odd ? kFirst : 0, kCopies = kCopiesAll - kSkip;
     // of `count` things dealt over the instructions from .. from + len - 1, those out behind k
     constexpr auto dealt = [](int k, int from, int len, int count) {
       const int n = k < from ? 0 : (k - from + 1) * count / len;
@@ -632,11 +636,19 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
     auto issue = [&](auto kc) {
       constexpr int k = decltype(kc)::value;
       if constexpr (kApart) {
-        unroll<copied(k - 1), copied(k)>([&](auto c) { copy(c, m0); });
-        unroll<aimed(k - 1), aimed(k)>([&](auto c) { m0 = aim_copy(c, Odd{}, sbuf); });
+        unroll<kSkip + copied(k - 1), kSkip + copied(k)>([&](auto c) { copy(c, m0); });
+        unroll<kSkip + aimed(k - 1), kSkip + aimed(k)>(
+            [&](auto c) { m0 = aim_copy(c, Odd{}, sbuf); });
       } else {
-        unroll<copied(k - 1), copied(k)>([&](auto c) { copy_now(c, Odd{}, sbuf); });
+        unroll<kSkip + copied(k - 1), kSkip + copied(k)>(
+            [&](auto c) { copy_now(c, Odd{}, sbuf); });
       }
+    };
+    auto scale_reads = [&](auto kc) {
+      constexpr int k = decltype(kc)::value, from = kRelease + 1, len = kPublish - kRelease;
+      if constexpr (odd)
+        unroll<dealt(k - 1, from, len, kReads + kLag), dealt(k, from, len, kReads + kLag)>(
+            [&](auto j) { read_scale(j, st >> 1, sbuf); });
     };
     bound(st);
     unroll<0, kMma>([&](auto kc) {
@@ -646,8 +658,11 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
           [&](auto j) { read(j, C1{}, Odd{}); });
       if constexpr (k == kRelease) {
         __builtin_amdgcn_s_waitcnt(0xc07f);           // lgkmcnt(0): my reads of this stage are done
+        // the next group's scales have landed; behind them the last stage's copies were issued
+        if constexpr (odd) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
         __builtin_amdgcn_s_barrier();
       }
+      scale_reads(kc);
       issue(kc);
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -663,13 +678,10 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
         else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(own) : "memory");
         __builtin_amdgcn_s_barrier();
       }
-      constexpr int r0 = kPublish + 1, r1 = r0 + kWindow / 2;
+      constexpr int r0 = kPublish + 1;
       unroll<dealt(k - 1, r0, kWindow, kReads), dealt(k, r0, kWindow, kReads)>(
           [&](auto j) { read(j, C0{}, Other{}); });
-      constexpr int len = kWindow * 5 / 4 < 2 * kMma - r1 ? kWindow * 5 / 4 : 2 * kMma - r1;
-      if constexpr (odd)
-        unroll<dealt(k - 1, r1, len, kReads + kLag), dealt(k, r1, len, kReads + kLag)>(
-            [&](auto j) { read_scale(j, st >> 1, sbuf); });
+      scale_reads(kc);
       issue(kc);
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -691,10 +703,9 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   int sbuf = 0;                                       // buffer of the current group's scales
   aim(at);
   bound(0);
-  unroll<S::kLoads, S::kLoads + S::kScaleLoads>([&](auto i) { copy_now(i, C0{}, 0); });
-  unroll<0, S::kLoads>([&](auto i) { copy_now(i, C0{}, 0); });
+  unroll<0, kCopiesAll>([&](auto i) { copy_now(i, C0{}, 0); });
   bound(1);
-  unroll<0, S::kLoads>([&](auto i) { copy_now(i, C1{}, 0); });
+  unroll<kFirst, kCopiesAll>([&](auto i) { copy_now(i, C1{}, 0); });
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
   __builtin_amdgcn_s_barrier();
   unroll<0, FW + TW>([&](auto j) { read(j, C0{}, C0{}); });
