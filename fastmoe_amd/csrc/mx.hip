@@ -7,6 +7,9 @@
 // and the codes come from the conversion instruction that divides by the power of two itself.
 // The form for tokens writes a row to its top_k places in expert order, which makes the
 // dispatch of a 4-bit layer part of this pass: 4.25 bits written per value and place.
+// With many rows a wave takes four chunks of 512 values, so that codes are stored 16 bytes a lane.
+// Measured: 114688 x 4096 in bf16 to 4 bits and back in 446 us, 2.38 GB at 5.3 TB/s (a large copy
+// reaches 5.2); 1000 x 300 in f32 2.7 us either way, a launch alone 2.1.
 #include <algorithm>
 
 #include "mx.h"
