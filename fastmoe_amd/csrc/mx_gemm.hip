@@ -97,18 +97,38 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_bias_rows(const MxGemmArgs&
   const int64_t bytes = (int64_t)a.out_feat * (a.dtype == FMOE_F32 ? 4 : 2);
   return mx_resource((const char*)a.bias + e * bytes, a.bias ? bytes : 0);
 }
+// 8 values of the bias's 16-bit type.
+__device__ __forceinline__ void mx_widen(const MxGemmArgs& a, i32x4 u, float (&b)[8]) {
+  if (a.dtype == FMOE_BF16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      b[i] = __uint_as_float(i & 1 ? (uint32_t)u[i >> 1] & 0xffff0000u : (uint32_t)u[i >> 1] << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      b[i] = __half2float(__builtin_bit_cast(__half, (uint16_t)((uint32_t)u[i >> 1] >> (16 * (i & 1)))));
+  }
+}
 // The bias of 8 consecutive features from n0 on (zeros where there is none).
 __device__ __forceinline__ void mx_load_bias(const MxGemmArgs& a, __amdgpu_buffer_rsrc_t rows,
                                              int n0, float (&b)[8]) {
+  // (one test for all, or every load is waited for by itself)
+  if (a.bias == nullptr) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (a.dtype == FMOE_F32) {
+    for (int i = 0; i < 8; ++i) b[i] = 0.f;
+  } else if (a.dtype == FMOE_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
       b[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, (n0 + i) * 4, 0, 0));
-    } else {
-      const uint16_t u = __builtin_amdgcn_raw_buffer_load_b16(rows, (n0 + i) * 2, 0, 0);
-      b[i] = a.dtype == FMOE_BF16 ? __uint_as_float((uint32_t)u << 16)
-                                  : __half2float(__builtin_bit_cast(__half, u));
-    }
+  } else {
+    uint16_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      u[i] = __builtin_amdgcn_raw_buffer_load_b16(rows, (n0 + i) * 2, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      b[i] = a.dtype == FMOE_BF16 ? __uint_as_float((uint32_t)u[i] << 16)
+                                  : __half2float(__builtin_bit_cast(__half, u[i]));
   }
 }
 
@@ -138,7 +158,7 @@ template <typename T, int MODE> struct MxOutput {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (MODE == kMxQuantGelu) v[i] = mx_gelu(v[i]);
-      if (MODE == kMxQuantRelu) v[i] = v[i] < 0.f ? 0.f : v[i];     // (a NaN stays)
+      if (MODE == kMxQuantRelu) v[i] = __builtin_elementwise_maximum(v[i], 0.f);   // (a NaN stays)
     }
   }
 
@@ -563,6 +583,11 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
 #pragma unroll
     for (int i = 0; i < S::kScaleLoads; ++i) s_rsrc[i][2] = past ? 0 : s_rsrc[i][2];
   };
+  // the bias comes by LDS where it is words throughout; it has x's type, which is y's
+  constexpr int kBiasCopies = 2;                     // (16-bit types need only the first)
+  const bool wide = mx_quantises(MODE) ? a.dtype == FMOE_F32 : std::is_same<T, float>::value;
+  const bool bias_by_lds = a.bias != nullptr &&
+                           (wide || (a.out_feat % 2 == 0 && (uintptr_t)a.bias % 4 == 0));
   const int m = lane & 15, g = lane >> 4, wn = wave >> 1, wm = wave & 1;
   const int frag0 = m * 128 + (g ^ ((m >> 1) & 7)) * 16;      // step 0; step 1 has packs 4..7
   const char* const w_lds = lds + wn * (TN / 2) * 128;
@@ -682,11 +707,15 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
       constexpr int k = decltype(kc)::value, i = (k - kMma) / FW, f = (k - kMma) % FW;
       mx_mfma_at<2 * odd + 1>(wf[1][f], wsc[f], xf[1][i], xsc[i], acc[i][f]);
       if constexpr (k == kPublish) {
-        // everything but this stage's own copies has landed; the last tile's results, which lie
-        // between a tile's second stage and its third, may still be on their way
-        constexpr int own = copied(kPublish - 1), sent = own + kSent < 63 ? own + kSent : 63;
+        // everything but this stage's own copies has landed; the last tile's results and the bias,
+        // which lie between a tile's second stage and its third, may still be on their way
+        constexpr int own = copied(kPublish - 1), most = 63;
+        constexpr int sent = own + kSent < most ? own + kSent : most;
+        constexpr int sent_bias = own + kSent + kBiasCopies < most ? own + kSent + kBiasCopies : most;
         static_assert(own < 64, "vmcnt is a 6-bit counter");
-        if (!odd && first) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(sent) : "memory");
+        if (!odd && first && bias_by_lds && kSent > 0)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(sent_bias) : "memory");
+        else if (!odd && first) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(sent) : "memory");
         else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(own) : "memory");
         __builtin_amdgcn_s_barrier();
       }
@@ -701,10 +730,6 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   };
 
   char* const stage = lds + 2 * (S::kStageBytes + S::kScaleBytes) + wave * (16 * S::kOutRow);
-  // by LDS where it is words throughout
-  const bool wide = a.dtype == FMOE_F32;
-  const bool bias_by_lds = a.bias != nullptr &&
-                           (wide || (a.out_feat % 2 == 0 && (uintptr_t)a.bias % 4 == 0));
   // (the last group's missing steps, if any, multiply zeros)
   const int groups = (steps + 3) >> 2;
   int pid = blockIdx.x;
@@ -731,7 +756,7 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
       const uint32_t dst = lds0 + (uint32_t)(stage - lds);
       const uint32_t off = (uint32_t)((at.base + wn * (TN / 2)) * (wide ? 4 : 2) + lane * 4);
       dma4(dst, off, rsrc);
-      if (wide) dma4(dst + 256, off + 256, rsrc);
+      dma4(dst + 256, off + 256, rsrc);
     }
 #pragma unroll
     for (int i = 0; i < TW; ++i)
@@ -770,12 +795,7 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
           for (int i = 0; i < 8; ++i) b[p][i] = *(const float*)(at_g + p * 128 + i * 4);
         } else {
           const i32x4 u = *(const i32x4*)(at_g + p * 64);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t bits = ((uint32_t)u[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-            b[p][i] = a.dtype == FMOE_BF16 ? __uint_as_float(bits << 16)
-                                           : __half2float(__builtin_bit_cast(__half, (uint16_t)bits));
-          }
+          mx_widen(a, u, b[p]);
         }
       }
     } else {

@@ -323,6 +323,33 @@ def test_every_tile_shape_comes_out_quantised(k, n, counts):
         assert not tail.any()
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("case", BY_RULE)
+def test_no_bias_is_a_bias_of_zeros(case, dt):
+    from fastmoe_amd import fmoe_cuda, mx
+
+    counts, k, n = BY_RULE[case]
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(sum(counts), k, device="cuda", generator=g).to(DTYPES[dt])
+    wq = mx.quantize(torch.randn(len(counts), n, k, device="cuda", generator=g))
+    zeros = torch.zeros(len(counts), n, device="cuda", dtype=DTYPES[dt])
+    # (one value further on: rows of the bias that start inside a word)
+    inside = torch.zeros(len(counts) * n + 1, device="cuda", dtype=DTYPES[dt])[1:].view(zeros.shape)
+    y = mx.linear(x, torch.tensor(counts), wq)
+    assert torch.equal(y, mx.linear(x, torch.tensor(counts), wq, zeros))
+    assert torch.equal(y, mx.linear(x, torch.tensor(counts), wq, inside))
+    xq = mx.quantize(x)
+    seg = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32).cuda()
+    for act in (0, 1, 2):
+        run = lambda b: fmoe_cuda.mx_linear_act_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k,
+                                                    b, seg, act)
+        blocks = -(-n // 128) * 4                     # (scales further on are not written)
+        (c0, s0), (c1, s1), (c2, s2) = run(None), run(zeros), run(inside)
+        assert torch.equal(c0, c1) and torch.equal(c0, c2)
+        assert torch.equal(s0[:, :blocks], s1[:, :blocks])
+        assert torch.equal(s0[:, :blocks], s2[:, :blocks])
+
+
 def test_counts_that_do_not_fit_are_cut_off():
     """On the device nobody looks at them: negative counts are none, rows there are not are left."""
     from fastmoe_amd import mx
