@@ -57,23 +57,28 @@ __device__ __forceinline__ i32x4 mx_descriptor(const void* p, int64_t bytes) {
 }
 
 // gelu(x) = x Phi(x) with Phi(x) = 1 / (1 + 2^z), z = -log2(Phi(x) / Phi(-x)) = x P(x^2) for
-// |x| <= 6 and x P(36) outside: P of degree 9, a reweighted least-squares fit on Chebyshev nodes.
-// Within 0.8e-6 of gelu everywhere and, for |x| <= 6, within 2.6e-5 of its value, so that blocks
-// whose values all lie in the negative tail keep their digits as well.  22 issue slots where erff
-// takes about 60, with branches, and loses the tail: with one wave on a SIMD nothing hides them
-// (a 256 x 256 tile of 4096 features: 27 us of matrix instructions, 26 us of erff).
+// |x| <= 6 and x P(36) outside: P of degree 12 in x^2 / 18 - 1, a reweighted least-squares fit on
+// Chebyshev nodes.  Within 1.4e-7 + 1e-7 |gelu| of gelu everywhere, so that hardly more codes than
+// the sums' own rounding makes land on the other side of a boundary (degree 9, three instructions
+// less, was off by 7e-7), and, for |x| <= 6, within 3.4e-6 of its value, so that blocks whose values
+// all lie in the negative tail keep their digits as well.  26 issue slots where erff takes about
+// 60, with branches, and loses the tail: with one wave on a SIMD nothing hides them (a 256 x 256
+// tile of 4096 features: 27 us of matrix instructions, 26 us of erff).
 __device__ __forceinline__ float mx_gelu(float x) {
-  const float u = fminf(x * x, 36.f);
-  float p = 2.19136148e-14f;
-  p = fmaf(p, u, -4.54144361e-12f);
-  p = fmaf(p, u, 4.11870843e-10f);
-  p = fmaf(p, u, -2.14399911e-08f);
-  p = fmaf(p, u, 7.0298131e-07f);
-  p = fmaf(p, u, -1.47544906e-05f);
-  p = fmaf(p, u, 0.000177562615f);
-  p = fmaf(p, u, 4.6205645e-05f);
-  p = fmaf(p, u, -0.104784109f);
-  p = fmaf(p, u, -2.30222034f);
+  const float t = fminf(fmaf(x * x, 1.f / 18.f, -1.f), 1.f);
+  float p = 0.00220932276f;
+  p = fmaf(p, t, -0.00235819351f);
+  p = fmaf(p, t, -0.00623256993f);
+  p = fmaf(p, t, 0.0106137199f);
+  p = fmaf(p, t, -0.00437692506f);
+  p = fmaf(p, t, 0.0022452944f);
+  p = fmaf(p, t, -0.00346183078f);
+  p = fmaf(p, t, -0.00412944285f);
+  p = fmaf(p, t, 0.0250278097f);
+  p = fmaf(p, t, -0.0735082775f);
+  p = fmaf(p, t, 0.223777682f);
+  p = fmaf(p, t, -1.27482498f);
+  p = fmaf(p, t, -3.8811202f);
   // (2^z overflows to infinity far down, its inverse is 0 there)
   return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * p));
 }
