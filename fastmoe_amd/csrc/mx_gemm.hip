@@ -400,8 +400,8 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
 // into pieces of 256 bytes of a row (stored from the registers, 64 bytes of each of 16 rows at a
 // time, they took 16 us a tile instead of 9).
 //
-// Measured: 32768 rows of 8 experts, 16384 -> 4096, 926 us, 4.75 PFLOP/s; 4096 -> 14336 965 us,
-// 3.99.  A loop of these matrix instructions alone reaches 7.3 on random codes (9.7 on zeros: the
+// Measured: 32768 rows of 8 experts, 16384 -> 4096, 926 us, 4.75 PFLOP/s; 4096 -> 14336 938 us,
+// 4.10.  A loop of these matrix instructions alone reaches 7.3 on random codes (9.7 on zeros: the
 // card's power limit sets the clock).  Of the first shape's 1.68 M cycles at 1.9 GHz the matrix
 // pipes are busy for 1.05; without copies it takes 1.45 M, without fragment reads as many as with
 // them.  128 x 128 tiles on 15560 rows of 128 experts, 2048 -> 1408: 61 us, 257 MB at 4.2 TB/s.
