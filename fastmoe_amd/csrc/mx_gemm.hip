@@ -471,7 +471,7 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
   constexpr int FW = TN / 32, TW = TM / 32;         // fragments of a wave
   constexpr int kMma = FW * TW;
   extern __shared__ __align__(16) char lds[];
-  // (the first wave's corner, behind the bias)
+  // (the first wave's corner, behind the bias; results on their way out may pass over it)
   int* const s_find = (int*)(lds + 2 * (S::kStageBytes + S::kScaleBytes) + 1024);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   RowTiles<TM, kOneHeight, 4> tiles;
@@ -825,6 +825,10 @@ __global__ __launch_bounds__(256, (MxTile<TN, TM>::kGroups)) void mx_tile_kernel
     first = true;
     // (the corner is read out before the next bias lands there)
     __builtin_amdgcn_s_waitcnt(0xc07f);
+    // With more experts than lanes, place() writes to the first wave's corner from another one.  A
+    // tile of one group calls it before the K loop's first barrier, so it waits here until the
+    // first wave's results have left.
+    if (groups == 1 && !tiles.by_lane) __syncthreads();
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS after the end
 }

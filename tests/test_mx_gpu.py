@@ -323,6 +323,43 @@ def test_every_tile_shape_comes_out_quantised(k, n, counts):
         assert not tail.any()
 
 
+# More experts than lanes, where the owner of a row tile is looked up through LDS, K of one group
+# of scales, and several tiles per workgroup: the next tile is looked up while the last one's
+# results pass through the same LDS.
+@pytest.mark.parametrize("dt", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("counts", [[60, 0, 200, 1] * 32, [30, 0, 65, 17] * 32],
+                         ids=["tiles of 128 rows", "tiles of 64 rows"])
+@pytest.mark.parametrize("k,n", [(96, 1504), (512, 1504), (512, 1499), (300, 3001)])
+def test_short_rows_of_many_experts(dt, counts, k, n):
+    from fastmoe_amd import fmoe_cuda, mx
+
+    g = torch.Generator(device="cuda").manual_seed(k + n)
+    draw = lambda *shape: torch.randn(*shape, device="cuda", generator=g)
+    x, b = draw(sum(counts), k).to(DTYPES[dt]), draw(len(counts), n).to(DTYPES[dt])
+    wq, xq = mx.quantize(draw(len(counts), n, k) * 0.05), mx.quantize(x)
+    y = mx.linear(x, torch.tensor(counts), wq, b)
+    xv, at = xq.dequantize(torch.float32).double(), 0
+    for e, c in enumerate(counts):
+        rows = xv[at:at + c]
+        we = mx.MXTensor(wq.codes[e], wq.scales[e], k).dequantize(torch.float32).double()
+        want = rows @ we.T + b[e].double()
+        mag = rows.abs() @ we.abs().T + b[e].double().abs()
+        # as above: the instructions' sums and the bias in f32, then the output's rounding
+        tol = UNIT[dt] * want.abs() + 2.0 ** -23 * (k / 128 + 4) * mag
+        assert ((y[at:at + c].double() - want).abs() <= tol).all(), e
+        at += c
+    for _ in range(5):
+        assert torch.equal(mx.linear(x, torch.tensor(counts), wq, b), y)
+    seg = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32).cuda()
+    y32 = fmoe_cuda.mx_linear_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k, b.float(), seg,
+                                  torch.empty(sum(counts), n, device="cuda"))
+    for act, h in ((0, y32), (2, y32.relu())):
+        codes, scales = fmoe_cuda.mx_linear_act_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k,
+                                                    b, seg, act)
+        assert torch.equal(mx.MXTensor(codes, scales, n).dequantize(torch.float32),
+                           mx.quantize(h).dequantize(torch.float32))
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32", "f16"])
 @pytest.mark.parametrize("case", BY_RULE)
 def test_no_bias_is_a_bias_of_zeros(case, dt):
