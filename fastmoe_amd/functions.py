@@ -135,14 +135,17 @@ class SegmentTable:
 
 
 class RoutePlan:
-    """Everything the dispatch needs about one routing decision."""
+    """Everything the dispatch needs about one routing decision; `routed` is what
+    fmoe_cuda.route made of it, where that is at hand."""
 
-    def __init__(self, gate: torch.Tensor, num_expert: int):
+    def __init__(self, gate: torch.Tensor, num_expert: int, routed=None):
         self.top_k = gate.shape[-1] if gate.dim() >= 2 else 1
         self.n_slots = gate.numel()
         self.n_tokens = self.n_slots // max(self.top_k, 1)
-        with torch.no_grad():
-            pos, counts, seg_off, inv = fmoe_cuda.route(gate.contiguous(), num_expert)
+        if routed is None:
+            with torch.no_grad():
+                routed = fmoe_cuda.route(gate.contiguous(), num_expert)
+        pos, counts, seg_off, inv = routed
         self.pos = pos
         self.inv = inv
         self.segments = SegmentTable(seg_off, counts)

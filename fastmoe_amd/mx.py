@@ -52,12 +52,7 @@ class MXTensor:
         if native is not None:
             return native.mx_dequantize_rows(self.codes.contiguous(), self.scales.contiguous(),
                                              self.features, dtype)
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        if out.numel():
-            fmoe_cuda.mx_dequantize(
-                self.codes.reshape(-1, self.codes.shape[-1]).contiguous(),
-                self.scales.reshape(-1, self.scales.shape[-1]).contiguous(), out.view(-1, self.features))
-        return out
+        return _Dequantize.apply(self.codes, self.scales, self.features, dtype)
 
     @classmethod
     def from_blocks(cls, codes: torch.Tensor, scales: torch.Tensor) -> "MXTensor":
@@ -72,6 +67,41 @@ class MXTensor:
                    pad(scales, (0, -(-k // 512) * 16 - scales.shape[-1])), k)
 
 
+# Where the extension's own nodes do not apply (fmoe_cuda.native()), somebody may be looking at
+# torch operations: tracing records these functions where an operator called directly would leave
+# the example's results behind as constants, and forward-mode differentiation is refused by them
+# where such an operator would drop the tangents.
+class _Quantize(Function):
+    @staticmethod
+    def forward(ctx, x):
+        k = x.shape[-1]
+        codes, scales = fmoe_cuda.mx_quantize(x.reshape(-1, k).contiguous())
+        codes = codes.view(*x.shape[:-1], codes.shape[-1])
+        scales = scales.view(*x.shape[:-1], scales.shape[-1])
+        ctx.mark_non_differentiable(codes, scales)
+        return codes, scales
+
+    @staticmethod
+    def backward(ctx, *_grads):
+        return None
+
+
+class _Dequantize(Function):
+    @staticmethod
+    def forward(ctx, codes, scales, features, dtype):
+        out = torch.empty((*codes.shape[:-1], features), dtype=dtype, device=codes.device)
+        if out.numel():
+            fmoe_cuda.mx_dequantize(codes.reshape(-1, codes.shape[-1]).contiguous(),
+                                    scales.reshape(-1, scales.shape[-1]).contiguous(),
+                                    out.view(-1, features))
+        ctx.mark_non_differentiable(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, _grad):
+        return None, None, None, None
+
+
 def quantize(x: torch.Tensor) -> MXTensor:
     r"""x [..., features] (float32, float16 or bfloat16, on the GPU) in MXFP4.  The scale of a
     block is 2^(floor(log2(max |x|)) - 2); values are rounded to nearest, ties to the even
@@ -80,10 +110,7 @@ def quantize(x: torch.Tensor) -> MXTensor:
     native = fmoe_cuda.native()
     if native is not None:
         return MXTensor(*native.mx_quantize_rows(x), k)
-    x = x.detach()
-    codes, scales = fmoe_cuda.mx_quantize(x.reshape(-1, k).contiguous())
-    return MXTensor(codes.view(*x.shape[:-1], codes.shape[-1]),
-                    scales.view(*x.shape[:-1], scales.shape[-1]), k)
+    return MXTensor(*_Quantize.apply(x.detach()), k)
 
 
 class MXLinear(Function):
@@ -91,12 +118,21 @@ class MXLinear(Function):
     rows is that of the weights' values, straight through the rounding of the rows."""
 
     @staticmethod
-    def forward(ctx, x, seg_off, w_codes, w_scales, bias):
+    def forward(ctx, x, counts, w_codes, w_scales, bias):
+        r"""`counts`: a SegmentTable, int64 counts on the host or on the device, or the segment
+        bounds themselves (int32 on the device)."""
         in_feat = x.shape[1]
-        if seg_off.dtype == torch.int64:      # counts on the device
-            codes, scales, seg_off = fmoe_cuda.mx_quantize_counted(x.contiguous(), seg_off)
+        x = x.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        on_device = isinstance(counts, torch.Tensor) and counts.is_cuda
+        if on_device and counts.dtype == torch.int64:
+            codes, scales, seg_off = fmoe_cuda.mx_quantize_counted(x, counts.contiguous())
         else:
-            codes, scales = fmoe_cuda.mx_quantize(x.contiguous())
+            if isinstance(counts, torch.Tensor) and not on_device and (
+                    bool((counts < 0).any()) or int(counts.sum()) > x.shape[0]):
+                raise RuntimeError("expert counts are negative or claim more rows than x holds")
+            seg_off = counts.contiguous() if on_device else _segments(counts, x.device)
+            codes, scales = fmoe_cuda.mx_quantize(x)
         out = torch.empty((x.shape[0], w_codes.shape[1]), dtype=x.dtype, device=x.device)
         fmoe_cuda.mx_linear_fwd(codes, scales, w_codes, w_scales, in_feat, bias, seg_off, out)
         ctx.in_feat = in_feat
@@ -125,13 +161,69 @@ def linear(x: torch.Tensor, fwd_expert_count, weight: MXTensor, bias=None) -> to
         return native.mx_linear(x, segments, weight.codes, weight.scales, weight.features, bias)
     if x.dim() != 2 or x.shape[1] != weight.features or not x.is_cuda:
         raise RuntimeError(f"x must be a CUDA tensor [rows, {weight.features}]")
-    if isinstance(fwd_expert_count, torch.Tensor) and not fwd_expert_count.is_cuda and (
-            bool((fwd_expert_count < 0).any()) or int(fwd_expert_count.sum()) > x.shape[0]):
-        raise RuntimeError("expert counts are negative or claim more rows than x holds")
-    if not isinstance(fwd_expert_count, torch.Tensor) or not fwd_expert_count.is_cuda:
-        fwd_expert_count = _segments(fwd_expert_count, x.device)
-    return MXLinear.apply(x, fwd_expert_count.contiguous(), weight.codes, weight.scales,
-                          None if bias is None else bias.contiguous())
+    return MXLinear.apply(x, fwd_expert_count, weight.codes, weight.scales, bias)
+
+
+class _Route(Function):
+    r"""fmoe_cuda.route as an operation that tracing records."""
+
+    @staticmethod
+    def forward(ctx, gate_idx, n_expert):
+        routed = fmoe_cuda.route(gate_idx.contiguous(), n_expert)
+        ctx.mark_non_differentiable(*routed)
+        return tuple(routed)
+
+    @staticmethod
+    def backward(ctx, *_grads):
+        return None, None
+
+
+class _Scatter(Function):
+    r"""FusedScatter on the tensors of its plan, for tracing (a plan would be a constant)."""
+
+    @staticmethod
+    def forward(ctx, x, gate_idx, n_expert, *routed):
+        return FusedScatter.forward(ctx, x, RoutePlan(gate_idx, n_expert, routed))
+
+    @staticmethod
+    def backward(ctx, grad_buf):
+        return (FusedScatter.backward(ctx, grad_buf)[0],) + (None,) * 6
+
+
+class _Combine(Function):
+    r"""FusedGatherCombine on the tensors of its plan, for tracing."""
+
+    @staticmethod
+    def forward(ctx, buf, score, gate_idx, n_expert, *routed):
+        return FusedGatherCombine.forward(ctx, buf, score, RoutePlan(gate_idx, n_expert, routed))
+
+    @staticmethod
+    def backward(ctx, grad_y):
+        return FusedGatherCombine.backward(ctx, grad_y)[:2] + (None,) * 6
+
+
+class MXExpertLayer(Function):
+    r"""The layer without gradients (see expert_layer) operator by operator."""
+
+    @staticmethod
+    def forward(ctx, x, gate_idx, score, w1_codes, w1_scales, in_feat, b1, w2_codes, w2_scales,
+                hidden, b2, act):
+        n_tokens, top_k = gate_idx.shape
+        x = x.contiguous()
+        _pos, _counts, seg_off, inv = fmoe_cuda.route(gate_idx.contiguous(), w1_codes.shape[0])
+        codes, scales = fmoe_cuda.mx_quantize_tokens(x, inv, top_k)
+        codes, scales = fmoe_cuda.mx_linear_act_fwd(
+            codes, scales, w1_codes, w1_scales, in_feat, None if b1 is None else b1.contiguous(),
+            seg_off, act)
+        out = torch.empty((n_tokens * top_k, w2_codes.shape[1]), dtype=x.dtype, device=x.device)
+        fmoe_cuda.mx_linear_fwd(codes, scales, w2_codes, w2_scales, hidden,
+                                None if b2 is None else b2.contiguous(), seg_off, out)
+        score = score.reshape(n_tokens, top_k).contiguous().to(x.dtype)
+        return fmoe_cuda.gather_combine_fwd(out, inv, score, n_tokens, top_k)
+
+    @staticmethod
+    def backward(ctx, _grad):
+        raise RuntimeError("mx.expert_layer was called (or traced) without gradients")
 
 
 def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w1: MXTensor, b1,
@@ -149,27 +241,26 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
     act = native_act(activation, x)
     grads = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, score, b1, b2))
+    gate_idx = gate_idx.reshape(-1, top_k)
     if grads or not act or x.dtype == torch.float64:
-        plan = RoutePlan(gate_idx.reshape(-1, top_k), n_expert)
-        h = linear(FusedScatter.apply(x, plan), plan.segments, w1, b1)
-        h = apply_activation(activation, h, plan.n_rows_dev)
-        y = linear(h, plan.segments, w2, b2)
-        return FusedGatherCombine.apply(y, score.reshape(-1, top_k), plan)
+        score = score.reshape(-1, top_k)
+        if torch._C._get_tracing_state() is not None:
+            routed = _Route.apply(gate_idx, n_expert)
+            segments, live = routed[2], routed[2][-1:]
+            h = _Scatter.apply(x, gate_idx, n_expert, *routed)
+        else:
+            plan = RoutePlan(gate_idx, n_expert)
+            segments, live = plan.segments, plan.n_rows_dev
+            h = FusedScatter.apply(x, plan)
+        h = apply_activation(activation, linear(h, segments, w1, b1), live)
+        y = linear(h, segments, w2, b2)
+        if torch._C._get_tracing_state() is not None:
+            return _Combine.apply(y, score, gate_idx, n_expert, *routed)
+        return FusedGatherCombine.apply(y, score, plan)
     native = fmoe_cuda.native()
-    if native is not None:
-        return native.mx_expert_layer(x, gate_idx.reshape(-1, top_k), score, w1.codes, w1.scales,
-                                      w1.features, b1, w2.codes, w2.scales, w2.features, b2, act)
-    x = x.contiguous()
-    n_tokens = x.shape[0]
-    _pos, _counts, seg_off, inv = fmoe_cuda.route(gate_idx.reshape(-1, top_k).contiguous(),
-                                                  n_expert)
-    codes, scales = fmoe_cuda.mx_quantize_tokens(x, inv, top_k)
-    codes, scales = fmoe_cuda.mx_linear_act_fwd(codes, scales, w1.codes, w1.scales, w1.features,
-                                                b1, seg_off, act)
-    out = torch.empty((n_tokens * top_k, w2.codes.shape[1]), dtype=x.dtype, device=x.device)
-    fmoe_cuda.mx_linear_fwd(codes, scales, w2.codes, w2.scales, w2.features, b2, seg_off, out)
-    score = score.reshape(n_tokens, top_k).contiguous().to(x.dtype)
-    return fmoe_cuda.gather_combine_fwd(out, inv, score, n_tokens, top_k)
+    run = MXExpertLayer.apply if native is None else native.mx_expert_layer
+    return run(x, gate_idx, score, w1.codes, w1.scales, w1.features, b1, w2.codes, w2.scales,
+               w2.features, b2, act)
 
 
 class MXExpert(nn.Module):

@@ -1,0 +1,123 @@
+"""4-bit experts on the GPU as user programs call them: traced, under forward-mode
+differentiation, with counts, dtypes and modules that differ from the plain ones."""
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import mx_reference as R
+from helpers import DTYPES, make_gate
+
+pytestmark = pytest.mark.gpu
+
+
+def _layer(n_expert=8, d_model=96, d_hidden=160, dtype=torch.bfloat16, **kwargs):
+    import fastmoe_amd as fm
+    from fastmoe_amd import mx
+
+    torch.manual_seed(3)
+    layer = fm.FMoETransformerMLP(num_expert=n_expert, d_model=d_model, d_hidden=d_hidden,
+                                  gate=fm.ScoreGate, **kwargs).to(dtype).cuda()
+    with torch.no_grad():
+        for p in (layer.experts.htoh4.bias, layer.experts.h4toh.bias):
+            p.normal_(0, 0.1)
+    return mx.quantize_experts(layer)
+
+
+# ------------------------------------------------------------------ tracing, forward mode
+@pytest.mark.parametrize("act", [torch.nn.GELU(), torch.nn.ReLU(), torch.nn.SiLU()])
+def test_traced_layer_follows_its_input(act):
+    layer = _layer(activation=act).eval()
+    rows = [torch.randn(n, 96, device="cuda").bfloat16() for n in (40, 40, 40)]
+    with torch.no_grad():
+        traced = torch.jit.trace(layer, rows[0], check_trace=False)
+        for x in rows:
+            assert torch.equal(traced(x), layer(x))
+        assert not torch.equal(layer(rows[1]), layer(rows[2]))
+    # and its gradients, traced with them
+    traced = torch.jit.trace(layer, rows[0].clone().requires_grad_(True), check_trace=False)
+    for x in rows:
+        grads = []
+        for run in (traced, layer):
+            a = x.clone().requires_grad_(True)
+            y = run(a)
+            y.float().square().sum().backward()
+            grads.append((y.detach(), a.grad))
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+        assert grads[0][1].any()
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+def test_traced_linear_and_quantisation_follow_their_inputs(where):
+    from fastmoe_amd import mx
+
+    w = mx.quantize(torch.randn(3, 48, 96, device="cuda"))
+    b = torch.randn(3, 48, device="cuda")
+    run = lambda x, counts: mx.linear(x, counts, w, b)
+    there_and_back = lambda x: mx.quantize(x).dequantize(torch.float32)
+    counts = [torch.tensor(c, device=where) for c in ([10, 0, 20], [0, 30, 0], [7, 11, 12])]
+    rows = [torch.randn(30, 96, device="cuda") for _ in counts]
+    with torch.no_grad():
+        traced = torch.jit.trace(run, (rows[0], counts[0]), check_trace=False)
+        back = torch.jit.trace(there_and_back, rows[0], check_trace=False)
+        for x, c in zip(rows, counts):
+            assert torch.equal(traced(x, c), run(x, c))
+            assert torch.equal(back(x), there_and_back(x))
+
+
+def test_forward_mode_differentiation_is_refused():
+    from fastmoe_amd import mx
+
+    layer = _layer().eval()
+    for p in layer.parameters():
+        p.requires_grad_(False)
+    ex = layer.experts
+    x = torch.randn(20, 96, device="cuda").bfloat16()
+    idx, score = layer.gate(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for act in (torch.nn.GELU(), torch.nn.SiLU()):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                mx.expert_layer(dual, idx, score, ex.w1, ex.b1, ex.w2, ex.b2, act)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            mx.expert_layer(x, idx, forward_ad.make_dual(score, torch.ones_like(score)), ex.w1,
+                            ex.b1, ex.w2, ex.b2, torch.nn.GELU())
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            mx.linear(dual, torch.tensor([20] + [0] * 7), ex.w1, ex.b1)
+        # codes carry no tangent, and nothing else is lost
+        q = mx.quantize(dual)
+        assert torch.equal(q.codes, mx.quantize(x).codes)
+        y = mx.expert_layer(x, idx, score, ex.w1, ex.b1, ex.w2, ex.b2, torch.nn.GELU())
+    with torch.no_grad():
+        assert torch.equal(y, layer(x))
+
+
+@pytest.mark.parametrize("act", [torch.nn.GELU(), torch.nn.ReLU(), torch.nn.SiLU()])
+def test_operator_by_operator_gives_the_same_bits(act):
+    """While somebody watches the single operators, the layer runs them one by one."""
+    from fastmoe_amd import fmoe_cuda
+
+    layer = _layer(activation=act).eval()
+    x = torch.randn(50, 96, device="cuda").bfloat16()
+
+    def both(fn):
+        a = fn()
+        names = []
+        fmoe_cuda.profile_hook = lambda name, *events: names.append(name)
+        try:
+            b = fn()
+        finally:
+            fmoe_cuda.profile_hook = None
+        assert "route" in names
+        return zip(a, b)
+
+    def train():
+        layer.zero_grad()
+        a = x.clone().requires_grad_(True)
+        y = layer(a)
+        y.float().square().sum().backward()
+        return [y.detach(), a.grad, layer.experts.b1.grad.clone(), layer.experts.b2.grad.clone()]
+
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in both(lambda: [layer(x)]))
+    assert all(torch.equal(a, b) for a, b in both(train))

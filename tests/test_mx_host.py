@@ -1,0 +1,107 @@
+"""4-bit experts, what needs no GPU: how the layer is called, not what its kernels compute.  The
+operators are opaque stand-ins that autograd and tracing cannot look into, like the real ones."""
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+E, D, H = 3, 32, 64
+
+
+def _weight(out, features, seed):
+    from fastmoe_amd import mx
+
+    rng = np.random.default_rng(seed)
+    return mx.MXTensor(
+        torch.from_numpy(rng.integers(0, 256, (E, out, -(-features // 128) * 64)).astype(np.uint8)),
+        torch.from_numpy(rng.integers(120, 130, (E, out, -(-features // 512) * 16)).astype(np.uint8)),
+        features)
+
+
+@pytest.fixture
+def operators(monkeypatch):
+    """Operators on the CPU whose results depend on their inputs; the list of their calls."""
+    from fastmoe_amd import fmoe_cuda
+
+    calls = []
+
+    def stand_in(name, fn):
+        def op(*args, **kwargs):
+            calls.append(name)
+            with torch.no_grad():
+                return fn(*args, **kwargs)
+        monkeypatch.setattr(fmoe_cuda, name, op)
+
+    def opaque(a):
+        return torch.from_numpy(a.detach().float().numpy().copy())
+
+    def route(gate, n_expert, want_inv=True):
+        g = gate.numpy().reshape(-1)
+        order = np.argsort(np.where(g < 0, n_expert, g), kind="stable")
+        live = int((g >= 0).sum())
+        inv = np.full(g.size, -1, dtype=np.int32)
+        inv[order[:live]] = np.arange(live)
+        counts = np.bincount(g[g >= 0], minlength=n_expert)
+        seg = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        return tuple(torch.from_numpy(a.copy()) for a in (order, counts, seg, inv))
+
+    def quantize_tokens(x, inv, top_k):
+        rows = torch.zeros(x.shape[0] * top_k, x.shape[1])
+        keep = inv >= 0
+        rows[inv[keep].long()] = opaque(x).repeat_interleave(top_k, 0)[keep]
+        return rows, torch.zeros(rows.shape[0], 16)
+
+    def linear_act(codes, scales, wc, ws, k, bias, seg, act):
+        return codes.mean(1, keepdim=True).repeat(1, wc.shape[1]), scales
+
+    def linear_fwd(codes, scales, wc, ws, k, bias, seg, out):
+        return out.copy_(codes.mean(1, keepdim=True).to(out.dtype))
+
+    def combine(buf, inv, score, n_tokens, top_k):
+        rows = buf[inv.clamp(min=0).long()].view(n_tokens, top_k, -1)
+        return (rows * (opaque(score) * (inv >= 0).view(n_tokens, top_k))[..., None]).sum(1)
+
+    for name, fn in (("route", route), ("mx_quantize_tokens", quantize_tokens),
+                     ("mx_linear_act_fwd", linear_act), ("mx_linear_fwd", linear_fwd),
+                     ("gather_combine_fwd", combine)):
+        stand_in(name, fn)
+    monkeypatch.setattr(fmoe_cuda, "_compiled", None)      # (the other binding's way)
+    return calls
+
+
+def _inputs(seed, tokens=5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(tokens, D, generator=g)
+    idx = torch.randint(-1, E, (tokens, 2), generator=g)
+    return x, idx, torch.rand(tokens, 2, generator=g) + 0.5
+
+
+def test_traced_expert_layer_follows_its_inputs(operators):
+    from fastmoe_amd import mx
+
+    w1, w2 = _weight(H, D, 1), _weight(D, H, 2)
+
+    def layer(x, idx, score):
+        return mx.expert_layer(x, idx, score, w1, None, w2, None, torch.nn.ReLU())
+
+    with torch.no_grad():
+        traced = torch.jit.trace(layer, _inputs(0), check_trace=False)
+        for seed in (0, 1, 2):
+            new = _inputs(seed)
+            want = layer(*new)
+            assert want.any() and torch.equal(traced(*new), want)
+        assert not torch.equal(layer(*_inputs(1)), layer(*_inputs(2)))
+
+
+@pytest.mark.parametrize("which", ["x", "score"])
+def test_forward_mode_differentiation_is_refused(operators, which):
+    from fastmoe_amd import mx
+
+    w1, w2 = _weight(H, D, 1), _weight(D, H, 2)
+    x, idx, score = _inputs(0)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x if which == "x" else score,
+                                    torch.ones_like(x if which == "x" else score))
+        x, score = (dual, score) if which == "x" else (x, dual)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            mx.expert_layer(x, idx, score, w1, None, w2, None, torch.nn.ReLU())
