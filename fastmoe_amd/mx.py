@@ -16,11 +16,13 @@ import torch
 import torch.nn as nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import fmoe_cuda
 from .functions import (FusedGatherCombine, FusedScatter, RoutePlan, SegmentTable,
                         apply_activation)
-from .linear import _segments, native_act
+from .linear import _segments, is_exact_gelu, native_act
+from .transformer import _Expert, _watched
 
 BLOCK = 32      # features that share a scale
 
@@ -164,6 +166,11 @@ def linear(x: torch.Tensor, fwd_expert_count, weight: MXTensor, bias=None) -> to
     return MXLinear.apply(x, fwd_expert_count, weight.codes, weight.scales, bias)
 
 
+def _activate(activation, x, n_rows_dev):
+    r"""`activation(x)`, called as the module it is where somebody watches it."""
+    return activation(x) if _watched(activation) else apply_activation(activation, x, n_rows_dev)
+
+
 class _Route(Function):
     r"""fmoe_cuda.route as an operation that tracing records."""
 
@@ -233,12 +240,13 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
     w2 [E, out, hidden].  Without gradients and for GELU and ReLU: routing, one pass that
     quantises the tokens into expert order, the first product with bias, activation and
     quantisation in its epilogue, the second product, the weighted combine.  Otherwise the
-    chain of single operators, in which the hidden layer is rounded to x's dtype on its way."""
+    chain of single operators, in which the hidden layer is rounded to x's dtype on its way.
+    An activation module with hooks, or a `forward` set on it, is called (the chain, too)."""
     top_k = gate_idx.shape[-1] if gate_idx.dim() >= 2 else 1
     if x.dim() != 2 or x.shape[1] != w1.features or w1.codes.shape[-2] != w2.features:
         raise RuntimeError("x [tokens, in], w1 [E, hidden, in] and w2 [E, out, hidden] disagree")
     n_expert = w1.codes.shape[0]
-    act = native_act(activation, x)
+    act = 0 if _watched(activation) else native_act(activation, x)
     grads = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, score, b1, b2))
     gate_idx = gate_idx.reshape(-1, top_k)
@@ -252,7 +260,7 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
             plan = RoutePlan(gate_idx, n_expert)
             segments, live = plan.segments, plan.n_rows_dev
             h = FusedScatter.apply(x, plan)
-        h = apply_activation(activation, linear(h, segments, w1, b1), live)
+        h = _activate(activation, linear(h, segments, w1, b1), live)
         y = linear(h, segments, w2, b2)
         if torch._C._get_tracing_state() is not None:
             return _Combine.apply(y, score, gate_idx, n_expert, *routed)
@@ -305,13 +313,15 @@ class MXExpert(nn.Module):
     def forward(self, inp, fwd_expert_count):
         x = linear(inp, fwd_expert_count, self.w1, self.b1)
         live = fwd_expert_count.seg_off[-1:] if isinstance(fwd_expert_count, SegmentTable) else None
-        x = apply_activation(self.activation, x, live)
+        x = _activate(self.activation, x, live)
         return linear(x, fwd_expert_count, self.w2, self.b2)
 
     # what FMoE.forward asks of a module that can run the whole dispatch
     def can_run_layer(self, inp, top_k) -> bool:
         return (torch.is_tensor(inp) and inp.dim() == 2 and inp.is_cuda and 1 <= top_k <= 64
                 and "forward" not in self.__dict__ and type(self).forward is MXExpert.forward
+                # (hooks on all modules see experts called where they see `_Expert` called)
+                and (is_exact_gelu(self.activation, inp) or not _has_any_global_hook())
                 and not (self._forward_hooks or self._forward_pre_hooks or self._backward_hooks
                          or self._backward_pre_hooks))
 
@@ -329,8 +339,6 @@ class MXExpert(nn.Module):
 def quantize_experts(layer):
     r"""Puts the fused experts of an `FMoE` layer on the GPU into 4 bits, in place; returns the
     layer.  Its state dict then holds `experts.w1_codes` and so on; gate and hooks stay."""
-    from .transformer import _Expert
-
     if not isinstance(layer.experts, _Expert):
         raise TypeError("only a layer whose experts are one fused module can be quantised")
     layer.experts = MXExpert.from_expert(layer.experts)

@@ -121,3 +121,76 @@ def test_operator_by_operator_gives_the_same_bits(act):
     with torch.no_grad():
         assert all(torch.equal(a, b) for a, b in both(lambda: [layer(x)]))
     assert all(torch.equal(a, b) for a, b in both(train))
+
+
+# ------------------------------------------------------------------ hooks
+@pytest.mark.parametrize("grads", [False, True])
+@pytest.mark.parametrize("act", [torch.nn.GELU, torch.nn.ReLU, torch.nn.SiLU])
+def test_hooks_on_the_activation_run(act, grads):
+    from fastmoe_amd import mx
+
+    layer = _layer(activation=act()).eval()
+    ex, x = layer.experts, torch.randn(30, 96, device="cuda").bfloat16().requires_grad_(grads)
+    idx, score = (t.detach() for t in layer.gate(x))
+    live = int((idx >= 0).sum())
+    counts = torch.tensor([5, 0, 10, 15, 0, 0, 0, 0])
+    calls = {"layer": lambda: layer(x), "experts": lambda: ex(x, counts),
+             "function": lambda: mx.expert_layer(x, idx, score, ex.w1, ex.b1, ex.w2, ex.b2,
+                                                 ex.activation)}
+    with torch.set_grad_enabled(grads):
+        for name, call in calls.items():
+            seen = []
+            plain = call()
+            rows = 30 if name == "experts" else live
+            hooks = [ex.activation.register_forward_hook(lambda m, i, o: seen.append(o.shape)),
+                     ex.activation.register_forward_pre_hook(lambda m, i: seen.append("before"))]
+            if grads:
+                hooks.append(ex.activation.register_full_backward_hook(
+                    lambda m, i, o: seen.append("back")))
+            watched = call()
+            if grads:
+                watched.float().sum().backward()
+            for h in hooks:
+                h.remove()
+            assert seen[0] == "before" and seen[1] == (rows, 160), name
+            assert seen[2:] == (["back"] if grads else []), name
+            # the chain of single operators: the fused form but for the hidden layer's rounding
+            err = (watched - plain).float().norm() / plain.float().norm()
+            assert err < 0.05, name
+            # and what a hook returns counts
+            h = ex.activation.register_forward_hook(lambda m, i, o: o * 0)
+            none = call()
+            h.remove()
+            b2 = ex.b2.detach()
+            if name == "experts":
+                want = b2.repeat_interleave(counts.cuda(), 0)
+                assert torch.equal(none, want)
+            else:
+                want = (b2[idx].float() * score[..., None].float()).sum(1)
+                assert (none.float() - want).abs().max() <= 2 ** -7 * want.abs().max()
+        ex.activation.forward = lambda t: t * 0
+        assert torch.equal(ex(x, counts), b2.repeat_interleave(counts.cuda(), 0))
+        assert torch.equal(layer(x), none)
+
+
+@pytest.mark.parametrize("act", [torch.nn.GELU, torch.nn.ReLU])
+def test_hooks_on_all_modules_see_what_they_saw_before(act):
+    import fastmoe_amd as fm
+    from fastmoe_amd import mx
+
+    full = fm.FMoETransformerMLP(num_expert=4, d_model=64, d_hidden=96, activation=act()).cuda()
+    x = torch.randn(20, 64, device="cuda")
+
+    def seen(layer):
+        names = []
+        hook = torch.nn.modules.module.register_module_forward_hook(
+            lambda m, *_: names.append(type(m).__name__))
+        try:
+            with torch.no_grad():
+                layer(x)
+        finally:
+            hook.remove()
+        return [n.replace("MXExpert", "_Expert") for n in names]
+
+    before = seen(full)
+    assert seen(mx.quantize_experts(full)) == before
