@@ -839,7 +839,8 @@ def mx_linear_bwd(dy: torch.Tensor, seg_off: torch.Tensor, w_codes: torch.Tensor
                   w_scales: torch.Tensor, in_feat: int, need_dx: bool = True,
                   need_bias: bool = False
                   ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """(dx, dbias) in front of frozen MXFP4 weights: dx[seg_e] = dy[seg_e] @ w[e]."""
+    """(dx, dbias) in front of frozen MXFP4 weights: dx[seg_e] = dy[seg_e] @ w[e], zero in rows
+    that no expert owns."""
     _dev(dy, "dy")
     _mx_check(w_codes, w_scales, in_feat, "weight")
     _dev(seg_off, "seg_off", torch.int32)
@@ -852,8 +853,14 @@ def mx_linear_bwd(dy: torch.Tensor, seg_off: torch.Tensor, w_codes: torch.Tensor
     dx = db = w = None
     if need_dx:
         w = dy.new_empty((e * out_f, in_feat))
-        mx_dequantize(w_codes.view(e * out_f, -1), w_scales.view(e * out_f, -1), w)
         dx = dy.new_empty((dy.shape[0], in_feat))
+        with _launch(dy, "mx_dequantize"):
+            _lib.check(
+                _L.fmoe_mx_dequantize_bwd(w_codes.data_ptr(), w_scales.data_ptr(),
+                                          seg_off.data_ptr(), w.data_ptr(), dx.data_ptr(),
+                                          dy.shape[0], in_feat, out_f, e, _dt(dy, "dy"),
+                                          _stream(dy)),
+                "mx_dequantize_bwd")
     if need_bias:
         db = dy.new_empty((e, out_f))
     if need_dx or need_bias:

@@ -104,6 +104,7 @@ SIGNATURES = {
     "fmoe_mx_quantize_tokens": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
                                         c_void_p, c_int, c_void_p]),
     "fmoe_mx_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "fmoe_mx_dequantize_bwd": (c_int, [c_void_p] * 5 + [c_int64] * 4 + [c_int, c_void_p]),
     "fmoe_mx_linear_fwd": (c_int, [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int64] * 4
                            + [c_int, c_void_p]),
     "fmoe_scatter_tokens": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,

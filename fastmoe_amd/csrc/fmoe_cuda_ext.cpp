@@ -687,7 +687,7 @@ std::tuple<Tensor, Tensor> mx_linear_act_fwd(Tensor xc, Tensor xs, Tensor wc, Te
 }
 
 // Gradients of the rows and of the bias in front of frozen 4-bit weights: the weights' values in
-// dy's dtype, then the grouped product of the other weights.
+// dy's dtype, then the grouped product of the other weights.  Rows that no expert owns get zeros.
 std::tuple<OptTensor, OptTensor> mx_linear_bwd(Tensor dy, Tensor seg_off, Tensor wc, Tensor ws,
                                                int64_t in_f, bool need_dx, bool need_bias) {
   dev(dy, "dy");
@@ -703,8 +703,11 @@ std::tuple<OptTensor, OptTensor> mx_linear_bwd(Tensor dy, Tensor seg_off, Tensor
   Tensor w;
   if (need_dx) {
     w = torch::empty({e * out_f, in_f}, dy.options());
-    mx_dequantize(wc.view({e * out_f, -1}), ws.view({e * out_f, -1}), w);
     dx = torch::empty({dy.size(0), in_f}, dy.options());
+    check(fmoe_mx_dequantize_bwd(wc.data_ptr(), ws.data_ptr(), seg_off.data_ptr<int32_t>(),
+                                 w.data_ptr(), dx->data_ptr(), dy.size(0), in_f, out_f, e,
+                                 dt(dy, "dy"), stream_of(dy)),
+          "mx_dequantize_bwd");
   }
   if (need_bias) db = torch::empty({e, out_f}, dy.options());
   if (need_dx || need_bias)   // (the layer's input takes part in the weight gradient alone)

@@ -176,10 +176,26 @@ __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(
   }
 }
 
+// The rows of a gradient that no expert owns, for mx_dequantize_kernel to clear in passing: rows
+// *end .. n_rows - 1 of k values at p.
+template <typename T> struct MxTail {
+  const int32_t* end = nullptr;
+  T* p = nullptr;
+  int64_t n_rows = 0;
+
+  __device__ __forceinline__ void clear(int k) const {
+    const int64_t stride = (int64_t)gridDim.x * kMxThreads;
+    for (int64_t i = (int64_t)max(*end, 0) * k + (int64_t)blockIdx.x * kMxThreads + threadIdx.x;
+         i < n_rows * k; i += stride)
+      p[i] = Elem<T>::from_acc(0.f);
+  }
+};
+
 template <typename T, int N, int U>
 __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_rows, int k,
-    T* __restrict__ out) {
+    T* __restrict__ out, MxTail<T> tail) {
+  if (tail.p) tail.clear(k);
   const int lane = threadIdx.x & (kWave - 1);
   const int chunks = (k + kMxChunk - 1) / kMxChunk;
   const int64_t code_row = mx_code_bytes(k), scale_row = mx_scale_bytes(k);
@@ -266,13 +282,14 @@ static int launch_quantize(const void* x, int64_t n_rows, int k, const int32_t* 
 
 template <typename T>
 static int launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, int k,
-                             void* out, hipStream_t s) {
+                             void* out, const int32_t* tail_end, void* tail, int64_t tail_rows,
+                             hipStream_t s) {
   const int run = run_length<T>(out, k);
   const MxGrid g(n_rows, k);
   const dim3 grid(g.blocks);
 #define FMOE_CALL(N, U)                                                                        \
   hipLaunchKernelGGL((mx_dequantize_kernel<T, N, U>), grid, dim3(kMxThreads), 0, s, codes,   \
-                     scales, n_rows, k, (T*)out)
+                     scales, n_rows, k, (T*)out, MxTail<T>{tail_end, (T*)tail, tail_rows})
   FMOE_RUNS(FMOE_CALL);
 #undef FMOE_CALL
   FMOE_LAUNCH_CHECK("mx_dequantize");
@@ -298,6 +315,28 @@ static int quantize(const void* x, int64_t n_rows, int64_t k, const int32_t* n_r
       return launch_quantize<__half>(x, n_rows, (int)k, n_rows_dev, inv, (int)top_k, c, sc, segments, s);
     default:
       return launch_quantize<__hip_bfloat16>(x, n_rows, (int)k, n_rows_dev, inv, (int)top_k, c, sc, segments, s);
+  }
+}
+
+static int dequantize(const void* codes, const void* scales, int64_t n_rows, int64_t k, void* out,
+                      const int32_t* tail_end, void* tail, int64_t tail_rows, int dtype,
+                      hipStream_t s) {
+  FMOE_REQUIRE(n_rows >= 0 && k >= 1 && k <= FMOE_MX_MAX_FEATURES, FMOE_ERR_INVALID,
+               "mx_dequantize: bad sizes");
+  FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_F16 || dtype == FMOE_BF16, FMOE_ERR_UNSUPPORTED,
+               "mx_dequantize: unsupported dtype %d", dtype);
+  if (n_rows == 0) return FMOE_OK;
+  FMOE_REQUIRE(codes && scales && out, FMOE_ERR_INVALID, "mx_dequantize: null pointer");
+  FMOE_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, FMOE_ERR_INVALID,
+               "mx_dequantize: codes and scales must be 16-byte aligned");
+  const uint8_t *c = (const uint8_t*)codes, *sc = (const uint8_t*)scales;
+  switch (dtype) {
+    case FMOE_F32:
+      return launch_dequantize<float>(c, sc, n_rows, (int)k, out, tail_end, tail, tail_rows, s);
+    case FMOE_F16:
+      return launch_dequantize<__half>(c, sc, n_rows, (int)k, out, tail_end, tail, tail_rows, s);
+    default:
+      return launch_dequantize<__hip_bfloat16>(c, sc, n_rows, (int)k, out, tail_end, tail, tail_rows, s);
   }
 }
 
@@ -344,20 +383,18 @@ extern "C" int fmoe_mx_quantize_tokens(const void* x, const int32_t* inv, int64_
 
 extern "C" int fmoe_mx_dequantize(const void* codes, const void* scales, int64_t n_rows,
                                   int64_t features, void* out, int dtype, void* stream) {
-  using namespace fmoe;
-  FMOE_REQUIRE(n_rows >= 0 && features >= 1 && features <= FMOE_MX_MAX_FEATURES, FMOE_ERR_INVALID,
-               "mx_dequantize: bad sizes");
-  FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_F16 || dtype == FMOE_BF16, FMOE_ERR_UNSUPPORTED,
-               "mx_dequantize: unsupported dtype %d", dtype);
-  if (n_rows == 0) return FMOE_OK;
-  FMOE_REQUIRE(codes && scales && out, FMOE_ERR_INVALID, "mx_dequantize: null pointer");
-  FMOE_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, FMOE_ERR_INVALID,
-               "mx_dequantize: codes and scales must be 16-byte aligned");
-  const uint8_t *c = (const uint8_t*)codes, *sc = (const uint8_t*)scales;
-  hipStream_t s = (hipStream_t)stream;
-  switch (dtype) {
-    case FMOE_F32: return launch_dequantize<float>(c, sc, n_rows, (int)features, out, s);
-    case FMOE_F16: return launch_dequantize<__half>(c, sc, n_rows, (int)features, out, s);
-    default: return launch_dequantize<__hip_bfloat16>(c, sc, n_rows, (int)features, out, s);
-  }
+  return fmoe::dequantize(codes, scales, n_rows, features, out, nullptr, nullptr, 0, dtype,
+                          (hipStream_t)stream);
+}
+
+extern "C" int fmoe_mx_dequantize_bwd(const void* w_codes, const void* w_scales,
+                                      const int32_t* seg_off, void* w, void* dx, int64_t n_rows,
+                                      int64_t in_feat, int64_t out_feat, int64_t n_expert,
+                                      int dtype, void* stream) {
+  FMOE_REQUIRE(n_rows >= 0 && n_rows < INT32_MAX && n_expert >= 1 && n_expert < INT32_MAX &&
+                   out_feat >= 1 && out_feat <= FMOE_MX_MAX_FEATURES,
+               FMOE_ERR_INVALID, "mx_dequantize_bwd: bad sizes");
+  FMOE_REQUIRE(seg_off && (dx || n_rows == 0), FMOE_ERR_INVALID, "mx_dequantize_bwd: null pointer");
+  return fmoe::dequantize(w_codes, w_scales, n_expert * out_feat, in_feat, w, seg_off + n_expert,
+                          n_rows ? dx : nullptr, n_rows, dtype, (hipStream_t)stream);
 }

@@ -155,7 +155,9 @@ def linear(x: torch.Tensor, fwd_expert_count, weight: MXTensor, bias=None) -> to
     r"""y[rows of e] = x[rows of e] @ weight[e].T + bias[e]: the grouped linear layer of
     `FMoELinear` with 4-bit weights [E, out, in].  x [rows, in] holds the rows in expert
     order and is quantised on the way; `fwd_expert_count` is an int64 tensor of row counts
-    (host or device) or a SegmentTable; bias [E, out] has x's dtype, as has the result."""
+    (host or device) or a SegmentTable; bias [E, out] has x's dtype, as has the result.  Rows of
+    x that the counts do not cover are in no product: their rows of y are left as they were
+    allocated, their gradient is zero."""
     native = fmoe_cuda.native()
     if native is not None:
         segments = (fwd_expert_count.seg_off if isinstance(fwd_expert_count, SegmentTable)

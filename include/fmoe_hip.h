@@ -522,6 +522,10 @@ int fmoe_score_topk_bwd(const void* dweight, const void* logits, const int64_t* 
  *                     [n_expert + 1]) from their DEVICE int64 counts: a linear layer that is
  *                     handed counts then needs no launch of its own for them.
  *   _dequantize       the values, rounded to dtype where that is too narrow for them.
+ *   _dequantize_bwd   what stands in front of fmoe_grouped_linear_bwd for frozen 4-bit weights:
+ *                     w [n_expert * out_feat, in_feat] = their values, and zeros in the rows of
+ *                     dx [n_rows, in_feat] at or behind seg_off[n_expert] (DEVICE), which that
+ *                     call leaves as they are.
  * dtype: f32, f16 or bf16.  The reference has no such format.
  */
 int64_t fmoe_mx_code_bytes(int64_t features);
@@ -535,6 +539,9 @@ int fmoe_mx_quantize_tokens(const void* x, const int32_t* inv, int64_t n_tokens,
                             int64_t features, void* codes, void* scales, int dtype, void* stream);
 int fmoe_mx_dequantize(const void* codes, const void* scales, int64_t n_rows, int64_t features,
                        void* out, int dtype, void* stream);
+int fmoe_mx_dequantize_bwd(const void* w_codes, const void* w_scales, const int32_t* seg_off,
+                           void* w, void* dx, int64_t n_rows, int64_t in_feat, int64_t out_feat,
+                           int64_t n_expert, int dtype, void* stream);
 
 /*
  * The grouped linear layer (fmoe_grouped_linear_fwd) on MXFP4 operands:

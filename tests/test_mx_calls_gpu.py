@@ -194,3 +194,47 @@ def test_hooks_on_all_modules_see_what_they_saw_before(act):
 
     before = seen(full)
     assert seen(mx.quantize_experts(full)) == before
+
+
+# ------------------------------------------------------------------ counts that leave rows over
+def _nan_memory(*shape, dtype):
+    """Leaves NaN behind in the memory that the next tensor of this size gets."""
+    held = [torch.full(shape, float("nan"), dtype=dtype, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("counts", [[0, 0, 0], [7, 0, 60], [100, 30, 0], [0, 0, 131]])
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+def test_rows_that_no_expert_owns_have_no_gradient(dt, counts, where):
+    from fastmoe_amd import mx
+
+    rows, k, n, dtype = 131, 72, 40, DTYPES[dt]
+    w = mx.quantize(torch.randn(3, n, k, device="cuda"))
+    counts = torch.tensor(counts)
+    live = int(counts.sum())
+    dy = torch.randn(rows, n, device="cuda").to(dtype)
+    x = torch.randn(rows, k, device="cuda").to(dtype).requires_grad_(True)
+    y = mx.linear(x, counts.to(where), w)
+    _nan_memory(rows, k, dtype=dtype)
+    y.backward(dy)
+    assert not x.grad[live:].any()
+    # the covered rows as if the others were not there
+    z = x.detach()[:live].clone().requires_grad_(True)
+    mx.linear(z, counts, w).backward(dy[:live])
+    assert torch.equal(x.grad[:live], z.grad)
+
+
+def test_both_bindings_clear_what_no_expert_owns():
+    from fastmoe_amd import _ext, fmoe_cuda, mx
+
+    w = mx.quantize(torch.randn(2, 40, 300, device="cuda"))
+    dy = torch.randn(3000, 40, device="cuda").bfloat16()
+    for bounds in ([0, 0, 0], [0, 1000, 1777], [0, 5, 3000]):
+        seg = torch.tensor(bounds, dtype=torch.int32).cuda()
+        got = []
+        for ops in (fmoe_cuda.ctypes_ops, _ext.load()):
+            _nan_memory(3000, 300, dtype=torch.bfloat16)
+            got.append(ops.mx_linear_bwd(dy, seg, w.codes, w.scales, 300)[0])
+        assert torch.equal(*got) and not got[0][bounds[-1]:].any()
