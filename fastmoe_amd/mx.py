@@ -21,7 +21,7 @@ from torch.nn.modules.module import _has_any_global_hook
 from . import fmoe_cuda
 from .functions import (FusedGatherCombine, FusedScatter, RoutePlan, SegmentTable,
                         apply_activation)
-from .linear import _segments, is_exact_gelu, native_act
+from .linear import FMoELinear, _segments, is_exact_gelu, native_act
 from .transformer import _Expert, _watched
 
 BLOCK = 32      # features that share a scale
@@ -300,9 +300,22 @@ class MXExpert(nn.Module):
 
     @classmethod
     def from_expert(cls, expert) -> "MXExpert":
-        r"""From a fused `_Expert` on the GPU, its weights quantised."""
+        r"""From a fused `_Expert` on the GPU, its weights quantised.  The biases keep their
+        `dp_comm` tags and what else was set on them, the module its training flag; hooks on
+        the expert module and on its two linear layers do not come along.  An expert with a
+        `forward` other than `_Expert`'s, in itself or a linear layer, is refused."""
         l1, l2 = expert.htoh4, expert.h4toh
-        return cls(quantize(l1.weight), l1.bias, quantize(l2.weight), l2.bias, expert.activation)
+        for module, kind in ((expert, _Expert), (l1, FMoELinear), (l2, FMoELinear)):
+            if type(module).forward is not kind.forward or "forward" in module.__dict__:
+                raise TypeError(f"{type(module).__name__} computes something of its own and "
+                                "cannot be quantised")
+        new = cls(quantize(l1.weight), l1.bias, quantize(l2.weight), l2.bias, expert.activation)
+        for old, b in ((l1.bias, new.b1), (l2.bias, new.b2)):
+            if b is not None:
+                b.__dict__.update(old.__dict__)
+        # (not train(): the activation is shared)
+        new.training = expert.training
+        return new
 
     @property
     def w1(self) -> MXTensor:
@@ -340,7 +353,8 @@ class MXExpert(nn.Module):
 
 def quantize_experts(layer):
     r"""Puts the fused experts of an `FMoE` layer on the GPU into 4 bits, in place; returns the
-    layer.  Its state dict then holds `experts.w1_codes` and so on; gate and hooks stay."""
+    layer.  Its state dict then holds `experts.w1_codes` and so on.  The gate stays, and hooks
+    on the layer, the gate and the activation; see MXExpert.from_expert for the experts."""
     if not isinstance(layer.experts, _Expert):
         raise TypeError("only a layer whose experts are one fused module can be quantised")
     layer.experts = MXExpert.from_expert(layer.experts)

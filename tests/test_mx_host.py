@@ -105,3 +105,78 @@ def test_forward_mode_differentiation_is_refused(operators, which):
         x, score = (dual, score) if which == "x" else (x, dual)
         with pytest.raises((RuntimeError, NotImplementedError)):
             mx.expert_layer(x, idx, score, w1, None, w2, None, torch.nn.ReLU())
+
+
+# ------------------------------------------------------------------ quantising a layer
+@pytest.fixture
+def quantised(monkeypatch):
+    """mx.quantize_experts on the CPU: codes and scales of the right shapes."""
+    from fastmoe_amd import mx
+
+    def quantize(x):
+        k = x.shape[-1]
+        return mx.MXTensor(*(torch.zeros(*x.shape[:-1], n, dtype=torch.uint8)
+                             for n in (-(-k // 128) * 64, -(-k // 512) * 16)), k)
+
+    monkeypatch.setattr(mx, "quantize", quantize)
+    return mx.quantize_experts
+
+
+def _layer(**kwargs):
+    from fastmoe_amd import FMoETransformerMLP
+
+    return FMoETransformerMLP(num_expert=E, d_model=D, d_hidden=H, **kwargs)
+
+
+@pytest.mark.parametrize("comm", ["none", "dp"])
+def test_quantised_experts_keep_tags_flags_and_gradients(quantised, comm):
+    layer = _layer(expert_dp_comm=comm).eval()
+    layer.experts.activation.train()
+    layer.experts.h4toh.bias.requires_grad_(False)
+    layer.experts.htoh4.bias.lr_scale = 3.0
+    quantised(layer)
+    ex = layer.experts
+    assert not layer.training and not ex.training and ex.activation.training
+    assert ex.b1.dp_comm == ex.b2.dp_comm == comm and ex.b1.lr_scale == 3.0
+    assert ex.b1.requires_grad and not ex.b2.requires_grad
+    assert quantised(_layer()).experts.training
+
+
+def test_experts_without_biases_are_quantised(quantised):
+    layer = _layer()
+    layer.experts.htoh4.register_parameter("bias", None)
+    quantised(layer)
+    assert layer.experts.b1 is None and layer.experts.b2.dp_comm == "none"
+
+
+def test_experts_that_compute_something_else_are_refused(quantised):
+    from fastmoe_amd import FMoELinear
+    from fastmoe_amd.transformer import _Expert
+
+    class Doubled(_Expert):
+        def forward(self, inp, fwd_expert_count):
+            return 2 * super().forward(inp, fwd_expert_count)
+
+    class Scaled(FMoELinear):
+        def forward(self, inp, fwd_expert_count):
+            return 2 * super().forward(inp, fwd_expert_count)
+
+    def own_forward(layer):
+        layer.experts.forward = lambda inp, counts: inp
+
+    def own_linear(layer):
+        layer.experts.htoh4 = Scaled(E, D, H)
+
+    def own_linear_forward(layer):
+        layer.experts.h4toh.forward = lambda inp, counts: inp
+
+    def own_class(layer):
+        layer.experts = Doubled(E, D, H, torch.nn.GELU())
+
+    for change in (own_forward, own_linear, own_linear_forward, own_class):
+        layer = _layer()
+        change(layer)
+        before = layer.experts
+        with pytest.raises(TypeError):
+            quantised(layer)
+        assert layer.experts is before
