@@ -173,6 +173,10 @@ def _activate(activation, x, n_rows_dev):
     return activation(x) if _watched(activation) else apply_activation(activation, x, n_rows_dev)
 
 
+def _as(x, bias):
+    return x if bias is None else x.type_as(bias)
+
+
 class _Route(Function):
     r"""fmoe_cuda.route as an operation that tracing records."""
 
@@ -243,7 +247,8 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
     quantises the tokens into expert order, the first product with bias, activation and
     quantisation in its epilogue, the second product, the weighted combine.  Otherwise the
     chain of single operators, in which the hidden layer is rounded to x's dtype on its way.
-    An activation module with hooks, or a `forward` set on it, is called (the chain, too)."""
+    An activation module with hooks, or a `forward` set on it, is called (the chain, too).
+    The result has x's dtype; biases of another are taken in it (b1, without gradients, as it is)."""
     top_k = gate_idx.shape[-1] if gate_idx.dim() >= 2 else 1
     if x.dim() != 2 or x.shape[1] != w1.features or w1.codes.shape[-2] != w2.features:
         raise RuntimeError("x [tokens, in], w1 [E, hidden, in] and w2 [E, out, hidden] disagree")
@@ -252,6 +257,7 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
     grads = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, score, b1, b2))
     gate_idx = gate_idx.reshape(-1, top_k)
+    b2 = None if b2 is None else b2.to(x.dtype)
     if grads or not act or x.dtype == torch.float64:
         score = score.reshape(-1, top_k)
         if torch._C._get_tracing_state() is not None:
@@ -262,6 +268,7 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
             plan = RoutePlan(gate_idx, n_expert)
             segments, live = plan.segments, plan.n_rows_dev
             h = FusedScatter.apply(x, plan)
+        b1 = None if b1 is None else b1.to(x.dtype)
         h = _activate(activation, linear(h, segments, w1, b1), live)
         y = linear(h, segments, w2, b2)
         if torch._C._get_tracing_state() is not None:
@@ -277,7 +284,8 @@ class MXExpert(nn.Module):
     r"""The experts of a layer (`linear -> activation -> linear`) with 4-bit weights, in the
     place of the fused `_Expert`: `layer.experts = MXExpert.from_expert(layer.experts)`, or
     `quantize_experts(layer)`.  Weights are uint8 buffers and frozen; the biases stay
-    parameters.  Accepts host counts or a device-side SegmentTable, as `_Expert` does."""
+    parameters.  Accepts host counts or a device-side SegmentTable, and casts its rows to its
+    parameters' dtype, as `_Expert` does."""
 
     accepts_segment_table = True
 
@@ -326,14 +334,15 @@ class MXExpert(nn.Module):
         return MXTensor(self.w2_codes, self.w2_scales, self.hidden_features)
 
     def forward(self, inp, fwd_expert_count):
-        x = linear(inp, fwd_expert_count, self.w1, self.b1)
+        x = linear(_as(inp, self.b1), fwd_expert_count, self.w1, self.b1)
         live = fwd_expert_count.seg_off[-1:] if isinstance(fwd_expert_count, SegmentTable) else None
         x = _activate(self.activation, x, live)
-        return linear(x, fwd_expert_count, self.w2, self.b2)
+        return linear(_as(x, self.b2), fwd_expert_count, self.w2, self.b2)
 
     # what FMoE.forward asks of a module that can run the whole dispatch
     def can_run_layer(self, inp, top_k) -> bool:
         return (torch.is_tensor(inp) and inp.dim() == 2 and inp.is_cuda and 1 <= top_k <= 64
+                and all(b is None or b.dtype == inp.dtype for b in (self.b1, self.b2))
                 and "forward" not in self.__dict__ and type(self).forward is MXExpert.forward
                 # (hooks on all modules see experts called where they see `_Expert` called)
                 and (is_exact_gelu(self.activation, inp) or not _has_any_global_hook())

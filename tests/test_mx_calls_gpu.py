@@ -238,3 +238,65 @@ def test_both_bindings_clear_what_no_expert_owns():
             _nan_memory(3000, 300, dtype=torch.bfloat16)
             got.append(ops.mx_linear_bwd(dy, seg, w.codes, w.scales, 300)[0])
         assert torch.equal(*got) and not got[0][bounds[-1]:].any()
+
+
+# ------------------------------------------------------------------ dtypes
+def test_layer_takes_rows_of_another_dtype_as_before():
+    """`_Expert` casts its rows to its parameters' dtype; so do the experts in its place."""
+    import fastmoe_amd as fm
+    from fastmoe_amd import mx
+
+    torch.manual_seed(0)
+    layer = fm.FMoETransformerMLP(num_expert=4, d_model=64, d_hidden=96).cuda().eval()
+    x, counts = torch.randn(30, 64, device="cuda"), torch.tensor([5, 0, 10, 15])
+    half = x.bfloat16()
+
+    def run():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            return layer(half)
+
+    full = run()
+    mx.quantize_experts(layer)
+    ex = layer.experts
+    for rows in (half, x.half(), x.double()):
+        assert torch.equal(ex(rows, counts), ex(rows.float(), counts))
+    for grads in (False, True):
+        with torch.set_grad_enabled(grads):
+            y = run()
+            assert y.dtype == full.dtype == torch.float32
+            assert 0.01 < (y - full).norm() / full.norm() < 0.5
+            if grads:
+                y.sum().backward()
+                assert ex.b1.grad.dtype == torch.float32 and ex.b1.grad.any()
+    # a first layer of another dtype than the second
+    ex.b1.data = ex.b1.data.half()
+    ex.b1.grad = None
+    y = ex(half, counts)
+    assert y.dtype == torch.float32 and torch.equal(y, ex(half.half(), counts))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert layer(half).dtype == torch.float32
+
+
+@pytest.mark.parametrize("act", [torch.nn.GELU(), torch.nn.SiLU()])
+def test_expert_layer_takes_biases_of_another_dtype(act):
+    from fastmoe_amd import mx
+
+    ex = _layer(dtype=torch.float32).experts
+    x = torch.randn(40, 96, device="cuda").bfloat16()
+    idx = torch.from_numpy(make_gate(40, 2, 8, drop=0.1)).cuda()
+    score = torch.rand(40, 2, device="cuda")
+    run = lambda b1, b2: mx.expert_layer(x, idx, score, ex.w1, b1, ex.w2, b2, act)
+    b1, b2 = ex.b1.detach(), ex.b2.detach()
+    with torch.no_grad():
+        want = run(b1.bfloat16(), b2.bfloat16())
+        assert torch.equal(run(b1.bfloat16(), b2), want) and want.dtype == torch.bfloat16
+        got = run(b1, b2)
+        assert (got - want).float().norm() <= 0.02 * want.float().norm()
+    leaf1, leaf2 = ex.b1, ex.b2
+    y = run(leaf1, leaf2)
+    y.float().square().sum().backward()
+    same1, same2 = (b.bfloat16().requires_grad_(True) for b in (b1, b2))
+    z = run(same1, same2)
+    z.float().square().sum().backward()
+    assert torch.equal(y, z)
+    assert torch.equal(leaf1.grad, same1.grad.float()) and torch.equal(leaf2.grad, same2.grad.float())
