@@ -707,7 +707,7 @@ def _mx_check(codes: torch.Tensor, scales: torch.Tensor, features: int, name: st
     _dev(codes, name, torch.uint8)
     _dev(scales, name, torch.uint8)
     _need(features >= 1, f"{name}: features must be positive")
-    _need(codes.dim() >= 2 and scales.dim() == codes.dim()
+    _need(codes.dim() >= 1 and scales.dim() == codes.dim()
           and codes.shape[:-1] == scales.shape[:-1]
           and (codes.shape[-1], scales.shape[-1]) == _mx_bytes(features)
           and codes.device == scales.device,

@@ -573,7 +573,7 @@ void mx_check(const Tensor& codes, const Tensor& scales, int64_t features, const
   dev(codes, name, at::kByte);
   dev(scales, name, at::kByte);
   need(features >= 1, std::string(name) + ": features must be positive");
-  need(codes.dim() >= 2 && scales.dim() == codes.dim() &&
+  need(codes.dim() >= 1 && scales.dim() == codes.dim() &&
            codes.sizes().slice(0, codes.dim() - 1) == scales.sizes().slice(0, codes.dim() - 1) &&
            codes.size(-1) == fmoe_mx_code_bytes(features) &&
            scales.size(-1) == fmoe_mx_scale_bytes(features) && codes.device() == scales.device(),

@@ -300,3 +300,23 @@ def test_expert_layer_takes_biases_of_another_dtype(act):
     z.float().square().sum().backward()
     assert torch.equal(y, z)
     assert torch.equal(leaf1.grad, same1.grad.float()) and torch.equal(leaf2.grad, same2.grad.float())
+
+
+@pytest.mark.parametrize("k", [1, 32, 300, 513])
+def test_a_single_row_without_leading_dimensions(k):
+    from fastmoe_amd import fmoe_cuda, mx
+
+    x = torch.randn(k, device="cuda")
+    q, rows = mx.quantize(x), mx.quantize(x[None])
+    assert q.shape == (k,) and torch.equal(q.codes, rows.codes[0])
+    back = q.dequantize(torch.float32)
+    assert back.shape == (k,) and torch.equal(back, rows.dequantize(torch.float32)[0])
+    fmoe_cuda.profile_hook = lambda *event: None          # (the operators one by one)
+    try:
+        assert torch.equal(mx.quantize(x).dequantize(torch.float32), back)
+    finally:
+        fmoe_cuda.profile_hook = None
+    with pytest.raises(RuntimeError):
+        mx.linear(x, torch.tensor([1]), mx.quantize(torch.randn(1, 8, k, device="cuda")))
+    with pytest.raises(RuntimeError):                      # a weight is [E, out, in]
+        mx.linear(x[None], torch.tensor([1]), q)
