@@ -37,10 +37,15 @@ class ScoreGate(NaiveGate):
 
     @classmethod
     def configured(cls, **options):
-        r"""A subclass whose constructor's defaults are `options`."""
+        r"""A subclass whose constructor's defaults are `options`.  What it makes are instances of
+        this class (the options are theirs), so that they can be pickled."""
         def init(self, *args, **kwargs):
             cls.__init__(self, *args, **{**options, **kwargs})
-        return type(cls.__name__, (cls,), {"__init__": init})
+            if type(self) is made:
+                self.__class__ = made._made_from
+        made = type(cls.__name__, (cls,), {
+            "__init__": init, "_made_from": cls.__dict__.get("_made_from", cls)})
+        return made
 
     def _apply(self, fn, recurse=True):
         bias = self.balance_bias
