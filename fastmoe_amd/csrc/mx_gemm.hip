@@ -58,10 +58,12 @@ __device__ __forceinline__ i32x4 mx_descriptor(const void* p, int64_t bytes) {
 
 // gelu(x) = x Phi(x) with Phi(x) = 1 / (1 + 2^z), z = -log2(Phi(x) / Phi(-x)) = x P(x^2) for
 // |x| <= 6 and x P(36) outside: P of degree 12 in x^2 / 18 - 1, a reweighted least-squares fit on
-// Chebyshev nodes.  Within 1.4e-7 + 1e-7 |gelu| of gelu everywhere, so that hardly more codes than
-// the sums' own rounding makes land on the other side of a boundary (degree 9, three instructions
-// less, was off by 7e-7), and, for |x| <= 6, within 3.4e-6 of its value, so that blocks whose values
-// all lie in the negative tail keep their digits as well.  26 issue slots where erff takes about
+// Chebyshev nodes.  Within 2e-7 + 3e-7 |gelu| of gelu everywhere (the fit, evaluated in f32 with an
+// exact exponential and quotient: 1.42e-7 + 1e-7 |gelu|; the two instructions for these are good to
+// 1.2e-7 each), so that hardly more codes than the sums' own rounding makes land on the other side
+// of a boundary (degree 9, three instructions less, was off by 7e-7), and, for |x| <= 6, within
+// 5e-6 of its value (3.7e-6 likewise), so that blocks whose values all lie in the negative tail
+// keep their digits as well.  26 issue slots where erff takes about
 // 60, with branches, and loses the tail: with one wave on a SIMD nothing hides them (a 256 x 256
 // tile of 4096 features: 27 us of matrix instructions, 26 us of erff).
 __device__ __forceinline__ float mx_gelu(float x) {

@@ -5,7 +5,6 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-import mx_reference as R
 from helpers import DTYPES, make_gate
 
 pytestmark = pytest.mark.gpu
@@ -320,3 +319,42 @@ def test_a_single_row_without_leading_dimensions(k):
         mx.linear(x, torch.tensor([1]), mx.quantize(torch.randn(1, 8, k, device="cuda")))
     with pytest.raises(RuntimeError):                      # a weight is [E, out, in]
         mx.linear(x[None], torch.tensor([1]), q)
+
+
+# ------------------------------------------------------------------ GELU between the products
+@pytest.mark.parametrize("k,n,counts", [
+    (200, 6020, [3001, 0, 700, 2500]), (4100, 13000, [9000, 0, 4001, 7000]),
+    (1030, 260, [60, 0, 200, 1] * 20), (520, 1500, [1, 30, 0, 65, 17] * 30),
+    (512, 1499, [60, 0, 200, 1] * 32)])
+def test_gelu_moves_only_codes_on_a_boundary(k, n, counts):
+    """The kernel's GELU is within 2e-7 + 3e-7 |gelu| of gelu, the 64-bit one behind it is rounded
+    to f32 here (6e-8): a code may be another only where a rounding boundary is as near as that,
+    and a block's scale only where its largest value is as near to a power of two."""
+    from fastmoe_amd import fmoe_cuda, mx
+
+    g = torch.Generator(device="cuda").manual_seed(k)
+    draw = lambda *shape: torch.randn(*shape, device="cuda", generator=g)
+    xq, wq = mx.quantize(draw(sum(counts), k)), mx.quantize(draw(len(counts), n, k) * 0.1)
+    b = draw(len(counts), n)
+    seg = torch.cat([torch.zeros(1, dtype=torch.int64), torch.tensor(counts).cumsum(0)]).int().cuda()
+    y = fmoe_cuda.mx_linear_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k, b, seg,
+                                torch.empty(sum(counts), n, device="cuda"))
+    codes, scales = fmoe_cuda.mx_linear_act_fwd(xq.codes, xq.scales, wq.codes, wq.scales, k, b,
+                                                seg, 1)
+    got = mx.MXTensor(codes, scales, n).dequantize(torch.float32).double()
+    assert torch.isfinite(got).all()
+    y = y.double()
+    h = 0.5 * y * torch.special.erfc(-y / 2 ** 0.5)
+    want = mx.quantize(h.float())
+    row, col = torch.nonzero(got != want.dequantize(torch.float32).double(), as_tuple=True)
+    assert len(row) <= 1e-4 * got.numel()
+    near = lambda v: 2e-7 + 4e-7 * v.abs()
+    got, other, true = got[row, col], want.dequantize(torch.float32)[row, col].double(), h[row, col]
+    on_boundary = (true - (got + other) / 2).abs() <= near(true)
+    block = col // 32
+    mine, theirs = scales[row, block], want.scales[row, block]
+    pad = torch.nn.functional.pad(h, (0, -n % 32)).view(len(h), -1, 32)
+    top = pad[row, block].abs().amax(-1)
+    power = torch.exp2(torch.round(torch.log2(top)))
+    assert ((mine == theirs) | ((top - power).abs() <= near(top))).all()
+    assert (on_boundary | (mine != theirs)).all()

@@ -1,9 +1,14 @@
 """4-bit experts, what needs no GPU: how the layer is called, not what its kernels compute.  The
 operators are opaque stand-ins that autograd and tracing cannot look into, like the real ones."""
+import os
+import re
+
 import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
+
+from conftest import ROOT
 
 E, D, H = 3, 32, 64
 
@@ -180,3 +185,43 @@ def test_experts_that_compute_something_else_are_refused(quantised):
         with pytest.raises(TypeError):
             quantised(layer)
         assert layer.experts is before
+
+
+# ------------------------------------------------------------------ the GELU between the products
+def test_fitted_gelu_keeps_its_bounds():
+    """mx_gelu of csrc/mx_gemm.hip in f32 arithmetic, its exponential and quotient correctly
+    rounded: 2e-7 + 1e-7 |gelu| everywhere (the kernel's stated bound leaves 2e-7 |gelu| for the two
+    approximate instructions) and 4e-6 of the value for |x| <= 6 (stated: 5e-6)."""
+    from scipy.special import erfc
+
+    with open(os.path.join(ROOT, "fastmoe_amd", "csrc", "mx_gemm.hip")) as f:
+        body = re.search(r"float mx_gelu\(float x\) \{(.*?)\n\}", f.read(), re.S)[1]
+    first, *rest = re.findall(r"p = (?:fmaf\(p, t, )?(-?[\d.e-]+)f\)?;", body)
+    assert len(rest) == 12
+
+    def exact(x):
+        x = x.astype(np.float64)
+        return 0.5 * x * erfc(-x / np.sqrt(2))
+
+    def fitted(x):
+        f32, wide = np.float32, np.float64
+
+        def fma(a, b, c):                     # (a product of two f32 is exact in 64 bits)
+            return (a.astype(wide) * b + wide(c)).astype(f32)
+        t = np.minimum(fma(x * x, wide(f32(1 / 18)), -1.0), f32(1))
+        p = np.full_like(x, f32(first))
+        for c in rest:
+            p = fma(p, t.astype(wide), f32(c))
+        with np.errstate(over="ignore"):
+            power = np.exp2((x * p).astype(wide)).astype(f32)
+            quotient = (1 / (f32(1) + power).astype(wide)).astype(f32)
+        return x * quotient
+
+    everywhere = np.concatenate([np.linspace(-30, 30, 2_000_001), np.linspace(-2, 2, 1_000_001),
+                                 -np.logspace(-20, 20, 100_001), np.logspace(-20, 20, 100_001)])
+    x = everywhere.astype(np.float32)
+    want = exact(x)
+    assert (np.abs(fitted(x) - want) <= 2e-7 + 1e-7 * np.abs(want)).all()
+    x = np.linspace(-6, 6, 2_000_000).astype(np.float32)
+    want = exact(x)
+    assert (np.abs(fitted(x) - want) <= 4e-6 * np.abs(want)).all()
