@@ -16,7 +16,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "act_math.h"
 #include "dma_desc.h"
 #include "gemm_tiles.h"
 #include "mx.h"
@@ -34,7 +33,7 @@ struct MxGemmArgs {
   void* y;                     // [n_rows, out], or null with yc
   uint8_t *yc, *ys;            // rows of `out` features
   int64_t n_rows;
-  int in_feat, out_feat, n_expert, act, dtype;
+  int in_feat, out_feat, n_expert, dtype;
 };
 
 __device__ __forceinline__ f32x4 mx_mfma(i32x4 a, int sa, i32x4 b, int sb, f32x4 c) {
@@ -931,7 +930,7 @@ extern "C" int fmoe_mx_linear_fwd(const void* x_codes, const void* x_scales, con
                FMOE_ERR_INVALID, "mx_linear: codes and scales must be 16-byte aligned");
   const MxGemmArgs a{(const uint8_t*)x_codes, (const uint8_t*)x_scales, (const uint8_t*)w_codes,
                      (const uint8_t*)w_scales, bias, seg_off, y, (uint8_t*)y_codes,
-                     (uint8_t*)y_scales, n_rows, (int)in_feat, (int)out_feat, (int)n_expert, act, dtype};
+                     (uint8_t*)y_scales, n_rows, (int)in_feat, (int)out_feat, (int)n_expert, dtype};
   hipStream_t s = (hipStream_t)stream;
   if (y_codes)      // (the element type then is that of the bias alone, which is read as it comes)
     return act == FMOE_ACT_GELU   ? launch<float, kMxQuantGelu>(a, s)
