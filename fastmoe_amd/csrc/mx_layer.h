@@ -91,7 +91,7 @@ Tensor mx_dequantize_rows(const Tensor& codes, const Tensor& scales, int64_t fea
 }
 
 // x in MXFP4 and the segment table of `counts` (int64 row counts on x's device, or on the host),
-// unless that is at hand.
+// unless that is at hand: then rows behind its end, those of dropped slots, are left out.
 struct MxRows {
   Tensor codes, scales, seg;
   MxRows(const Tensor& x, const Tensor& counts_or_seg) {
@@ -102,7 +102,9 @@ struct MxRows {
       return;
     }
     seg = counts ? seg_off_from_counts(counts_or_seg, x, x.size(0)) : counts_or_seg;
-    std::tie(codes, scales) = mx_quantize(x, c10::nullopt);
+    OptTensor live;
+    if (!counts && seg.dim() == 1 && seg.numel() > 0) live = seg.narrow(0, seg.numel() - 1, 1);
+    std::tie(codes, scales) = mx_quantize(x, live);
   }
 };
 

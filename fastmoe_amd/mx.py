@@ -134,7 +134,9 @@ class MXLinear(Function):
                     bool((counts < 0).any()) or int(counts.sum()) > x.shape[0]):
                 raise RuntimeError("expert counts are negative or claim more rows than x holds")
             seg_off = counts.contiguous() if on_device else _segments(counts, x.device)
-            codes, scales = fmoe_cuda.mx_quantize(x)
+            # (rows behind a segment table's end, those of dropped slots, are left out)
+            host = isinstance(counts, torch.Tensor) and not on_device
+            codes, scales = fmoe_cuda.mx_quantize(x, None if host else seg_off[-1:])
         out = torch.empty((x.shape[0], w_codes.shape[1]), dtype=x.dtype, device=x.device)
         fmoe_cuda.mx_linear_fwd(codes, scales, w_codes, w_scales, in_feat, bias, seg_off, out)
         ctx.in_feat = in_feat

@@ -358,3 +358,25 @@ def test_gelu_moves_only_codes_on_a_boundary(k, n, counts):
     power = torch.exp2(torch.round(torch.log2(top)))
     assert ((mine == theirs) | ((top - power).abs() <= near(top))).all()
     assert (on_boundary | (mine != theirs)).all()
+
+
+def test_rows_of_dropped_slots_are_not_quantised(monkeypatch):
+    from fastmoe_amd import fmoe_cuda, mx
+    from fastmoe_amd.functions import RoutePlan
+
+    w = mx.quantize(torch.randn(9, 40, 96, device="cuda"))
+    plan = RoutePlan(torch.from_numpy(make_gate(200, 2, 9, drop=0.4)).cuda(), 9)
+    live = int(plan.n_rows_dev)
+    x = torch.randn(400, 96, device="cuda")
+    y = mx.linear(x, plan.segments, w)
+    assert 0 < live < 300 and torch.equal(y[:live], mx.linear(x, plan.segments.counts, w)[:live])
+    told = []
+    quantize = fmoe_cuda.mx_quantize
+    monkeypatch.setattr(fmoe_cuda, "mx_quantize",
+                        lambda x, n=None: told.append(n) or quantize(x, n))
+    monkeypatch.setattr(fmoe_cuda, "profile_hook", lambda *event: None)
+    assert torch.equal(mx.linear(x, plan.segments, w)[:live], y[:live])
+    assert [int(n) for n in told] == [live]
+    assert torch.equal(mx.linear(x, plan.segments.cpu(), w)[:live], y[:live]) and told[1] is None
+    with pytest.raises(RuntimeError):                      # no segment table
+        mx.linear(x, torch.empty(0, dtype=torch.int32, device="cuda"), w)
