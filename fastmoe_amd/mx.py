@@ -282,12 +282,40 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
                w2.features, b2, act)
 
 
+def _experts(inp, counts, w1, b1, w2, b2, activation):
+    r"""The experts on rows in expert order, operator by operator."""
+    x = linear(_as(inp, b1), counts, w1, b1)
+    live = counts.seg_off[-1:] if isinstance(counts, SegmentTable) else None
+    x = _activate(activation, x, live)
+    return linear(_as(x, b2), counts, w2, b2)
+
+
+class _MXExpertView:
+    r"""`experts[i]` of an MXExpert: called like an MXExpert of one expert, on views of the
+    weights `w1`, `w2` (MXTensor [1, out, in]) and of the biases `b1`, `b2` (gradients flow into
+    the parameters)."""
+
+    def __init__(self, parent: "MXExpert", i: int):
+        def one(w):
+            return MXTensor(w.codes[i:i + 1], w.scales[i:i + 1], w.features)
+        self.w1, self.w2 = one(parent.w1), one(parent.w2)
+        self.b1, self.b2 = (None if b is None else b[i:i + 1] for b in (parent.b1, parent.b2))
+        self.activation = parent.activation
+
+    def __call__(self, inp, fwd_expert_count):
+        return _experts(inp, fwd_expert_count, self.w1, self.b1, self.w2, self.b2,
+                        self.activation)
+
+    def parameters(self):
+        return (b for b in (self.b1, self.b2) if b is not None)
+
+
 class MXExpert(nn.Module):
     r"""The experts of a layer (`linear -> activation -> linear`) with 4-bit weights, in the
     place of the fused `_Expert`: `layer.experts = MXExpert.from_expert(layer.experts)`, or
     `quantize_experts(layer)`.  Weights are uint8 buffers and frozen; the biases stay
-    parameters.  Accepts host counts or a device-side SegmentTable, and casts its rows to its
-    parameters' dtype, as `_Expert` does."""
+    parameters.  Accepts host counts or a device-side SegmentTable, casts its rows to its
+    parameters' dtype, and gives views of single experts, as `_Expert` does."""
 
     accepts_segment_table = True
 
@@ -336,10 +364,8 @@ class MXExpert(nn.Module):
         return MXTensor(self.w2_codes, self.w2_scales, self.hidden_features)
 
     def forward(self, inp, fwd_expert_count):
-        x = linear(_as(inp, self.b1), fwd_expert_count, self.w1, self.b1)
-        live = fwd_expert_count.seg_off[-1:] if isinstance(fwd_expert_count, SegmentTable) else None
-        x = _activate(self.activation, x, live)
-        return linear(_as(x, self.b2), fwd_expert_count, self.w2, self.b2)
+        return _experts(inp, fwd_expert_count, self.w1, self.b1, self.w2, self.b2,
+                        self.activation)
 
     # what FMoE.forward asks of a module that can run the whole dispatch
     def can_run_layer(self, inp, top_k) -> bool:
@@ -360,6 +386,14 @@ class MXExpert(nn.Module):
 
     def __len__(self):
         return self.num_expert
+
+    def __getitem__(self, i):
+        if not -self.num_expert <= i < self.num_expert:
+            raise IndexError(f"expert {i} of {self.num_expert}")
+        return _MXExpertView(self, i % self.num_expert)
+
+    def __iter__(self):
+        return (_MXExpertView(self, i) for i in range(self.num_expert))
 
 
 def quantize_experts(layer):

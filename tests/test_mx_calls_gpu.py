@@ -380,3 +380,30 @@ def test_rows_of_dropped_slots_are_not_quantised(monkeypatch):
     assert torch.equal(mx.linear(x, plan.segments.cpu(), w)[:live], y[:live]) and told[1] is None
     with pytest.raises(RuntimeError):                      # no segment table
         mx.linear(x, torch.empty(0, dtype=torch.int32, device="cuda"), w)
+
+
+# ------------------------------------------------------------------ single experts
+def test_single_experts_are_views_of_the_module():
+    ex = _layer(dtype=torch.float32).experts
+    x, counts = torch.randn(40, 96, device="cuda"), [5, 0, 10, 15, 0, 3, 0, 7]
+    whole = ex(x, torch.tensor(counts))
+    dy = torch.randn_like(whole)
+    whole.backward(dy)
+    grads = [b.grad.clone() for b in (ex.b1, ex.b2)]
+    ex.zero_grad()
+    at = 0
+    assert len(list(ex)) == len(ex) == 8
+    for i, (one, c) in enumerate(zip(ex, counts)):
+        y = one(x[at:at + c], torch.tensor([c]))
+        assert torch.equal(y, ex[i - 8](x[at:at + c], torch.tensor([c])))
+        # (fewer rows may take a kernel that adds in another order: 1e-6, and a hidden value in
+        # 10^5 on the other side of a rounding boundary)
+        assert (y - whole[at:at + c]).norm() <= 2e-3 * whole.norm()
+        assert len(list(one.parameters())) == 2
+        y.backward(dy[at:at + c])
+        at += c
+    for b, g in zip((ex.b1, ex.b2), grads):
+        assert (b.grad - g).norm() <= 2e-3 * g.norm()
+    for i in (8, -9):
+        with pytest.raises(IndexError):
+            ex[i]
