@@ -407,3 +407,105 @@ def test_single_experts_are_views_of_the_module():
     for i in (8, -9):
         with pytest.raises(IndexError):
             ex[i]
+
+
+# ------------------------------------------------------------------ values of whole layers
+# The hidden values are taken from the kernels, in 4 bits (other tests hold what these may be), so
+# that no code on the other side of a rounding boundary blurs the rest.
+UNIT = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}      # bounds of one rounding
+
+
+def _problem(dt, n_expert=6, tokens=150, top_k=3, d=160, h=288):
+    from fastmoe_amd import mx
+
+    g = torch.Generator(device="cuda").manual_seed(len(dt) + d)
+    draw = lambda *shape: torch.randn(*shape, device="cuda", generator=g)
+    idx = torch.from_numpy(make_gate(tokens, top_k, n_expert, drop=0.15, seed=4)).cuda()
+    idx[7] = -1
+    w1, w2 = mx.quantize(draw(n_expert, h, d) * 0.1), mx.quantize(draw(n_expert, d, h) * 0.1)
+    put = lambda a: a.to(DTYPES[dt])
+    return (idx, w1, w2, put(draw(tokens, d)), put(draw(tokens, top_k).abs()),
+            put(draw(n_expert, h) * 0.2), put(draw(n_expert, d) * 0.2), put(draw(tokens, d)))
+
+
+def _rows(idx, n_expert):
+    """(token, slot, expert) of the live rows in expert order."""
+    flat = idx.reshape(-1)
+    order = flat.sort(stable=True)[1][int((flat < 0).sum()):]
+    return order // idx.shape[1], order % idx.shape[1], flat[order]
+
+
+def _values64(w):
+    return w.dequantize(torch.float32).double()
+
+
+def _per_row(rows, w, expert):
+    """rows @ w[expert of the row].T"""
+    out = rows.new_zeros(len(rows), w.shape[1])
+    for e in range(w.shape[0]):
+        out[expert == e] = rows[expert == e] @ w[e].T
+    return out
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("act", [1, 2])
+def test_expert_layer_value_by_value(dt, act):
+    from fastmoe_amd import fmoe_cuda, mx
+
+    idx, w1, w2, x, score, b1, b2, _ = _problem(dt)
+    module = (torch.nn.GELU(), torch.nn.ReLU())[act - 1]
+    got = mx.expert_layer(x, idx, score, w1, b1, w2, b2, module)
+    tok, slot, expert = _rows(idx, 6)
+    seg = torch.bincount(expert, minlength=6).cumsum(0)
+    seg = torch.cat([seg.new_zeros(1), seg]).int()
+    q = mx.quantize(x[tok])
+    hidden = mx.MXTensor(*fmoe_cuda.mx_linear_act_fwd(q.codes, q.scales, w1.codes, w1.scales,
+                                                      160, b1, seg, act), 288)
+    hidden, v2 = _values64(hidden), _values64(w2)
+    y = _per_row(hidden, v2, expert) + b2.double()[expert]
+    mag = _per_row(hidden.abs(), v2.abs(), expert) + b2.double().abs()[expert]
+    s = score.double()[tok, slot, None]
+    zero = torch.zeros(len(x), 160, dtype=torch.float64, device="cuda")
+    want = zero.index_add(0, tok, s * y)
+    # a row's sum in f32, its rounding to the type, the weighted sum, its rounding to the type
+    tol = UNIT[dt] * (zero.index_add(0, tok, s * y.abs()) + want.abs()) + \
+        2.0 ** -22 * (288 / 128 + 8) * zero.index_add(0, tok, s * mag)
+    assert ((got.double() - want).abs() <= tol).all()
+    assert not got[7].any()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("act", [torch.nn.GELU(), torch.nn.ReLU(), torch.nn.SiLU()])
+def test_expert_layer_trains_in_every_type(dt, act):
+    from fastmoe_amd import functions, mx
+
+    idx, w1, w2, *tensors = _problem(dt)
+    x, score, b1, b2 = (t.clone().requires_grad_(True) for t in tensors[:4])
+    dy = tensors[4]
+    got = mx.expert_layer(x, idx, score, w1, b1, w2, b2, act)
+    got.backward(dy)
+    got = [got.detach(), x.grad, score.grad, b1.grad, b2.grad]
+    assert all(g.dtype == DTYPES[dt] for g in got)
+    x, score, b1, b2 = tensors[:4]
+    tok, slot, expert = _rows(idx, 6)
+    counts = torch.bincount(expert, minlength=6)
+    pre = mx.linear(x[tok], counts, w1, b1)
+    hidden = _values64(mx.quantize(functions.apply_activation(act, pre)))
+    v1, v2, s, g = _values64(w1), _values64(w2), score.double()[tok, slot, None], dy.double()[tok]
+    y = _per_row(hidden, v2, expert) + b2.double()[expert]
+    # the rounding of the hidden layer passes its gradient straight through
+    leaf = pre.double().requires_grad_(True)
+    act(leaf).backward(_per_row(s * g, v2.transpose(1, 2), expert))
+    zero = torch.zeros(len(x), 160, dtype=torch.float64, device="cuda")
+    by_expert = lambda a: a.new_zeros(6, a.shape[1]).index_add(0, expert, a)
+    dscore = torch.zeros(idx.shape, dtype=torch.float64, device="cuda")
+    dscore[tok, slot] = (g * y).sum(1)
+    want = [zero.index_add(0, tok, s * y),
+            zero.index_add(0, tok, _per_row(leaf.grad, v1.transpose(1, 2), expert)), dscore,
+            by_expert(leaf.grad), by_expert(s * g)]
+    # at most eight roundings to the type in a row (dx: the row of dy, of dh, of the activation's
+    # gradient, of dx, their sum), in the norm; in f32 also sums of up to 450 terms
+    tol = 8 * UNIT[dt] + 450 * 2.0 ** -24
+    for a, b, name in zip(got, want, ("y", "dx", "dscore", "db1", "db2")):
+        assert (a.double() - b).norm() <= tol * b.norm(), name
+    assert not got[1][7].any() and not got[2][idx < 0].any()
