@@ -401,8 +401,8 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(MxGemmArgs a) {
 // into pieces of 256 bytes of a row (stored from the registers, 64 bytes of each of 16 rows at a
 // time, they took 16 us a tile instead of 9).
 //
-// Measured: 32768 rows of 8 experts, 16384 -> 4096, 926 us, 4.75 PFLOP/s; 4096 -> 14336 938 us,
-// 4.10.  A loop of these matrix instructions alone reaches 7.3 on random codes (9.7 on zeros: the
+// Measured: 32768 rows of 8 experts, 16384 -> 4096, 926 us, 4.75 PFLOP/s; 4096 -> 14336 917 us,
+// 4.20.  A loop of these matrix instructions alone reaches 7.3 on random codes (9.7 on zeros: the
 // card's power limit sets the clock).  Of the first shape's 1.68 M cycles at 1.9 GHz the matrix
 // pipes are busy for 1.05; without copies it takes 1.45 M, without fragment reads as many as with
 // them.  128 x 128 tiles on 15560 rows of 128 experts, 2048 -> 1408: 61 us, 257 MB at 4.2 TB/s.
@@ -838,17 +838,19 @@ constexpr int kCus = 256;
 
 // Which kernel: by the mean number of rows per expert, the features and the number of tiles this
 // makes.  Measured with three sets of operands in turn (us; GELU and quantisation behind the
-// products marked q):
-//   rows  experts  in -> out        stream   128x64  128x128  256x256
-//    128   16    4096 -> 1024           10       13       15       29
-//     64   16    1024 -> 4096           12       10       11       17
-//    128    8    4096 -> 14336 q        90       56       62       99
-//   4096   32    4096 -> 1024          140       29       25       32
-//  15560  128    2048 -> 1408 q        325       83       68      109
-//  30000   16    2048 -> 2048          729      116       89       84
-//  32768    8    4096 -> 14336                           1239      980
-//  16384    4    4096 -> 11008 q                          542      549
-//  32768    8    4096 -> 14336 q                         1376     1311
+// products marked q), with even loads and, behind the slash, with half of all rows on one expert;
+// two runs differ by up to 10 % below 100 us:
+//   rows  experts  in -> out        stream     128x64   128x128  256x256
+//    128   16    4096 -> 1024      11 / 13    12 / 12   14 / 14   27 / 27
+//     64   16    1024 -> 4096      12 / 12    10 / 10   11 / 11   16 / 15
+//    128    8    4096 -> 14336 q   68 / 85    54 / 51   60 / 62   91 / 90
+//   4096   32    4096 -> 1024     114 / 118   18 / 26   18 / 25   29 / 29
+//  15560  128    2048 -> 1408 q   338 / 280   78 / 75   62 / 78  102 / 130
+//  30000   16    2048 -> 2048     727 / 725  110 / 109  80 / 79   74 / 74
+//  32768    8    4096 -> 14336              1649 / 1661 1222 / 1231 917 / 959
+//  16384    4    4096 -> 11008 q             696 / 706  510 / 526  495 / 515
+//  32768    8    4096 -> 14336 q            1806 / 1825 1326 / 1384 1235 / 1272
+// The mean stands for both: what it picks is within 5 % of the best under these uneven loads too.
 // Few rows and few tiles: the kernel that splits K.  The largest tiles move the least through L2
 // and win where K is long and there are rounds enough of them; smaller ones share a CU by two, so
 // that one's beginning and end (with GELU, half its time) are the other's middle.

@@ -171,6 +171,10 @@ Tensor mx_expert_layer(const Tensor& x_in, const Tensor& gate_idx, const Tensor&
   const Tensor &seg = std::get<2>(r), &inv = *std::get<3>(r);
   auto q = mx_quantize_tokens(x, inv, k);
   auto h = mx_linear_act_fwd(std::get<0>(q), std::get<1>(q), w1c, w1s, in_f, contiguous(b1), seg, act);
+  // The experts' rows have x's type on their way to the combine, as those of the 16-bit experts
+  // do.  Kept in f32 the result's error against 64 bits would be one rounding's, not 1.4 times
+  // that; 8192 tokens x top-2 of 1024 features in f16 would take 9 us more of 155 (product 53 ->
+  // 54, combine 8 -> 16), 2047 x top-8 of 2048 in bf16 14 of 181 (63 -> 67, 12 -> 22).
   Tensor y = torch::empty({t * k, w2c.size(1)}, x.options());
   mx_linear_fwd(std::get<0>(h), std::get<1>(h), w2c, w2s, hidden, contiguous(b2), seg, y);
   return gather_combine_fwd(y, inv, score_in.reshape({t, k}).contiguous().to(x.scalar_type()), t, k);

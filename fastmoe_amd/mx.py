@@ -230,6 +230,7 @@ class MXExpertLayer(Function):
         codes, scales = fmoe_cuda.mx_linear_act_fwd(
             codes, scales, w1_codes, w1_scales, in_feat, None if b1 is None else b1.contiguous(),
             seg_off, act)
+        # (in x's dtype, not in f32: csrc/mx_layer.h says why)
         out = torch.empty((n_tokens * top_k, w2_codes.shape[1]), dtype=x.dtype, device=x.device)
         fmoe_cuda.mx_linear_fwd(codes, scales, w2_codes, w2_scales, hidden,
                                 None if b2 is None else b2.contiguous(), seg_off, out)
@@ -261,6 +262,8 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
     gate_idx = gate_idx.reshape(-1, top_k)
     b2 = None if b2 is None else b2.to(x.dtype)
     if grads or not act or x.dtype == torch.float64:
+        # (the hidden layer in x's dtype: any activation takes it so, and what its gradient keeps
+        # until the backward pass is half of f32's size)
         score = score.reshape(-1, top_k)
         if torch._C._get_tracing_state() is not None:
             routed = _Route.apply(gate_idx, n_expert)
