@@ -165,6 +165,9 @@ def linear(x: torch.Tensor, fwd_expert_count, weight: MXTensor, bias=None) -> to
         segments = (fwd_expert_count.seg_off if isinstance(fwd_expert_count, SegmentTable)
                     else fwd_expert_count)
         return native.mx_linear(x, segments, weight.codes, weight.scales, weight.features, bias)
+    if isinstance(fwd_expert_count, SegmentTable) and torch._C._get_tracing_state() is not None:
+        raise RuntimeError("a SegmentTable would be a constant of the trace: trace the layer or "
+                           "mx.expert_layer, or hand over counts")
     if x.dim() != 2 or x.shape[1] != weight.features or not x.is_cuda:
         raise RuntimeError(f"x must be a CUDA tensor [rows, {weight.features}]")
     return MXLinear.apply(x, fwd_expert_count, weight.codes, weight.scales, bias)

@@ -112,6 +112,72 @@ def test_forward_mode_differentiation_is_refused(operators, which):
             mx.expert_layer(x, idx, score, w1, None, w2, None, torch.nn.ReLU())
 
 
+def _inputs_of(graph, kind):
+    return [i.node().kind() for n in graph.nodes() if n.kind() == kind for i in n.inputs()]
+
+
+@pytest.mark.parametrize("act", [torch.nn.ReLU(), torch.nn.SiLU()])
+def test_traces_hand_no_uninitialised_memory_to_operators(operators, monkeypatch, act):
+    """Real operators allocate their results with torch.empty and fill them behind tracing's back:
+    a traced call may only ever see what a recorded function returned."""
+    from fastmoe_amd import fmoe_cuda, mx
+
+    def unseen(fn):
+        def op(*args, **kwargs):
+            def copy(t):
+                out = torch.empty(t.shape, dtype=t.dtype)
+                out.numpy()[...] = t.numpy()
+                return out
+            res = fn(*args, **kwargs)
+            return tuple(map(copy, res)) if isinstance(res, tuple) else copy(res)
+        return op
+
+    for name in ("route", "mx_quantize_tokens", "mx_linear_act_fwd", "gather_combine_fwd"):
+        monkeypatch.setattr(fmoe_cuda, name, unseen(getattr(fmoe_cuda, name)))
+    monkeypatch.setattr(fmoe_cuda, "local_scatter", unseen(
+        lambda x, pos, top_k, live: x.detach()[pos // top_k] + 0))
+
+    class Linear(torch.autograd.Function):     # (MXLinear, which wants the GPU)
+        @staticmethod
+        def forward(ctx, x, seg, out_features):
+            y = x.detach().mean(1, keepdim=True).repeat(1, out_features)
+            y[int(seg[-1]):] = 0
+            return y
+
+        @staticmethod
+        def backward(ctx, grad):
+            return None, None, None
+
+    def linear(x, counts, w, b):
+        seg = counts if torch.is_tensor(counts) else counts.seg_off
+        return Linear.apply(x, seg, int(w.codes.shape[-2]))
+
+    monkeypatch.setattr(mx, "linear", linear)
+    w1, w2 = _weight(H, D, 1), _weight(D, H, 2)
+
+    def layer(x, idx, score):
+        return mx.expert_layer(x, idx, score, w1, None, w2, None, act)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(layer, _inputs(0), check_trace=False)
+        for seed in (0, 1, 2):
+            assert torch.equal(traced(*_inputs(seed)), layer(*_inputs(seed)))
+        assert "aten::empty" not in _inputs_of(traced.graph, "prim::PythonOp")
+        assert "prim::PythonOp" in [n.kind() for n in traced.graph.nodes()]
+
+
+def test_a_segment_table_is_no_constant_of_a_trace():
+    from fastmoe_amd import mx
+    from fastmoe_amd.functions import SegmentTable
+
+    w1, w2 = _weight(H, D, 1), _weight(D, H, 2)
+    experts = mx.MXExpert(w1, None, w2, None, torch.nn.ReLU())
+    segments = SegmentTable(torch.tensor([0, 2, 2, 5], dtype=torch.int32), torch.tensor([2, 0, 3]))
+    for call in (lambda x: mx.linear(x, segments, w1), lambda x: experts(x, segments)):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, torch.randn(5, D), check_trace=False)
+
+
 # ------------------------------------------------------------------ quantising a layer
 @pytest.fixture
 def quantised(monkeypatch):
