@@ -9,7 +9,7 @@ from .gates import BaseGate, GShardGate, NaiveGate, ScoreGate, SwitchGate
 from .layers import FMoE
 from .linear import FMoELinear
 from .transformer import FMoETransformerMLP
-from . import mx
+from . import i8, mx
 
 
 def install_as_fmoe_cuda(compiled: bool = True) -> None:
@@ -44,4 +44,4 @@ def graphed(layer, sample_input, num_warmup_iters: int = 3):
 
 
 __all__ = ["FMoE", "FMoELinear", "FMoETransformerMLP", "BaseGate", "NaiveGate",
-           "GShardGate", "ScoreGate", "SwitchGate", "fmoe_cuda", "mx", "install_as_fmoe_cuda", "graphed"]
+           "GShardGate", "ScoreGate", "SwitchGate", "fmoe_cuda", "i8", "mx", "install_as_fmoe_cuda", "graphed"]

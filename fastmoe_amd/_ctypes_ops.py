@@ -874,6 +874,279 @@ def mx_linear_bwd(dy: torch.Tensor, seg_off: torch.Tensor, w_codes: torch.Tensor
     return dx, db
 
 
+# --------------------------------------------------------------------------
+# Rows in 8-bit integers
+# --------------------------------------------------------------------------
+def _i8_bytes(features: int) -> int:
+    n = _L.fmoe_i8_row_bytes(features)
+    _lib.check(min(n, 0), "i8 row size")
+    return n
+
+
+def _i8_empty(rows: int, features: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    return (torch.empty((rows, _i8_bytes(features)), dtype=torch.int8, device=device),
+            torch.empty(rows, dtype=torch.float32, device=device))
+
+
+def _i8_check(codes: torch.Tensor, scales: torch.Tensor, features: int, name: str) -> None:
+    _dev(codes, name, torch.int8)
+    _dev(scales, name, torch.float32)
+    _need(features >= 1, f"{name}: features must be positive")
+    _need(codes.dim() >= 1 and codes.shape[:-1] == scales.shape
+          and codes.shape[-1] == _i8_bytes(features) and codes.device == scales.device,
+          f"{name}: codes and scales do not hold rows of that many features")
+
+
+def i8_quantize(x: torch.Tensor, n_rows_dev: Optional[torch.Tensor] = None
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of the rows of x [rows, features] in 8 bits (fmoe_i8_quantize)."""
+    _dev(x, "x")
+    _need(x.dim() == 2 and x.shape[1] >= 1, "x must be [rows, features]")
+    if n_rows_dev is not None:
+        _dev(n_rows_dev, "n_rows_dev", torch.int32)
+        _need(n_rows_dev.numel() >= 1 and n_rows_dev.device == x.device,
+              "n_rows_dev must be an int32 on x's device")
+    codes, scales = _i8_empty(x.shape[0], x.shape[1], x.device)
+    with _launch(x, "i8_quantize"):
+        _lib.check(
+            _L.fmoe_i8_quantize(x.data_ptr(), x.shape[0], x.shape[1], _ptr(n_rows_dev),
+                                codes.data_ptr(), scales.data_ptr(), _dt(x, "x"), _stream(x)),
+            "i8_quantize")
+    return codes, scales
+
+
+def i8_quantize_counted(x: torch.Tensor, expert_count: Optional[torch.Tensor] = None
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """i8_quantize of expert-ordered rows and, in the same launch, the seg_off (device
+    int32[E+1]) of their device int64 counts; without counts one expert has all rows."""
+    _dev(x, "x")
+    _need(x.dim() == 2 and x.shape[1] >= 1, "x must be [rows, features]")
+    if expert_count is not None:
+        _dev(expert_count, "expert_count", torch.int64)
+        _need(expert_count.numel() >= 1 and expert_count.device == x.device,
+              "expert_count must lie on x's device")
+    n_expert = 1 if expert_count is None else expert_count.numel()
+    codes, scales = _i8_empty(x.shape[0], x.shape[1], x.device)
+    seg = torch.empty(n_expert + 1, dtype=torch.int32, device=x.device)
+    with _launch(x, "i8_quantize_counted"):
+        _lib.check(
+            _L.fmoe_i8_quantize_counted(x.data_ptr(), x.shape[0], x.shape[1], _ptr(expert_count),
+                                        n_expert, seg.data_ptr(), codes.data_ptr(),
+                                        scales.data_ptr(), _dt(x, "x"), _stream(x)),
+            "i8_quantize_counted")
+    return codes, scales, seg
+
+
+def i8_quantize_tokens(x: torch.Tensor, inv: torch.Tensor, top_k: int
+                       ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """i8_quantize of token rows, written to their places in expert order: rows
+    inv[t * top_k + j] (-1: dropped) of [tokens * top_k] rows."""
+    _dev(x, "x")
+    _dev(inv, "inv", torch.int32)
+    _need(x.dim() == 2 and x.shape[1] >= 1, "x must be [tokens, features]")
+    _need(top_k >= 1 and inv.numel() == x.shape[0] * top_k and inv.device == x.device,
+          "inv must have tokens * top_k entries on x's device")
+    codes, scales = _i8_empty(x.shape[0] * top_k, x.shape[1], x.device)
+    with _launch(x, "i8_quantize_tokens"):
+        _lib.check(
+            _L.fmoe_i8_quantize_tokens(x.data_ptr(), inv.data_ptr(), x.shape[0], top_k,
+                                       x.shape[1], codes.data_ptr(), scales.data_ptr(),
+                                       _dt(x, "x"), _stream(x)),
+            "i8_quantize_tokens")
+    return codes, scales
+
+
+def i8_dequantize(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """Writes the values of 8-bit rows into out [rows, features] and returns it."""
+    _dev(out, "out")
+    _need(out.dim() == 2 and out.shape[1] >= 1, "out must be [rows, features]")
+    _i8_check(codes, scales, out.shape[1], "i8_dequantize")
+    _need(codes.dim() == 2 and codes.shape[0] == out.shape[0] and codes.device == out.device,
+          "i8_dequantize: out has other rows")
+    with _launch(out, "i8_dequantize"):
+        _lib.check(
+            _L.fmoe_i8_dequantize(codes.data_ptr(), scales.data_ptr(), out.shape[0], out.shape[1],
+                                  out.data_ptr(), _dt(out, "out"), _stream(out)),
+            "i8_dequantize")
+    return out
+
+
+def i8_linear_fwd(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.Tensor,
+                  w_scales: torch.Tensor, in_feat: int, bias: Optional[torch.Tensor],
+                  seg_off: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """out[seg_e] = x[seg_e] @ w[e].T + bias[e] on 8-bit rows and weights; returns out."""
+    _i8_check(x_codes, x_scales, in_feat, "x")
+    _i8_check(w_codes, w_scales, in_feat, "weight")
+    _dev(seg_off, "seg_off", torch.int32)
+    _dev(out, "out")
+    _need(x_codes.dim() == 2 and w_codes.dim() == 3, "x must be 2-d and weight 3-d")
+    _need(x_codes.device == w_codes.device == seg_off.device == out.device,
+          "x, weight, seg_off and out must share a device")
+    _need(seg_off.numel() == w_codes.shape[0] + 1, "seg_off must have E+1 entries")
+    _need(out.dim() == 2 and out.shape == (x_codes.shape[0], w_codes.shape[1]),
+          "out must be [rows, out]")
+    if bias is not None:
+        _dev(bias, "bias", out.dtype)
+        _need(bias.dim() == 2 and bias.shape == w_codes.shape[:2] and bias.device == out.device,
+              "bias must be [E, out]")
+    with _launch(out, "i8_linear_fwd"):
+        _lib.check(
+            _L.fmoe_i8_linear_fwd(x_codes.data_ptr(), x_scales.data_ptr(), w_codes.data_ptr(),
+                                  w_scales.data_ptr(), _ptr(bias), seg_off.data_ptr(),
+                                  out.data_ptr(), x_codes.shape[0], in_feat, w_codes.shape[1],
+                                  w_codes.shape[0], _dt(out, "out"), _stream(out)),
+            "i8_linear_fwd")
+    return out
+
+
+def i8_linear_bwd(dy: torch.Tensor, seg_off: torch.Tensor, w_codes: torch.Tensor,
+                  w_scales: torch.Tensor, in_feat: int, need_dx: bool = True,
+                  need_bias: bool = False
+                  ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dbias) in front of frozen 8-bit weights: dx[seg_e] = dy[seg_e] @ w[e], zero in rows
+    that no expert owns."""
+    _dev(dy, "dy")
+    _i8_check(w_codes, w_scales, in_feat, "weight")
+    _dev(seg_off, "seg_off", torch.int32)
+    _need(dy.dim() == 2 and w_codes.dim() == 3 and dy.shape[1] == w_codes.shape[1],
+          "dy must be [rows, out]")
+    _need(dy.device == w_codes.device == seg_off.device,
+          "dy, weight and seg_off must share a device")
+    _need(seg_off.numel() == w_codes.shape[0] + 1, "seg_off must have E+1 entries")
+    e, out_f = w_codes.shape[:2]
+    dx = db = w = None
+    if need_dx:
+        w = dy.new_empty((e * out_f, in_feat))
+        dx = dy.new_empty((dy.shape[0], in_feat))
+        with _launch(dy, "i8_dequantize"):
+            _lib.check(
+                _L.fmoe_i8_dequantize_bwd(w_codes.data_ptr(), w_scales.data_ptr(),
+                                          seg_off.data_ptr(), w.data_ptr(), dx.data_ptr(),
+                                          dy.shape[0], in_feat, out_f, e, _dt(dy, "dy"),
+                                          _stream(dy)),
+                "i8_dequantize_bwd")
+    if need_bias:
+        db = dy.new_empty((e, out_f))
+    if need_dx or need_bias:
+        with _launch(dy, "i8_linear_bwd"):
+            _lib.check(
+                _L.fmoe_grouped_linear_bwd(dy.data_ptr(), dy.data_ptr(), _ptr(w),
+                                           seg_off.data_ptr(), _ptr(dx), None, _ptr(db),
+                                           dy.shape[0], in_feat, out_f, e, _dt(dy, "dy"),
+                                           _stream(dy)),
+                "i8_linear_bwd")
+    return dx, db
+
+
+# --------------------------------------------------------------------------
+# Tokens sorted by expert along a map of truth values
+# --------------------------------------------------------------------------
+MAP_MAX_EXPERTS = 1024   # FMOE_MAP_MAX_EXPERTS of the C ABI
+
+
+def map_plan(routing_map: torch.Tensor, max_rows: int
+             ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(counts int64 [E], seg_off int32 [E+1], token_off int32 [T+1], pairs int32 [max_rows, 2]) of
+    a bool map [T, E] (fmoe_map_plan)."""
+    _dev(routing_map, "routing_map", torch.bool)
+    _need(routing_map.dim() == 2 and routing_map.shape[1] >= 1,
+          "routing_map must be [tokens, experts]")
+    _need(max_rows >= 0, "max_rows must not be negative")
+    t, e = routing_map.shape
+    dev = routing_map.device
+    pairs = torch.empty((max_rows, 2), dtype=torch.int32, device=dev)
+    if t == 0:
+        return (torch.zeros(e, dtype=torch.int64, device=dev),
+                torch.zeros(e + 1, dtype=torch.int32, device=dev),
+                torch.zeros(1, dtype=torch.int32, device=dev), pairs)
+    _need(e <= MAP_MAX_EXPERTS, f"routing_map has more than {MAP_MAX_EXPERTS} experts")
+    counts = torch.empty(e, dtype=torch.int64, device=dev)
+    seg = torch.empty(e + 1, dtype=torch.int32, device=dev)
+    off = torch.empty(t + 1, dtype=torch.int32, device=dev)
+    need = _L.fmoe_map_workspace_bytes(t, e)
+    _lib.check(min(need, 0), "map_plan")
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    with _launch(routing_map, "map_plan"):
+        _lib.check(
+            _L.fmoe_map_plan(routing_map.data_ptr(), t, e, max_rows, counts.data_ptr(),
+                             seg.data_ptr(), off.data_ptr(), pairs.data_ptr(), ws.data_ptr(),
+                             ws.numel(), _stream(routing_map)),
+            "map_plan")
+    return counts, seg, off, pairs
+
+
+def _map_check(given, name, count, weight, seg_off, token_off, pairs) -> None:
+    _dev(given, name)
+    for t, what in ((seg_off, "seg_off"), (token_off, "token_off"), (pairs, "pairs")):
+        _dev(t, what, torch.int32)
+    _need(pairs.dim() == 2 and pairs.shape[1] == 2 and token_off.numel() >= 1
+          and seg_off.numel() >= 2, "the plan's tensors do not belong together")
+    _need(given.dim() == 2 and given.shape[0] == count and given.shape[1] >= 1,
+          f"{name} must be [{count}, features]")
+    _need(given.device == seg_off.device == token_off.device == pairs.device,
+          f"{name} and the plan must share a device")
+    if weight is not None:
+        _dev(weight, "weight")
+        _need(weight.dim() == 2 and weight.shape == (token_off.numel() - 1, seg_off.numel() - 1)
+              and weight.device == given.device,
+              "weight must be [tokens, experts] on the plan's device")
+        _need(weight.dtype in (torch.float32, given.dtype),
+              "weight must be float32 or of the rows' dtype")
+
+
+def map_expand(tokens: torch.Tensor, weight: Optional[torch.Tensor], seg_off: torch.Tensor,
+               token_off: torch.Tensor, pairs: torch.Tensor,
+               given: Optional[torch.Tensor] = None, clear: bool = False
+               ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(rows [max_rows, d]: weight[t, e] * tokens[t] at the row of every pair; with `given` rows also
+    the weights' gradient <tokens[t], given[row]>).  `clear`: rows behind the last are zero."""
+    _map_check(tokens, "tokens", token_off.numel() - 1, weight, seg_off, token_off, pairs)
+    if given is not None:
+        _map_check(given, "rows", pairs.shape[0], weight, seg_off, token_off, pairs)
+        _need(weight is not None and given.shape[1] == tokens.shape[1]
+              and given.dtype == tokens.dtype,
+              "a gradient of weights needs them, and rows like the tokens")
+    rows = tokens.new_empty((pairs.shape[0], tokens.shape[1]))
+    dw = None if given is None else torch.empty_like(weight)
+    if tokens.shape[0] == 0:
+        return (rows.zero_() if clear else rows), dw
+    with _launch(tokens, "map_expand"):
+        _lib.check(
+            _L.fmoe_map_expand(tokens.data_ptr(), _ptr(given), _ptr(weight), token_off.data_ptr(),
+                               pairs.data_ptr(), seg_off[-1:].data_ptr() if clear else None,
+                               rows.data_ptr(), _ptr(dw), tokens.shape[0], tokens.shape[1],
+                               seg_off.numel() - 1, pairs.shape[0], _dt(tokens, "tokens"),
+                               0 if weight is None else _dt(weight, "weight"), _stream(tokens)),
+            "map_expand")
+    return rows, dw
+
+
+def map_reduce(rows: torch.Tensor, weight: Optional[torch.Tensor], seg_off: torch.Tensor,
+               token_off: torch.Tensor, pairs: torch.Tensor,
+               given: Optional[torch.Tensor] = None
+               ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(tokens [T, d]: the sum of weight[t, e] * rows[row] over a token's pairs; with `given` tokens
+    also the weights' gradient <given[t], rows[row]>)."""
+    _map_check(rows, "rows", pairs.shape[0], weight, seg_off, token_off, pairs)
+    if given is not None:
+        _map_check(given, "tokens", token_off.numel() - 1, weight, seg_off, token_off, pairs)
+        _need(weight is not None and given.shape[1] == rows.shape[1] and given.dtype == rows.dtype,
+              "a gradient of weights needs them, and tokens like the rows")
+    tokens = rows.new_empty((token_off.numel() - 1, rows.shape[1]))
+    dw = None if given is None else torch.empty_like(weight)
+    if tokens.shape[0] == 0:
+        return tokens, dw
+    with _launch(rows, "map_reduce"):
+        _lib.check(
+            _L.fmoe_map_reduce(rows.data_ptr(), _ptr(given), _ptr(weight), token_off.data_ptr(),
+                               pairs.data_ptr(), tokens.data_ptr(), _ptr(dw), tokens.shape[0],
+                               rows.shape[1], seg_off.numel() - 1, pairs.shape[0],
+                               _dt(rows, "rows"), 0 if weight is None else _dt(weight, "weight"),
+                               _stream(rows)),
+            "map_reduce")
+    return tokens, dw
+
+
 def _row_len(x: torch.Tensor) -> int:
     return x.shape[-1] if x.dim() >= 1 and x.numel() else 0
 

@@ -95,6 +95,23 @@ SIGNATURES = {
                                     c_void_p]),
     "fmoe_score_topk_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int,
                                     c_int, c_float, c_void_p, c_int, c_void_p]),
+    "fmoe_map_workspace_bytes": (c_int64, [c_int64, c_int32]),
+    "fmoe_map_plan": (c_int, [c_void_p, c_int64, c_int32, c_int64] + [c_void_p] * 5
+                      + [c_int64, c_void_p]),
+    "fmoe_map_expand": (c_int, [c_void_p] * 8 + [c_int64, c_int64, c_int32, c_int64, c_int, c_int,
+                                                 c_void_p]),
+    "fmoe_map_reduce": (c_int, [c_void_p] * 7 + [c_int64, c_int64, c_int32, c_int64, c_int, c_int,
+                                                 c_void_p]),
+    "fmoe_i8_row_bytes": (c_int64, [c_int64]),
+    "fmoe_i8_quantize": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int,
+                                 c_void_p]),
+    "fmoe_i8_quantize_counted": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                         c_void_p, c_void_p, c_int, c_void_p]),
+    "fmoe_i8_quantize_tokens": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                                        c_void_p, c_int, c_void_p]),
+    "fmoe_i8_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "fmoe_i8_dequantize_bwd": (c_int, [c_void_p] * 5 + [c_int64] * 4 + [c_int, c_void_p]),
+    "fmoe_i8_linear_fwd": (c_int, [c_void_p] * 7 + [c_int64] * 4 + [c_int, c_void_p]),
     "fmoe_mx_code_bytes": (c_int64, [c_int64]),
     "fmoe_mx_scale_bytes": (c_int64, [c_int64]),
     "fmoe_mx_quantize": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int,

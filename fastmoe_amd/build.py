@@ -20,9 +20,10 @@ LIB_PATH = os.path.join(LIB_DIR, "libfmoe_hip.so")
 
 # the two heavy translation units first, so that they compile side by side
 SOURCES = ["gemm_mfma_bf16.hip", "gemm_mfma_f16.hip", "api.hip", "route.hip", "dispatch.hip",
-           "gate.hip", "score_gate.hip", "mx.hip", "mx_gemm.hip", "gate_grad.hip", "act.hip", "gemm_simt.hip", "gemm_mfma.hip", "gemm_plain.hip",
+           "gate.hip", "score_gate.hip", "mx.hip", "mx_gemm.hip", "i8.hip",
+           "i8_gemm.hip", "map.hip", "gate_grad.hip", "act.hip", "gemm_simt.hip", "gemm_mfma.hip", "gemm_plain.hip",
            "gemm_mfma_wide.hip"]
-HEADERS = ["common.h", "gemm.h", "gemm_tiles.h", "act_math.h", "mx.h",
+HEADERS = ["common.h", "gemm.h", "gemm_tiles.h", "act_math.h", "mx.h", "i8.h", "rows.h", "quant_gemm.h",
            "dma_desc.h", "gemm_mfma_impl.h",
            os.path.join("..", "..", "include", "fmoe_hip.h")]
 # the library carries a digest of the files it was built from behind this marker
@@ -120,6 +121,7 @@ def ext_source_hash() -> str:
 
     h = hashlib.sha256()
     for path in (EXT_SRC, os.path.join(CSRC, "moe_layer.h"), os.path.join(CSRC, "mx_layer.h"),
+                 os.path.join(CSRC, "i8_layer.h"), os.path.join(CSRC, "map_layer.h"),
                  os.path.join(PKG_DIR, "..", "include", "fmoe_hip.h")):
         with open(path, "rb") as f:
             h.update(f.read() + b"\0")

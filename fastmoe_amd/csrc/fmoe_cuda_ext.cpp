@@ -746,6 +746,8 @@ Tensor gelu_bwd(Tensor dy, Tensor x, OptTensor n_rows_dev) {
 
 #include "moe_layer.h"   // the whole layer as one native autograd node
 #include "mx_layer.h"    // scored routing and 4-bit experts
+#include "i8_layer.h"    // 8-bit rows and products
+#include "map_layer.h"   // tokens sorted by expert along a map
 
 namespace {
 
@@ -817,6 +819,28 @@ PYBIND11_MODULE(fmoe_cuda, m) {
   m.def("mx_linear_bwd", &mx_linear_bwd, py::arg("dy"), py::arg("seg_off"), py::arg("w_codes"),
         py::arg("w_scales"), py::arg("in_feat"), py::arg("need_dx") = true,
         py::arg("need_bias") = false);
+  m.def("i8_quantize", &i8_quantize, py::arg("x"), py::arg("n_rows_dev") = py::none());
+  m.def("i8_quantize_counted", &i8_quantize_counted, py::arg("x"),
+        py::arg("expert_count") = py::none());
+  m.def("i8_quantize_tokens", &i8_quantize_tokens, py::arg("x"), py::arg("inv"), py::arg("top_k"));
+  m.def("i8_dequantize", &i8_dequantize, py::arg("codes"), py::arg("scales"), py::arg("out"));
+  m.def("i8_linear_fwd", &i8_linear_fwd, py::arg("x_codes"), py::arg("x_scales"),
+        py::arg("w_codes"), py::arg("w_scales"), py::arg("in_feat"), py::arg("bias"),
+        py::arg("seg_off"), py::arg("out"));
+  m.def("i8_linear_bwd", &i8_linear_bwd, py::arg("dy"), py::arg("seg_off"), py::arg("w_codes"),
+        py::arg("w_scales"), py::arg("in_feat"), py::arg("need_dx") = true,
+        py::arg("need_bias") = false);
+  m.def("i8_quantize_rows", &i8_quantize_rows);
+  m.def("i8_dequantize_rows", &i8_dequantize_rows);
+  m.def("i8_linear", &i8_linear);
+  m.def("map_plan", &map_plan, py::arg("routing_map"), py::arg("max_rows"));
+  m.def("map_expand", &map_expand, py::arg("tokens"), py::arg("weight"), py::arg("seg_off"),
+        py::arg("token_off"), py::arg("pairs"), py::arg("given") = py::none(),
+        py::arg("clear") = false);
+  m.def("map_reduce", &map_reduce, py::arg("rows"), py::arg("weight"), py::arg("seg_off"),
+        py::arg("token_off"), py::arg("pairs"), py::arg("given") = py::none());
+  m.def("sort_tokens", &sort_tokens);
+  m.def("unsort_tokens", &unsort_tokens);
   m.def("gelu_fwd", &gelu_fwd, py::arg("x"), py::arg("n_rows_dev") = py::none());
   m.def("gelu_bwd", &gelu_bwd, py::arg("dy"), py::arg("x"), py::arg("n_rows_dev") = py::none());
   py::class_<ParamTables>(m, "ParamTables").def(py::init<>());

@@ -1,0 +1,166 @@
+// Tokens sorted by expert and back along a map of truth values: the operators, and each as a native
+// autograd node whose gradient is the other.  Part of the extension (fmoe_cuda_ext.cpp);
+// csrc/mx_layer.h says why such nodes are native.
+#pragma once
+#include <torch/extension.h>
+
+#include <ATen/core/grad_mode.h>
+
+namespace {
+
+// (counts int64 [E], seg_off int32 [E + 1], token_off int32 [T + 1], pairs int32 [max_rows, 2])
+std::tuple<Tensor, Tensor, Tensor, Tensor> map_plan(Tensor map, int64_t max_rows) {
+  dev(map, "routing_map", at::kBool);
+  need(map.dim() == 2 && map.size(1) >= 1, "routing_map must be [tokens, experts]");
+  need(max_rows >= 0, "max_rows must not be negative");
+  c10::DeviceGuard guard(map.device());
+  const int64_t t = map.size(0), e = map.size(1);
+  const auto ints = map.options().dtype(at::kInt);
+  Tensor pairs = torch::empty({max_rows, 2}, ints);
+  if (t == 0)
+    return {torch::zeros({e}, map.options().dtype(at::kLong)), torch::zeros({e + 1}, ints),
+            torch::zeros({1}, ints), pairs};
+  Tensor counts = torch::empty({e}, map.options().dtype(at::kLong));
+  Tensor seg = torch::empty({e + 1}, ints), off = torch::empty({t + 1}, ints);
+  need(e <= FMOE_MAP_MAX_EXPERTS, "routing_map has more than " +
+                                      std::to_string(FMOE_MAP_MAX_EXPERTS) + " experts");
+  const int64_t bytes = fmoe_map_workspace_bytes(t, (int32_t)e);
+  check(bytes < 0 ? (int)bytes : 0, "map_plan");
+  Tensor ws = workspace_of(bytes, map);
+  check(fmoe_map_plan((const uint8_t*)map.data_ptr(), t, (int32_t)e, max_rows,
+                      counts.data_ptr<int64_t>(), seg.data_ptr<int32_t>(), off.data_ptr<int32_t>(),
+                      pairs.data_ptr<int32_t>(), ws.data_ptr(), ws.numel(), stream_of(map)),
+        "map_plan");
+  return {counts, seg, off, pairs};
+}
+
+// What both directions check: rows [max_rows, d] and tokens [T, d] against a plan, and the weight.
+void map_check(const Tensor& given, const char* name, int64_t count, const OptTensor& weight,
+               const Tensor& seg_off, const Tensor& token_off, const Tensor& pairs) {
+  dev(given, name);
+  dev(seg_off, "seg_off", at::kInt);
+  dev(token_off, "token_off", at::kInt);
+  dev(pairs, "pairs", at::kInt);
+  need(pairs.dim() == 2 && pairs.size(1) == 2 && token_off.numel() >= 1 && seg_off.numel() >= 2,
+       "the plan's tensors do not belong together");
+  need(given.dim() == 2 && given.size(0) == count && given.size(1) >= 1,
+       std::string(name) + " must be [" + std::to_string(count) + ", features]");
+  need(given.device() == seg_off.device() && given.device() == token_off.device() &&
+           given.device() == pairs.device(),
+       std::string(name) + " and the plan must share a device");
+  if (weight.has_value() && weight->defined()) {
+    dev(*weight, "weight");
+    need(weight->dim() == 2 && weight->size(0) == token_off.numel() - 1 &&
+             weight->size(1) == seg_off.numel() - 1 && weight->device() == given.device(),
+         "weight must be [tokens, experts] on the plan's device");
+    need(weight->scalar_type() == at::kFloat || weight->scalar_type() == given.scalar_type(),
+         "weight must be float32 or of the rows' dtype");
+  }
+}
+int weight_dtype(const OptTensor& weight) {
+  return weight.has_value() && weight->defined() ? dt(*weight, "weight") : FMOE_F32;
+}
+const Tensor* defined(const OptTensor& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
+
+// (rows [max_rows, d], the weights' gradient if `given` rows are handed over)
+std::tuple<Tensor, OptTensor> map_expand(Tensor tokens, OptTensor weight, Tensor seg_off,
+                                         Tensor token_off, Tensor pairs, OptTensor given,
+                                         bool clear) {
+  map_check(tokens, "tokens", token_off.numel() - 1, weight, seg_off, token_off, pairs);
+  OptTensor dw;
+  if (const Tensor* g = defined(given)) {
+    map_check(*g, "rows", pairs.size(0), weight, seg_off, token_off, pairs);
+    need(defined(weight) && g->sizes()[1] == tokens.size(1) && g->scalar_type() == tokens.scalar_type(),
+         "a gradient of weights needs them, and rows like the tokens");
+  }
+  c10::DeviceGuard guard(tokens.device());
+  Tensor rows = torch::empty({pairs.size(0), tokens.size(1)}, tokens.options());
+  if (defined(given)) dw = torch::empty_like(*weight);
+  if (tokens.size(0) == 0) {
+    if (clear) rows.zero_();
+    return {rows, dw};
+  }
+  check(fmoe_map_expand(tokens.data_ptr(), ptr(given), ptr(weight), token_off.data_ptr<int32_t>(),
+                        pairs.data_ptr<int32_t>(),
+                        clear ? seg_off.data_ptr<int32_t>() + seg_off.numel() - 1 : nullptr,
+                        rows.data_ptr(), ptr(dw), tokens.size(0), tokens.size(1),
+                        (int32_t)(seg_off.numel() - 1), pairs.size(0), dt(tokens, "tokens"),
+                        weight_dtype(weight), stream_of(tokens)),
+        "map_expand");
+  return {rows, dw};
+}
+
+// (tokens [T, d], the weights' gradient if `given` tokens are handed over)
+std::tuple<Tensor, OptTensor> map_reduce(Tensor rows, OptTensor weight, Tensor seg_off,
+                                         Tensor token_off, Tensor pairs, OptTensor given) {
+  map_check(rows, "rows", pairs.size(0), weight, seg_off, token_off, pairs);
+  if (const Tensor* g = defined(given)) {
+    map_check(*g, "tokens", token_off.numel() - 1, weight, seg_off, token_off, pairs);
+    need(defined(weight) && g->sizes()[1] == rows.size(1) && g->scalar_type() == rows.scalar_type(),
+         "a gradient of weights needs them, and tokens like the rows");
+  }
+  c10::DeviceGuard guard(rows.device());
+  OptTensor dw;
+  Tensor tokens = torch::empty({token_off.numel() - 1, rows.size(1)}, rows.options());
+  if (defined(given)) dw = torch::empty_like(*weight);
+  if (tokens.size(0) == 0) return {tokens, dw};
+  check(fmoe_map_reduce(rows.data_ptr(), ptr(given), ptr(weight), token_off.data_ptr<int32_t>(),
+                        pairs.data_ptr<int32_t>(), tokens.data_ptr(), ptr(dw), tokens.size(0),
+                        rows.size(1), (int32_t)(seg_off.numel() - 1), pairs.size(0),
+                        dt(rows, "rows"), weight_dtype(weight), stream_of(rows)),
+        "map_reduce");
+  return {tokens, dw};
+}
+
+// EXPAND: functions.sort_tokens; otherwise functions.unsort_tokens
+template <bool EXPAND> struct MapNode : public torch::autograd::Function<MapNode<EXPAND>> {
+  static Tensor run(const Tensor& from, const OptTensor& weight, const Tensor& seg_off,
+                    const Tensor& token_off, const Tensor& pairs) {
+    return EXPAND ? std::get<0>(map_expand(from, weight, seg_off, token_off, pairs, c10::nullopt, false))
+                  : std::get<0>(map_reduce(from, weight, seg_off, token_off, pairs, c10::nullopt));
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& from_in, const Tensor& seg_off,
+                        const Tensor& token_off, const Tensor& pairs, const OptTensor& weight_in) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor from = from_in.contiguous();
+    OptTensor weight;
+    if (defined(weight_in)) weight = weight_in->contiguous();
+    const bool dot = weight.has_value() && weight_in->requires_grad();
+    ctx->save_for_backward({seg_off, token_off, pairs, weight.has_value() ? *weight : Tensor(),
+                            dot ? from : Tensor()});
+    return run(from, weight, seg_off, token_off, pairs);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list v = ctx->get_saved_variables();
+    c10::DeviceGuard guard(v[0].device());
+    const Tensor g = only_once(grads[0], EXPAND ? "sort_tokens" : "unsort_tokens");
+    auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    auto r = EXPAND ? map_reduce(g, opt(v[3]), v[0], v[1], v[2], opt(v[4]))
+                    : map_expand(g, opt(v[3]), v[0], v[1], v[2], opt(v[4]), true);
+    const OptTensor& dw = std::get<1>(r);
+    return {std::get<0>(r), Tensor(), Tensor(), Tensor(), dw.has_value() ? *dw : Tensor()};
+  }
+};
+
+template <bool EXPAND>
+Tensor map_move(const Tensor& from, const OptTensor& weight, const Tensor& seg_off,
+                const Tensor& token_off, const Tensor& pairs) {
+  need(from.is_cuda(), "the input must be a CUDA tensor");
+  c10::DeviceGuard guard(from.device());
+  if (at::GradMode::is_enabled() &&
+      (from.requires_grad() || (defined(weight) && weight->requires_grad())))
+    return MapNode<EXPAND>::apply(from, seg_off, token_off, pairs, weight);
+  OptTensor w;
+  if (defined(weight)) w = weight->contiguous();
+  return MapNode<EXPAND>::run(from.contiguous(), w, seg_off, token_off, pairs);
+}
+Tensor sort_tokens(const Tensor& x, const OptTensor& weight, const Tensor& seg_off,
+                   const Tensor& token_off, const Tensor& pairs) {
+  return map_move<true>(x, weight, seg_off, token_off, pairs);
+}
+Tensor unsort_tokens(const Tensor& rows, const OptTensor& weight, const Tensor& seg_off,
+                     const Tensor& token_off, const Tensor& pairs) {
+  return map_move<false>(rows, weight, seg_off, token_off, pairs);
+}
+
+}  // namespace

@@ -13,6 +13,7 @@
 #include <algorithm>
 
 #include "mx.h"
+#include "rows.h"
 
 namespace fmoe {
 
@@ -20,35 +21,6 @@ constexpr int kMxThreads = 256;
 constexpr int kMxWaves = kMxThreads / kWave;
 constexpr int kMxChunk = kWave * 8;          // values of a row that a wave takes at once
 static_assert(kMxChunk == kMxGroup, "a chunk's scales are one 16-byte pack");
-
-// N values, moved as one.
-template <typename T, int N> struct alignas(sizeof(T) * N) Run { T v[N]; };
-
-// 8 values of a row from element k on, as f32; zeros from k_total on.  Rows are moved in runs of N
-// values, of which they hold whole ones.
-template <typename T, int N>
-__device__ __forceinline__ void load8(const T* row, int k, int k_total, float (&v)[8]) {
-#pragma unroll
-  for (int p = 0; p < 8; p += N) {
-    Run<T, N> x;
-    const bool in = k + p < k_total;
-    if (in) x = *reinterpret_cast<const Run<T, N>*>(row + k + p);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[p + i] = in ? Elem<T>::to_acc(x.v[i]) : 0.f;
-  }
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void store8(T* row, int k, int k_total, const float (&v)[8]) {
-#pragma unroll
-  for (int p = 0; p < 8; p += N) {
-    if (k + p >= k_total) break;
-    Run<T, N> x;
-#pragma unroll
-    for (int i = 0; i < N; ++i) x.v[i] = Elem<T>::from_acc(v[p + i]);
-    *reinterpret_cast<Run<T, N>*>(row + k + p) = x;
-  }
-}
 
 // Maximum over the four lanes of a block, in each of them.
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
@@ -80,30 +52,6 @@ __device__ __forceinline__ int of_four(const int (&v)[4], int i) {
   return i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
 }
 
-// Row counts of experts as segment bounds, for the call's first workgroup to leave behind.
-struct MxSegments {
-  const int64_t* count = nullptr;
-  int n_expert = 0;
-  int32_t* seg_off = nullptr;
-};
-
-// seg_off = exclusive prefix of the counts, by one wave.  Counts on the device nobody has looked
-// at: negative ones count as zero, and what lies beyond the rows there are is cut off.
-__device__ __forceinline__ void write_segments(const MxSegments& sg, int64_t n_rows, int lane) {
-  int64_t carry = 0;
-  for (int e0 = 0; e0 < sg.n_expert; e0 += kWave) {
-    const int64_t c = e0 + lane < sg.n_expert ? min(max(sg.count[e0 + lane], (int64_t)0), n_rows) : 0;
-    int64_t sum = c;
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int64_t o = __shfl_up(sum, d, kWave);
-      if (lane >= d) sum += o;
-    }
-    if (e0 + lane < sg.n_expert) sg.seg_off[e0 + lane] = (int32_t)min(carry + sum - c, n_rows);
-    carry += __shfl(sum, kWave - 1, kWave);
-  }
-  if (lane == 0) sg.seg_off[sg.n_expert] = (int32_t)min(carry, n_rows);
-}
-
 // The chunks of all rows are numbered row by row; a wave takes U consecutive ones at a time.
 struct MxChunk {
   int64_t row;
@@ -120,7 +68,7 @@ template <typename T, int N, int U>
 __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(
     const T* __restrict__ x, int64_t n_rows, int k, const int32_t* __restrict__ n_rows_dev,
     const int32_t* __restrict__ inv, int top_k, uint8_t* __restrict__ codes,
-    uint8_t* __restrict__ scales, MxSegments segments) {
+    uint8_t* __restrict__ scales, SegmentsOut segments) {
   static_assert(U == 1 || U == 4, "the lanes of a block share the chunks between them");
   const int lane = threadIdx.x & (kWave - 1);
   if (segments.seg_off && blockIdx.x == 0 && threadIdx.x < kWave) write_segments(segments, n_rows, lane);
@@ -176,25 +124,10 @@ __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(
   }
 }
 
-// The rows of a gradient that no expert owns, for mx_dequantize_kernel to clear in passing: rows
-// *end .. n_rows - 1 of k values at p.
-template <typename T> struct MxTail {
-  const int32_t* end = nullptr;
-  T* p = nullptr;
-  int64_t n_rows = 0;
-
-  __device__ __forceinline__ void clear(int k) const {
-    const int64_t stride = (int64_t)gridDim.x * kMxThreads;
-    for (int64_t i = (int64_t)max(*end, 0) * k + (int64_t)blockIdx.x * kMxThreads + threadIdx.x;
-         i < n_rows * k; i += stride)
-      p[i] = Elem<T>::from_acc(0.f);
-  }
-};
-
 template <typename T, int N, int U>
 __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_rows, int k,
-    T* __restrict__ out, MxTail<T> tail) {
+    T* __restrict__ out, ClearedTail<T> tail) {
   if (tail.p) tail.clear(k);
   const int lane = threadIdx.x & (kWave - 1);
   const int chunks = (k + kMxChunk - 1) / kMxChunk;
@@ -244,12 +177,6 @@ struct MxGrid {
   }
 };
 
-// The longest run (of at most 16 bytes) that every row holds a whole number of, at its alignment.
-template <typename T> static int run_length(const void* p, int k) {
-  int n = 16 / (int)sizeof(T);
-  while (n > 1 && (k % n || (uintptr_t)p % (n * sizeof(T)))) n /= 2;
-  return n;
-}
 #define FMOE_RUN(CALL, N)          \
   do {                             \
     if (g.many) CALL(N, 4);        \
@@ -267,7 +194,7 @@ template <typename T> static int run_length(const void* p, int k) {
 template <typename T>
 static int launch_quantize(const void* x, int64_t n_rows, int k, const int32_t* n_rows_dev,
                            const int32_t* inv, int top_k, uint8_t* codes, uint8_t* scales,
-                           const MxSegments& segments, hipStream_t s) {
+                           const SegmentsOut& segments, hipStream_t s) {
   const int run = run_length<T>(x, k);
   const MxGrid g(n_rows, k);
   const dim3 grid(g.blocks);
@@ -289,7 +216,7 @@ static int launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64_
   const dim3 grid(g.blocks);
 #define FMOE_CALL(N, U)                                                                        \
   hipLaunchKernelGGL((mx_dequantize_kernel<T, N, U>), grid, dim3(kMxThreads), 0, s, codes,   \
-                     scales, n_rows, k, (T*)out, MxTail<T>{tail_end, (T*)tail, tail_rows})
+                     scales, n_rows, k, (T*)out, ClearedTail<T>{tail_end, (T*)tail, tail_rows})
   FMOE_RUNS(FMOE_CALL);
 #undef FMOE_CALL
   FMOE_LAUNCH_CHECK("mx_dequantize");
@@ -298,7 +225,7 @@ static int launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64_
 
 static int quantize(const void* x, int64_t n_rows, int64_t k, const int32_t* n_rows_dev,
                     const int32_t* inv, int64_t top_k, void* codes, void* scales, int dtype,
-                    hipStream_t s, const MxSegments& segments = {}) {
+                    hipStream_t s, const SegmentsOut& segments = {}) {
   FMOE_REQUIRE(n_rows >= 0 && k >= 1 && k <= FMOE_MX_MAX_FEATURES, FMOE_ERR_INVALID,
                "mx_quantize: bad sizes");
   FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_F16 || dtype == FMOE_BF16, FMOE_ERR_UNSUPPORTED,

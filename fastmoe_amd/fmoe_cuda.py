@@ -40,6 +40,7 @@ profile_only = None
 
 MAX_GATE_TOP_K = ctypes_ops.MAX_GATE_TOP_K   # FMOE_MAX_GATE_TOP_K of the C ABI
 MAX_EXPERTS = ctypes_ops.MAX_EXPERTS         # FMOE_MAX_EXPERTS: what routing takes
+MAP_MAX_EXPERTS = ctypes_ops.MAP_MAX_EXPERTS # FMOE_MAP_MAX_EXPERTS: what a routing map takes
 init = ctypes_ops.init                       # one-time GPU set-up (fmoe_init), either binding
 
 OPERATORS = ("expert_count", "assign_pos", "linear_forward", "linear_backward",
@@ -50,7 +51,9 @@ OPERATORS = ("expert_count", "assign_pos", "linear_forward", "linear_backward",
              "scatter_reduce", "topk_softmax_fwd", "topk_softmax_bwd", "score_topk_fwd", "score_topk_bwd",
              "mx_quantize", "mx_quantize_counted", "mx_quantize_tokens", "mx_dequantize",
              "mx_linear_fwd",
-             "mx_linear_act_fwd", "mx_linear_bwd", "gelu_fwd", "gelu_bwd", "set_gemm_path", "_seg_off_from_counts")
+             "mx_linear_act_fwd", "mx_linear_bwd", "i8_quantize", "i8_quantize_counted",
+             "i8_quantize_tokens", "i8_dequantize", "i8_linear_fwd", "i8_linear_bwd", "map_plan",
+             "map_expand", "map_reduce", "gelu_fwd", "gelu_bwd", "set_gemm_path", "_seg_off_from_counts")
 
 
 def _hooked(op_name, fn):

@@ -199,6 +199,104 @@ class FusedGatherCombine(Function):
         return dbuf, dscore.view_as(score), None
 
 
+class MapPlan:
+    r"""Which rows tokens become where `routing_map` (bool [tokens, experts], on the GPU) says which
+    expert takes which token: any number of experts per token, as with experts that choose their
+    tokens or with thresholds.  Rows are numbered expert by expert, an expert's in token order.
+
+    `max_rows`: rows of the sorted buffers, e.g. experts * capacity; what the map has beyond is cut
+    off (the last experts' last tokens), and rows it does not fill stay as they were allocated.
+    Without it the map's entries are counted and read back to the host.
+
+    counts    int64[E]   rows per expert, on the device
+    segments  SegmentTable of them, as the expert layers take it
+    """
+
+    def __init__(self, routing_map: torch.Tensor, max_rows=None):
+        if routing_map.dim() != 2 or routing_map.dtype != torch.bool:
+            raise RuntimeError("routing_map must be bool [tokens, experts]")
+        with torch.no_grad():
+            if max_rows is None:
+                max_rows = int(routing_map.sum())
+            self.counts, seg_off, self.token_off, self.pairs = fmoe_cuda.map_plan(
+                routing_map.contiguous(), int(max_rows))
+        self.n_tokens, self.num_expert = routing_map.shape
+        self.max_rows = int(max_rows)
+        self.segments = SegmentTable(seg_off, self.counts)
+
+    @property
+    def n_rows_dev(self) -> torch.Tensor:
+        """Device int32 holding the number of live rows (= seg_off[E])."""
+        return self.segments.seg_off[-1:]
+
+    def _tensors(self):
+        return self.segments.seg_off, self.token_off, self.pairs
+
+
+class _MapExpand(Function):
+    r"""sort_tokens operator by operator; map_reduce is its gradient."""
+
+    @staticmethod
+    def forward(ctx, x, weight, *plan):
+        x = x.contiguous()
+        weight = None if weight is None else weight.contiguous()
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight, *plan)
+        return fmoe_cuda.map_expand(x, weight, *plan)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, *plan = ctx.saved_tensors
+        dx, dw = fmoe_cuda.map_reduce(grad.contiguous(), weight, *plan, x)
+        return dx, dw, None, None, None
+
+
+class _MapReduce(Function):
+    r"""unsort_tokens operator by operator; map_expand is its gradient."""
+
+    @staticmethod
+    def forward(ctx, rows, weight, *plan):
+        rows = rows.contiguous()
+        weight = None if weight is None else weight.contiguous()
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weight, *plan)
+        return fmoe_cuda.map_reduce(rows, weight, *plan)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        rows, weight, *plan = ctx.saved_tensors
+        drows, dw = fmoe_cuda.map_expand(grad.contiguous(), weight, *plan, rows, True)
+        return drows, dw, None, None, None
+
+
+def _no_trace(name):
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{name}: a MapPlan would be a constant of the trace")
+
+
+def sort_tokens(x: torch.Tensor, plan: MapPlan, weight=None) -> torch.Tensor:
+    r"""rows [plan.max_rows, d]: weight[t, e] * x[t] for every token t that expert e takes, in the
+    order of `plan`.  x [tokens, d] float32, float16 or bfloat16; weight [tokens, experts] float32
+    or of x's dtype (None: ones), read where the map is true; both get gradients, the weight's zero
+    elsewhere."""
+    native = fmoe_cuda.native()
+    if native is not None:
+        return native.sort_tokens(x, weight, *plan._tensors())
+    _no_trace("sort_tokens")
+    return _MapExpand.apply(x, weight, *plan._tensors())
+
+
+def unsort_tokens(rows: torch.Tensor, plan: MapPlan, weight=None) -> torch.Tensor:
+    r"""y [tokens, d]: the sum over the experts e that take token t of weight[t, e] * (t's row of
+    e's), summed in float32 in the order of the experts; zero for a token that nobody takes.  Types
+    and gradients as of sort_tokens; rows behind the last of the map's get a gradient of zero."""
+    native = fmoe_cuda.native()
+    if native is not None:
+        return native.unsort_tokens(rows, weight, *plan._tensors())
+    _no_trace("unsort_tokens")
+    return _MapReduce.apply(rows, weight, *plan._tensors())
+
+
 class TopKSoftmax(Function):
     r"""(idx, score) = top-k of the logits and the softmax over the k values,
     the two torch calls of fmoe/gates/naive_gate.py:31-38 as one kernel each

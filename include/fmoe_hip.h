@@ -558,6 +558,89 @@ int fmoe_mx_linear_fwd(const void* x_codes, const void* x_scales, const void* w_
                        int64_t out_feat, int64_t n_expert, int dtype, void* stream);
 
 /*
+ * Tokens sorted by expert and back where `map` [n_tokens, n_expert] (a byte each, not 0: the expert
+ * takes the token) says who takes whom: any number of experts per token, as with experts that
+ * choose their tokens or with thresholds.  Rows are numbered expert by expert, an expert's in token
+ * order; those from max_rows on are cut off.
+ *   _plan    counts int64[n_expert] and seg_off int32[n_expert + 1] of the rows there are, and each
+ *            token's (row, expert) pairs, experts ascending: pairs int32[max_rows][2], those of
+ *            token t from token_off[t] to token_off[t + 1] - 1 (int32[n_tokens + 1]).  n_tokens >= 1.
+ *            The workspace (fmoe_map_workspace_bytes) is 16-byte aligned, pairs 8-byte aligned.
+ *   _expand  rows[r] = weight[t][e] tokens[t] for all pairs (r, e) of t; dweight (if not NULL)
+ *            [t][e] = <tokens[t], given[r]>, 0 without a row.  With n_rows_dev (DEVICE int32, =
+ *            seg_off[n_expert]) the rows from there to max_rows are cleared; without, left as they are.
+ *   _reduce  tokens[t] = sum over the pairs (r, e) of t of weight[t][e] rows[r], 0 without any;
+ *            dweight (if not NULL) [t][e] = <given[t], rows[r]>, 0 without a row.
+ * Each is the other's gradient.  weight and dweight [n_tokens, n_expert] of weight_dtype, which is
+ * f32 or dtype; weight NULL: ones (and no dweight).  Sums in f32, in the order of the experts.
+ * dtype: f32, f16 or bf16.  n_expert <= FMOE_MAP_MAX_EXPERTS, n_tokens * n_expert < 2^31.
+ * They stand beside _local_scatter and _local_gather of fmoe/functions.py:78-90, which take a fixed
+ * number of experts per token.
+ */
+#define FMOE_MAP_MAX_EXPERTS 1024
+int64_t fmoe_map_workspace_bytes(int64_t n_tokens, int32_t n_expert);
+int fmoe_map_plan(const uint8_t* map, int64_t n_tokens, int32_t n_expert, int64_t max_rows,
+                  int64_t* counts, int32_t* seg_off, int32_t* token_off, int32_t* pairs,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+int fmoe_map_expand(const void* tokens, const void* given, const void* weight,
+                    const int32_t* token_off, const int32_t* pairs, const int32_t* n_rows_dev,
+                    void* rows, void* dweight, int64_t n_tokens, int64_t d, int32_t n_expert,
+                    int64_t max_rows, int dtype, int weight_dtype, void* stream);
+int fmoe_map_reduce(const void* rows, const void* given, const void* weight,
+                    const int32_t* token_off, const int32_t* pairs, void* tokens, void* dweight,
+                    int64_t n_tokens, int64_t d, int32_t n_expert, int64_t max_rows, int dtype,
+                    int weight_dtype, void* stream);
+
+/*
+ * Rows in 8-bit integers with one scale each: with a = max |x| over a row, the scale is a / 127
+ * (f32) and the code of x the integer nearest to 127 x / a, ties to even.  A row of zeros has
+ * scale 0; one with an infinity or a NaN has scale NaN and codes 0, i.e. all of it is NaN.  A row
+ * of `features` values takes fmoe_i8_row_bytes() = 128 ceil(features / 128) bytes of codes, zeros
+ * behind the last feature; codes are 16-byte aligned.  features <= FMOE_I8_MAX_FEATURES.
+ *
+ *   _quantize         the rows of x; the first *n_rows_dev rows only, if n_rows_dev (DEVICE int32)
+ *                     is not NULL.
+ *   _quantize_tokens  row t goes to the rows inv[t * top_k + j] that are not -1 (inv of
+ *                     fmoe_route): the dispatch of fmoe_scatter_tokens in the same pass.
+ *   _quantize_counted _quantize of rows in expert order that also writes seg_off (int32
+ *                     [n_expert + 1]) from their DEVICE int64 counts (negative ones count as zero,
+ *                     rows that are not there are cut off); counts NULL: one expert has them all.
+ *   _dequantize       the values, rounded to dtype where that is too narrow for them.
+ *   _dequantize_bwd   what stands in front of fmoe_grouped_linear_bwd for frozen 8-bit weights:
+ *                     w [n_expert * out_feat, in_feat] = their values, and zeros in the rows of
+ *                     dx [n_rows, in_feat] at or behind seg_off[n_expert] (DEVICE), which that
+ *                     call leaves as they are.
+ * dtype: f32, f16 or bf16.  The reference has no such format.
+ */
+#define FMOE_I8_MAX_FEATURES 131072   /* 127 * 127 * 2^17 < 2^31: sums of products are exact */
+int64_t fmoe_i8_row_bytes(int64_t features);
+int fmoe_i8_quantize(const void* x, int64_t n_rows, int64_t features, const int32_t* n_rows_dev,
+                     void* codes, float* scales, int dtype, void* stream);
+int fmoe_i8_quantize_counted(const void* x, int64_t n_rows, int64_t features,
+                             const int64_t* expert_count, int64_t n_expert, int32_t* seg_off,
+                             void* codes, float* scales, int dtype, void* stream);
+int fmoe_i8_quantize_tokens(const void* x, const int32_t* inv, int64_t n_tokens, int64_t top_k,
+                            int64_t features, void* codes, float* scales, int dtype, void* stream);
+int fmoe_i8_dequantize(const void* codes, const float* scales, int64_t n_rows, int64_t features,
+                       void* out, int dtype, void* stream);
+int fmoe_i8_dequantize_bwd(const void* w_codes, const float* w_scales, const int32_t* seg_off,
+                           void* w, void* dx, int64_t n_rows, int64_t in_feat, int64_t out_feat,
+                           int64_t n_expert, int dtype, void* stream);
+
+/*
+ * The grouped linear layer (fmoe_grouped_linear_fwd) on 8-bit operands:
+ *   y[r][n] = x_scales[r] * w_scales[e][n] * sum_k x[r][k] w_e[n][k] + bias[e][n],  r in seg_e
+ * with the sum of integer products exact, and f32 from there on.  x: n_rows rows of in_feat
+ * features; w: n_expert * out_feat rows of in_feat features; bias [n_expert, out_feat] of `dtype`
+ * or NULL; y [n_rows, out_feat] of `dtype` (f32, f16 or bf16).  Rows at or behind
+ * seg_off[n_expert] are not written.
+ */
+int fmoe_i8_linear_fwd(const void* x_codes, const float* x_scales, const void* w_codes,
+                       const float* w_scales, const void* bias, const int32_t* seg_off, void* y,
+                       int64_t n_rows, int64_t in_feat, int64_t out_feat, int64_t n_expert,
+                       int dtype, void* stream);
+
+/*
  * y[i] = gelu(x[i]) = 0.5 x (1 + erf(x / sqrt 2)) over n elements, and
  * dx[i] = dy[i] * gelu'(x[i]): the activation between the two expert layers,
  * fmoe/transformer.py:28-30 with the default torch.nn.GELU() of
