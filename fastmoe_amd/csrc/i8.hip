@@ -1,14 +1,20 @@
 // Quantisation of rows to 8-bit integers and back on gfx950 (the format: i8.h).
 //
 // Both directions are bound by HBM: a value costs its own 2 or 4 bytes plus one.  The scale needs
-// the whole row before the first code, so a wave, or four, keeps a row in registers between the two
-// (up to 4096 or 16384 values; what is longer is read a second time, from L2 as a rule).
+// the whole row before the first code, so up to eight waves keep a row in registers between the two
+// (4 KiB each; what is longer is read a second time, from L2 as a rule), and the next row is on its
+// way meanwhile.
 //
-// A code is one multiply-add: t = x (127 / a) + 1.5 * 2^23 rounds the product to an integer whose
-// low byte is the code.  That is wrong at most for products within 2^-15 of a half-way point (the
-// quotient's error is 2^-24 of at most 127); a lane that holds one decides it exactly, by the sign
-// of 127 |x| - (k + 1/2) a, whose terms have at most 19 bits for 16-bit x (32 for f32, where the
-// sign is taken in f64).
+// A code is one multiply-add: t = x (127 / a) + 1.5 * 2^23 rounds the product, taken exactly, to an
+// integer whose low byte is the code.  The quotient is off by up to 2^-23 of itself, and so is the
+// product r = 127 x / a near a half-way point k + 1/2.  The distance there is |254 x - (2 k + 1) a| /
+// (2 a): with x and a of m bits, it is zero or at least 2^-m / 254 of r, so that for 16-bit types
+// (m = 8, 11) only exact ties can go wrong.  254 x = (2 k + 1) a needs 127 to divide 2 k + 1, which
+// is k = 63, or the digits of a.  The first goes to the even 64 if the quotient is rounded up, which
+// it is; rows with the second, 1 in 128, decide every code by the sign of 127 |x| - (k + 1/2) a,
+// whose terms have at most 19 bits.  f32 values do so, in f64, where a product is within 2^-15 of a
+// half-way point.  (Looking for such products in 16-bit rows as well, where every x = a / 2 is one,
+// took 25 instructions a value in place of @@, and 306 us for 114688 x 4096.)
 #include <algorithm>
 
 #include "i8.h"
@@ -16,59 +22,72 @@
 
 namespace fmoe {
 
-constexpr int kI8Threads = 256;
-constexpr int kI8Waves = kI8Threads / kWave;
+constexpr int kI8Threads = 256;              // of a block that dequantises
 constexpr int kI8Chunk = kWave * 8;          // values that a wave takes at once
-constexpr int kI8Held = 8;                   // chunks of a row in a wave's registers
+constexpr int kI8HeldBytes = 4096;           // of a row in a wave's registers
+constexpr float kI8Magic = 12582912.f;       // 1.5 * 2^23: a float there has integers as its steps
 
 // What turns a row's values into codes.
 struct I8Row {
   float unit;       // power of two that keeps everything below in range
   float top;        // the largest magnitude, times unit
-  float inv;        // 127 / top
+  float inv;        // 127 / top, rounded up
   float scale;      // 0 for a row of zeros, NaN for one that is not finite
   bool finite;
+  bool ties;        // of 16-bit values: there may be ties other than top / 2
 
   __device__ __forceinline__ explicit I8Row(uint32_t top_bits) {
     finite = top_bits < 0x7f800000u;
     const float a = __uint_as_float(finite ? top_bits : 0u);
     unit = a < 0x1p-60f ? 0x1p64f : a > 0x1p60f ? 0x1p-64f : 1.f;
     top = a * unit;
-    inv = top > 0.f ? 127.f / top : 0.f;
+    inv = 127.f / top;
+    if (fmaf(inv, top, -127.f) < 0.f) inv = __uint_as_float(__float_as_uint(inv) + 1);
+    if (!(top > 0.f)) inv = 0.f;
+    ties = ((__float_as_uint(top) & 0x7fffffu) | 0x800000u) % 127 == 0;
     scale = finite ? a / 127.f : __uint_as_float(0x7fc00000u);
   }
-};
 
-constexpr float kI8Magic = 12582912.f;       // 1.5 * 2^23: a float there has integers as its steps
-
-// The codes of 8 values, v[0] in the lowest byte.  EXACT: f32 for 16-bit values, f64 for f32.
-template <typename EXACT>
-__device__ __forceinline__ uint2 i8_codes(const float (&v)[8], const I8Row& row) {
-  float t[8], off = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = v[i] * row.unit;
-    t[i] = fmaf(x, row.inv, kI8Magic);
-    off = fmaxf(off, fabsf(fmaf(x, row.inv, kI8Magic - t[i])));
+  // The code of x, as a float, decided exactly.
+  template <typename EXACT> __device__ __forceinline__ float decide(float x) const {
+    const float k = floorf(fabsf(x) * inv);
+    const EXACT side = fma(-((EXACT)k + (EXACT)0.5), (EXACT)top, (EXACT)127 * (EXACT)fabsf(x));
+    const bool odd = (int)k & 1;
+    return copysignf(side > 0 || (side == 0 && odd) ? k + 1.f : k, x);
   }
-  if (off > 0.5f - 0x1p-15f) {
+
+  // The codes of 8 values, v[0] in the lowest byte.
+  template <typename T> __device__ __forceinline__ uint2 codes(const Eight<T>& from) const {
+    float v[8], t[8];
+    from.widen(v);
+    if (unit != 1.f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = fabsf(v[i] * row.unit);
-      const float k = floorf(x * row.inv);
-      const EXACT side = fma(-((EXACT)k + (EXACT)0.5), (EXACT)row.top, (EXACT)127 * (EXACT)x);
-      const bool odd = (int)k & 1;
-      const float q = side > 0 || (side == 0 && odd) ? k + 1.f : k;
-      t[i] = copysignf(q, v[i]) + kI8Magic;
+      for (int i = 0; i < 8; ++i) v[i] *= unit;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = fmaf(v[i], inv, kI8Magic);
+    if constexpr (sizeof(T) == 2) {
+      if (ties) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = decide<float>(v[i]) + kI8Magic;
+      }
+    } else {
+      float off = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) off = fmaxf(off, fabsf(fmaf(v[i], inv, kI8Magic - t[i])));
+      if (off > 0.5f - 0x1p-15f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = decide<double>(v[i]) + kI8Magic;
+      }
+    }
+    auto four = [&](int i) {
+      const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(t[i + 1]), __float_as_uint(t[i]), 0x0c0c0400u);
+      const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(t[i + 3]), __float_as_uint(t[i + 2]), 0x04000c0cu);
+      return lo | hi;
+    };
+    return finite ? make_uint2(four(0), four(4)) : make_uint2(0, 0);
   }
-  auto four = [&](int i) {
-    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(t[i + 1]), __float_as_uint(t[i]), 0x0c0c0400u);
-    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(t[i + 3]), __float_as_uint(t[i + 2]), 0x04000c0cu);
-    return lo | hi;
-  };
-  return row.finite ? make_uint2(four(0), four(4)) : make_uint2(0, 0);
-}
+};
 
 __device__ __forceinline__ void i8_values(uint2 codes, float scale, float (&v)[8]) {
 #pragma unroll
@@ -80,13 +99,19 @@ __device__ __forceinline__ void i8_values(uint2 codes, float scale, float (&v)[8
   }
 }
 
-// The largest magnitude's bits (NaN > infinity > numbers) among the waves of a row.
-template <int W>
-__device__ __forceinline__ uint32_t row_max(uint32_t m) {
-#pragma unroll
-  for (int d = kWave / 2; d > 0; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, kWave));
+// The maximum of m over the waves of a block; `part` is not the one of the call before.
+template <int W> __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t* part) {
+#define FMOE_MAX(CTRL, ROWS) \
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, ROWS, 0xf, false))
+  FMOE_MAX(0x111, 0xf);   // row_shr:1
+  FMOE_MAX(0x112, 0xf);
+  FMOE_MAX(0x114, 0xf);
+  FMOE_MAX(0x118, 0xf);
+  FMOE_MAX(0x142, 0xa);   // row_bcast:15
+  FMOE_MAX(0x143, 0xc);   // row_bcast:31
+#undef FMOE_MAX
+  m = (uint32_t)__builtin_amdgcn_readlane((int)m, kWave - 1);
   if constexpr (W > 1) {
-    __shared__ uint32_t part[W];
     if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = m;
     __syncthreads();
 #pragma unroll
@@ -95,86 +120,106 @@ __device__ __forceinline__ uint32_t row_max(uint32_t m) {
   return m;
 }
 
-// inv == nullptr: row r goes to row r, and rows from *n_rows_dev on (if given) are skipped; else
-// row t goes to the rows inv[t * top_k + j] that are not -1.  W waves take a row.
-template <typename T, int N, int W>
-__global__ __launch_bounds__(kI8Threads) void i8_quantize_kernel(
+// Row r goes to row r, and rows from *n_rows_dev on (if given) are skipped; or, PLACED, row t to the
+// rows inv[t * top_k + j] that are not -1.  A block of W waves takes row after row, the next one's
+// loads under way while it works on one's values.
+template <typename T, int W, bool PLACED>
+__global__ __launch_bounds__(W * kWave) void i8_quantize_kernel(
     const T* __restrict__ x, int64_t n_rows, int k, const int32_t* __restrict__ n_rows_dev,
     const int32_t* __restrict__ inv, int top_k, uint8_t* __restrict__ codes,
     float* __restrict__ scales, SegmentsOut segments) {
-  static_assert(W == 1 || W == kI8Waves, "rows do not share a block's barrier");
-  using Exact = std::conditional_t<sizeof(T) == 4, double, float>;
+  constexpr int kHeld = kI8HeldBytes / (8 * kWave * (int)sizeof(T));     // chunks in registers
+  constexpr int kSpan = W * kI8Chunk;
+  __shared__ uint32_t part[2][W];
   if (segments.seg_off && blockIdx.x == 0 && threadIdx.x < kWave)
     write_segments(segments, n_rows, threadIdx.x);
-  const int at = (threadIdx.x & (W * kWave - 1)) * 8;      // first value of the thread's in a chunk
-  const int64_t r = (int64_t)blockIdx.x * (kI8Waves / W) + (W > 1 ? 0 : threadIdx.x / kWave);
+  const int at = threadIdx.x * 8;                      // first value of the thread's in a chunk
+  const bool odd = threadIdx.x & 1;
+  const int row_bytes = (int)i8_row_bytes(k);
   int64_t rows = n_rows;
   if (n_rows_dev) rows = min(rows, (int64_t)*n_rows_dev);
-  if (r >= rows) return;
-  constexpr int kSpan = W * kI8Chunk;
-  const T* const src = x + r * k;
-  float v[kI8Held][8];
-  uint32_t m = 0;
-  auto widest = [&](const float (&u)[8]) {
+  Eight<T> held[kHeld];
+  auto fetch = [&](int64_t row) {
+    const T* const src = x + row * k;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(u[i]) & 0x7fffffffu);
-  };
-#pragma unroll
-  for (int c = 0; c < kI8Held; ++c)
-    if (c * kSpan < k) load8<T, N>(src, c * kSpan + at, k, v[c]);
-#pragma unroll
-  for (int c = 0; c < kI8Held; ++c)
-    if (c * kSpan < k) widest(v[c]);
-  for (int c = kI8Held * kSpan; c < k; c += kSpan) {
-    float u[8];
-    load8<T, N>(src, c + at, k, u);
-    widest(u);
-  }
-  const I8Row row(row_max<W>(m));
-  const int64_t row_bytes = i8_row_bytes(k);
-  auto put = [&](int c, const float (&u)[8]) {
-    if (c + at >= row_bytes) return;
-    const uint2 w = i8_codes<Exact>(u, row);
-    if (inv == nullptr) {
-      *reinterpret_cast<uint2*>(codes + r * row_bytes + c + at) = w;
-    } else {
-      for (int j = 0; j < top_k; ++j) {
-        const int64_t to = inv[r * top_k + j];
-        if (to >= 0) *reinterpret_cast<uint2*>(codes + to * row_bytes + c + at) = w;
-      }
+    for (int c = 0; c < kHeld; ++c) {
+      if ((c + 1) * kSpan <= k) __builtin_memcpy(&held[c], src + c * kSpan + at, sizeof(held[c]));
+      else if (c * kSpan < k) held[c].load(src, c * kSpan + at, k);
     }
   };
+  int64_t r = blockIdx.x;
+  if (r < rows) fetch(r);
+  for (int turn = 0; r < rows; r += gridDim.x, turn ^= 1) {
+    Eight<T> v[kHeld];
+    uint32_t m = 0;
 #pragma unroll
-  for (int c = 0; c < kI8Held; ++c)
-    if (c * kSpan < k) put(c * kSpan, v[c]);
-  for (int c = kI8Held * kSpan; c < k; c += kSpan) {
-    float u[8];
-    load8<T, N>(src, c + at, k, u);
-    put(c, u);
-  }
-  if (at != 0) return;
-  if (inv == nullptr) {
-    scales[r] = row.scale;
-  } else {
-    for (int j = 0; j < top_k; ++j) {
-      const int64_t to = inv[r * top_k + j];
-      if (to >= 0) scales[to] = row.scale;
+    for (int c = 0; c < kHeld; ++c) {
+      if (c * kSpan >= k) break;
+      m = held[c].widest(m);
+      v[c] = held[c];
+    }
+    if (r + gridDim.x < rows) fetch(r + gridDim.x);
+    for (int c = kHeld * kSpan; c < k; c += kSpan) {
+      Eight<T> u;
+      u.load(x + r * k, c + at, k);
+      m = u.widest(m);
+    }
+    const I8Row row(row_max<W>(Eight<T>::f32_bits(m), part[turn]));
+    // The codes of the chunks from c and c + kSpan on: neighbouring lanes exchange halves, so that
+    // a lane stores 16 bytes of one of the two.
+    auto put = [&](int c, const Eight<T>& a, const Eight<T>& b, bool second) {
+      const uint2 ca = row.codes(a), cb = second ? row.codes(b) : make_uint2(0, 0);
+      const uint32_t s0 = odd ? ca.x : cb.x, s1 = odd ? ca.y : cb.y;
+      const uint32_t g0 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)s0, 0xb1, 0xf, 0xf, false);
+      const uint32_t g1 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)s1, 0xb1, 0xf, 0xf, false);
+      const uint4 w = odd ? make_uint4(g0, g1, cb.x, cb.y) : make_uint4(ca.x, ca.y, g0, g1);
+      const int to = c + (odd ? kSpan : 0) + (at & ~15);
+      if (to >= row_bytes) return;
+      if constexpr (!PLACED) {
+        *reinterpret_cast<uint4*>(codes + r * row_bytes + to) = w;
+      } else {
+        for (int j = 0; j < top_k; ++j) {
+          const int64_t place = inv[r * top_k + j];
+          if (place >= 0) *reinterpret_cast<uint4*>(codes + place * row_bytes + to) = w;
+        }
+      }
+    };
+#pragma unroll
+    for (int c = 0; c < kHeld; c += 2) {
+      if (c * kSpan >= k) break;
+      put(c * kSpan, v[c], v[c + 1], (c + 1) * kSpan < k);
+    }
+    for (int c = kHeld * kSpan; c < k; c += 2 * kSpan) {
+      Eight<T> a, b;
+      a.load(x + r * k, c + at, k);
+      b.load(x + r * k, c + kSpan + at, k);
+      put(c, a, b, c + kSpan < k);
+    }
+    if (threadIdx.x != 0) continue;
+    if constexpr (!PLACED) {
+      scales[r] = row.scale;
+    } else {
+      for (int j = 0; j < top_k; ++j) {
+        const int64_t place = inv[r * top_k + j];
+        if (place >= 0) scales[place] = row.scale;
+      }
     }
   }
 }
 
 // The chunks of all rows are numbered row by row; a wave takes U consecutive ones at a time.
-template <typename T, int N, int U>
+template <typename T, int U>
 __global__ __launch_bounds__(kI8Threads) void i8_dequantize_kernel(
     const uint8_t* __restrict__ codes, const float* __restrict__ scales, int64_t n_rows, int k,
     T* __restrict__ out, ClearedTail<T> tail) {
+  constexpr int kWaves = kI8Threads / kWave;
   if (tail.p) tail.clear(k);
   const int lane = threadIdx.x & (kWave - 1);
   const int chunks = (k + kI8Chunk - 1) / kI8Chunk;
   const int64_t row_bytes = i8_row_bytes(k);
-  const int64_t items = n_rows * chunks, stride = (int64_t)gridDim.x * kI8Waves * U;
+  const int64_t items = n_rows * chunks, stride = (int64_t)gridDim.x * kWaves * U;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  for (int64_t it = ((int64_t)blockIdx.x * kI8Waves + wave) * U; it < items; it += stride) {
+  for (int64_t it = ((int64_t)blockIdx.x * kWaves + wave) * U; it < items; it += stride) {
     uint2 w[U];
     float s[U];
     int64_t row[U];
@@ -194,41 +239,42 @@ __global__ __launch_bounds__(kI8Threads) void i8_dequantize_kernel(
       if (at[u] >= k) continue;
       float v[8];
       i8_values(w[u], s[u], v);
-      store8<T, N>(out + row[u] * k, at[u], k, v);
+      store_any(out + row[u] * k, at[u], k, v);
     }
   }
 }
 
-#define FMOE_RUNS(CALL)                                             \
-  do {                                                              \
-    constexpr int kMost = 16 / (int)sizeof(T);                      \
-    if (run == 8) CALL(kMost);                                      \
-    else if (run == 4) CALL(4);                                     \
-    else if (run == 2) CALL(2);                                     \
-    else CALL(1);                                                   \
-  } while (0)
+// Waves of a row: as many as hold it, or, where rows are few, as many as find a chunk in it.
+constexpr int64_t kI8FewRows = 2048;
+constexpr int64_t kI8Waves = 256 * 16;     // as many as their registers allow on the chip
 
-// One wave a row where rows are enough to fill the chip and short enough for its registers.
-constexpr int64_t kI8ManyRows = 256 * 16;
+template <typename T, int W>
+static void start_quantize(const void* x, int64_t n_rows, int k, const int32_t* n_rows_dev,
+                           const int32_t* inv, int top_k, uint8_t* codes, float* scales,
+                           const SegmentsOut& segments, hipStream_t s) {
+  const dim3 grid((unsigned)std::max<int64_t>(std::min(n_rows, kI8Waves / W), 1));
+  if (inv)
+    hipLaunchKernelGGL((i8_quantize_kernel<T, W, true>), grid, dim3(W * kWave), 0, s, (const T*)x,
+                       n_rows, k, n_rows_dev, inv, top_k, codes, scales, segments);
+  else
+    hipLaunchKernelGGL((i8_quantize_kernel<T, W, false>), grid, dim3(W * kWave), 0, s, (const T*)x,
+                       n_rows, k, n_rows_dev, inv, top_k, codes, scales, segments);
+}
 
 template <typename T>
 static int launch_quantize(const void* x, int64_t n_rows, int k, const int32_t* n_rows_dev,
                            const int32_t* inv, int top_k, uint8_t* codes, float* scales,
                            const SegmentsOut& segments, hipStream_t s) {
-  const int run = run_length<T>(x, k);
-  const bool one = k <= kI8Chunk || (n_rows >= kI8ManyRows && k <= kI8Held * kI8Chunk);
-  const dim3 grid((unsigned)std::max<int64_t>(one ? (n_rows + kI8Waves - 1) / kI8Waves : n_rows, 1));
-#define FMOE_CALL(N)                                                                             \
-  do {                                                                                           \
-    if (one)                                                                                     \
-      hipLaunchKernelGGL((i8_quantize_kernel<T, N, 1>), grid, dim3(kI8Threads), 0, s,            \
-                         (const T*)x, n_rows, k, n_rows_dev, inv, top_k, codes, scales, segments); \
-    else                                                                                         \
-      hipLaunchKernelGGL((i8_quantize_kernel<T, N, kI8Waves>), grid, dim3(kI8Threads), 0, s,     \
-                         (const T*)x, n_rows, k, n_rows_dev, inv, top_k, codes, scales, segments); \
-  } while (0)
-  FMOE_RUNS(FMOE_CALL);
-#undef FMOE_CALL
+  const int64_t need = n_rows < kI8FewRows
+                           ? ((int64_t)k + kI8Chunk - 1) / kI8Chunk
+                           : ((int64_t)k * (int)sizeof(T) + kI8HeldBytes - 1) / kI8HeldBytes;
+#define FMOE_START(W) \
+  start_quantize<T, W>(x, n_rows, k, n_rows_dev, inv, top_k, codes, scales, segments, s)
+  if (need <= 1) FMOE_START(1);
+  else if (need <= 2) FMOE_START(2);
+  else if (need <= 4) FMOE_START(4);
+  else FMOE_START(8);
+#undef FMOE_START
   FMOE_LAUNCH_CHECK("i8_quantize");
   return FMOE_OK;
 }
@@ -240,23 +286,17 @@ template <typename T>
 static int launch_dequantize(const uint8_t* codes, const float* scales, int64_t n_rows, int k,
                              void* out, const int32_t* tail_end, void* tail, int64_t tail_rows,
                              hipStream_t s) {
-  const int run = run_length<T>(out, k);
   const int64_t items = n_rows * ((k + kI8Chunk - 1) / kI8Chunk);
   const bool many = items >= kI8ManyItems;
-  const int64_t per_block = kI8Waves * (many ? 4 : 1);
+  const int64_t per_block = kI8Threads / kWave * (many ? 4 : 1);
   const dim3 grid((unsigned)std::max<int64_t>(std::min<int64_t>((items + per_block - 1) / per_block, 256 * 64), 1));
   const ClearedTail<T> cleared{tail_end, (T*)tail, tail_rows};
-#define FMOE_CALL(N)                                                                            \
-  do {                                                                                          \
-    if (many)                                                                                   \
-      hipLaunchKernelGGL((i8_dequantize_kernel<T, N, 4>), grid, dim3(kI8Threads), 0, s, codes,  \
-                         scales, n_rows, k, (T*)out, cleared);                                  \
-    else                                                                                        \
-      hipLaunchKernelGGL((i8_dequantize_kernel<T, N, 1>), grid, dim3(kI8Threads), 0, s, codes,  \
-                         scales, n_rows, k, (T*)out, cleared);                                  \
-  } while (0)
-  FMOE_RUNS(FMOE_CALL);
-#undef FMOE_CALL
+  if (many)
+    hipLaunchKernelGGL((i8_dequantize_kernel<T, 4>), grid, dim3(kI8Threads), 0, s, codes, scales,
+                       n_rows, k, (T*)out, cleared);
+  else
+    hipLaunchKernelGGL((i8_dequantize_kernel<T, 1>), grid, dim3(kI8Threads), 0, s, codes, scales,
+                       n_rows, k, (T*)out, cleared);
   FMOE_LAUNCH_CHECK("i8_dequantize");
   return FMOE_OK;
 }

@@ -93,13 +93,16 @@ enum I8Kernel { kStream, kTile128x64, kTile128x128, kTile256x256 };
 static I8Kernel choose_kernel(const QuantGemmArgs& a, bool packed) {
   const double live = (double)std::min<int64_t>(a.n_expert, a.n_rows);
   const double mean = (double)a.n_rows / a.n_expert;
-  // (an expert's last tile is half empty on average)
+  // (of several experts the last tile is half empty on average)
   auto tiles = [&](int tn, int tm) {
-    return std::max((double)a.n_rows / tm + live / 2, live) * ceil_div(a.out_feat, tn);
+    const double rows = live == 1 ? ceil_div(a.n_rows, tm) : (double)a.n_rows / tm + live / 2;
+    return std::max(rows, live) * ceil_div(a.out_feat, tn);
   };
   if (mean <= 16 && tiles(128, 64) <= kCus / 2) return kStream;
   if (mean < 56) return kTile128x64;
-  if (packed && mean >= 192 && a.in_feat >= 2048 && tiles(256, 256) >= 600) return kTile256x256;
+  if (packed && mean >= 192 && a.in_feat >= 1024 &&
+      std::max(tiles(256, 256) / kCus, 1.) <= 0.73 * std::max(tiles(128, 128) / (2 * kCus), 1.))
+    return kTile256x256;
   return kTile128x128;
 }
 

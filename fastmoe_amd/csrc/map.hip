@@ -15,153 +15,170 @@
 
 namespace fmoe {
 
-constexpr int kMapThreads = 256;
-constexpr int kMapWaves = kMapThreads / kWave;
-
 // ------------------------------------------------------------------------- plan
-// Two launches, or one for up to kMapUnit tokens: a histogram per block of tokens, then, in every
-// block, the sums of the histograms in front of its own and of all (16-bit counts, 16 bytes a load:
-// 16384 tokens of 128 experts are 64 KiB a block, from L2) and the places of its own tokens.
-constexpr int kMapUnit = 64;           // tokens of the smallest block
-constexpr int kMapBlocks = 256;        // at most; more tokens make larger blocks
-constexpr int kMapStage = 4096;        // bytes of truth values a wave holds in LDS
-static_assert(FMOE_MAP_MAX_EXPERTS <= 1024 && FMOE_MAP_MAX_EXPERTS <= kMapStage, "a token's fit");
+// Two launches, or one for up to 64 tokens: a histogram per block of tokens, then, in every block,
+// the sums of the histograms in front of its own and of all, and the places of its own tokens.
+//
+// A wave takes up to 16 tokens in a round.  Their truth values pass through LDS into one 16-bit mask per
+// expert, which a lane holds; from there on a token's row is the expert's first one plus the bits
+// below the token's in the mask, and its place in the token's list the bits below the lane's in a
+// ballot, so that no step waits for the one before (a counter per expert in LDS, advanced token by
+// token, took 11 us for 8192 tokens of 16 experts where this takes @@).
+constexpr int kMapThreads = 1024;
+constexpr int kMapWaves = kMapThreads / kWave;
+constexpr int kMapRound = 16;          // most tokens of a wave at a time
+constexpr int kMapUnit = 64;           // tokens of the smallest block, 4 for each wave
+constexpr int kMapBlocks = 256;        // at most; more tokens make more rounds
+constexpr int kMapStage = 2048;        // bytes of truth values a wave holds in LDS
+constexpr int64_t kMapMostTokens = (int64_t)1 << 23;    // a block's counts have 16 bits
+static_assert(FMOE_MAP_MAX_EXPERTS <= kMapStage, "a token's truth values fit");
+static_assert(kMapMostTokens / kMapBlocks < 65536, "counts fit");
 
 struct MapBlocks {
   int per_block, per_wave, blocks;     // tokens of a block and of a wave; blocks
   __host__ __device__ explicit MapBlocks(int64_t n_tokens) {
     const int64_t units = (n_tokens + kMapUnit - 1) / kMapUnit;
-    per_block = (int)((units + kMapBlocks - 1) / kMapBlocks) * kMapUnit;
-    if (per_block == 0) per_block = kMapUnit;
-    per_wave = per_block / kMapWaves;
+    const int64_t waves = (units < kMapBlocks ? units : kMapBlocks) * kMapWaves;
+    per_wave = (int)((n_tokens + waves - 1) / waves);
+    per_block = per_wave * kMapWaves;
     blocks = (int)((n_tokens + per_block - 1) / per_block);
   }
 };
 __host__ __device__ inline int map_hist_row(int n_expert) { return (n_expert + 7) & ~7; }
 
-// A wave's truth values, `batch` tokens at a time, through its own LDS.
-struct MapStage {
+// A wave's tokens and its part of LDS.
+struct MapWave {
   const uint8_t* map;
-  uint8_t* lds;
-  int n_expert, batch;
-  int64_t end;                         // one behind the wave's last token
-  int64_t at = -1;                     // first token held
+  uint8_t* stage;                      // [kMapStage]
+  uint16_t* mask;                      // [n_expert]: the round's tokens that an expert takes
+  int n_expert, lane;
+  int64_t first, end;
 
-  // (whole wave) the tokens t .. held() - 1
-  __device__ __forceinline__ void hold(int64_t t, int lane) {
-    if (t == at) return;
-    at = t;
-    const int bytes = (int)(min(t + batch, end) - t) * n_expert;
-    const uint8_t* const src = map + t * n_expert;
-    for (int i = lane * 16; i < bytes; i += kWave * 16) {
-      if (i + 16 <= bytes) {
-        uint4 v;
-        __builtin_memcpy(&v, src + i, 16);
-        *reinterpret_cast<uint4*>(lds + i) = v;
-      } else {
-        for (int j = i; j < bytes; ++j) lds[j] = src[j];
+  __device__ __forceinline__ MapWave(const uint8_t* map_, int64_t n_tokens, int n_expert_,
+                                     const MapBlocks& b, uint8_t* stages, uint16_t* masks) {
+    const int wave = threadIdx.x / kWave;
+    map = map_;
+    stage = stages + wave * kMapStage;
+    mask = masks + wave * n_expert_;
+    n_expert = n_expert_;
+    lane = threadIdx.x & (kWave - 1);
+    first = min((int64_t)blockIdx.x * b.per_block + wave * b.per_wave, n_tokens);
+    end = min(first + b.per_wave, n_tokens);
+  }
+
+  // The masks of tokens t .. t + n - 1 (n <= kMapRound).
+  __device__ __forceinline__ void round(int64_t t, int n) {
+    const int batch = min(kMapStage / n_expert, n);
+    for (int at = 0; at < n; at += batch) {
+      const int tokens = min(batch, n - at), bytes = tokens * n_expert;
+      const uint8_t* const src = map + (t + at) * n_expert;
+      for (int i = lane * 16; i < bytes; i += kWave * 16) {
+        if (i + 16 <= bytes) {
+          uint4 v;
+          __builtin_memcpy(&v, src + i, 16);
+          *reinterpret_cast<uint4*>(stage + i) = v;
+        } else {
+          for (int j = i; j < bytes; ++j) stage[j] = src[j];
+        }
       }
+      wave_fence();
+      for (int e = lane; e < n_expert; e += kWave) {
+        uint32_t m = at == 0 ? 0 : mask[e];
+#pragma unroll
+        for (int i = 0; i < kMapRound; ++i) {
+          if (i >= tokens) break;
+          m |= (uint32_t)(stage[i * n_expert + e] != 0) << (at + i);
+        }
+        mask[e] = (uint16_t)m;
+      }
+      wave_fence();
     }
+  }
+  // (a wave's LDS accesses run in order; this keeps the compiler's order, too)
+  static __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
-  __device__ __forceinline__ int64_t held() const { return min(at + batch, end); }
-  __device__ __forceinline__ bool takes(int64_t t, int e) const {
-    return e < n_expert && lds[(int)(t - at) * n_expert + e] != 0;
-  }
 };
-
-// Tokens that the wave's experts take, counted into cnt[0 .. n_expert - 1].
-__device__ __forceinline__ void map_count(MapStage& st, int64_t first, int32_t* cnt, int lane) {
-  for (int e = lane; e < st.n_expert; e += kWave) cnt[e] = 0;
-  for (int64_t t = first; t < st.end; t = st.held()) {
-    st.hold(t, lane);
-    const int64_t stop = st.held();
-    for (int e = lane; e < st.n_expert; e += kWave) {
-      int c = 0;
-      for (int64_t u = t; u < stop; ++u) c += st.takes(u, e);
-      cnt[e] += c;
-    }
-  }
-}
-
-__device__ __forceinline__ MapStage map_stage(const uint8_t* map, uint8_t* lds, int64_t n_tokens,
-                                              int n_expert, const MapBlocks& b, int wave,
-                                              int64_t& first) {
-  first = min((int64_t)blockIdx.x * b.per_block + wave * b.per_wave, n_tokens);
-  MapStage st;
-  st.map = map;
-  st.lds = lds + wave * kMapStage;
-  st.n_expert = n_expert;
-  st.batch = kMapStage / n_expert;
-  st.end = min(first + b.per_wave, n_tokens);
-  return st;
-}
 
 __global__ __launch_bounds__(kMapThreads) void map_count_kernel(const uint8_t* __restrict__ map,
                                                                 int64_t n_tokens, int n_expert,
                                                                 uint16_t* __restrict__ hist) {
-  __shared__ __align__(16) uint8_t stage[kMapWaves * kMapStage];
-  extern __shared__ int32_t cnt[];     // [waves][n_expert]
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const MapBlocks b(n_tokens);
-  int64_t first;
-  MapStage st = map_stage(map, stage, n_tokens, n_expert, b, wave, first);
-  map_count(st, first, cnt + wave * n_expert, lane);
-  __syncthreads();
+  extern __shared__ __align__(16) uint8_t lds[];
+  uint16_t* const masks = (uint16_t*)(lds + kMapWaves * kMapStage);
   const int row = map_hist_row(n_expert);
-  for (int e = threadIdx.x; e < row; e += kMapThreads) {
-    int c = 0;
-    if (e < n_expert)
-      for (int w = 0; w < kMapWaves; ++w) c += cnt[w * n_expert + e];
-    hist[(int64_t)blockIdx.x * row + e] = (uint16_t)c;
+  int32_t* const count = (int32_t*)(masks + kMapWaves * row);
+  const MapBlocks b(n_tokens);
+  MapWave w(map, n_tokens, n_expert, b, lds, masks);
+  for (int e = threadIdx.x; e < row; e += kMapThreads) count[e] = 0;
+  __syncthreads();
+  for (int64_t t = w.first; t < w.end; t += kMapRound) {
+    w.round(t, (int)min((int64_t)kMapRound, w.end - t));
+    for (int e = w.lane; e < n_expert; e += kWave)
+      if (const int c = __popc(w.mask[e])) atomicAdd(&count[e], c);       // (integers: any order)
   }
+  __syncthreads();
+  for (int e = threadIdx.x; e < row; e += kMapThreads)
+    hist[(int64_t)blockIdx.x * row + e] = (uint16_t)count[e];
 }
 
 __global__ __launch_bounds__(kMapThreads) void map_place_kernel(
     const uint8_t* __restrict__ map, int64_t n_tokens, int n_expert, int max_rows,
     const uint16_t* __restrict__ hist, int64_t* __restrict__ counts, int32_t* __restrict__ seg_off,
     int32_t* __restrict__ token_off, int2* __restrict__ pairs) {
-  __shared__ __align__(16) uint8_t stage[kMapWaves * kMapStage];
-  extern __shared__ int32_t lds[];
+  extern __shared__ __align__(16) uint8_t lds[];
   const int row = map_hist_row(n_expert);
-  int32_t* const cnt = lds;                          // [waves][n_expert]
-  int32_t* const total = cnt + kMapWaves * n_expert; // [row] tokens of an expert
-  int32_t* const before = total + row;               // [row] of those, in blocks in front
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  uint16_t* const masks = (uint16_t*)(lds + kMapWaves * kMapStage);
+  uint16_t* const taken = masks + kMapWaves * row;             // [waves][n_expert]
+  int32_t* const total = (int32_t*)(taken + kMapWaves * row);  // [row] tokens of an expert
+  int32_t* const before = total + row;                         // [row] of those, in earlier blocks
   const MapBlocks b(n_tokens);
-  int64_t first;
-  MapStage st = map_stage(map, stage, n_tokens, n_expert, b, wave, first);
+  MapWave w(map, n_tokens, n_expert, b, lds, masks);
+  const int lane = w.lane, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  uint16_t* const mine = taken + wave * n_expert;
 
   for (int e = threadIdx.x; e < row; e += kMapThreads) total[e] = before[e] = 0;
-  map_count(st, first, cnt + wave * n_expert, lane);
+  for (int e = lane; e < n_expert; e += kWave) mine[e] = 0;
+  for (int64_t t = w.first; t < w.end; t += kMapRound) {
+    w.round(t, (int)min((int64_t)kMapRound, w.end - t));
+    for (int e = lane; e < n_expert; e += kWave) mine[e] += (uint16_t)__popc(w.mask[e]);
+  }
   __syncthreads();
-  if (hist == nullptr) {
-    for (int e = threadIdx.x; e < n_expert; e += kMapThreads)
-      for (int w = 0; w < kMapWaves; ++w) total[e] += cnt[w * n_expert + e];
-  } else {
+  if (hist) {
     const int packs = row / 8;                       // (at most 128)
     const int p = threadIdx.x % packs, from = threadIdx.x / packs, step = kMapThreads / packs;
-    int32_t all[8] = {}, mine[8] = {};
+    int32_t all[8] = {}, front[8] = {};
     if (from < step) {
-#pragma unroll 4
+#pragma unroll 8
       for (int k = from; k < b.blocks; k += step) {
         const uint4 v = *reinterpret_cast<const uint4*>(hist + (int64_t)k * row + p * 8);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
         const bool in_front = k < (int)blockIdx.x;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int32_t c = (int32_t)((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+          const int32_t c = (int32_t)((u[i >> 1] >> (16 * (i & 1))) & 0xffffu);
           all[i] += c;
-          mine[i] += in_front ? c : 0;
+          front[i] += in_front ? c : 0;
         }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {                  // (integers: any order)
-        atomicAdd(&total[p * 8 + i], all[i]);
-        atomicAdd(&before[p * 8 + i], mine[i]);
+        if (all[i]) atomicAdd(&total[p * 8 + i], all[i]);
+        if (front[i]) atomicAdd(&before[p * 8 + i], front[i]);
       }
     }
+  }
+  // every wave's counts become those of the waves in front of it
+  for (int e = threadIdx.x; e < n_expert; e += kMapThreads) {
+    int c[kMapWaves], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kMapWaves; ++k) c[k] = taken[k * n_expert + e];
+#pragma unroll
+    for (int k = 0; k < kMapWaves; ++k) {
+      taken[k * n_expert + e] = (uint16_t)sum;
+      sum += c[k];
+    }
+    if (!hist) total[e] = sum;
   }
   __syncthreads();
   // first row of every expert, in total's place; all waves need them, one makes them
@@ -183,72 +200,81 @@ __global__ __launch_bounds__(kMapThreads) void map_place_kernel(
     if (blockIdx.x == 0 && lane == 0) seg_off[n_expert] = min(carry, max_rows);
   }
   __syncthreads();
-  // The next row of the wave's experts, in LDS too (by the lane that alone uses it), and the number
-  // of pairs of the tokens in front of the wave's.  Rows from max_rows on are nobody's.
-  int32_t* const next = cnt + wave * n_expert;
+  // pairs of the tokens in front of the wave's (rows from max_rows on are nobody's)
   int pairs_before = 0;
-  for (int e = lane; e < n_expert; e += kWave) {
-    int c = before[e];
-    for (int w = 0; w < wave; ++w) c += cnt[w * n_expert + e];
-    pairs_before += min(c, max(max_rows - total[e], 0));
-    before[row * (wave + 1) + e] = total[e] + c;     // (others still read cnt)
-  }
+  for (int e = lane; e < n_expert; e += kWave)
+    pairs_before += min(before[e] + mine[e], max(max_rows - total[e], 0));
   int at = __builtin_amdgcn_readlane(wave_inclusive_sum(pairs_before), kWave - 1);
-  __syncthreads();
-  for (int e = lane; e < n_expert; e += kWave) next[e] = before[row * (wave + 1) + e];
   const unsigned long long below = (1ull << lane) - 1;
-  for (int64_t t = first; t < st.end;) {
-    st.hold(t, lane);
-    const int64_t stop = st.held();
-    for (; t < stop; ++t) {
-      if (lane == 0) token_off[t] = at;
-      for (int e0 = 0; e0 < n_expert; e0 += kWave) {
-        const int e = e0 + lane;
-        const bool takes = st.takes(t, e);
-        int r = 0;
-        if (takes) {
-          r = next[e];
-          next[e] = r + 1;
+  const bool one_round = w.end - w.first <= kMapRound;
+  for (int64_t t = w.first; t < w.end; t += kMapRound) {
+    const int n = (int)min((int64_t)kMapRound, w.end - t);
+    if (!one_round) w.round(t, n);
+    // lane i: pairs of token i
+    int tokens = 0;
+    for (int e0 = 0; e0 < n_expert; e0 += kWave) {
+      const int e = e0 + lane;
+      uint32_t m = 0;
+      if (e < n_expert) {
+        m = w.mask[e];
+        const int fit = max(max_rows - (total[e] + before[e] + mine[e]), 0);
+        if (__popc(m) > fit) {                       // the last ones are cut off
+          while (__popc(m) > fit) m &= ~(1u << (31 - __clz(m)));
+          w.mask[e] = (uint16_t)m;
         }
-        const bool kept = takes && r < max_rows;
-        const unsigned long long all = __ballot(kept);
-        if (kept) pairs[at + __popcll(all & below)] = make_int2(r, e);
-        at += __popcll(all);
+      }
+#pragma unroll
+      for (int i = 0; i < kMapRound; ++i) {
+        if (i >= n) break;
+        const int c = __popcll(__ballot((m >> i) & 1));
+        tokens += lane == i ? c : 0;
+      }
+    }
+    const int incl = wave_inclusive_sum(tokens);
+    int start = at + incl - tokens;
+    if (lane < n) token_off[t + lane] = start;
+    at += __builtin_amdgcn_readlane(incl, kWave - 1);
+    for (int e0 = 0; e0 < n_expert; e0 += kWave) {
+      const int e = e0 + lane;
+      uint32_t m = 0;
+      int r = 0;
+      if (e < n_expert) {
+        m = w.mask[e];
+        r = total[e] + before[e] + mine[e];
+        mine[e] += (uint16_t)__popc(m);
+      }
+#pragma unroll
+      for (int i = 0; i < kMapRound; ++i) {
+        if (i >= n) break;
+        const bool takes = (m >> i) & 1;
+        const unsigned long long all = __ballot(takes);
+        const int to = __builtin_amdgcn_readlane(start, i) + __popcll(all & below);
+        if (takes) pairs[to] = make_int2(r + __popc(m & ((1u << i) - 1)), e);
+        start += lane == i ? __popcll(all) : 0;
       }
     }
   }
-  if (lane == 0 && st.end == n_tokens && first < n_tokens) token_off[n_tokens] = at;
+  if (lane == 0 && w.end == n_tokens && w.first < n_tokens) token_off[n_tokens] = at;
+}
+
+constexpr size_t map_lds(int n_expert, bool place) {
+  const int row = (n_expert + 7) & ~7;
+  return kMapWaves * kMapStage + (size_t)row * (place ? 2 * kMapWaves * 2 + 8 : kMapWaves * 2 + 4);
 }
 
 // ------------------------------------------------------------------------- rows
-// 8 values of a row from k on (zeros behind its end), rows of any alignment.
-template <typename T>
-__device__ __forceinline__ void load_any(const T* row, int k, int d, T (&v)[8]) {
-  if (k + 8 <= d) {
-    __builtin_memcpy(v, row + k, 8 * sizeof(T));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < d ? row[k + i] : Elem<T>::from_acc(0.f);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store_any(T* row, int k, int d, const float (&v)[8]) {
-  T o[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = Elem<T>::from_acc(v[i]);
-  if (k + 8 <= d) {
-    __builtin_memcpy(row + k, o, 8 * sizeof(T));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k + i < d) row[k + i] = o[i];
-  }
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int s = kWave / 2; s > 0; s >>= 1) v += __shfl_xor(v, s, kWave);
-  return v;
+// Sum over the wave, the same in every lane (the moves of wave_inclusive_sum()).
+__device__ __forceinline__ float wave_sum(float x) {
+#define FMOE_ADD(CTRL, ROWS) \
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWS, 0xf, false))
+  FMOE_ADD(0x111, 0xf);   // row_shr:1
+  FMOE_ADD(0x112, 0xf);
+  FMOE_ADD(0x114, 0xf);
+  FMOE_ADD(0x118, 0xf);
+  FMOE_ADD(0x142, 0xa);   // row_bcast:15
+  FMOE_ADD(0x143, 0xc);   // row_bcast:31
+#undef FMOE_ADD
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWave - 1));
 }
 
 struct MapMoveArgs {
@@ -261,18 +287,28 @@ struct MapMoveArgs {
 };
 
 // EXPAND: out[r] = w one[t] for a token's rows; else out[t] = sum of w many[r].  DOT: also
-// dweight[t][e] = <one[t], many[r]>, zero where the token has no row.  G threads take a token,
-// `H` chunks of 8 G values of its row at a time; without DOT a row's pieces of H chunks may be
-// different blocks' (blockIdx.y).
+// dweight[t][e] = <one[t], many[r]>, zero where the token has no row.
+//
+// A lane holds 8 values of a row, and U rows are under way at a time.  Without DOT a wave takes 512
+// values of a token's rows, whatever their length; with it a block of G threads takes a token,
+// H times 8 G values at a time, and its waves' shares of the products meet in LDS.
 template <typename T, typename W, int G, int H, bool EXPAND, bool DOT>
-__global__ __launch_bounds__(kMapThreads) void map_move_kernel(MapMoveArgs a, ClearedTail<T> tail) {
-  if (EXPAND && tail.p && blockIdx.y == 0) tail.clear(a.d);
+__global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, ClearedTail<T> tail) {
+  static_assert(DOT || (G == kWave && H == 1), "pieces of 512 values");
+  if (EXPAND && tail.p) tail.clear(a.d);
   extern __shared__ float s_dot[];                   // [waves][n_expert]
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t t = (int64_t)blockIdx.x * (kMapThreads / G) + (G == kWave ? wave : 0);
-  // (with G = 64 no barrier follows; with G = 256 the whole block leaves)
-  if (t >= a.n_tokens) return;
+  constexpr int kSpan = G * 8, kPiece = kSpan * H;
+  int64_t t = blockIdx.x;
+  int k0 = 0;
+  if constexpr (!DOT) {
+    const int pieces = (a.d + kPiece - 1) / kPiece;
+    const int64_t item = (int64_t)blockIdx.x * (256 / kWave) + wave;
+    t = item / pieces;
+    k0 = (int)(item - t * pieces) * kPiece;
+    if (t >= a.n_tokens) return;
+  }
   const T* const one = (const T*)a.one + t * a.d;
   const T* const many = (const T*)a.many;
   const W* const weight = (const W*)a.weight;
@@ -281,18 +317,16 @@ __global__ __launch_bounds__(kMapThreads) void map_move_kernel(MapMoveArgs a, Cl
   float* const dot = s_dot + wave * a.n_expert;
   if constexpr (DOT)
     for (int e = lane; e < a.n_expert; e += kWave) dot[e] = 0.f;
-  constexpr int kSpan = G * 8, kPiece = kSpan * H;
   const int at = (threadIdx.x & (G - 1)) * 8;
-  for (int k0 = blockIdx.y * kPiece; k0 < a.d; k0 += gridDim.y * kPiece) {
+  const int k_end = DOT ? a.d : k0 + 1;
+  for (; k0 < k_end; k0 += kPiece) {
     float x[H][8], sum[H][8];
     if constexpr (EXPAND || DOT) {
-      T raw[H][8];
+      Eight<T> raw[H];
 #pragma unroll
-      for (int h = 0; h < H; ++h) load_any(one, k0 + h * kSpan + at, a.d, raw[h]);
+      for (int h = 0; h < H; ++h) raw[h].load(one, k0 + h * kSpan + at, a.d);
 #pragma unroll
-      for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[h][i] = Elem<T>::to_acc(raw[h][i]);
+      for (int h = 0; h < H; ++h) raw[h].widen(x[h]);
     }
     if constexpr (!EXPAND) {
 #pragma unroll
@@ -309,15 +343,16 @@ __global__ __launch_bounds__(kMapThreads) void map_move_kernel(MapMoveArgs a, Cl
         if (weight) w = Elem<W>::to_acc(weight[t * a.n_expert + pair.y]);
       }
       const int n = min(p1 - b, kWave);
-      constexpr int U = EXPAND ? (DOT ? 2 : 1) : 8 / H;       // rows under way at a time
+      constexpr int U = EXPAND && !DOT ? 1 : 16 / (int)sizeof(T) / H;     // rows under way
       for (int j = 0; j < n; j += U) {
-        T raw[U][H][8];
+        Eight<T> raw[U][H];
         if constexpr (!EXPAND || DOT) {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const int64_t r = __builtin_amdgcn_readlane(pair.x, min(j + u, n - 1));
+            if (j + u >= n) break;
+            const int64_t r = __builtin_amdgcn_readlane(pair.x, j + u);
 #pragma unroll
-            for (int h = 0; h < H; ++h) load_any(many + r * a.d, k0 + h * kSpan + at, a.d, raw[u][h]);
+            for (int h = 0; h < H; ++h) raw[u][h].load(many + r * a.d, k0 + h * kSpan + at, a.d);
           }
         }
 #pragma unroll
@@ -330,9 +365,10 @@ __global__ __launch_bounds__(kMapThreads) void map_move_kernel(MapMoveArgs a, Cl
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
-              for (int i = 0; i < 8; ++i) s = fmaf(x[h][i], Elem<T>::to_acc(raw[u][h][i]), s);
+              for (int i = 0; i < 8; ++i) s = fmaf(x[h][i], raw[u][h][i], s);
             s = wave_sum(s);
-            if (lane == 0) dot[__builtin_amdgcn_readlane(pair.y, j + u)] += s;
+            const int e = __builtin_amdgcn_readlane(pair.y, j + u);
+            if (lane == 0) dot[e] = k0 == 0 ? s : dot[e] + s;
           }
 #pragma unroll
           for (int h = 0; h < H; ++h) {
@@ -344,7 +380,7 @@ __global__ __launch_bounds__(kMapThreads) void map_move_kernel(MapMoveArgs a, Cl
             } else {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                sum[h][i] = fmaf(Elem<T>::to_acc(raw[u][h][i]), wj, sum[h][i]);
+                sum[h][i] = fmaf(raw[u][h][i], wj, sum[h][i]);
             }
           }
         }
@@ -356,40 +392,35 @@ __global__ __launch_bounds__(kMapThreads) void map_move_kernel(MapMoveArgs a, Cl
     }
   }
   if constexpr (DOT) {
+    __syncthreads();
     W* const dw = (W*)a.dweight + t * a.n_expert;
-    if constexpr (G == kWave) {
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      for (int e = lane; e < a.n_expert; e += kWave) dw[e] = Elem<W>::from_acc(dot[e]);
-    } else {
-      __syncthreads();
-      for (int e = threadIdx.x; e < a.n_expert; e += kMapThreads) {
-        float s = 0.f;
+    for (int e = threadIdx.x; e < a.n_expert; e += G) {
+      float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kMapWaves; ++w) s += s_dot[w * a.n_expert + e];
-        dw[e] = Elem<W>::from_acc(s);
-      }
+      for (int w = 0; w < G / kWave; ++w) s += s_dot[w * a.n_expert + e];
+      dw[e] = Elem<W>::from_acc(s);
     }
   }
 }
 
-// A wave takes a token where there are enough of them, a block otherwise.
-constexpr int64_t kMapManyTokens = 256 * 8;
+template <typename T, typename W, int G, int H, bool EXPAND, bool DOT>
+static void start_move(const MapMoveArgs& a, const ClearedTail<T>& tail, hipStream_t s) {
+  const int64_t waves = a.n_tokens * ((a.d + kWave * 8 - 1) / (kWave * 8));
+  const dim3 grid((unsigned)(DOT ? a.n_tokens : (waves + 3) / 4)), block(DOT ? G : 256);
+  const size_t lds = DOT ? sizeof(float) * (G / kWave) * a.n_expert : 0;
+  hipLaunchKernelGGL((map_move_kernel<T, W, G, H, EXPAND, DOT>), grid, block, lds, s, a, tail);
+}
 
 template <typename T, typename W, bool EXPAND, bool DOT>
 static int launch_move(const MapMoveArgs& a, const ClearedTail<T>& tail, hipStream_t s) {
-  const size_t lds = DOT ? sizeof(float) * kMapWaves * a.n_expert : 0;
-  const bool wave = a.n_tokens >= kMapManyTokens;
-  constexpr int kHWave = 4, kHBlock = 2;
-  const int piece = wave ? kWave * 8 * kHWave : kMapThreads * 8 * kHBlock;
-  const dim3 grid((unsigned)(wave ? (a.n_tokens + kMapWaves - 1) / kMapWaves : a.n_tokens),
-                  DOT ? 1 : (unsigned)((a.d + piece - 1) / piece));
-  if (wave)
-    hipLaunchKernelGGL((map_move_kernel<T, W, kWave, kHWave, EXPAND, DOT>), grid, dim3(kMapThreads),
-                       lds, s, a, tail);
-  else
-    hipLaunchKernelGGL((map_move_kernel<T, W, kMapThreads, kHBlock, EXPAND, DOT>), grid,
-                       dim3(kMapThreads), lds, s, a, tail);
+  if constexpr (DOT) {
+    if (a.d <= 512) start_move<T, W, 64, 1, EXPAND, true>(a, tail, s);
+    else if (a.d <= 1024) start_move<T, W, 128, 1, EXPAND, true>(a, tail, s);
+    else if (a.d <= 2048) start_move<T, W, 256, 1, EXPAND, true>(a, tail, s);
+    else start_move<T, W, 256, 2, EXPAND, true>(a, tail, s);
+  } else {
+    start_move<T, W, 64, 1, EXPAND, false>(a, tail, s);
+  }
   FMOE_LAUNCH_CHECK(EXPAND ? "map_expand" : "map_reduce");
   return FMOE_OK;
 }
@@ -409,8 +440,9 @@ template <bool EXPAND>
 static int move(const MapMoveArgs& a, int dtype, int weight_dtype, const int32_t* n_rows_dev,
                 int64_t max_rows, hipStream_t s) {
   const char* const name = EXPAND ? "map_expand" : "map_reduce";
-  FMOE_REQUIRE(a.n_tokens >= 0 && a.n_tokens < INT32_MAX && a.d >= 1 && a.n_expert >= 1 &&
-                   a.n_expert <= FMOE_MAP_MAX_EXPERTS && max_rows >= 0 && max_rows < INT32_MAX,
+  FMOE_REQUIRE(a.n_tokens >= 0 && a.n_tokens <= kMapMostTokens && a.d >= 1 && a.n_expert >= 1 &&
+                   a.n_expert <= FMOE_MAP_MAX_EXPERTS && max_rows >= 0 && max_rows < INT32_MAX &&
+                   a.n_tokens * ((a.d + 511) / 512) < (int64_t)1 << 26,
                FMOE_ERR_INVALID, "%s: bad sizes", name);
   FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_F16 || dtype == FMOE_BF16, FMOE_ERR_UNSUPPORTED,
                "%s: unsupported dtype %d", name, dtype);
@@ -439,8 +471,8 @@ static int move(const MapMoveArgs& a, int dtype, int weight_dtype, const int32_t
 
 extern "C" int64_t fmoe_map_workspace_bytes(int64_t n_tokens, int32_t n_expert) {
   using namespace fmoe;
-  FMOE_REQUIRE(n_tokens >= 0 && n_expert >= 1 && n_expert <= FMOE_MAP_MAX_EXPERTS &&
-                   n_tokens <= INT32_MAX / n_expert,
+  FMOE_REQUIRE(n_tokens >= 0 && n_tokens <= kMapMostTokens && n_expert >= 1 &&
+                   n_expert <= FMOE_MAP_MAX_EXPERTS && n_tokens <= INT32_MAX / n_expert,
                FMOE_ERR_INVALID, "map: bad sizes");
   const MapBlocks b(n_tokens);
   return b.blocks <= 1 ? 0 : (int64_t)b.blocks * map_hist_row(n_expert) * (int64_t)sizeof(uint16_t);
@@ -463,16 +495,16 @@ extern "C" int fmoe_map_plan(const uint8_t* map, int64_t n_tokens, int32_t n_exp
                (long long)need);
   hipStream_t s = (hipStream_t)stream;
   const MapBlocks b(n_tokens);
-  const int row = map_hist_row(n_expert);
   uint16_t* const hist = b.blocks > 1 ? (uint16_t*)workspace : nullptr;
-  const size_t counters = sizeof(int32_t) * kMapWaves * n_expert;
+  FMOE_SET_DYNAMIC_LDS_ONCE(map_count_kernel, map_lds(FMOE_MAP_MAX_EXPERTS, false));
+  FMOE_SET_DYNAMIC_LDS_ONCE(map_place_kernel, map_lds(FMOE_MAP_MAX_EXPERTS, true));
   if (hist)
-    hipLaunchKernelGGL(map_count_kernel, dim3(b.blocks), dim3(kMapThreads), counters, s, map,
-                       n_tokens, n_expert, hist);
+    hipLaunchKernelGGL(map_count_kernel, dim3(b.blocks), dim3(kMapThreads), map_lds(n_expert, false),
+                       s, map, n_tokens, n_expert, hist);
   FMOE_LAUNCH_CHECK("map_count");
-  hipLaunchKernelGGL(map_place_kernel, dim3(b.blocks), dim3(kMapThreads),
-                     counters + sizeof(int32_t) * row * (2 + kMapWaves), s, map, n_tokens, n_expert,
-                     (int)max_rows, hist, counts, seg_off, token_off, (int2*)pairs);
+  hipLaunchKernelGGL(map_place_kernel, dim3(b.blocks), dim3(kMapThreads), map_lds(n_expert, true), s,
+                     map, n_tokens, n_expert, (int)max_rows, hist, counts, seg_off, token_off,
+                     (int2*)pairs);
   FMOE_LAUNCH_CHECK("map_place");
   return FMOE_OK;
 }

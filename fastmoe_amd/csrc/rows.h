@@ -1,6 +1,8 @@
 // Rows of values on their way into and out of quantised form: loads and stores of 8 values a lane,
 // segment bounds from counts, rows that a kernel clears in passing.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace fmoe {
@@ -31,6 +33,79 @@ __device__ __forceinline__ void store8(T* row, int k, int k_total, const float (
 #pragma unroll
     for (int i = 0; i < N; ++i) x.v[i] = Elem<T>::from_acc(v[p + i]);
     *reinterpret_cast<Run<T, N>*>(row + k + p) = x;
+  }
+}
+
+// 8 values as they lie in memory, in whole registers.
+template <typename T> struct Eight {
+  uint32_t w[2 * sizeof(T)];
+
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (std::is_same<T, float>::value) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __hip_bfloat16>::value) {
+      return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    } else {
+      return __half2float(__builtin_bit_cast(__half, (uint16_t)(w[i >> 1] >> (16 * (i & 1)))));
+    }
+  }
+  __device__ __forceinline__ void widen(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (*this)[i];
+  }
+
+  // Values k .. k + 7 of a row of any alignment, zeros from its end d on.
+  __device__ __forceinline__ void load(const T* row, int k, int d) {
+    if (k + 8 <= d) {
+      __builtin_memcpy(w, row + k, sizeof(w));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * (int)sizeof(T); ++i) w[i] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (k + i >= d) break;
+        if constexpr (sizeof(T) == 4) w[i] = __builtin_bit_cast(uint32_t, row[k + i]);
+        else w[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[k + i]) << (16 * (i & 1));
+      }
+    }
+  }
+
+  // The bits, as f32, of the largest magnitude (NaN > infinity > numbers) of these and of `bits`,
+  // what earlier calls returned (0 at first); f32_bits() of the last one is the answer.
+  __device__ __forceinline__ uint32_t widest(uint32_t bits) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) bits = max(bits, w[i] & 0x7fffffffu);
+    } else {
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 m = __builtin_bit_cast(u16x2, bits);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+      bits = __builtin_bit_cast(uint32_t, m);
+    }
+    return bits;
+  }
+  static __device__ __forceinline__ uint32_t f32_bits(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) return bits;
+    const uint32_t m = max(bits & 0xffffu, bits >> 16);
+    if constexpr (std::is_same<T, __hip_bfloat16>::value) return m << 16;
+    else return __float_as_uint(__half2float(__builtin_bit_cast(__half, (uint16_t)m)));
+  }
+};
+
+// 8 values into a row of any alignment, from k on, nothing behind its end d.
+template <typename T>
+__device__ __forceinline__ void store_any(T* row, int k, int d, const float (&v)[8]) {
+  T o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = Elem<T>::from_acc(v[i]);
+  if (k + 8 <= d) {
+    __builtin_memcpy(row + k, o, 8 * sizeof(T));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < d) row[k + i] = o[i];
   }
 }
 
