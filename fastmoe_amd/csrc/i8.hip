@@ -143,8 +143,8 @@ __global__ __launch_bounds__(W * kWave) void i8_quantize_kernel(
     const T* const src = x + row * k;
 #pragma unroll
     for (int c = 0; c < kHeld; ++c) {
-      if ((c + 1) * kSpan <= k) __builtin_memcpy(&held[c], src + c * kSpan + at, sizeof(held[c]));
-      else if (c * kSpan < k) held[c].load(src, c * kSpan + at, k);
+      if ((c + 1) * kSpan <= k) held[c].template load<true>(src + c * kSpan + at);
+      else if (c * kSpan < k) held[c].template load<true>(src, c * kSpan + at, k);
     }
   };
   int64_t r = blockIdx.x;

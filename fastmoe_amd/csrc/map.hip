@@ -36,7 +36,7 @@ static_assert(kMapMostTokens / kMapBlocks < 65536, "counts fit");
 
 struct MapBlocks {
   int per_block, per_wave, blocks;     // tokens of a block and of a wave; blocks
-  __host__ __device__ explicit MapBlocks(int64_t n_tokens) {
+  explicit MapBlocks(int64_t n_tokens) {
     const int64_t units = (n_tokens + kMapUnit - 1) / kMapUnit;
     const int64_t waves = (units < kMapBlocks ? units : kMapBlocks) * kMapWaves;
     per_wave = (int)((n_tokens + waves - 1) / waves);
@@ -103,12 +103,12 @@ struct MapWave {
 
 __global__ __launch_bounds__(kMapThreads) void map_count_kernel(const uint8_t* __restrict__ map,
                                                                 int64_t n_tokens, int n_expert,
+                                                                MapBlocks b,
                                                                 uint16_t* __restrict__ hist) {
   extern __shared__ __align__(16) uint8_t lds[];
   uint16_t* const masks = (uint16_t*)(lds + kMapWaves * kMapStage);
   const int row = map_hist_row(n_expert);
   int32_t* const count = (int32_t*)(masks + kMapWaves * row);
-  const MapBlocks b(n_tokens);
   MapWave w(map, n_tokens, n_expert, b, lds, masks);
   for (int e = threadIdx.x; e < row; e += kMapThreads) count[e] = 0;
   __syncthreads();
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kMapThreads) void map_count_kernel(const uint8_t* _
 }
 
 __global__ __launch_bounds__(kMapThreads) void map_place_kernel(
-    const uint8_t* __restrict__ map, int64_t n_tokens, int n_expert, int max_rows,
+    const uint8_t* __restrict__ map, int64_t n_tokens, int n_expert, int max_rows, MapBlocks b,
     const uint16_t* __restrict__ hist, int64_t* __restrict__ counts, int32_t* __restrict__ seg_off,
     int32_t* __restrict__ token_off, int2* __restrict__ pairs) {
   extern __shared__ __align__(16) uint8_t lds[];
@@ -132,7 +132,6 @@ __global__ __launch_bounds__(kMapThreads) void map_place_kernel(
   uint16_t* const taken = masks + kMapWaves * row;             // [waves][n_expert]
   int32_t* const total = (int32_t*)(taken + kMapWaves * row);  // [row] tokens of an expert
   int32_t* const before = total + row;                         // [row] of those, in earlier blocks
-  const MapBlocks b(n_tokens);
   MapWave w(map, n_tokens, n_expert, b, lds, masks);
   const int lane = w.lane, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   uint16_t* const mine = taken + wave * n_expert;
@@ -304,9 +303,9 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
   int k0 = 0;
   if constexpr (!DOT) {
     const int pieces = (a.d + kPiece - 1) / kPiece;
-    const int64_t item = (int64_t)blockIdx.x * (256 / kWave) + wave;
-    t = item / pieces;
-    k0 = (int)(item - t * pieces) * kPiece;
+    const uint32_t item = blockIdx.x * (256 / kWave) + wave;      // (below 2^26)
+    t = item / (uint32_t)pieces;
+    k0 = (int)(item - (uint32_t)t * pieces) * kPiece;
     if (t >= a.n_tokens) return;
   }
   const T* const one = (const T*)a.one + t * a.d;
@@ -352,7 +351,7 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
             if (j + u >= n) break;
             const int64_t r = __builtin_amdgcn_readlane(pair.x, j + u);
 #pragma unroll
-            for (int h = 0; h < H; ++h) raw[u][h].load(many + r * a.d, k0 + h * kSpan + at, a.d);
+            for (int h = 0; h < H; ++h) raw[u][h].template load<true>(many + r * a.d, k0 + h * kSpan + at, a.d);
           }
         }
 #pragma unroll
@@ -376,7 +375,7 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
               float v[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) v[i] = x[h][i] * wj;
-              store_any(out + r * a.d, k0 + h * kSpan + at, a.d, v);
+              store_any<true>(out + r * a.d, k0 + h * kSpan + at, a.d, v);
             } else {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
@@ -500,10 +499,10 @@ extern "C" int fmoe_map_plan(const uint8_t* map, int64_t n_tokens, int32_t n_exp
   FMOE_SET_DYNAMIC_LDS_ONCE(map_place_kernel, map_lds(FMOE_MAP_MAX_EXPERTS, true));
   if (hist)
     hipLaunchKernelGGL(map_count_kernel, dim3(b.blocks), dim3(kMapThreads), map_lds(n_expert, false),
-                       s, map, n_tokens, n_expert, hist);
+                       s, map, n_tokens, n_expert, b, hist);
   FMOE_LAUNCH_CHECK("map_count");
   hipLaunchKernelGGL(map_place_kernel, dim3(b.blocks), dim3(kMapThreads), map_lds(n_expert, true), s,
-                     map, n_tokens, n_expert, (int)max_rows, hist, counts, seg_off, token_off,
+                     map, n_tokens, n_expert, (int)max_rows, b, hist, counts, seg_off, token_off,
                      (int2*)pairs);
   FMOE_LAUNCH_CHECK("map_place");
   return FMOE_OK;

@@ -54,10 +54,23 @@ template <typename T> struct Eight {
     for (int i = 0; i < 8; ++i) v[i] = (*this)[i];
   }
 
-  // Values k .. k + 7 of a row of any alignment, zeros from its end d on.
-  __device__ __forceinline__ void load(const T* row, int k, int d) {
+  // Values k .. k + 7 of a row of any alignment, all of them there.  ONCE: nobody reads them again
+  // (the loads do not displace what the caches hold: 131072 rows of 2048 summed up by eights, 119 us
+  // without, 102 with).
+  template <bool ONCE = false> __device__ __forceinline__ void load(const T* p) {
+    typedef uint32_t Pack __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+    for (int i = 0; i < 2 * (int)sizeof(T); i += 4) {
+      const Pack* const from = reinterpret_cast<const Pack*>(p) + i / 4;
+      const Pack v = ONCE ? __builtin_nontemporal_load(from) : *from;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[i + j] = v[j];
+    }
+  }
+  // Likewise, zeros from the row's end d on.
+  template <bool ONCE = false> __device__ __forceinline__ void load(const T* row, int k, int d) {
     if (k + 8 <= d) {
-      __builtin_memcpy(w, row + k, sizeof(w));
+      load<ONCE>(row + k);
     } else {
 #pragma unroll
       for (int i = 0; i < 2 * (int)sizeof(T); ++i) w[i] = 0;
@@ -94,14 +107,22 @@ template <typename T> struct Eight {
   }
 };
 
-// 8 values into a row of any alignment, from k on, nothing behind its end d.
-template <typename T>
+// 8 values into a row of any alignment, from k on, nothing behind its end d.  ONCE: not to be read
+// before much else was written.
+template <bool ONCE = false, typename T>
 __device__ __forceinline__ void store_any(T* row, int k, int d, const float (&v)[8]) {
   T o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = Elem<T>::from_acc(v[i]);
   if (k + 8 <= d) {
-    __builtin_memcpy(row + k, o, 8 * sizeof(T));
+    typedef uint32_t Pack __attribute__((ext_vector_type(4), aligned(2)));
+    Pack p[sizeof(T) / 2];
+    __builtin_memcpy(p, o, sizeof(p));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      if constexpr (ONCE) __builtin_nontemporal_store(p[i], reinterpret_cast<Pack*>(row + k) + i);
+      else reinterpret_cast<Pack*>(row + k)[i] = p[i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)

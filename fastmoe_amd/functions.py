@@ -215,11 +215,10 @@ class MapPlan:
     def __init__(self, routing_map: torch.Tensor, max_rows=None):
         if routing_map.dim() != 2 or routing_map.dtype != torch.bool:
             raise RuntimeError("routing_map must be bool [tokens, experts]")
-        with torch.no_grad():
-            if max_rows is None:
-                max_rows = int(routing_map.sum())
-            self.counts, seg_off, self.token_off, self.pairs = fmoe_cuda.map_plan(
-                routing_map.contiguous(), int(max_rows))
+        if max_rows is None:
+            max_rows = int(routing_map.sum())
+        self.counts, seg_off, self.token_off, self.pairs = fmoe_cuda.map_plan(
+            routing_map.contiguous(), int(max_rows))
         self.n_tokens, self.num_expert = routing_map.shape
         self.max_rows = int(max_rows)
         self.segments = SegmentTable(seg_off, self.counts)
