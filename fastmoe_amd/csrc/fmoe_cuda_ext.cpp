@@ -833,6 +833,7 @@ PYBIND11_MODULE(fmoe_cuda, m) {
   m.def("i8_quantize_rows", &i8_quantize_rows);
   m.def("i8_dequantize_rows", &i8_dequantize_rows);
   m.def("i8_linear", &i8_linear);
+  m.def("i8_expert_layer", &i8_expert_layer);
   m.def("map_plan", &map_plan, py::arg("routing_map"), py::arg("max_rows"));
   m.def("map_expand", &map_expand, py::arg("tokens"), py::arg("weight"), py::arg("seg_off"),
         py::arg("token_off"), py::arg("pairs"), py::arg("given") = py::none(),

@@ -250,4 +250,37 @@ Tensor i8_linear(const Tensor& x, const OptTensor& counts_or_seg, const Tensor& 
   return I8LinearNode::run(rows, I8Rows(rows, counts_or_seg), wc, ws, b);
 }
 
+// i8.expert_layer without gradients, for an activation the library has: gate_idx and score
+// [tokens, top_k].  The hidden layer is rounded to x's type in front of its quantisation, as in the
+// chain of single operators, whose bits these are.
+Tensor i8_expert_layer(const Tensor& x_in, const Tensor& gate_idx, const Tensor& score_in,
+                       const Tensor& w1c, const Tensor& w1s, int64_t in_f, const OptTensor& b1,
+                       const Tensor& w2c, const Tensor& w2s, int64_t hidden, const OptTensor& b2,
+                       int64_t act) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  need(x_in.is_cuda() && x_in.dim() == 2, "x must be a 2-d CUDA tensor");
+  need(gate_idx.dim() == 2 && gate_idx.size(0) == x_in.size(0), "gate_idx must be [tokens, top_k]");
+  need(score_in.numel() == gate_idx.numel(), "score must be [tokens, top_k]");
+  need(w1c.dim() == 3 && w2c.dim() == 3 && w1c.size(0) == w2c.size(0) && w1c.size(1) == hidden,
+       "w1 must be [E, hidden, in] and w2 [E, out, hidden]");
+  need(act == FMOE_ACT_GELU || act == FMOE_ACT_RELU, "unknown activation");
+  c10::DeviceGuard guard(x_in.device());
+  const Tensor x = x_in.contiguous();
+  const int64_t t = x.size(0), k = gate_idx.size(1);
+  auto bias = [&](const OptTensor& b) {
+    return b.has_value() && b->defined() ? OptTensor(b->to(x.scalar_type()).contiguous()) : OptTensor();
+  };
+  auto r = route(gate_idx.contiguous(), w1c.size(0), true);
+  const Tensor &seg = std::get<2>(r), &inv = *std::get<3>(r);
+  const Tensor live = seg.narrow(0, seg.numel() - 1, 1);
+  auto q = i8_quantize_tokens(x, inv, k);
+  Tensor h = torch::empty({t * k, hidden}, x.options());
+  i8_linear_fwd(std::get<0>(q), std::get<1>(q), w1c, w1s, in_f, bias(b1), seg, h);
+  h = act == FMOE_ACT_GELU ? gelu_fwd(h, live) : h.relu_();
+  q = i8_quantize(h, live);
+  Tensor y = torch::empty({t * k, w2c.size(1)}, x.options());
+  i8_linear_fwd(std::get<0>(q), std::get<1>(q), w2c, w2s, hidden, bias(b2), seg, y);
+  return gather_combine_fwd(y, inv, score_in.reshape({t, k}).contiguous().to(x.scalar_type()), t, k);
+}
+
 }  // namespace

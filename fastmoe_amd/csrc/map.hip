@@ -37,9 +37,9 @@ static_assert(kMapMostTokens / kMapBlocks < 65536, "counts fit");
 struct MapBlocks {
   int per_block, per_wave, blocks;     // tokens of a block and of a wave; blocks
   explicit MapBlocks(int64_t n_tokens) {
-    const int64_t units = (n_tokens + kMapUnit - 1) / kMapUnit;
-    const int64_t waves = (units < kMapBlocks ? units : kMapBlocks) * kMapWaves;
-    per_wave = (int)((n_tokens + waves - 1) / waves);
+    const int64_t units = std::max<int64_t>((n_tokens + kMapUnit - 1) / kMapUnit, 1);
+    const int64_t waves = std::min<int64_t>(units, kMapBlocks) * kMapWaves;
+    per_wave = std::max((int)((n_tokens + waves - 1) / waves), 1);
     per_block = per_wave * kMapWaves;
     blocks = (int)((n_tokens + per_block - 1) / per_block);
   }

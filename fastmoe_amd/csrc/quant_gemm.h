@@ -41,34 +41,7 @@ __device__ __forceinline__ i32x4 mx_descriptor(const void* p, int64_t bytes) {
   return r;
 }
 
-// gelu(x) = x Phi(x) with Phi(x) = 1 / (1 + 2^z), z = -log2(Phi(x) / Phi(-x)) = x P(x^2) for
-// |x| <= 6 and x P(36) outside: P of degree 12 in x^2 / 18 - 1, a reweighted least-squares fit on
-// Chebyshev nodes.  Within 2e-7 + 3e-7 |gelu| of gelu everywhere (the fit, evaluated in f32 with an
-// exact exponential and quotient: 1.42e-7 + 1e-7 |gelu|; the two instructions for these are good to
-// 1.2e-7 each), so that hardly more codes than the sums' own rounding makes land on the other side
-// of a boundary (degree 9, three instructions less, was off by 7e-7), and, for |x| <= 6, within
-// 5e-6 of its value (3.7e-6 likewise), so that blocks whose values all lie in the negative tail
-// keep their digits as well.  26 issue slots where erff takes about
-// 60, with branches, and loses the tail: with one wave on a SIMD nothing hides them (a 256 x 256
-// tile of 4096 features: 27 us of matrix instructions, 26 us of erff).
-__device__ __forceinline__ float mx_gelu(float x) {
-  const float t = fminf(fmaf(x * x, 1.f / 18.f, -1.f), 1.f);
-  float p = 0.00220932276f;
-  p = fmaf(p, t, -0.00235819351f);
-  p = fmaf(p, t, -0.00623256993f);
-  p = fmaf(p, t, 0.0106137199f);
-  p = fmaf(p, t, -0.00437692506f);
-  p = fmaf(p, t, 0.0022452944f);
-  p = fmaf(p, t, -0.00346183078f);
-  p = fmaf(p, t, -0.00412944285f);
-  p = fmaf(p, t, 0.0250278097f);
-  p = fmaf(p, t, -0.0735082775f);
-  p = fmaf(p, t, 0.223777682f);
-  p = fmaf(p, t, -1.27482498f);
-  p = fmaf(p, t, -3.8811202f);
-  // (2^z overflows to infinity far down, its inverse is 0 there)
-  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * p));
-}
+__device__ __forceinline__ float mx_gelu(float x);     // (only the 4-bit product has it behind it)
 
 // How a product leaves: y where rows are whole 16-byte packs, any other y, or MXFP4 again behind
 // one of the activations.
@@ -149,8 +122,8 @@ template <typename T, int MODE> struct MxOutput {
   static __device__ __forceinline__ void activate(float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (MODE == kMxQuantGelu) v[i] = mx_gelu(v[i]);
-      if (MODE == kMxQuantRelu) v[i] = __builtin_elementwise_maximum(v[i], 0.f);   // (a NaN stays)
+      if constexpr (MODE == kMxQuantGelu) v[i] = mx_gelu(v[i]);
+      if constexpr (MODE == kMxQuantRelu) v[i] = __builtin_elementwise_maximum(v[i], 0.f);   // (a NaN stays)
     }
   }
 

@@ -17,8 +17,10 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import fmoe_cuda
+from .frozen import FrozenExpert, layer_chain
 from .functions import SegmentTable
-from .linear import _segments
+from .linear import _segments, native_act
+from .transformer import _watched
 
 STEP = 128      # rows of codes are padded with zeros to multiples of this
 
@@ -170,3 +172,63 @@ def linear(x: torch.Tensor, fwd_expert_count, weight: I8Tensor, bias=None) -> to
     if fwd_expert_count is None and (codes.dim() != 3 or codes.shape[0] != 1):
         raise RuntimeError("the rows of several experts need counts")
     return I8Linear.apply(x, fwd_expert_count, codes, scales, bias)
+
+
+def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w1: I8Tensor, b1,
+                 w2: I8Tensor, b2, activation) -> torch.Tensor:
+    r"""sum_j score[t, j] * expert_{gate_idx[t, j]}(x[t]) over the live slots (index >= 0), the
+    experts being `linear -> activation -> linear` with 8-bit weights w1 [E, hidden, in] and
+    w2 [E, out, hidden].  Without gradients and for GELU and ReLU tokens are quantised into expert
+    order in one pass; the bits are those of the chain of single operators, which runs otherwise.
+    An activation module with hooks, or a `forward` set on it, is called.  The hidden layer and the
+    result have x's dtype; biases of another are taken in it."""
+    top_k = gate_idx.shape[-1] if gate_idx.dim() >= 2 else 1
+    if x.dim() != 2 or x.shape[1] != w1.features or w1.codes.shape[-2] != w2.features:
+        raise RuntimeError("x [tokens, in], w1 [E, hidden, in] and w2 [E, out, hidden] disagree")
+    act = 0 if _watched(activation) else native_act(activation, x)
+    grads = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, score, b1, b2))
+    gate_idx = gate_idx.reshape(-1, top_k)
+    native = None if grads or not act or x.dtype == torch.float64 else fmoe_cuda.native()
+    if native is None:
+        return layer_chain(linear, x, gate_idx, score, w1, b1, w2, b2, activation)
+    return native.i8_expert_layer(x, gate_idx, score, w1.codes, w1.scales, w1.features, b1,
+                                  w2.codes, w2.scales, w2.features, b2, act)
+
+
+class I8Expert(FrozenExpert):
+    r"""The experts of a layer (`linear -> activation -> linear`) with 8-bit weights, in the place
+    of the fused `_Expert`: `layer.experts = I8Expert.from_expert(layer.experts)`, or
+    `quantize_experts(layer)`.  Codes and scales are buffers and frozen; the biases stay parameters.
+    Scales stay in float32 whatever dtype the module is cast to."""
+
+    tensor = I8Tensor
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = {name: getattr(self, name) for name in ("w1_scales", "w2_scales")}
+        super()._apply(fn, *args, **kwargs)
+        for name, scales in kept.items():
+            now = getattr(self, name)
+            if now.dtype != scales.dtype:
+                setattr(self, name, scales.to(now.device))
+        return self
+
+    @staticmethod
+    def quantize(weight):
+        return quantize(weight)
+
+    @staticmethod
+    def linear(x, counts, weight, bias):
+        return linear(x, counts, weight, bias)
+
+    @staticmethod
+    def layer(*args):
+        return expert_layer(*args)
+
+
+def quantize_experts(layer):
+    r"""Puts the fused experts of an `FMoE` layer on the GPU into 8 bits, in place; returns the
+    layer.  Its state dict then holds `experts.w1_codes`, `experts.w1_scales` and so on.  The gate
+    stays, and hooks on the layer, the gate and the activation; see FrozenExpert.from_expert for the
+    experts."""
+    return I8Expert.replace_in(layer)

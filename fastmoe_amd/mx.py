@@ -16,13 +16,12 @@ import torch
 import torch.nn as nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
-from torch.nn.modules.module import _has_any_global_hook
 
 from . import fmoe_cuda
-from .functions import (FusedGatherCombine, FusedScatter, RoutePlan, SegmentTable,
-                        apply_activation)
-from .linear import FMoELinear, _segments, is_exact_gelu, native_act
-from .transformer import _Expert, _watched
+from .frozen import FrozenExpert, layer_chain
+from .functions import SegmentTable
+from .linear import _segments, native_act
+from .transformer import _watched
 
 BLOCK = 32      # features that share a scale
 
@@ -173,53 +172,6 @@ def linear(x: torch.Tensor, fwd_expert_count, weight: MXTensor, bias=None) -> to
     return MXLinear.apply(x, fwd_expert_count, weight.codes, weight.scales, bias)
 
 
-def _activate(activation, x, n_rows_dev):
-    r"""`activation(x)`, called as the module it is where somebody watches it."""
-    return activation(x) if _watched(activation) else apply_activation(activation, x, n_rows_dev)
-
-
-def _as(x, bias):
-    return x if bias is None else x.type_as(bias)
-
-
-class _Route(Function):
-    r"""fmoe_cuda.route as an operation that tracing records."""
-
-    @staticmethod
-    def forward(ctx, gate_idx, n_expert):
-        routed = fmoe_cuda.route(gate_idx.contiguous(), n_expert)
-        ctx.mark_non_differentiable(*routed)
-        return tuple(routed)
-
-    @staticmethod
-    def backward(ctx, *_grads):
-        return None, None
-
-
-class _Scatter(Function):
-    r"""FusedScatter on the tensors of its plan, for tracing (a plan would be a constant)."""
-
-    @staticmethod
-    def forward(ctx, x, gate_idx, n_expert, *routed):
-        return FusedScatter.forward(ctx, x, RoutePlan(gate_idx, n_expert, routed))
-
-    @staticmethod
-    def backward(ctx, grad_buf):
-        return (FusedScatter.backward(ctx, grad_buf)[0],) + (None,) * 6
-
-
-class _Combine(Function):
-    r"""FusedGatherCombine on the tensors of its plan, for tracing."""
-
-    @staticmethod
-    def forward(ctx, buf, score, gate_idx, n_expert, *routed):
-        return FusedGatherCombine.forward(ctx, buf, score, RoutePlan(gate_idx, n_expert, routed))
-
-    @staticmethod
-    def backward(ctx, grad_y):
-        return FusedGatherCombine.backward(ctx, grad_y)[:2] + (None,) * 6
-
-
 class MXExpertLayer(Function):
     r"""The layer without gradients (see expert_layer) operator by operator."""
 
@@ -267,146 +219,37 @@ def expert_layer(x: torch.Tensor, gate_idx: torch.Tensor, score: torch.Tensor, w
     if grads or not act or x.dtype == torch.float64:
         # (the hidden layer in x's dtype: any activation takes it so, and what its gradient keeps
         # until the backward pass is half of f32's size)
-        score = score.reshape(-1, top_k)
-        if torch._C._get_tracing_state() is not None:
-            routed = _Route.apply(gate_idx, n_expert)
-            segments, live = routed[2], routed[2][-1:]
-            h = _Scatter.apply(x, gate_idx, n_expert, *routed)
-        else:
-            plan = RoutePlan(gate_idx, n_expert)
-            segments, live = plan.segments, plan.n_rows_dev
-            h = FusedScatter.apply(x, plan)
-        b1 = None if b1 is None else b1.to(x.dtype)
-        h = _activate(activation, linear(h, segments, w1, b1), live)
-        y = linear(h, segments, w2, b2)
-        if torch._C._get_tracing_state() is not None:
-            return _Combine.apply(y, score, gate_idx, n_expert, *routed)
-        return FusedGatherCombine.apply(y, score, plan)
+        return layer_chain(linear, x, gate_idx, score, w1, b1, w2, b2, activation)
     native = fmoe_cuda.native()
     run = MXExpertLayer.apply if native is None else native.mx_expert_layer
     return run(x, gate_idx, score, w1.codes, w1.scales, w1.features, b1, w2.codes, w2.scales,
                w2.features, b2, act)
 
 
-def _experts(inp, counts, w1, b1, w2, b2, activation):
-    r"""The experts on rows in expert order, operator by operator."""
-    x = linear(_as(inp, b1), counts, w1, b1)
-    live = counts.seg_off[-1:] if isinstance(counts, SegmentTable) else None
-    x = _activate(activation, x, live)
-    return linear(_as(x, b2), counts, w2, b2)
-
-
-class _MXExpertView:
-    r"""`experts[i]` of an MXExpert: called like an MXExpert of one expert, on views of the
-    weights `w1`, `w2` (MXTensor [1, out, in]) and of the biases `b1`, `b2` (gradients flow into
-    the parameters)."""
-
-    def __init__(self, parent: "MXExpert", i: int):
-        def one(w):
-            return MXTensor(w.codes[i:i + 1], w.scales[i:i + 1], w.features)
-        self.w1, self.w2 = one(parent.w1), one(parent.w2)
-        self.b1, self.b2 = (None if b is None else b[i:i + 1] for b in (parent.b1, parent.b2))
-        self.activation = parent.activation
-
-    def __call__(self, inp, fwd_expert_count):
-        return _experts(inp, fwd_expert_count, self.w1, self.b1, self.w2, self.b2,
-                        self.activation)
-
-    def parameters(self):
-        return (b for b in (self.b1, self.b2) if b is not None)
-
-
-class MXExpert(nn.Module):
+class MXExpert(FrozenExpert):
     r"""The experts of a layer (`linear -> activation -> linear`) with 4-bit weights, in the
     place of the fused `_Expert`: `layer.experts = MXExpert.from_expert(layer.experts)`, or
     `quantize_experts(layer)`.  Weights are uint8 buffers and frozen; the biases stay
     parameters.  Accepts host counts or a device-side SegmentTable, casts its rows to its
     parameters' dtype, and gives views of single experts, as `_Expert` does."""
 
-    accepts_segment_table = True
+    tensor = MXTensor
 
-    def __init__(self, w1: MXTensor, b1, w2: MXTensor, b2, activation):
-        super().__init__()
-        if w1.codes.dim() != 3 or w2.codes.dim() != 3 or w1.shape[0] != w2.shape[0] or \
-                w1.shape[1] != w2.features:
-            raise ValueError(f"w1 [E, hidden, in] and w2 [E, out, hidden] disagree: "
-                             f"{tuple(w1.shape)}, {tuple(w2.shape)}")
-        for name, w in (("w1", w1), ("w2", w2)):
-            self.register_buffer(name + "_codes", w.codes.contiguous())
-            self.register_buffer(name + "_scales", w.scales.contiguous())
-        self.in_features, self.hidden_features = w1.features, w2.features
-        self.num_expert = w1.shape[0]
-        for name, b in (("b1", b1), ("b2", b2)):
-            b = None if b is None else nn.Parameter(b.detach().clone(),
-                                                    requires_grad=b.requires_grad)
-            self.register_parameter(name, b)
-        self.activation = activation
+    @staticmethod
+    def quantize(weight):
+        return quantize(weight)
 
-    @classmethod
-    def from_expert(cls, expert) -> "MXExpert":
-        r"""From a fused `_Expert` on the GPU, its weights quantised.  The biases keep their
-        `dp_comm` tags and what else was set on them, the module its training flag; hooks on
-        the expert module and on its two linear layers do not come along.  An expert with a
-        `forward` other than `_Expert`'s, in itself or a linear layer, is refused."""
-        l1, l2 = expert.htoh4, expert.h4toh
-        for module, kind in ((expert, _Expert), (l1, FMoELinear), (l2, FMoELinear)):
-            if type(module).forward is not kind.forward or "forward" in module.__dict__:
-                raise TypeError(f"{type(module).__name__} computes something of its own and "
-                                "cannot be quantised")
-        new = cls(quantize(l1.weight), l1.bias, quantize(l2.weight), l2.bias, expert.activation)
-        for old, b in ((l1.bias, new.b1), (l2.bias, new.b2)):
-            if b is not None:
-                b.__dict__.update(old.__dict__)
-        # (not train(): the activation is shared)
-        new.training = expert.training
-        return new
+    @staticmethod
+    def linear(x, counts, weight, bias):
+        return linear(x, counts, weight, bias)
 
-    @property
-    def w1(self) -> MXTensor:
-        return MXTensor(self.w1_codes, self.w1_scales, self.in_features)
-
-    @property
-    def w2(self) -> MXTensor:
-        return MXTensor(self.w2_codes, self.w2_scales, self.hidden_features)
-
-    def forward(self, inp, fwd_expert_count):
-        return _experts(inp, fwd_expert_count, self.w1, self.b1, self.w2, self.b2,
-                        self.activation)
-
-    # what FMoE.forward asks of a module that can run the whole dispatch
-    def can_run_layer(self, inp, top_k) -> bool:
-        return (torch.is_tensor(inp) and inp.dim() == 2 and inp.is_cuda and 1 <= top_k <= 64
-                and all(b is None or b.dtype == inp.dtype for b in (self.b1, self.b2))
-                and "forward" not in self.__dict__ and type(self).forward is MXExpert.forward
-                # (hooks on all modules see experts called where they see `_Expert` called)
-                and (is_exact_gelu(self.activation, inp) or not _has_any_global_hook())
-                and not (self._forward_hooks or self._forward_pre_hooks or self._backward_hooks
-                         or self._backward_pre_hooks))
-
-    def run_layer(self, inp, gate_idx, score):
-        return expert_layer(inp, gate_idx, score, self.w1, self.b1, self.w2, self.b2,
-                            self.activation)
-
-    def run_gated_layer(self, gate, inp):
-        return None      # (the gate always runs as the module it is)
-
-    def __len__(self):
-        return self.num_expert
-
-    def __getitem__(self, i):
-        if not -self.num_expert <= i < self.num_expert:
-            raise IndexError(f"expert {i} of {self.num_expert}")
-        return _MXExpertView(self, i % self.num_expert)
-
-    def __iter__(self):
-        return (_MXExpertView(self, i) for i in range(self.num_expert))
+    @staticmethod
+    def layer(*args):
+        return expert_layer(*args)
 
 
 def quantize_experts(layer):
     r"""Puts the fused experts of an `FMoE` layer on the GPU into 4 bits, in place; returns the
     layer.  Its state dict then holds `experts.w1_codes` and so on.  The gate stays, and hooks
     on the layer, the gate and the activation; see MXExpert.from_expert for the experts."""
-    if not isinstance(layer.experts, _Expert):
-        raise TypeError("only a layer whose experts are one fused module can be quantised")
-    layer.experts = MXExpert.from_expert(layer.experts)
-    return layer
+    return MXExpert.replace_in(layer)
