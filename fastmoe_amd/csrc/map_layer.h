@@ -22,14 +22,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> map_plan(Tensor map, int64_t max_rows
             torch::zeros({1}, ints), pairs};
   Tensor counts = torch::empty({e}, map.options().dtype(at::kLong));
   Tensor seg = torch::empty({e + 1}, ints), off = torch::empty({t + 1}, ints);
-  need(e <= FMOE_MAP_MAX_EXPERTS, "routing_map has more than " +
-                                      std::to_string(FMOE_MAP_MAX_EXPERTS) + " experts");
+  need(e <= FMOE_MAP_MAX_EXPERTS, "routing_map has too many experts");
   const int64_t bytes = fmoe_map_workspace_bytes(t, (int32_t)e);
   check(bytes < 0 ? (int)bytes : 0, "map_plan");
-  Tensor ws = workspace_of(bytes, map);
+  Tensor ws;                           // (few tokens need none)
+  if (bytes > 0) ws = workspace_of(bytes, map);
   check(fmoe_map_plan((const uint8_t*)map.data_ptr(), t, (int32_t)e, max_rows,
                       counts.data_ptr<int64_t>(), seg.data_ptr<int32_t>(), off.data_ptr<int32_t>(),
-                      pairs.data_ptr<int32_t>(), ws.data_ptr(), ws.numel(), stream_of(map)),
+                      pairs.data_ptr<int32_t>(), bytes > 0 ? ws.data_ptr() : nullptr, bytes,
+                      stream_of(map)),
         "map_plan");
   return {counts, seg, off, pairs};
 }
@@ -43,11 +44,12 @@ void map_check(const Tensor& given, const char* name, int64_t count, const OptTe
   dev(pairs, "pairs", at::kInt);
   need(pairs.dim() == 2 && pairs.size(1) == 2 && token_off.numel() >= 1 && seg_off.numel() >= 2,
        "the plan's tensors do not belong together");
-  need(given.dim() == 2 && given.size(0) == count && given.size(1) >= 1,
-       std::string(name) + " must be [" + std::to_string(count) + ", features]");
-  need(given.device() == seg_off.device() && given.device() == token_off.device() &&
-           given.device() == pairs.device(),
-       std::string(name) + " and the plan must share a device");
+  // (texts are put together where they are wanted: a decode step's calls are all host time)
+  if (!(given.dim() == 2 && given.size(0) == count && given.size(1) >= 1))
+    need(false, std::string(name) + " must be [" + std::to_string(count) + ", features]");
+  if (!(given.device() == seg_off.device() && given.device() == token_off.device() &&
+        given.device() == pairs.device()))
+    need(false, std::string(name) + " and the plan must share a device");
   if (weight.has_value() && weight->defined()) {
     dev(*weight, "weight");
     need(weight->dim() == 2 && weight->size(0) == token_off.numel() - 1 &&

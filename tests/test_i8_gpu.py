@@ -328,6 +328,39 @@ def test_outputs_and_rows_beyond_32_bits():
     assert torch.equal(q.dequantize()[-3:], i8.quantize(x[-3:]).dequantize())
 
 
+@pytest.mark.parametrize("rows", [3, 60, 200])
+def test_the_largest_sums_fit(rows):
+    """131072 products of 127 * 127 are just below 2^31."""
+    x = torch.ones(rows, 131072, device="cuda")
+    x[1] = -1
+    w = i8.quantize(torch.ones(1, 8, 131072, device="cuda"))
+    y = i8.linear(x, None, w)
+    # two scales of 1 / 127, the sum, two products: 5 roundings of 2^-24
+    assert ((y - 131072 * x[:, :8]).abs() <= 5 * 2.0 ** -24 * 131072).all()
+
+
+def test_no_rows_and_experts_without_any():
+    w, b = weights(3, 16, 40, 2, torch.bfloat16)
+    b.requires_grad_()
+    for rows in (0, 4):
+        x = torch.ones(rows, 40, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        for counts in (torch.zeros(3, dtype=torch.int64), torch.zeros(3, dtype=torch.int64).cuda()):
+            b.grad = x.grad = None
+            y = i8.linear(x, counts, w, b)
+            assert y.shape == (rows, 16)
+            y.backward(torch.ones_like(y))
+            assert not x.grad.any() and not b.grad.any()
+
+
+def test_weights_changed_before_the_backward_pass_are_noticed():
+    x = randn((8, 64), torch.float32, 1).cuda().requires_grad_()
+    w, _ = weights(1, 32, 64, 2)
+    y = i8.linear(x, None, w)
+    w.scales.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_both_bindings_give_the_same_bits(monkeypatch):
     x = randn((60, 300), torch.float16, 1).cuda()
     w, b = weights(3, 136, 300, 2, torch.float16)

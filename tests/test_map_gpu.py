@@ -160,6 +160,39 @@ def test_rows_behind_the_last_and_rows_cut_off():
     assert len(tensors) == 3
 
 
+def test_no_rows_at_all():
+    m = make_map(70, 5, 0.5, 1).cuda()
+    for plan in (functions.MapPlan(m, 0), functions.MapPlan(torch.zeros_like(m), 4)):
+        x = randn((70, 24), torch.bfloat16, 1).cuda().requires_grad_()
+        w = torch.rand(70, 5, device="cuda", requires_grad=True)
+        rows = functions.sort_tokens(x, plan, w)
+        assert rows.shape == (plan.max_rows, 24) and plan.counts.tolist() == [0] * 5
+        rows.backward(torch.ones_like(rows))
+        assert not x.grad.any() and not w.grad.any()
+        r = torch.ones(plan.max_rows, 24, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        w.grad = None
+        y = functions.unsort_tokens(r, plan, w)
+        assert not y.any()
+        y.backward(torch.ones_like(y))
+        assert not r.grad.any() and not w.grad.any()
+
+
+def test_plans_used_twice_and_traces():
+    m = make_map(60, 7, 0.3, 2).cuda()
+    plan = functions.MapPlan(m)
+    x = randn((60, 40), torch.float32, 1).cuda().requires_grad_()
+    a, b = functions.sort_tokens(x, plan), functions.sort_tokens(x, plan)
+    (a.sum() + b.sum()).backward()
+    want = 2.0 * m.sum(1, keepdim=True).expand(60, 40)
+    assert torch.equal(x.grad, want)
+    y = functions.sort_tokens(x, plan)
+    plan.pairs.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError):
+        torch.jit.trace(lambda z: functions.sort_tokens(z, plan), x.detach())
+
+
 def test_values_that_are_not_finite_stay_where_they_are():
     m = torch.tensor([[True, False], [True, True], [False, False]])
     plan = functions.MapPlan(m.cuda())
