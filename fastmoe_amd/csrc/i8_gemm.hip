@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256, (QuantTile<true, TN, TM>::kGroups)) void i8_ti
 constexpr int kCus = 256;
 
 enum I8Kernel { kStream, kTile128x64, kTile128x128, kTile256x256 };
-static I8Kernel choose_kernel(const QuantGemmArgs& a, bool packed) {
+static I8Kernel choose_kernel(const QuantGemmArgs& a) {
   const double live = (double)std::min<int64_t>(a.n_expert, a.n_rows);
   const double mean = (double)a.n_rows / a.n_expert;
   // (of several experts the last tile is half empty on average)
@@ -100,7 +100,7 @@ static I8Kernel choose_kernel(const QuantGemmArgs& a, bool packed) {
   };
   if (mean <= 16 && tiles(128, 64) <= kCus / 2) return kStream;
   if (mean < 56) return kTile128x64;
-  if (packed && mean >= 192 && a.in_feat >= 1024 &&
+  if (mean >= 192 && a.in_feat >= 1024 &&
       std::max(tiles(256, 256) / kCus, 1.) <= 0.73 * std::max(tiles(128, 128) / (2 * kCus), 1.))
     return kTile256x256;
   return kTile128x128;
@@ -118,7 +118,7 @@ static int launch(const QuantGemmArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((i8_tile_kernel<T, TN, TM, MODE>), dim3(kCus * S::kGroups), dim3(256),    \
                        S::kLdsBytes, s, a);                                                      \
   } while (0)
-  switch (choose_kernel(a, MODE == kMxPacked)) {
+  switch (choose_kernel(a)) {
     case kStream: {
       const int64_t rows = a.n_rows / 16 + std::min<int64_t>(a.n_expert, a.n_rows);
       hipLaunchKernelGGL((i8_stream_kernel<T, MODE>),
@@ -128,9 +128,7 @@ static int launch(const QuantGemmArgs& a, hipStream_t s) {
     }
     case kTile128x64: FMOE_TILE(128, 64); break;
     case kTile128x128: FMOE_TILE(128, 128); break;
-    case kTile256x256:      // (only for packed rows: with any, its registers do not suffice)
-      if constexpr (MODE == kMxPacked) FMOE_TILE(256, 256);
-      break;
+    case kTile256x256: FMOE_TILE(256, 256); break;
   }
 #undef FMOE_TILE
   FMOE_LAUNCH_CHECK("i8_linear");

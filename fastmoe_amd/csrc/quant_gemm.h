@@ -345,7 +345,9 @@ template <bool INT8, int TN, int TM> struct QuantTile {
   static constexpr int kScaleBytes = kScaleLoads * 4096;
   static constexpr int kOutRow = TN <= 128 ? 128 : 256;            // bytes of a row on its way out
   static constexpr int kOutBytes = 4 * 16 * kOutRow;
-  static constexpr int kLdsBytes = 2 * (kStageBytes + kScaleBytes) + kOutBytes;
+  // (the floats of 8-bit rows, and the bias with them, in a place of their own: 2 KiB a wave)
+  static constexpr int kFactorBytes = INT8 ? 4 * 2048 : 0;
+  static constexpr int kLdsBytes = 2 * (kStageBytes + kScaleBytes) + kOutBytes + kFactorBytes;
   static constexpr int kGroups = kLdsBytes > 81920 ? 1 : 2;        // workgroups on a CU
   static_assert(TN % 128 == 0 && TM % 64 == 0 && TN <= 256 && TM <= 256, "even copies per wave");
 };
@@ -644,6 +646,8 @@ __device__ __forceinline__ void quant_tiles(const QuantGemmArgs& a) {
   };
 
   char* const stage = lds + 2 * (S::kStageBytes + S::kScaleBytes) + wave * (16 * S::kOutRow);
+  char* const factors = INT8 ? lds + 2 * (S::kStageBytes + S::kScaleBytes) + S::kOutBytes + wave * 2048
+                             : stage;
   // (the last group's missing steps, if any, multiply zeros)
   const int groups = (steps + 3) >> 2;
   int pid = blockIdx.x;
@@ -663,19 +667,19 @@ __device__ __forceinline__ void quant_tiles(const QuantGemmArgs& a) {
   unroll<0, FW + TW + kLag>([&](auto j) { read_scale(j, 0, 0); });
   next_scales();
   for (;;) {
-    // the bias waits out the K loop where the results will pass
+    // the bias waits out the K loop, of 4-bit rows where the results will pass
     if (bias_by_lds) {
       const int64_t row = (int64_t)a.out_feat * (wide ? 4 : 2);
       const i32x4 rsrc = mx_descriptor((const char*)a.bias + at.e * row, row);
-      const uint32_t dst = lds0 + (uint32_t)(stage - lds);
+      const uint32_t dst = lds0 + (uint32_t)(factors - lds);
       const uint32_t off = (uint32_t)((at.base + wn * (TN / 2)) * (wide ? 4 : 2) + lane * 4);
       dma4(dst, off, rsrc);
       dma4(dst + 256, off + 256, rsrc);
     }
-    // and the scales of 8-bit rows with it: the wave's features' at 512, its rows' at 1280 (128 of
+    // and the scales of 8-bit rows with it: the wave's features' at 512, its rows' at 1024 (128 of
     // either, which may be more than it has)
     if constexpr (INT8) {
-      const uint32_t dst = lds0 + (uint32_t)(stage - lds);
+      const uint32_t dst = lds0 + (uint32_t)(factors - lds);
       const i32x4 rw = mx_descriptor(a.ws + ((int64_t)at.e * a.out_feat + at.base) * 4,
                                      (int64_t)(a.out_feat - at.base) * 4);
       const i32x4 rx = mx_descriptor(a.xs + at.x0 * 4, (int64_t)at.rows * 4);
@@ -683,8 +687,8 @@ __device__ __forceinline__ void quant_tiles(const QuantGemmArgs& a) {
       const uint32_t x_off = (uint32_t)(wm * (TM / 2) + lane) * 4;
       dma4(dst + 512, w_off, rw);
       dma4(dst + 768, w_off + 256, rw);
-      dma4(dst + 1280, x_off, rx);
-      dma4(dst + 1536, x_off + 256, rx);
+      dma4(dst + 1024, x_off, rx);
+      dma4(dst + 1280, x_off + 256, rx);
     }
 #pragma unroll
     for (int i = 0; i < TW; ++i)
@@ -712,48 +716,54 @@ __device__ __forceinline__ void quant_tiles(const QuantGemmArgs& a) {
       first = false;
     } while (++q < groups);
     mx_mfma_done();
-    float b[FW / 2][8];
     const int fresh = mx_fresh(lane);
-    if (bias_by_lds) {
-      const char* const at_g = stage + (fresh >> 4) * (wide ? 32 : 16);
-#pragma unroll
-      for (int p = 0; p < FW / 2; ++p) {
+    auto read_bias = [&](int p, float (&b)[8]) {
+      if (bias_by_lds) {
+        const char* const at_g = factors + (fresh >> 4) * (wide ? 32 : 16);
         if (wide) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) b[p][i] = *(const float*)(at_g + p * 128 + i * 4);
+          for (int i = 0; i < 8; ++i) b[i] = *(const float*)(at_g + p * 128 + i * 4);
         } else {
           const i32x4 u = *(const i32x4*)(at_g + p * 64);
-          mx_widen(a, u, b[p]);
+          mx_widen(a, u, b);
         }
+      } else {
+        mx_load_bias(a, mx_bias_rows(a, at.e), at.base + wn * (TN / 2) + p * 32 + 8 * (fresh >> 4), b);
       }
-    } else {
-      const auto rows = mx_bias_rows(a, at.e);
+    };
+    auto read_factors = [&](int p, float (&sw)[8]) {
 #pragma unroll
-      for (int p = 0; p < FW / 2; ++p)
-        mx_load_bias(a, rows, at.base + wn * (TN / 2) + p * 32 + 8 * (fresh >> 4), b[p]);
-    }
-    float sw[FW / 2][8], sx[TW];                      // (all read before the first results pass)
-    if constexpr (INT8) {
+      for (int j = 0; j < 8; ++j)
+        sw[j] = *(const float*)(factors + 512 + (p * 32 + 8 * (fresh >> 4) + j) * 4);
+    };
+    // (held for all rows; but where rows are not whole packs and the tile is the largest, registers
+    // do not suffice, and these are read for every 16 rows)
+    constexpr bool kHold = !(INT8 && MODE == kMxAny && TN == 256);
+    float b[FW / 2][8], sw[FW / 2][8];
+    if constexpr (kHold) {
 #pragma unroll
-      for (int p = 0; p < FW / 2; ++p)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          sw[p][j] = *(const float*)(stage + 512 + (p * 32 + 8 * (fresh >> 4) + j) * 4);
-#pragma unroll
-      for (int i = 0; i < TW; ++i)
-        sx[i] = *(const float*)(stage + 1280 + (i * 16 + (fresh & 15)) * 4);
+      for (int p = 0; p < FW / 2; ++p) {
+        read_bias(p, b[p]);
+        if constexpr (INT8) read_factors(p, sw[p]);
+      }
     }
     const MxOutput<T, MODE> out(a, at.x0, at.rows);
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
-      float r[FW / 2][8];
+      float r[FW / 2][8], sx = 1.f;
+      if constexpr (INT8) sx = *(const float*)(factors + 1024 + (i * 16 + (fresh & 15)) * 4);
 #pragma unroll
-      for (int p = 0; p < FW / 2; ++p)
+      for (int p = 0; p < FW / 2; ++p) {
+        if constexpr (!kHold) {
+          read_bias(p, b[p]);
+          read_factors(p, sw[p]);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float v = mx_read(acc[i][2 * p + (j >> 2)][j & 3]);
-          r[p][j] = INT8 ? fmaf(v * sx[i], sw[p][j], b[p][j]) : v + b[p][j];
+          r[p][j] = INT8 ? fmaf(v * sx, sw[p][j], b[p][j]) : v + b[p][j];
         }
+      }
       out.template store_rows<FW / 2, S::kOutRow>(stage, fresh, wm * (TM / 2) + i * 16,
                                                   at.base + wn * (TN / 2), r);
     }

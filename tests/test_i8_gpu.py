@@ -175,7 +175,7 @@ CASES = [  # counts, in, out: the kernel of few rows, ...
     ([128, 0, 300, 1], 128, 128), ([500, 129], 384, 600), ([100] * 130, 256, 264),
     ([1000, 24], 1024, 4096), ([700], 777, 333), ([257, 3], 2048, 1000),
     # ... 256 x 256 tiles
-    ([6400, 0, 6300], 2048, 4096), ([12900], 2176, 4104),
+    ([6400, 0, 6300], 2048, 4096), ([12900], 2176, 4104), ([6300, 6600], 1100, 4103),
 ]
 
 

@@ -31,5 +31,5 @@ def test_compiler_leaves_the_hand_placed_instructions_alone():
                        check=True, capture_output=True)
         text = open(out).read()
     kernels = re.findall(r"^(_ZN4fmoe14i8_tile_kernel\S*):(.*?)^\.Lfunc_end", text, re.M | re.S)
-    assert len(kernels) == 15          # 3 types, 3 tiles of packed rows and 2 of any
+    assert len(kernels) == 18          # 3 types, 3 tiles, packed rows and any
     assert sum(loops.check(name, body) for name, body in kernels) == 0
