@@ -21,7 +21,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libfmoe_hip.so")
 # the two heavy translation units first, so that they compile side by side
 SOURCES = ["gemm_mfma_bf16.hip", "gemm_mfma_f16.hip", "api.hip", "route.hip", "dispatch.hip",
            "gate.hip", "score_gate.hip", "mx.hip", "mx_gemm.hip", "i8.hip",
-           "i8_gemm.hip", "map.hip", "gate_grad.hip", "act.hip", "gemm_simt.hip", "gemm_mfma.hip", "gemm_plain.hip",
+           "i8_gemm.hip", "i8_grad.hip", "map.hip", "gate_grad.hip", "act.hip", "gemm_simt.hip", "gemm_mfma.hip", "gemm_plain.hip",
            "gemm_mfma_wide.hip"]
 HEADERS = ["common.h", "gemm.h", "gemm_tiles.h", "act_math.h", "mx.h", "i8.h", "rows.h", "quant_gemm.h",
            "dma_desc.h", "gemm_mfma_impl.h",

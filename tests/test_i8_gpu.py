@@ -238,11 +238,15 @@ def test_rows_that_are_not_finite(counts):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("counts,k,n", [([3, 0, 5], 40, 24), ([70, 1, 0, 100], 300, 136),
-                                        ([9], 129, 77), ([300, 200], 512, 1024)],
+@pytest.mark.parametrize("counts,k,n", [([3, 0, 5], 40, 24), ([70, 1, 0, 100], 300, 136), ([1], 1, 1),
+                                        ([9], 129, 77), ([300, 200], 512, 1024), ([700], 300, 130),
+                                        ([20], 520, 4096), ([33, 0, 17], 1000, 2048),
+                                        ([2] * 70 + [40], 129, 65), ([16, 17, 32, 1], 1408, 999)],
                          ids=lambda c: str(c)[:24])
 def test_gradients(dtype, counts, k, n):
-    """dx = dy times the weights' values: their rounding to dtype, f32 sums, the result's rounding."""
+    """dx = dy times the weights' values.  Few rows: the result's rounding, f32 sums of f32 products
+    and, for 16-bit types, 2^-17 of a term that two bf16 numbers leave.  Many: the values' rounding
+    to dtype as well."""
     rows = sum(counts) + 6                       # some that nobody owns
     x = randn((rows, k), dtype, 1).cuda().requires_grad_()
     w, b = weights(len(counts), n, k, 2, dtype)
@@ -250,6 +254,8 @@ def test_gradients(dtype, counts, k, n):
     dy = randn((rows, n), dtype, 3).cuda()
     i8.linear(x, torch.tensor(counts, device="cuda"), w, b).backward(dy)
     half = torch.finfo(dtype).eps / 2
+    few = rows <= len(counts) * (192 if dtype == torch.float32 else 80)
+    term = half if not few else 0 if dtype == torch.float32 else 2.0 ** -17
     at = 0
     for e, c in enumerate(counts):
         r = slice(at, at + c)
@@ -258,11 +264,30 @@ def test_gradients(dtype, counts, k, n):
         g = dy[r].double()
         want, size = g @ v, g.abs() @ v.abs()
         # (f32's weights are rounded once, too)
-        tol = half_step(want, dtype) + (half + (n + 2) * 2.0 ** -24) * size
+        tol = half_step(want, dtype) + (term + (n + 20) * 2.0 ** -24) * size
         assert ((x.grad[r].double() - want).abs() <= tol).all()
         db, size = g.sum(0), g.abs().sum(0)
         assert ((b.grad[e].double() - db).abs() <= half_step(db, dtype) + c * 2.0 ** -24 * size).all()
     assert (x.grad[at:] == 0).all()
+
+
+def test_gradients_repeat_themselves_and_keep_infinities():
+    x = randn((40, 520), torch.bfloat16, 1).cuda().requires_grad_()
+    w, _ = weights(1, 2048, 520, 2)
+    dy = randn((40, 2048), torch.bfloat16, 3).cuda()
+    dy[3, 7], dy[20, 9], dy[30, 11] = float("inf"), float("nan"), 3e38
+    grads = []
+    for _ in range(3):
+        x.grad = None
+        i8.linear(x, None, w).backward(dy)
+        grads.append(x.grad)
+    for g in grads[1:]:
+        torch.testing.assert_close(g, grads[0], rtol=0, atol=0, equal_nan=True)
+    bad = ~grads[0].isfinite().all(1)
+    assert bad[3] and bad[20] and bad.sum() == 2          # 3e38 times a weight is a number
+    sign = w.codes[0, 7, :520].sign()
+    assert (grads[0][3][sign > 0] == float("inf")).all() and (grads[0][3][sign < 0] == -float("inf")).all()
+    assert grads[0][3][sign == 0].isnan().all() and grads[0][20].isnan().all()
 
 
 def test_gradient_against_differences():

@@ -42,6 +42,22 @@ def test_products_that_do_not_fit_are_refused():
         refused(call(**bad), b"i8_linear")
     assert call(rows=0) == 0
 
+    def grad(dy=P, w=P, ws=P, seg=P, dx=P, rows=4, k=8, n=8, e=2, work=P, size=1 << 30, dtype=0):
+        return lib.fmoe_i8_linear_dx(dy, w, ws, seg, dx, rows, k, n, e, work, size, dtype, None)
+
+    for bad in (dict(rows=-1), dict(k=0), dict(n=131073), dict(e=0), dict(dtype=1), dict(dy=None),
+                dict(w=None), dict(ws=None), dict(seg=None), dict(dx=None), dict(w=P + 4),
+                dict(ws=P + 2)):
+        refused(grad(**bad), b"i8_linear_dx")
+    assert grad(rows=0) == 0
+    # one expert, 5 column tiles: 8 blocks share the summed axis
+    assert lib.fmoe_i8_dx_workspace_bytes(20, 520, 4096, 1) == 8 * 20 * 520 * 4
+    for bad in (dict(work=None), dict(size=8 * 20 * 520 * 4 - 1), dict(work=P + 4)):
+        refused(grad(rows=20, k=520, n=4096, e=1, **bad), b"workspace")
+    assert lib.fmoe_i8_dx_workspace_bytes(5000, 4096, 4096, 8) == 0
+    assert lib.fmoe_i8_few_rows(160, 2, 3) == 1 and lib.fmoe_i8_few_rows(161, 2, 3) == 0
+    assert lib.fmoe_i8_few_rows(384, 2, 0) == 1 and lib.fmoe_i8_few_rows(385, 2, 0) == 0
+
 
 def test_plans_and_moves_that_do_not_fit_are_refused():
     assert lib.fmoe_map_workspace_bytes(64, 128) == 0
