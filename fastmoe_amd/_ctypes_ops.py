@@ -1019,7 +1019,7 @@ def i8_linear_bwd(dy: torch.Tensor, seg_off: torch.Tensor, w_codes: torch.Tensor
     if need_dx:
         dx = dy.new_empty((rows, in_feat))
     if need_dx and _L.fmoe_i8_few_rows(rows, e, _dt(dy, "dy")):
-        size = _L.fmoe_i8_dx_workspace_bytes(rows, in_feat, out_f, e)
+        size = _L.fmoe_i8_dx_workspace_bytes(rows, in_feat, out_f, e, _dt(dy, "dy"))
         _lib.check(min(size, 0), "i8_linear_dx")
         shares = torch.empty(size, dtype=torch.uint8, device=dy.device)
         with _launch(dy, "i8_linear_dx"):

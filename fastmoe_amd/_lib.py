@@ -112,7 +112,7 @@ SIGNATURES = {
     "fmoe_i8_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
     "fmoe_i8_dequantize_bwd": (c_int, [c_void_p] * 5 + [c_int64] * 4 + [c_int, c_void_p]),
     "fmoe_i8_few_rows": (c_int, [c_int64, c_int64, c_int]),
-    "fmoe_i8_dx_workspace_bytes": (c_int64, [c_int64] * 4),
+    "fmoe_i8_dx_workspace_bytes": (c_int64, [c_int64] * 4 + [c_int]),
     "fmoe_i8_linear_dx": (c_int, [c_void_p] * 5 + [c_int64] * 4 + [c_void_p, c_int64, c_int,
                                                                    c_void_p]),
     "fmoe_i8_linear_fwd": (c_int, [c_void_p] * 7 + [c_int64] * 4 + [c_int, c_void_p]),

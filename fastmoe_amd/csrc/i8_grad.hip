@@ -1,8 +1,8 @@
-// The gradient of an 8-bit product's rows, for few of them:
+// The gradient of an 8-bit product's rows:
 //   dx[r][k] = sum_n dy[r][n] s_e[n] q_e[n][k],   r in the rows of expert e
-// straight from the codes.  (Many rows go through weights laid out in the rows' type and the other
-// products' backward, which costs 5 bytes of traffic per weight whatever the rows; here it is one
-// per 32 rows of an expert.)
+// straight from the codes, for few rows and for f32.  (Many 16-bit rows go through weights laid out in
+// their type and the other products' backward, which costs 5 bytes of traffic per weight whatever the
+// rows; here it is one per 32 or 64 rows of an expert.)
 //
 // The sum runs over the codes' rows, so that v_mfma_f32_16x16x32_bf16 needs 8 rows' codes of one
 // feature in a lane, where memory has 8 features of one row.  A lane loads 8 bytes of 8 rows, and
@@ -27,25 +27,25 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kGradWaves = 8;          // share the summed axis
-constexpr int kGradRows = 32;          // of an expert, two fragments
 constexpr int kGradCols = 128;         // features: 8 fragments
 static_assert(kGradCols == kI8Step, "rows of codes are whole column tiles");
 
-// Mean rows per expert up to which this is the faster way.  Microseconds here and by weights laid out
-// (bf16; in f32, whose product by weights laid out runs at a sixteenth of the rate):
+// Mean rows per expert up to which this is the faster way in 16 bits; in f32, whose product by weights
+// laid out has a sixteenth of their rate, it always is.  Microseconds here and by weights laid out:
 //   rows  experts  in -> out        bf16          f32
-//     64   16    1024 -> 4096      21 /  67     26 /  172
+//     64   16    1024 -> 4096      20 /  67     22 /  172
 //   1024   16    1024 -> 4096      40 /  65     51 /  178
-//   2048   16    1024 -> 4096      75 /  70     98 /  220
-//   2048  128    2048 -> 1408     116 / 338    132 /  827
-//   8192  128    2048 -> 1408     276 / 347    336 /  838
-//  16384  128    2048 -> 1408     494 / 362    638 / 1165
-//     16    1    4096 -> 14336     21 / 125     30 /  350
-//    128    8    4096 -> 14336     99 / 444    118 / 1080
-//    768    8    4096 -> 14336    324 / 442    435 / 1497
-// (469 MB at 4.8 TB/s in the last but one; with more rows the conversions and the split of dy, 160
-// instructions a step and 16 rows, set the time.)
-constexpr int64_t kGradFewRows = 80, kGradFewRowsF32 = 192;
+//   2048   16    1024 -> 4096      60 /  70     98 /  220
+//   4096   16    1024 -> 4096     113 /  81    200 /  339
+//   2048  128    2048 -> 1408     117 / 338    132 /  827
+//   8192  128    2048 -> 1408     223 / 347    336 /  838
+//  16384  128    2048 -> 1408     410 / 364    638 / 1165
+//     16    1    4096 -> 14336     21 / 125     23 /  350
+//    128    8    4096 -> 14336     97 / 444    107 / 1080
+//    768    8    4096 -> 14336    324 / 444    435 / 1497
+// (469 MB at 4.8 TB/s in the last but one; with more rows the split of dy and the conversions, 70 and
+// 96 instructions per 16 and 64 rows in a step of 4 KiB, set the time.)
+constexpr int64_t kGradFewRows = 96;
 constexpr int64_t kGradBlocks = 256;   // one on a CU
 
 struct I8GradArgs {
@@ -99,14 +99,15 @@ __device__ __forceinline__ void store_four(T* to, int k, int d, const float (&v)
   }
 }
 
-template <typename T>
+// A block takes 16 F rows of an expert.
+template <typename T, int F>
 __global__ __launch_bounds__(kGradWaves* kWave) void i8_grad_kernel(I8GradArgs a, ClearedTail<T> tail) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
   __shared__ float part[kGradWaves][32][kWave];
   if (blockIdx.y == 0) tail.clear(a.in_feat);
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  RowTiles<kGradRows, kOneHeight, kGradWaves> tiles;
+  RowTiles<16 * F, kOneHeight, kGradWaves> tiles;
   int* const s_find = (int*)part;
   tiles.scan(a.seg_off, a.n_expert, s_find);
   const int row_bytes = (int)i8_row_bytes(a.in_feat), n_cols = row_bytes / kGradCols;
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(kGradWaves* kWave) void i8_grad_kernel(I8GradArgs a
   if (!tiles.by_lane) __syncthreads();     // (before that place holds anything else)
 
   const int m = lane & 15, g = lane >> 4;
-  const int rows = min(kGradRows, t.cnt - t.m0);
+  const int rows = min(16 * F, t.cnt - t.m0);
   const T* const dy = (const T*)a.dy + ((int64_t)t.row0 + t.m0) * a.out_feat;
   const float* const scale = a.ws + (int64_t)t.e * a.out_feat;
   const uint8_t* const w = a.wc + (int64_t)t.e * a.out_feat * row_bytes + col * kGradCols + m * 8;
@@ -125,26 +126,26 @@ __global__ __launch_bounds__(kGradWaves* kWave) void i8_grad_kernel(I8GradArgs a
   const int steps = (a.out_feat + 31) / 32;
   const int deal = (int)gridDim.y * kGradWaves, at = (int)blockIdx.y * kGradWaves + wave;
   const int s1 = (int)((int64_t)(at + 1) * steps / deal);
-  f32x4 acc[2][8];
+  f32x4 acc[F][8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < F; ++h)
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const bool second = rows > 16;
+  const int frags = (rows + 15) / 16;      // that hold rows
   // what a step reads: codes of rows 32 s + 8 g .. + 7 (behind the last: that one's, which meet
   // zeros), these rows' scales and values of dy (rows of dy behind the last repeat it; their results
   // are not stored)
   struct Step {
     uint2 code[8];
     Eight<float> scale;
-    Eight<T> dy[2];
+    Eight<T> dy[F];
   };
   auto fetch = [&](int s, Step& to) {
     const int n = s * 32 + g * 8;
     to.scale.load(scale, n, a.out_feat);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (h == 0 || second)
+    for (int h = 0; h < F; ++h)
+      if (h < frags)
         to.dy[h].load(dy + (int64_t)min(h * 16 + m, rows - 1) * a.out_feat, n, a.out_feat);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -155,45 +156,44 @@ __global__ __launch_bounds__(kGradWaves* kWave) void i8_grad_kernel(I8GradArgs a
   if (s < s1) fetch(s, now);
   for (; s < s1; ++s) {
     if (s + 1 < s1) fetch(s + 1, next);
-    u32x4 b[2][kParts];
+    u32x4 q[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h == 1 && !second) break;
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = now.dy[h][i] * now.scale[i];
-      split_bf16<kParts>(p, b[h]);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      u32x4 q;
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t lo = j < 4 ? now.code[2 * i].x : now.code[2 * i].y;
         const uint32_t hi = j < 4 ? now.code[2 * i + 1].x : now.code[2 * i + 1].y;
         const float x = (float)(int8_t)(lo >> (8 * (j & 3))), y = (float)(int8_t)(hi >> (8 * (j & 3)));
-        q[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+        q[j][i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h == 1 && !second) break;
+    for (int h = 0; h < F; ++h) {
+      if (h >= frags) break;
+      float p[8];
 #pragma unroll
-        for (int p = 0; p < kParts; ++p)
+      for (int i = 0; i < 8; ++i) p[i] = now.dy[h][i] * now.scale[i];
+      u32x4 b[kParts];
+      split_bf16<kParts>(p, b);
+#pragma unroll
+      for (int u = 0; u < kParts; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
           acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8, q), __builtin_bit_cast(bf16x8, b[h][p]), acc[h][j], 0, 0, 0);
-      }
+              __builtin_bit_cast(bf16x8, q[j]), __builtin_bit_cast(bf16x8, b[u]), acc[h][j], 0, 0, 0);
     }
     now = next;
   }
   // The waves' shares meet in LDS, 16 rows at a time, in the order of the waves: wave u adds up
   // features 8 (4 g + u / 2) + 4 (u % 2) .. + 3 of lane group g.
   const int i0 = wave >> 1, j0 = 4 * (wave & 1);
-  for (int h = 0; h < (second ? 2 : 1); ++h) {
-    if (h == 1) __syncthreads();
+#pragma unroll
+  for (int h = 0; h < F; ++h) {
+    if (h >= frags) break;
+    if (h > 0) __syncthreads();
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[wave][i * 8 + j][lane] = h ? acc[1][j][i] : acc[0][j][i];
+      for (int i = 0; i < 4; ++i) part[wave][i * 8 + j][lane] = acc[h][j][i];
     __syncthreads();
     const int r = h * 16 + m, k = col * kGradCols + 8 * (4 * g + i0) + j0;
     float sum[4];
@@ -223,23 +223,40 @@ __global__ __launch_bounds__(256) void i8_grad_sum_kernel(const float* __restric
   }
 }
 
-// Blocks that share the summed axis: so many that there are enough for the chip's memory, while a
+// Fragments of 16 rows in a block, and blocks that share the summed axis: so many that there are enough for the chip's memory, while a
 // wave keeps two steps.  (4096 -> 14336 for 16 rows of one expert, 32 column tiles: 89 us in one
 // block each, 21 in eight.)
-static int grad_shares(int64_t n_rows, int64_t in_feat, int64_t out_feat, int64_t n_expert) {
-  const int64_t live = std::min(n_expert, n_rows);
-  const int64_t tiles = std::max(n_rows / kGradRows + live / 2, live) * (i8_row_bytes(in_feat) / kGradCols);
-  const int64_t steps = (out_feat + 31) / 32;
-  return (int)std::max<int64_t>(std::min({kGradBlocks / tiles, steps / (2 * kGradWaves), (int64_t)16}), 1);
-}
+struct GradShape {
+  int frags, shares;
+  GradShape(int64_t n_rows, int64_t in_feat, int64_t out_feat, int64_t n_expert, int dtype) {
+    const int64_t live = std::min(n_expert, n_rows), cols = i8_row_bytes(in_feat) / kGradCols;
+    auto tiles = [&](int f) { return std::max(n_rows / (16 * f) + live / 2, live) * cols; };
+    // Four fragments halve the conversions (384 rows of 8 experts, 4096 -> 14336: 219 -> 157 us),
+    // but leave CUs without a block where there were just enough (1024 of 16, 1024 -> 4096: 40 -> 53);
+    // f32's do not fit the registers.
+    frags = 2;
+    if (dtype != FMOE_F32 && n_rows > n_expert * 32 &&
+        (tiles(4) >= kGradBlocks || tiles(4) <= kGradBlocks / 2))
+      frags = 4;
+    const int64_t steps = (out_feat + 31) / 32;
+    shares = (int)std::max<int64_t>(
+        std::min({kGradBlocks / tiles(frags), steps / (2 * kGradWaves), (int64_t)16}), 1);
+  }
+};
 
-template <typename T> static int launch_grad(const I8GradArgs& a, int shares, hipStream_t s) {
-  const int64_t rows = a.n_rows / kGradRows + std::min<int64_t>(a.n_expert, a.n_rows);
+template <typename T>
+static int launch_grad(const I8GradArgs& a, const GradShape& shape, hipStream_t s) {
+  const int frags = shape.frags, shares = shape.shares;
+  const int64_t rows = a.n_rows / (16 * frags) + std::min<int64_t>(a.n_expert, a.n_rows);
   const int64_t blocks = rows * (i8_row_bytes(a.in_feat) / kGradCols);
   FMOE_REQUIRE(blocks * (kGradWaves * kWave) <= UINT32_MAX, FMOE_ERR_UNSUPPORTED,
                "i8_linear_dx: too many tiles");
-  hipLaunchKernelGGL((i8_grad_kernel<T>), dim3((unsigned)blocks, shares), dim3(kGradWaves * kWave), 0,
-                     s, a, ClearedTail<T>{a.seg_off + a.n_expert, (T*)a.dx, a.n_rows});
+  const ClearedTail<T> tail{a.seg_off + a.n_expert, (T*)a.dx, a.n_rows};
+  const dim3 grid((unsigned)blocks, shares), block(kGradWaves * kWave);
+  if constexpr (sizeof(T) == 2) {
+    if (frags == 4) hipLaunchKernelGGL((i8_grad_kernel<T, 4>), grid, block, 0, s, a, tail);
+  }
+  if (frags == 2) hipLaunchKernelGGL((i8_grad_kernel<T, 2>), grid, block, 0, s, a, tail);
   FMOE_LAUNCH_CHECK("i8_linear_dx");
   if (shares > 1) {
     const int64_t size = a.n_rows * a.in_feat;
@@ -254,18 +271,18 @@ template <typename T> static int launch_grad(const I8GradArgs& a, int shares, hi
 }  // namespace fmoe
 
 extern "C" int fmoe_i8_few_rows(int64_t n_rows, int64_t n_expert, int dtype) {
-  return n_rows <= n_expert * (dtype == FMOE_F32 ? fmoe::kGradFewRowsF32 : fmoe::kGradFewRows);
+  return dtype == FMOE_F32 || n_rows <= n_expert * fmoe::kGradFewRows;
 }
 
 extern "C" int64_t fmoe_i8_dx_workspace_bytes(int64_t n_rows, int64_t in_feat, int64_t out_feat,
-                                              int64_t n_expert) {
+                                              int64_t n_expert, int dtype) {
   using namespace fmoe;
   FMOE_REQUIRE(n_rows >= 0 && n_rows < INT32_MAX && n_expert >= 1 && n_expert < INT32_MAX &&
                    in_feat >= 1 && out_feat >= 1 && in_feat <= FMOE_I8_MAX_FEATURES &&
                    out_feat <= FMOE_I8_MAX_FEATURES,
                FMOE_ERR_INVALID, "i8_linear_dx: bad sizes");
   if (n_rows == 0) return 0;
-  const int shares = grad_shares(n_rows, in_feat, out_feat, n_expert);
+  const int shares = GradShape(n_rows, in_feat, out_feat, n_expert, dtype).shares;
   return shares > 1 ? (int64_t)sizeof(float) * shares * n_rows * in_feat : 0;
 }
 
@@ -274,7 +291,7 @@ extern "C" int fmoe_i8_linear_dx(const void* dy, const void* w_codes, const floa
                                  int64_t out_feat, int64_t n_expert, void* workspace,
                                  int64_t workspace_bytes, int dtype, void* stream) {
   using namespace fmoe;
-  const int64_t need = fmoe_i8_dx_workspace_bytes(n_rows, in_feat, out_feat, n_expert);
+  const int64_t need = fmoe_i8_dx_workspace_bytes(n_rows, in_feat, out_feat, n_expert, dtype);
   if (need < 0) return (int)need;
   FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_F16 || dtype == FMOE_BF16, FMOE_ERR_UNSUPPORTED,
                "i8_linear_dx: unsupported dtype %d", dtype);
@@ -289,11 +306,11 @@ extern "C" int fmoe_i8_linear_dx(const void* dy, const void* w_codes, const floa
   const I8GradArgs a{dy, (const uint8_t*)w_codes, w_scales, seg_off, dx,
                      need ? (float*)workspace : nullptr, n_rows,
                      (int)in_feat, (int)out_feat, (int)n_expert};
-  const int shares = grad_shares(n_rows, in_feat, out_feat, n_expert);
+  const GradShape shape(n_rows, in_feat, out_feat, n_expert, dtype);
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
-    case FMOE_F32: return launch_grad<float>(a, shares, s);
-    case FMOE_F16: return launch_grad<__half>(a, shares, s);
-    default: return launch_grad<__hip_bfloat16>(a, shares, s);
+    case FMOE_F32: return launch_grad<float>(a, shape, s);
+    case FMOE_F16: return launch_grad<__half>(a, shape, s);
+    default: return launch_grad<__hip_bfloat16>(a, shape, s);
   }
 }

@@ -144,7 +144,7 @@ std::tuple<OptTensor, OptTensor> i8_linear_bwd(Tensor dy, Tensor seg_off, Tensor
   Tensor w;
   if (need_dx) dx = torch::empty({dy.size(0), in_f}, dy.options());
   if (need_dx && fmoe_i8_few_rows(dy.size(0), e, dt(dy, "dy"))) {
-    const int64_t bytes = fmoe_i8_dx_workspace_bytes(dy.size(0), in_f, out_f, e);
+    const int64_t bytes = fmoe_i8_dx_workspace_bytes(dy.size(0), in_f, out_f, e, dt(dy, "dy"));
     check(bytes < 0 ? (int)bytes : 0, "i8_linear_dx");
     // (a tensor of its own: a backward pass does not hold the interpreter lock)
     Tensor shares = torch::empty({bytes}, dy.options().dtype(at::kByte));

@@ -644,7 +644,7 @@ int fmoe_i8_linear_fwd(const void* x_codes, const float* x_scales, const void* w
 /*
  * dx[r][k] = sum_n dy[r][n] * w_scales[e][n] * w_e[n][k], r in seg_e: the gradient of that product's
  * rows, straight from the codes, and zeros in the rows at or behind seg_off[n_expert].  For any
- * number of rows, but made for few per expert (each 32 of them read the expert's codes once):
+ * number of rows, but made for few per expert (each 32 or 64 of them read its codes once) and for f32:
  * fmoe_i8_dequantize_bwd and fmoe_grouped_linear_bwd serve many.  fmoe_i8_few_rows: 1 where it is
  * the faster of the two for so many rows, else 0.  dy [n_rows, out_feat] and
  * dx [n_rows, in_feat] of dtype (f32, f16 or bf16).  The workspace is 16-byte aligned
@@ -652,7 +652,7 @@ int fmoe_i8_linear_fwd(const void* x_codes, const float* x_scales, const void* w
  */
 int fmoe_i8_few_rows(int64_t n_rows, int64_t n_expert, int dtype);
 int64_t fmoe_i8_dx_workspace_bytes(int64_t n_rows, int64_t in_feat, int64_t out_feat,
-                                   int64_t n_expert);
+                                   int64_t n_expert, int dtype);
 int fmoe_i8_linear_dx(const void* dy, const void* w_codes, const float* w_scales,
                       const int32_t* seg_off, void* dx, int64_t n_rows, int64_t in_feat,
                       int64_t out_feat, int64_t n_expert, void* workspace, int64_t workspace_bytes,

@@ -241,7 +241,8 @@ def test_rows_that_are_not_finite(counts):
 @pytest.mark.parametrize("counts,k,n", [([3, 0, 5], 40, 24), ([70, 1, 0, 100], 300, 136), ([1], 1, 1),
                                         ([9], 129, 77), ([300, 200], 512, 1024), ([700], 300, 130),
                                         ([20], 520, 4096), ([33, 0, 17], 1000, 2048),
-                                        ([2] * 70 + [40], 129, 65), ([16, 17, 32, 1], 1408, 999)],
+                                        ([2] * 70 + [40], 129, 65), ([16, 17, 32, 1], 1408, 999),
+                                        ([70], 300, 600), ([64, 0, 80, 33], 4096, 1000)],
                          ids=lambda c: str(c)[:24])
 def test_gradients(dtype, counts, k, n):
     """dx = dy times the weights' values.  Few rows: the result's rounding, f32 sums of f32 products
@@ -254,7 +255,7 @@ def test_gradients(dtype, counts, k, n):
     dy = randn((rows, n), dtype, 3).cuda()
     i8.linear(x, torch.tensor(counts, device="cuda"), w, b).backward(dy)
     half = torch.finfo(dtype).eps / 2
-    few = rows <= len(counts) * (192 if dtype == torch.float32 else 80)
+    few = dtype == torch.float32 or rows <= len(counts) * 96
     term = half if not few else 0 if dtype == torch.float32 else 2.0 ** -17
     at = 0
     for e, c in enumerate(counts):

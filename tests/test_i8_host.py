@@ -51,12 +51,12 @@ def test_products_that_do_not_fit_are_refused():
         refused(grad(**bad), b"i8_linear_dx")
     assert grad(rows=0) == 0
     # one expert, 5 column tiles: 8 blocks share the summed axis
-    assert lib.fmoe_i8_dx_workspace_bytes(20, 520, 4096, 1) == 8 * 20 * 520 * 4
+    assert lib.fmoe_i8_dx_workspace_bytes(20, 520, 4096, 1, 0) == 8 * 20 * 520 * 4
     for bad in (dict(work=None), dict(size=8 * 20 * 520 * 4 - 1), dict(work=P + 4)):
         refused(grad(rows=20, k=520, n=4096, e=1, **bad), b"workspace")
-    assert lib.fmoe_i8_dx_workspace_bytes(5000, 4096, 4096, 8) == 0
-    assert lib.fmoe_i8_few_rows(160, 2, 3) == 1 and lib.fmoe_i8_few_rows(161, 2, 3) == 0
-    assert lib.fmoe_i8_few_rows(384, 2, 0) == 1 and lib.fmoe_i8_few_rows(385, 2, 0) == 0
+    assert lib.fmoe_i8_dx_workspace_bytes(5000, 4096, 4096, 8, 3) == 0
+    assert lib.fmoe_i8_few_rows(192, 2, 3) == 1 and lib.fmoe_i8_few_rows(193, 2, 3) == 0
+    assert lib.fmoe_i8_few_rows(100000, 2, 0) == 1
 
 
 def test_plans_and_moves_that_do_not_fit_are_refused():
