@@ -3,7 +3,8 @@
 // Both directions are bound by HBM: a value costs its own 2 or 4 bytes plus one.  The scale needs
 // the whole row before the first code, so up to eight waves keep a row in registers between the two
 // (4 KiB each; what is longer is read a second time, from L2 as a rule), and the next row is on its
-// way meanwhile.
+// way meanwhile.  Measured: 114688 x 4096 in bf16 to 8 bits 240 us, 1.41 GB at 5.9 TB/s, and back 238,
+// at 5.9 (a large copy reaches 5.2); 1000 x 300 in f32 3.8 and 3.0, a launch alone 2.1.
 //
 // A code is one multiply-add: t = x (127 / a) + 1.5 * 2^23 rounds the product, taken exactly, to an
 // integer whose low byte is the code.  The quotient is off by up to 2^-23 of itself, and so is the
@@ -89,16 +90,6 @@ struct I8Row {
     return finite ? make_uint2(four(0), four(4)) : make_uint2(0, 0);
   }
 };
-
-__device__ __forceinline__ void i8_values(uint2 codes, float scale, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = (float)(int8_t)((i < 4 ? codes.x : codes.y) >> (8 * (i & 3))) * scale;
-    // (an f32 product, always: left alone, the compiler makes it and a conversion to f16 one
-    // instruction with one rounding, here and there)
-    asm("" : "+v"(v[i]));
-  }
-}
 
 // The maximum of m over the waves of a block; `part` is not the one of the call before.
 template <int W> __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t* part) {
@@ -208,12 +199,13 @@ __global__ __launch_bounds__(W * kWave) void i8_quantize_kernel(
   }
 }
 
-// The chunks of all rows are numbered row by row; a wave takes U consecutive ones at a time.
-template <typename T, int U>
+// The chunks of all rows are numbered row by row; a wave takes U consecutive ones at a time, a lane 16
+// bytes of values, N, of each of a chunk's 8 / N parts.  ONCE: nobody reads them at once.
+template <typename T, int U, bool ONCE>
 __global__ __launch_bounds__(kI8Threads) void i8_dequantize_kernel(
     const uint8_t* __restrict__ codes, const float* __restrict__ scales, int64_t n_rows, int k,
     T* __restrict__ out, ClearedTail<T> tail) {
-  constexpr int kWaves = kI8Threads / kWave;
+  constexpr int kWaves = kI8Threads / kWave, N = 16 / (int)sizeof(T), kParts = 8 / N;
   if (tail.p) tail.clear(k);
   const int lane = threadIdx.x & (kWave - 1);
   const int chunks = (k + kI8Chunk - 1) / kI8Chunk;
@@ -221,7 +213,7 @@ __global__ __launch_bounds__(kI8Threads) void i8_dequantize_kernel(
   const int64_t items = n_rows * chunks, stride = (int64_t)gridDim.x * kWaves * U;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   for (int64_t it = ((int64_t)blockIdx.x * kWaves + wave) * U; it < items; it += stride) {
-    uint2 w[U];
+    uint32_t w[U][kParts][N / 4];
     float s[U];
     int64_t row[U];
     int at[U];
@@ -229,23 +221,33 @@ __global__ __launch_bounds__(kI8Threads) void i8_dequantize_kernel(
     for (int u = 0; u < U; ++u) {
       const int64_t number = min(it + u, items - 1);
       row[u] = number / chunks;
-      at[u] = (int)(number - row[u] * chunks) * kI8Chunk + lane * 8;
+      at[u] = (int)(number - row[u] * chunks) * kI8Chunk + lane * N;
       if (it + u >= items) at[u] = k;
-      w[u] = make_uint2(0, 0);
-      if (at[u] < k) w[u] = *reinterpret_cast<const uint2*>(codes + row[u] * row_bytes + at[u]);
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) {
+        const int from = at[u] + q * kWave * N;        // (codes reach to the next 128 features)
+        if (from < k) __builtin_memcpy(w[u][q], codes + row[u] * row_bytes + from, N);
+      }
       s[u] = scales[row[u]];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (at[u] >= k) continue;
       float v[8];
-      i8_values(w[u], s[u], v);
-      store_any(out + row[u] * k, at[u], k, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = (float)(int8_t)(w[u][i / N][i % N / 4] >> (8 * (i & 3))) * s[u];
+        // (an f32 product, always: left alone, the compiler makes it and a conversion to f16 one
+        // instruction with one rounding, here and there)
+        asm("" : "+v"(v[i]));
+      }
+      Eight<T>::template store<ONCE>(out + row[u] * k, at[u], k, v, kWave * N);
     }
   }
 }
 
-// Waves of a row: as many as hold it, or, where rows are few, as many as find a chunk in it.
+// Waves of a row: as many as hold it, or, where rows are few, as many as find a chunk in it (2047 x
+// 2048 in bf16: 5.9 us, otherwise 6.9; 4000 x 4096: 18.2, otherwise 13.8).
 constexpr int64_t kI8FewRows = 2048;
 constexpr int64_t kI8Waves = 256 * 16;     // as many as their registers allow on the chip
 
@@ -280,26 +282,35 @@ static int launch_quantize(const void* x, int64_t n_rows, int k, const int32_t* 
   return FMOE_OK;
 }
 
-// Four chunks at a time where that leaves every CU several waves.
+// Four chunks at a time where that leaves every CU several waves (114688 x 4096 in bf16: 243 us, one at
+// a time 291; 16376 x 2048 23 and 21).
 constexpr int64_t kI8ManyItems = 256 * 32;
 
-template <typename T>
+template <typename T, bool ONCE>
 static int launch_dequantize(const uint8_t* codes, const float* scales, int64_t n_rows, int k,
-                             void* out, const int32_t* tail_end, void* tail, int64_t tail_rows,
-                             hipStream_t s) {
+                             void* out, const ClearedTail<T>& cleared, hipStream_t s) {
   const int64_t items = n_rows * ((k + kI8Chunk - 1) / kI8Chunk);
   const bool many = items >= kI8ManyItems;
   const int64_t per_block = kI8Threads / kWave * (many ? 4 : 1);
   const dim3 grid((unsigned)std::max<int64_t>(std::min<int64_t>((items + per_block - 1) / per_block, 256 * 64), 1));
-  const ClearedTail<T> cleared{tail_end, (T*)tail, tail_rows};
   if (many)
-    hipLaunchKernelGGL((i8_dequantize_kernel<T, 4>), grid, dim3(kI8Threads), 0, s, codes, scales,
+    hipLaunchKernelGGL((i8_dequantize_kernel<T, 4, ONCE>), grid, dim3(kI8Threads), 0, s, codes, scales,
                        n_rows, k, (T*)out, cleared);
   else
-    hipLaunchKernelGGL((i8_dequantize_kernel<T, 1>), grid, dim3(kI8Threads), 0, s, codes, scales,
+    hipLaunchKernelGGL((i8_dequantize_kernel<T, 1, ONCE>), grid, dim3(kI8Threads), 0, s, codes, scales,
                        n_rows, k, (T*)out, cleared);
   FMOE_LAUNCH_CHECK("i8_dequantize");
   return FMOE_OK;
+}
+
+// (weights that a product reads next stay in the caches, others pass them by: 232 in place of 243 us)
+template <typename T>
+static int launch_dequantize(const uint8_t* codes, const float* scales, int64_t n_rows, int k,
+                             void* out, const int32_t* tail_end, void* tail, int64_t tail_rows,
+                             hipStream_t s) {
+  const ClearedTail<T> cleared{tail_end, (T*)tail, tail_rows};
+  return tail_end ? launch_dequantize<T, false>(codes, scales, n_rows, k, out, cleared, s)
+                  : launch_dequantize<T, true>(codes, scales, n_rows, k, out, cleared, s);
 }
 
 static int i8_quantize(const void* x, int64_t n_rows, int64_t k, const int32_t* n_rows_dev,

@@ -5,9 +5,10 @@
 //   reduce  y[t] = sum_e w[t][e] rows[r(t, e)]          (dw[t][e] = <given[t], rows[r]>)
 // Each is the other's gradient, the product for dw taken while the row is at hand.
 //
-// Both move rows and are bound by HBM.  They go token by token, along a list of each token's
-// (row, expert) pairs, so that x[t] is read once for all its rows and a sum needs no atomics: its
-// order is that of the experts, always.
+// Both move rows and are bound by HBM (131072 rows of 16384 tokens, 2048 in bf16: summed up 103 us,
+// 604 MB at 5.9 TB/s; expanded with the weights' gradient 205, 1.15 GB at 5.6).  They go token by
+// token, along a list of each token's (row, expert) pairs, so that x[t] is read once for all its rows
+// and a sum needs no atomics: its order is that of the experts, always.
 #include <algorithm>
 
 #include "gemm_tiles.h"
@@ -19,8 +20,8 @@ namespace fmoe {
 // Two launches, or one for up to 64 tokens: a histogram per block of tokens, then, in every block,
 // the sums of the histograms in front of its own and of all, and the places of its own tokens.
 //
-// A wave takes up to 16 tokens in a round.  Their truth values pass through LDS into one 16-bit mask per
-// expert, which a lane holds; from there on a token's row is the expert's first one plus the bits
+// A wave takes up to 16 tokens in a round.  Their truth values pass through LDS into one 16-bit mask
+// per expert, which a lane holds; from there on a token's row is the expert's first one plus the bits
 // below the token's in the mask, and its place in the token's list the bits below the lane's in a
 // ballot, so that no step waits for the one before (a counter per expert in LDS, advanced token by
 // token, took 11 us for 8192 tokens of 16 experts where this takes 7.8).
@@ -286,7 +287,7 @@ struct MapMoveArgs {
 // EXPAND: out[r] = w one[t] for a token's rows; else out[t] = sum of w many[r].  DOT: also
 // dweight[t][e] = <one[t], many[r]>, zero where the token has no row.
 //
-// A lane holds 8 values of a row, and U rows are under way at a time.  Without DOT a wave takes 512
+// A lane holds 8 values of a piece of a row, and U rows are under way at a time.  Without DOT a wave takes 512
 // values of a token's rows, whatever their length; with it a block of G threads takes a token,
 // H times 8 G values at a time, and its waves' shares of the products meet in LDS.
 template <typename T, typename W, int G, int H, bool EXPAND, bool DOT>
@@ -314,14 +315,16 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
   float* const dot = s_dot + wave * a.n_expert;
   if constexpr (DOT)
     for (int e = lane; e < a.n_expert; e += kWave) dot[e] = 0.f;
-  const int at = (threadIdx.x & (G - 1)) * 8;
+  // (a lane's values are runs of 16 bytes, so that a wave's stores are whole lines in f32, too)
+  constexpr int kGap = G * Eight<T>::N;
+  const int at = (threadIdx.x & (G - 1)) * Eight<T>::N;
   const int k_end = DOT ? a.d : k0 + 1;
   for (; k0 < k_end; k0 += kPiece) {
     float x[H][8], sum[H][8];
     if constexpr (EXPAND || DOT) {
       Eight<T> raw[H];
 #pragma unroll
-      for (int h = 0; h < H; ++h) raw[h].load(one, k0 + h * kSpan + at, a.d);
+      for (int h = 0; h < H; ++h) raw[h].load(one, k0 + h * kSpan + at, a.d, kGap);
 #pragma unroll
       for (int h = 0; h < H; ++h) raw[h].widen(x[h]);
     }
@@ -349,7 +352,8 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
             if (j + u >= n) break;
             const int64_t r = __builtin_amdgcn_readlane(pair.x, j + u);
 #pragma unroll
-            for (int h = 0; h < H; ++h) raw[u][h].template load<true>(many + r * a.d, k0 + h * kSpan + at, a.d);
+            for (int h = 0; h < H; ++h)
+              raw[u][h].template load<true>(many + r * a.d, k0 + h * kSpan + at, a.d, kGap);
           }
         }
 #pragma unroll
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
               float v[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) v[i] = x[h][i] * wj;
-              store_any<true>(out + r * a.d, k0 + h * kSpan + at, a.d, v);
+              Eight<T>::template store<true>(out + r * a.d, k0 + h * kSpan + at, a.d, v, kGap);
             } else {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
     }
     if constexpr (!EXPAND) {
 #pragma unroll
-      for (int h = 0; h < H; ++h) store_any(out + t * a.d, k0 + h * kSpan + at, a.d, sum[h]);
+      for (int h = 0; h < H; ++h) Eight<T>::store(out + t * a.d, k0 + h * kSpan + at, a.d, sum[h], kGap);
     }
   }
   if constexpr (DOT) {

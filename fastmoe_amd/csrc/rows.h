@@ -54,31 +54,57 @@ template <typename T> struct Eight {
     for (int i = 0; i < 8; ++i) v[i] = (*this)[i];
   }
 
-  // Values k .. k + 7 of a row of any alignment, all of them there.  ONCE: nobody reads them again
-  // (the loads do not displace what the caches hold: 131072 rows of 2048 summed up by eights, 119 us
-  // without, 102 with).
-  template <bool ONCE = false> __device__ __forceinline__ void load(const T* p) {
-    typedef uint32_t Pack __attribute__((ext_vector_type(4), aligned(2)));
+  // The values are runs of 16 bytes, N each, at k, k + gap (consecutive by default: values k .. k + 7).
+  static constexpr int N = 16 / (int)sizeof(T);
+  typedef uint32_t Pack __attribute__((ext_vector_type(4), aligned(2)));     // rows of any alignment
+
+  // From p on, all of them there.  ONCE: nobody reads them again (the loads do not displace what the
+  // caches hold: 131072 rows of 2048 summed up by eights, 119 us without, 102 with).
+  template <bool ONCE = false> __device__ __forceinline__ void load(const T* p, int gap = N) {
 #pragma unroll
-    for (int i = 0; i < 2 * (int)sizeof(T); i += 4) {
-      const Pack* const from = reinterpret_cast<const Pack*>(p) + i / 4;
+    for (int q = 0; q < 8 / N; ++q) {
+      const Pack* const from = reinterpret_cast<const Pack*>(p + q * gap);
       const Pack v = ONCE ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[i + j] = v[j];
+      for (int j = 0; j < 4; ++j) w[4 * q + j] = v[j];
     }
   }
-  // Likewise, zeros from the row's end d on.
-  template <bool ONCE = false> __device__ __forceinline__ void load(const T* row, int k, int d) {
-    if (k + 8 <= d) {
-      load<ONCE>(row + k);
+  // From k on, zeros from the row's end d on.
+  template <bool ONCE = false>
+  __device__ __forceinline__ void load(const T* row, int k, int d, int gap = N) {
+    if (k + 7 / N * gap + N <= d) {
+      load<ONCE>(row + k, gap);
     } else {
 #pragma unroll
       for (int i = 0; i < 2 * (int)sizeof(T); ++i) w[i] = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (k + i >= d) break;
-        if constexpr (sizeof(T) == 4) w[i] = __builtin_bit_cast(uint32_t, row[k + i]);
-        else w[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[k + i]) << (16 * (i & 1));
+        const int at = k + i / N * gap + i % N;
+        if (at >= d) continue;
+        if constexpr (sizeof(T) == 4) w[i] = __builtin_bit_cast(uint32_t, row[at]);
+        else w[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[at]) << (16 * (i & 1));
+      }
+    }
+  }
+  // 8 values, rounded, likewise, nothing behind the row's end d.  ONCE: not to be read before much
+  // else was written.
+  template <bool ONCE = false>
+  static __device__ __forceinline__ void store(T* row, int k, int d, const float (&v)[8], int gap = N) {
+    T o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = Elem<T>::from_acc(v[i]);
+#pragma unroll
+    for (int q = 0; q < 8 / N; ++q) {
+      const int at = k + q * gap;
+      if (at + N <= d) {
+        Pack p;
+        __builtin_memcpy(&p, o + q * N, 16);
+        if constexpr (ONCE) __builtin_nontemporal_store(p, reinterpret_cast<Pack*>(row + at));
+        else *reinterpret_cast<Pack*>(row + at) = p;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (at + i < d) row[at + i] = o[q * N + i];
       }
     }
   }
@@ -106,29 +132,6 @@ template <typename T> struct Eight {
     else return __float_as_uint(__half2float(__builtin_bit_cast(__half, (uint16_t)m)));
   }
 };
-
-// 8 values into a row of any alignment, from k on, nothing behind its end d.  ONCE: not to be read
-// before much else was written.
-template <bool ONCE = false, typename T>
-__device__ __forceinline__ void store_any(T* row, int k, int d, const float (&v)[8]) {
-  T o[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = Elem<T>::from_acc(v[i]);
-  if (k + 8 <= d) {
-    typedef uint32_t Pack __attribute__((ext_vector_type(4), aligned(2)));
-    Pack p[sizeof(T) / 2];
-    __builtin_memcpy(p, o, sizeof(p));
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-      if constexpr (ONCE) __builtin_nontemporal_store(p[i], reinterpret_cast<Pack*>(row + k) + i);
-      else reinterpret_cast<Pack*>(row + k)[i] = p[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k + i < d) row[k + i] = o[i];
-  }
-}
 
 // Row counts of experts as segment bounds, for the call's first workgroup to leave behind.
 struct SegmentsOut {
