@@ -8,6 +8,15 @@
 
 namespace {
 
+// `sizes` of a tensor's values from `offset` on, as a tensor of its own on the same memory.
+Tensor part_of(const Tensor& whole, int64_t offset, at::IntArrayRef sizes) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(),
+                                                      whole.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(whole.storage_offset() + offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
 // (counts int64 [E], seg_off int32 [E + 1], token_off int32 [T + 1], pairs int32 [max_rows, 2])
 std::tuple<Tensor, Tensor, Tensor, Tensor> map_plan(Tensor map, int64_t max_rows) {
   dev(map, "routing_map", at::kBool);
@@ -16,12 +25,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> map_plan(Tensor map, int64_t max_rows
   c10::DeviceGuard guard(map.device());
   const int64_t t = map.size(0), e = map.size(1);
   const auto ints = map.options().dtype(at::kInt);
-  Tensor pairs = torch::empty({max_rows, 2}, ints);
+  // (one allocation, the host's share of a decode step's plan; what a user may keep, the counts, apart)
+  const int64_t at_off = (e + 2) & ~1, at_pairs = at_off + ((t + 2) & ~1);
+  Tensor whole = torch::empty({at_pairs + 2 * max_rows}, ints);
+  Tensor pairs = part_of(whole, at_pairs, {max_rows, 2});
   if (t == 0)
     return {torch::zeros({e}, map.options().dtype(at::kLong)), torch::zeros({e + 1}, ints),
             torch::zeros({1}, ints), pairs};
   Tensor counts = torch::empty({e}, map.options().dtype(at::kLong));
-  Tensor seg = torch::empty({e + 1}, ints), off = torch::empty({t + 1}, ints);
+  Tensor seg = part_of(whole, 0, {e + 1}), off = part_of(whole, at_off, {t + 1});
   need(e <= FMOE_MAP_MAX_EXPERTS, "routing_map has too many experts");
   const int64_t bytes = fmoe_map_workspace_bytes(t, (int32_t)e);
   check(bytes < 0 ? (int)bytes : 0, "map_plan");

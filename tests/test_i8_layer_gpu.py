@@ -194,3 +194,21 @@ def test_refusals():
                  (x.double(), gate, score.double(), w1, b1, w2, b2)):
         with pytest.raises(RuntimeError), torch.no_grad():
             i8.expert_layer(*args, relu)
+
+
+def test_traces_follow_their_inputs_and_forward_mode_is_refused():
+    x, gate, score, w1, b1, w2, b2 = parts(30, 4, 2, 64, 96, torch.float32)
+    relu = torch.nn.ReLU()
+    counts = torch.tensor([10, 0, 12, 8], device="cuda")
+    with torch.no_grad():
+        one = torch.jit.trace(lambda z, c: i8.linear(z, c, w1, b1), (x, counts))
+        whole = torch.jit.trace(lambda z, g, s: i8.expert_layer(z, g, s, w1, b1, w2, b2, relu),
+                                (x, gate, score))
+        z, other = randn((30, 64), torch.float32, 7).cuda(), torch.tensor([0, 30, 0, 0], device="cuda")
+        assert torch.equal(one(z, other), i8.linear(z, other, w1, b1))
+        flipped = gate.flip(0)
+        assert torch.equal(whole(z, flipped, score.flip(0)),
+                           i8.expert_layer(z, flipped, score.flip(0), w1, b1, w2, b2, relu))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        i8.linear(dual, counts, w1, b1)
