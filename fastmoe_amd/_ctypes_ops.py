@@ -1014,39 +1014,30 @@ def i8_linear_bwd(dy: torch.Tensor, seg_off: torch.Tensor, w_codes: torch.Tensor
           "dy, weight and seg_off must share a device")
     _need(seg_off.numel() == w_codes.shape[0] + 1, "seg_off must have E+1 entries")
     e, out_f = w_codes.shape[:2]
-    dx = db = w = None
+    dx = db = None
     rows = dy.shape[0]
     if need_dx:
+        few = _L.fmoe_i8_few_rows(rows, e, _dt(dy, "dy"))
+        size_of, run, name = ((_L.fmoe_i8_dx_workspace_bytes, _L.fmoe_i8_linear_dx, "i8_linear_dx")
+                              if few else (_L.fmoe_i8_dx_many_workspace_bytes,
+                                           _L.fmoe_i8_linear_dx_many, "i8_linear_dx_many"))
+        size = size_of(rows, in_feat, out_f, e, _dt(dy, "dy"))
+        _lib.check(min(size, 0), name)
         dx = dy.new_empty((rows, in_feat))
-    if need_dx and _L.fmoe_i8_few_rows(rows, e, _dt(dy, "dy")):
-        size = _L.fmoe_i8_dx_workspace_bytes(rows, in_feat, out_f, e, _dt(dy, "dy"))
-        _lib.check(min(size, 0), "i8_linear_dx")
-        shares = torch.empty(size, dtype=torch.uint8, device=dy.device)
-        with _launch(dy, "i8_linear_dx"):
+        work = torch.empty(size, dtype=torch.uint8, device=dy.device)
+        with _launch(dy, name):
             _lib.check(
-                _L.fmoe_i8_linear_dx(dy.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(),
-                                     seg_off.data_ptr(), dx.data_ptr(), rows, in_feat, out_f, e,
-                                     shares.data_ptr(), size, _dt(dy, "dy"), _stream(dy)),
-                "i8_linear_dx")
-        need_dx = False
-    if need_dx:
-        w = dy.new_empty((e * out_f, in_feat))
-        with _launch(dy, "i8_dequantize"):
-            _lib.check(
-                _L.fmoe_i8_dequantize_bwd(w_codes.data_ptr(), w_scales.data_ptr(),
-                                          seg_off.data_ptr(), w.data_ptr(), dx.data_ptr(),
-                                          dy.shape[0], in_feat, out_f, e, _dt(dy, "dy"),
-                                          _stream(dy)),
-                "i8_dequantize_bwd")
+                run(dy.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), seg_off.data_ptr(),
+                    dx.data_ptr(), rows, in_feat, out_f, e, work.data_ptr(), size, _dt(dy, "dy"),
+                    _stream(dy)),
+                name)
     if need_bias:
         db = dy.new_empty((e, out_f))
-    if need_dx or need_bias:
         with _launch(dy, "i8_linear_bwd"):
             _lib.check(
-                _L.fmoe_grouped_linear_bwd(dy.data_ptr(), dy.data_ptr(), _ptr(w),
-                                           seg_off.data_ptr(), _ptr(dx) if need_dx else None, None,
-                                           _ptr(db), dy.shape[0], in_feat, out_f, e, _dt(dy, "dy"),
-                                           _stream(dy)),
+                _L.fmoe_grouped_linear_bwd(dy.data_ptr(), dy.data_ptr(), None, seg_off.data_ptr(),
+                                           None, None, db.data_ptr(), rows, in_feat, out_f, e,
+                                           _dt(dy, "dy"), _stream(dy)),
                 "i8_linear_bwd")
     return dx, db
 

@@ -115,6 +115,9 @@ SIGNATURES = {
     "fmoe_i8_dx_workspace_bytes": (c_int64, [c_int64] * 4 + [c_int]),
     "fmoe_i8_linear_dx": (c_int, [c_void_p] * 5 + [c_int64] * 4 + [c_void_p, c_int64, c_int,
                                                                    c_void_p]),
+    "fmoe_i8_dx_many_workspace_bytes": (c_int64, [c_int64] * 4 + [c_int]),
+    "fmoe_i8_linear_dx_many": (c_int, [c_void_p] * 5 + [c_int64] * 4 + [c_void_p, c_int64, c_int,
+                                                                        c_void_p]),
     "fmoe_i8_linear_fwd": (c_int, [c_void_p] * 7 + [c_int64] * 4 + [c_int, c_void_p]),
     "fmoe_mx_code_bytes": (c_int64, [c_int64]),
     "fmoe_mx_scale_bytes": (c_int64, [c_int64]),

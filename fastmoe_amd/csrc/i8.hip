@@ -93,16 +93,7 @@ struct I8Row {
 
 // The maximum of m over the waves of a block; `part` is not the one of the call before.
 template <int W> __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t* part) {
-#define FMOE_MAX(CTRL, ROWS) \
-  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, ROWS, 0xf, false))
-  FMOE_MAX(0x111, 0xf);   // row_shr:1
-  FMOE_MAX(0x112, 0xf);
-  FMOE_MAX(0x114, 0xf);
-  FMOE_MAX(0x118, 0xf);
-  FMOE_MAX(0x142, 0xa);   // row_bcast:15
-  FMOE_MAX(0x143, 0xc);   // row_bcast:31
-#undef FMOE_MAX
-  m = (uint32_t)__builtin_amdgcn_readlane((int)m, kWave - 1);
+  m = wave_max(m);
   if constexpr (W > 1) {
     if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = m;
     __syncthreads();

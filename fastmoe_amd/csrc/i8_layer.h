@@ -123,12 +123,8 @@ Tensor i8_linear_fwd(Tensor xc, Tensor xs, Tensor wc, Tensor ws, int64_t in_f, O
   return out;
 }
 
-// Gradients of the rows and of the bias in front of frozen 8-bit weights: for few rows from the codes,
-// else the weights' values in dy's dtype, then the grouped product of the other weights.  Rows that
-// no expert owns get zeros.
-// (A value rounded to 16 bits is off by half a step like the result itself, so that for many rows the
-// gradient's error is 1.4 times one rounding's; the scale is on the axis that is summed over, so that
-// without this rounding dy would have to take it, in two products instead of one.)
+// Gradients of the rows and of the bias in front of frozen 8-bit weights, the former by the faster of
+// two ways (csrc/i8_grad.hip).  Rows that no expert owns get zeros.
 std::tuple<OptTensor, OptTensor> i8_linear_bwd(Tensor dy, Tensor seg_off, Tensor wc, Tensor ws,
                                                int64_t in_f, bool need_dx, bool need_bias) {
   dev(dy, "dy");
@@ -140,34 +136,29 @@ std::tuple<OptTensor, OptTensor> i8_linear_bwd(Tensor dy, Tensor seg_off, Tensor
   need(seg_off.numel() == wc.size(0) + 1, "seg_off must have E+1 entries");
   c10::DeviceGuard guard(dy.device());
   const int64_t e = wc.size(0), out_f = wc.size(1);
+  const int64_t rows = dy.size(0);
+  const int type = dt(dy, "dy");
   OptTensor dx, db;
-  Tensor w;
-  if (need_dx) dx = torch::empty({dy.size(0), in_f}, dy.options());
-  if (need_dx && fmoe_i8_few_rows(dy.size(0), e, dt(dy, "dy"))) {
-    const int64_t bytes = fmoe_i8_dx_workspace_bytes(dy.size(0), in_f, out_f, e, dt(dy, "dy"));
-    check(bytes < 0 ? (int)bytes : 0, "i8_linear_dx");
-    // (a tensor of its own: a backward pass does not hold the interpreter lock)
-    Tensor shares = torch::empty({bytes}, dy.options().dtype(at::kByte));
-    check(fmoe_i8_linear_dx(dy.data_ptr(), wc.data_ptr(), ws.data_ptr<float>(),
-                            seg_off.data_ptr<int32_t>(), dx->data_ptr(), dy.size(0), in_f, out_f, e,
-                            shares.data_ptr(), bytes, dt(dy, "dy"), stream_of(dy)),
-          "i8_linear_dx");
-    need_dx = false;
-  }
   if (need_dx) {
-    w = torch::empty({e * out_f, in_f}, dy.options());
-    check(fmoe_i8_dequantize_bwd(wc.data_ptr(), ws.data_ptr<float>(), seg_off.data_ptr<int32_t>(),
-                                 w.data_ptr(), dx->data_ptr(), dy.size(0), in_f, out_f, e,
-                                 dt(dy, "dy"), stream_of(dy)),
-          "i8_dequantize_bwd");
+    const bool few = fmoe_i8_few_rows(rows, e, type);
+    const int64_t bytes = few ? fmoe_i8_dx_workspace_bytes(rows, in_f, out_f, e, type)
+                              : fmoe_i8_dx_many_workspace_bytes(rows, in_f, out_f, e, type);
+    check(bytes < 0 ? (int)bytes : 0, "i8_linear_dx");
+    dx = torch::empty({rows, in_f}, dy.options());
+    // (a tensor of its own: a backward pass does not hold the interpreter lock)
+    Tensor work = torch::empty({bytes}, dy.options().dtype(at::kByte));
+    check((few ? fmoe_i8_linear_dx : fmoe_i8_linear_dx_many)(
+              dy.data_ptr(), wc.data_ptr(), ws.data_ptr<float>(), seg_off.data_ptr<int32_t>(),
+              dx->data_ptr(), rows, in_f, out_f, e, work.data_ptr(), bytes, type, stream_of(dy)),
+          "i8_linear_dx");
   }
-  if (need_bias) db = torch::empty({e, out_f}, dy.options());
-  if (need_dx || need_bias)   // (the layer's input takes part in the weight gradient alone)
-    check(fmoe_grouped_linear_bwd(dy.data_ptr(), dy.data_ptr(), need_dx ? w.data_ptr() : nullptr,
-                                  seg_off.data_ptr<int32_t>(), need_dx ? dx->data_ptr() : nullptr,
-                                  nullptr, ptr(db), dy.size(0), in_f, out_f, e, dt(dy, "dy"),
+  if (need_bias) {   // (the weights and the layer's input have no part in it)
+    db = torch::empty({e, out_f}, dy.options());
+    check(fmoe_grouped_linear_bwd(dy.data_ptr(), dy.data_ptr(), nullptr, seg_off.data_ptr<int32_t>(),
+                                  nullptr, nullptr, db->data_ptr(), rows, in_f, out_f, e, type,
                                   stream_of(dy)),
           "i8_linear_bwd");
+  }
   return {dx, db};
 }
 

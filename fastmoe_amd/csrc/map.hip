@@ -261,20 +261,6 @@ constexpr size_t map_lds(int n_expert, bool place) {
 }
 
 // ------------------------------------------------------------------------- rows
-// Sum over the wave, the same in every lane (the moves of wave_inclusive_sum()).
-__device__ __forceinline__ float wave_sum(float x) {
-#define FMOE_ADD(CTRL, ROWS) \
-  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWS, 0xf, false))
-  FMOE_ADD(0x111, 0xf);   // row_shr:1
-  FMOE_ADD(0x112, 0xf);
-  FMOE_ADD(0x114, 0xf);
-  FMOE_ADD(0x118, 0xf);
-  FMOE_ADD(0x142, 0xa);   // row_bcast:15
-  FMOE_ADD(0x143, 0xc);   // row_bcast:31
-#undef FMOE_ADD
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWave - 1));
-}
-
 struct MapMoveArgs {
   const void *one, *many, *weight;     // [tokens, d], [rows, d], [tokens, experts] or null (ones)
   const int32_t* token_off;

@@ -133,6 +133,26 @@ template <typename T> struct Eight {
   }
 };
 
+// Sum and maximum over the wave, the same in every lane (the moves of wave_inclusive_sum()).
+#define FMOE_ROW_MOVES(STEP) \
+  STEP(0x111, 0xf) /* row_shr:1 */ STEP(0x112, 0xf) STEP(0x114, 0xf) STEP(0x118, 0xf) \
+  STEP(0x142, 0xa) /* row_bcast:15 */ STEP(0x143, 0xc) /* row_bcast:31 */
+__device__ __forceinline__ float wave_sum(float x) {
+#define FMOE_ADD(CTRL, ROWS) \
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWS, 0xf, false));
+  FMOE_ROW_MOVES(FMOE_ADD)
+#undef FMOE_ADD
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWave - 1));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t m) {
+#define FMOE_MAX(CTRL, ROWS) \
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, ROWS, 0xf, false));
+  FMOE_ROW_MOVES(FMOE_MAX)
+#undef FMOE_MAX
+  return (uint32_t)__builtin_amdgcn_readlane((int)m, kWave - 1);
+}
+#undef FMOE_ROW_MOVES
+
 // Row counts of experts as segment bounds, for the call's first workgroup to leave behind.
 struct SegmentsOut {
   const int64_t* count = nullptr;

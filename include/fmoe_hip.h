@@ -608,10 +608,12 @@ int fmoe_map_reduce(const void* rows, const void* given, const void* weight,
  *                     [n_expert + 1]) from their DEVICE int64 counts (negative ones count as zero,
  *                     rows that are not there are cut off); counts NULL: one expert has them all.
  *   _dequantize       the values, rounded to dtype where that is too narrow for them.
- *   _dequantize_bwd   what stands in front of fmoe_grouped_linear_bwd for frozen 8-bit weights:
- *                     w [n_expert * out_feat, in_feat] = their values, and zeros in the rows of
+ *   _dequantize_bwd   the weights' values, rounded to dtype, for fmoe_grouped_linear_bwd:
+ *                     w [n_expert * out_feat, in_feat], and zeros in the rows of
  *                     dx [n_rows, in_feat] at or behind seg_off[n_expert] (DEVICE), which that
- *                     call leaves as they are.
+ *                     call leaves as they are.  (Rounded to 16 bits they cost the gradient 1.4
+ *                     times its own rounding, and f16 has no values above 65504 or, to its full
+ *                     precision, below 2^-14: fmoe_i8_linear_dx_many has neither limit.)
  * dtype: f32, f16 or bf16.  The reference has no such format.
  */
 #define FMOE_I8_MAX_FEATURES 131072   /* 127 * 127 * 2^17 < 2^31: sums of products are exact */
@@ -645,11 +647,13 @@ int fmoe_i8_linear_fwd(const void* x_codes, const float* x_scales, const void* w
 /*
  * dx[r][k] = sum_n dy[r][n] * w_scales[e][n] * w_e[n][k], r in seg_e: the gradient of that product's
  * rows, straight from the codes, and zeros in the rows at or behind seg_off[n_expert].  For any
- * number of rows, but made for few per expert (each 32 or 64 of them read its codes once) and for f32:
- * fmoe_i8_dequantize_bwd and fmoe_grouped_linear_bwd serve many.  fmoe_i8_few_rows: 1 where it is
- * the faster of the two for so many rows, else 0.  dy [n_rows, out_feat] and
- * dx [n_rows, in_feat] of dtype (f32, f16 or bf16).  The workspace is 16-byte aligned
- * (fmoe_i8_dx_workspace_bytes; none where that is 0).
+ * number of rows, but made for few per expert (each 32 or 64 of them read its codes once) and for f32.
+ * _dx_many: the same for many rows of f16 or bf16, by the products of fmoe_grouped_linear_bwd, to the
+ * same precision: dx is off by at most 1.03 times its own rounding.  fmoe_i8_few_rows: 1 where
+ * _dx is the faster of the two for so many rows, or the only one, else 0.  dy [n_rows, out_feat] and
+ * dx [n_rows, in_feat] of dtype (f32, f16 or bf16).  The workspaces are 16-byte aligned
+ * (fmoe_i8_dx_workspace_bytes, none where that is 0; fmoe_i8_dx_many_workspace_bytes, n_expert <=
+ * 65535).
  */
 int fmoe_i8_few_rows(int64_t n_rows, int64_t n_expert, int dtype);
 int64_t fmoe_i8_dx_workspace_bytes(int64_t n_rows, int64_t in_feat, int64_t out_feat,
@@ -658,6 +662,12 @@ int fmoe_i8_linear_dx(const void* dy, const void* w_codes, const float* w_scales
                       const int32_t* seg_off, void* dx, int64_t n_rows, int64_t in_feat,
                       int64_t out_feat, int64_t n_expert, void* workspace, int64_t workspace_bytes,
                       int dtype, void* stream);
+int64_t fmoe_i8_dx_many_workspace_bytes(int64_t n_rows, int64_t in_feat, int64_t out_feat,
+                                        int64_t n_expert, int dtype);
+int fmoe_i8_linear_dx_many(const void* dy, const void* w_codes, const float* w_scales,
+                           const int32_t* seg_off, void* dx, int64_t n_rows, int64_t in_feat,
+                           int64_t out_feat, int64_t n_expert, void* workspace,
+                           int64_t workspace_bytes, int dtype, void* stream);
 
 /*
  * y[i] = gelu(x[i]) = 0.5 x (1 + erf(x / sqrt 2)) over n elements, and

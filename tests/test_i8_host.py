@@ -150,3 +150,24 @@ def test_experts_in_8_bits_keep_what_they_should(quantised):
         i8.quantize_experts(quantised)
     state = quantised.state_dict()
     assert state["experts.w2_codes"].dtype == torch.int8 and "experts.w1_scales" in state
+
+
+def test_gradients_of_many_rows_that_do_not_fit_are_refused():
+    size = lib.fmoe_i8_dx_many_workspace_bytes
+
+    def grad(dy=P, w=P, ws=P, seg=P, dx=P, rows=400, k=8, n=24, e=2, work=P, room=1 << 30, dtype=3):
+        return lib.fmoe_i8_linear_dx_many(dy, w, ws, seg, dx, rows, k, n, e, work, room, dtype, None)
+
+    # rows, weights and a float a row, each to whole 256 bytes; twice the first two in f16
+    assert size(400, 8, 24, 2, 3) == 400 * 24 * 2 + 2 * 24 * 8 * 2 + 1792
+    assert size(400, 8, 24, 2, 2) == 2 * 400 * 24 * 2 + 2 * 2 * 24 * 8 * 2 + 1792
+    assert size(0, 8, 24, 2, 3) == 0
+    # (sizes past 32 bits)
+    assert size(1 << 20, 4096, 14336, 8, 2) > 2 * 2 * ((1 << 20) + 8 * 4096) * 14336
+    for bad in (dict(rows=-1), dict(rows=1 << 31), dict(k=0), dict(k=131073), dict(n=131073),
+                dict(e=0), dict(e=65536), dict(dtype=0), dict(dtype=1), dict(dy=None), dict(w=None),
+                dict(ws=None), dict(seg=None), dict(dx=None), dict(w=P + 4), dict(ws=P + 2)):
+        refused(grad(**bad), b"i8_linear_dx_many")
+    for bad in (dict(work=None), dict(room=size(400, 8, 24, 2, 3) - 1), dict(work=P + 4)):
+        refused(grad(**bad), b"workspace")
+    assert grad(rows=0) == 0
