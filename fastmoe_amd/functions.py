@@ -110,18 +110,36 @@ class MOEGather(Function):
 # --------------------------------------------------------------------------
 # Fused, synchronisation-free path
 # --------------------------------------------------------------------------
+def bounds_within(seg_off: torch.Tensor, n_rows: int) -> torch.Tensor:
+    """Segment bounds nobody has looked at, for a buffer of n_rows rows: what lies beyond the rows
+    there are is cut off, and bounds below the one before are that one.  (The products take their
+    rows from the bounds alone.)"""
+    if not seg_off.numel():
+        return seg_off
+    return seg_off.clamp(0, min(n_rows, 2 ** 31 - 1)).cummax(0)[0]
+
+
 class SegmentTable:
     """Per-expert row segments kept on the device.
 
     seg_off  int32[E+1]  exclusive prefix of the row counts
     counts   int64[E]    rows per expert (what the reference calls
                          fwd_expert_count, fmoe/functions.py:66-67)
+    n_rows   rows that the bounds are known to stay within (None: not known)
     """
 
-    def __init__(self, seg_off: torch.Tensor, counts: torch.Tensor):
+    def __init__(self, seg_off: torch.Tensor, counts: torch.Tensor, n_rows=None):
         self.seg_off = seg_off
         self.counts = counts
+        self.n_rows = n_rows
         self._host = None
+
+    def bounds(self, x: torch.Tensor) -> torch.Tensor:
+        """seg_off for the rows of x, cut off where x has fewer than the table may name."""
+        rows = x.shape[0] if x.dim() else 0
+        if self.n_rows is not None and rows >= self.n_rows:
+            return self.seg_off
+        return bounds_within(self.seg_off, rows)
 
     @property
     def num_expert(self) -> int:
@@ -132,6 +150,16 @@ class SegmentTable:
         if self._host is None:
             self._host = self.counts.cpu()
         return self._host
+
+
+def segments_for(counts, x: torch.Tensor):
+    """What a product takes for the rows of x: a table's bounds, or bounds themselves, within x; row
+    counts (int64, or none) as they are."""
+    if isinstance(counts, SegmentTable):
+        return counts.bounds(x)
+    if isinstance(counts, torch.Tensor) and counts.dtype == torch.int32:
+        return bounds_within(counts, x.shape[0] if x.dim() else 0)
+    return counts
 
 
 class RoutePlan:
@@ -148,7 +176,7 @@ class RoutePlan:
         pos, counts, seg_off, inv = routed
         self.pos = pos
         self.inv = inv
-        self.segments = SegmentTable(seg_off, counts)
+        self.segments = SegmentTable(seg_off, counts, self.n_slots)
 
     @property
     def n_rows_dev(self) -> torch.Tensor:
@@ -221,7 +249,7 @@ class MapPlan:
             routing_map.contiguous(), int(max_rows))
         self.n_tokens, self.num_expert = routing_map.shape
         self.max_rows = int(max_rows)
-        self.segments = SegmentTable(seg_off, self.counts)
+        self.segments = SegmentTable(seg_off, self.counts, self.max_rows)
 
     @property
     def n_rows_dev(self) -> torch.Tensor:

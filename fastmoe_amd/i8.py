@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 
 from . import fmoe_cuda
 from .frozen import FrozenExpert, layer_chain
-from .functions import SegmentTable
+from .functions import SegmentTable, bounds_within, segments_for
 from .linear import _segments, native_act
 from .transformer import _watched
 
@@ -126,7 +126,8 @@ class I8Linear(Function):
             if isinstance(counts, torch.Tensor) and not on_device and (
                     bool((counts < 0).any()) or int(counts.sum()) > x.shape[0]):
                 raise RuntimeError("expert counts are negative or claim more rows than x holds")
-            seg_off = counts.contiguous() if on_device else _segments(counts, x.device)
+            seg_off = (bounds_within(counts, x.shape[0]).contiguous() if on_device
+                       else _segments(counts, x))
             # (rows behind a segment table's end, those of dropped slots, are left out)
             host = isinstance(counts, torch.Tensor) and not on_device
             codes, scales = fmoe_cuda.i8_quantize(x, None if host else seg_off[-1:])
@@ -162,8 +163,7 @@ def linear(x: torch.Tensor, fwd_expert_count, weight: I8Tensor, bias=None) -> to
         bias = None if bias is None else bias.unsqueeze(0)
     native = fmoe_cuda.native()
     if native is not None:
-        segments = (fwd_expert_count.seg_off if isinstance(fwd_expert_count, SegmentTable)
-                    else fwd_expert_count)
+        segments = segments_for(fwd_expert_count, x)
         return native.i8_linear(x, segments, codes, scales, weight.features, bias)
     if isinstance(fwd_expert_count, SegmentTable) and torch._C._get_tracing_state() is not None:
         raise RuntimeError("a SegmentTable would be a constant of the trace: hand over counts")

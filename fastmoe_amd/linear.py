@@ -12,10 +12,10 @@ from . import fmoe_cuda
 from .functions import SegmentTable, apply_activation
 
 
-def _segments(fwd_expert_count, device) -> torch.Tensor:
+def _segments(fwd_expert_count, x) -> torch.Tensor:
     if isinstance(fwd_expert_count, SegmentTable):
-        return fwd_expert_count.seg_off
-    return fmoe_cuda._seg_off_from_counts(fwd_expert_count, device)
+        return fwd_expert_count.bounds(x)
+    return fmoe_cuda._seg_off_from_counts(fwd_expert_count, x.device)
 
 
 class MOELinear(Function):
@@ -27,7 +27,7 @@ class MOELinear(Function):
     @staticmethod
     def forward(ctx, global_input_buf, fwd_expert_count, weight, bias=None):
         x = global_input_buf.contiguous()
-        seg_off = _segments(fwd_expert_count, x.device)
+        seg_off = _segments(fwd_expert_count, x)
         out = fmoe_cuda.grouped_linear_fwd(x, seg_off, weight.contiguous(),
                                            None if bias is None else bias.contiguous())
         ctx.save_for_backward(x, seg_off, weight, bias)
@@ -54,7 +54,7 @@ class MOELinearGelu(Function):
     @staticmethod
     def forward(ctx, global_input_buf, fwd_expert_count, weight, bias=None):
         x = global_input_buf.contiguous()
-        seg_off = _segments(fwd_expert_count, x.device)
+        seg_off = _segments(fwd_expert_count, x)
         pre, act = fmoe_cuda.grouped_linear_fwd(
             x, seg_off, weight.contiguous(), None if bias is None else bias.contiguous(),
             with_gelu=True)
@@ -88,7 +88,7 @@ class MOEGeluLinear(Function):
     @staticmethod
     def forward(ctx, pre, fwd_expert_count, weight, bias=None, act=None):
         pre = pre.contiguous()
-        seg_off = _segments(fwd_expert_count, pre.device)
+        seg_off = _segments(fwd_expert_count, pre)
         if act is None:   # (MOELinearGelu hands over gelu(pre) with the pre-activations)
             act = fmoe_cuda.gelu_fwd(pre, seg_off[-1:])  # rows past the last segment are dead
         out = fmoe_cuda.grouped_linear_fwd(act, seg_off, weight.contiguous(),
@@ -175,7 +175,7 @@ class MOELinearList(Function):
     def forward(ctx, global_input_buf, fwd_expert_count, w_table, b_table, n_expert, has_bias,
                 *params):
         x = global_input_buf.contiguous()
-        seg_off = _segments(fwd_expert_count, x.device)
+        seg_off = _segments(fwd_expert_count, x)
         out = fmoe_cuda.grouped_linear_fwd_ptrs(x, seg_off, w_table, b_table,
                                                 params[0].shape[1])
         ctx.n_expert, ctx.has_bias, ctx.n_fixed = n_expert, has_bias, MOELinearList.n_fixed
@@ -204,7 +204,7 @@ class MOELinearGeluList(Function):
     def forward(ctx, global_input_buf, fwd_expert_count, w_table, b_table, n_expert, has_bias,
                 *params):
         x = global_input_buf.contiguous()
-        seg_off = _segments(fwd_expert_count, x.device)
+        seg_off = _segments(fwd_expert_count, x)
         pre, act = fmoe_cuda.grouped_linear_fwd_ptrs(x, seg_off, w_table, b_table,
                                                      params[0].shape[1], with_gelu=True)
         ctx.n_expert, ctx.has_bias, ctx.n_fixed = n_expert, has_bias, MOELinearGeluList.n_fixed
@@ -238,7 +238,7 @@ class MOEGeluLinearList(Function):
     @staticmethod
     def forward(ctx, pre, fwd_expert_count, w_table, b_table, n_expert, has_bias, act, *params):
         pre = pre.contiguous()
-        seg_off = _segments(fwd_expert_count, pre.device)
+        seg_off = _segments(fwd_expert_count, pre)
         if act is None:
             act = fmoe_cuda.gelu_fwd(pre, seg_off[-1:])
         out = fmoe_cuda.grouped_linear_fwd_ptrs(act, seg_off, w_table, b_table,

@@ -637,7 +637,8 @@ int fmoe_i8_dequantize_bwd(const void* w_codes, const float* w_scales, const int
  * with the sum of integer products exact, and f32 from there on.  x: n_rows rows of in_feat
  * features; w: n_expert * out_feat rows of in_feat features; bias [n_expert, out_feat] of `dtype`
  * or NULL; y [n_rows, out_feat] of `dtype` (f32, f16 or bf16).  Rows at or behind
- * seg_off[n_expert] are not written.
+ * seg_off[n_expert] are not written.  (seg_off is trusted, here and in the gradients: it ascends from
+ * 0 to at most n_rows.)
  */
 int fmoe_i8_linear_fwd(const void* x_codes, const float* x_scales, const void* w_codes,
                        const float* w_scales, const void* bias, const int32_t* seg_off, void* y,
