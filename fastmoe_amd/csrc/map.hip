@@ -32,6 +32,7 @@ constexpr int kMapUnit = 64;           // tokens of the smallest block, 4 for ea
 constexpr int kMapBlocks = 256;        // at most; more tokens make more rounds
 constexpr int kMapStage = 2048;        // bytes of truth values a wave holds in LDS
 constexpr int64_t kMapMostTokens = (int64_t)1 << 23;    // a block's counts have 16 bits
+constexpr int64_t kMapMostPieces = (int64_t)1 << 26;
 static_assert(FMOE_MAP_MAX_EXPERTS <= kMapStage, "a token's truth values fit");
 static_assert(kMapMostTokens / kMapBlocks < 65536, "counts fit");
 
@@ -428,9 +429,13 @@ static int move(const MapMoveArgs& a, int dtype, int weight_dtype, const int32_t
                 int64_t max_rows, hipStream_t s) {
   const char* const name = EXPAND ? "map_expand" : "map_reduce";
   FMOE_REQUIRE(a.n_tokens >= 0 && a.n_tokens <= kMapMostTokens && a.d >= 1 && a.n_expert >= 1 &&
-                   a.n_expert <= FMOE_MAP_MAX_EXPERTS && max_rows >= 0 && max_rows < INT32_MAX &&
-                   a.n_tokens * ((a.d + 511) / 512) < (int64_t)1 << 26,
+                   a.n_expert <= FMOE_MAP_MAX_EXPERTS && max_rows >= 0 && max_rows < INT32_MAX,
                FMOE_ERR_INVALID, "%s: bad sizes", name);
+  // (a wave for each piece of 512 values, and fewer than 2^32 threads in a launch; with dweight it is a
+  // block for each token)
+  FMOE_REQUIRE(a.dweight || a.n_tokens * ((a.d + 511) / 512) < kMapMostPieces, FMOE_ERR_UNSUPPORTED,
+               "%s: %lld tokens of %d features: tokens times ceil(features / 512) must be below 2^26",
+               name, (long long)a.n_tokens, a.d);
   FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_F16 || dtype == FMOE_BF16, FMOE_ERR_UNSUPPORTED,
                "%s: unsupported dtype %d", name, dtype);
   FMOE_REQUIRE(weight_dtype == FMOE_F32 || weight_dtype == dtype, FMOE_ERR_UNSUPPORTED,

@@ -575,7 +575,8 @@ int fmoe_mx_linear_fwd(const void* x_codes, const void* x_scales, const void* w_
  * Each is the other's gradient.  weight and dweight [n_tokens, n_expert] of weight_dtype, which is
  * f32 or dtype; weight NULL: ones (and no dweight).  Sums in f32, in the order of the experts.
  * dtype: f32, f16 or bf16.  n_expert <= FMOE_MAP_MAX_EXPERTS, n_tokens <= 2^23 and
- * n_tokens * n_expert < 2^31.
+ * n_tokens * n_expert < 2^31; without dweight, n_tokens * ceil(d / 512) < 2^26 (2^23 tokens of up to
+ * 3584 features).
  * They stand beside _local_scatter and _local_gather of fmoe/functions.py:78-90, which take a fixed
  * number of experts per token.
  */

@@ -171,3 +171,19 @@ def test_gradients_of_many_rows_that_do_not_fit_are_refused():
     for bad in (dict(work=None), dict(room=size(400, 8, 24, 2, 3) - 1), dict(work=P + 4)):
         refused(grad(**bad), b"workspace")
     assert grad(rows=0) == 0
+
+
+def test_the_most_tokens_and_features_of_a_move():
+    """Sizes are looked at before pointers: what passes them is refused for its missing offsets."""
+    def expand(t, d, dw=None):
+        return lib.fmoe_map_expand(P, dw, P, None, P, None, P, dw, t, d, 4, 8, 3, 0, None)
+
+    def reduce(t, d, dw=None):
+        return lib.fmoe_map_reduce(P, dw, P, None, P, P, dw, t, d, 4, 8, 3, 0, None)
+
+    for f in (expand, reduce):
+        for t, d in ((1 << 23, 3585), (1 << 22, 7681), ((1 << 23) - 1, 5000)):
+            refused(f(t, d), b"tokens times ceil(features / 512) must be below 2^26")
+            refused(f(t, d, P), b"null pointer")        # (a block per token, whatever its length)
+        for t, d in ((1 << 23, 3584), ((1 << 22) - 1, 8192)):
+            refused(f(t, d), b"null pointer")
