@@ -363,7 +363,13 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
             if constexpr (EXPAND) {
               float v[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = x[h][i] * wj;
+              for (int i = 0; i < 8; ++i) {
+                v[i] = x[h][i] * wj;
+                // (an f32 product, always: with the conversion to f16 the compiler would make it one
+                // instruction with one rounding, here and there, and a gradient's bits would depend on
+                // which others are wanted)
+                if constexpr (std::is_same<T, __half>::value) asm("" : "+v"(v[i]));
+              }
               Eight<T>::template store<true>(out + r * a.d, k0 + h * kSpan + at, a.d, v, kGap);
             } else {
 #pragma unroll
