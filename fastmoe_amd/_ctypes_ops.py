@@ -1100,25 +1100,28 @@ def _map_check(given, name, count, weight, seg_off, token_off, pairs) -> None:
 
 def map_expand(tokens: torch.Tensor, weight: Optional[torch.Tensor], seg_off: torch.Tensor,
                token_off: torch.Tensor, pairs: torch.Tensor,
-               given: Optional[torch.Tensor] = None, clear: bool = False
-               ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """(rows [max_rows, d]: weight[t, e] * tokens[t] at the row of every pair; with `given` rows also
-    the weights' gradient <tokens[t], given[row]>).  `clear`: rows behind the last are zero."""
+               given: Optional[torch.Tensor] = None, clear: bool = False, wanted: bool = True
+               ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(rows [max_rows, d]: weight[t, e] * tokens[t] at the row of every pair, unless they are not
+    `wanted`; with `given` rows also the weights' gradient <tokens[t], given[row]>).  `clear`: rows
+    behind the last are zero."""
     _map_check(tokens, "tokens", token_off.numel() - 1, weight, seg_off, token_off, pairs)
     if given is not None:
         _map_check(given, "rows", pairs.shape[0], weight, seg_off, token_off, pairs)
         _need(weight is not None and given.shape[1] == tokens.shape[1]
               and given.dtype == tokens.dtype,
               "a gradient of weights needs them, and rows like the tokens")
-    rows = tokens.new_empty((pairs.shape[0], tokens.shape[1]))
+    _need(wanted or given is not None,
+          "nothing to do without rows and without a gradient of weights")
+    rows = tokens.new_empty((pairs.shape[0], tokens.shape[1])) if wanted else None
     dw = None if given is None else torch.empty_like(weight)
     if tokens.shape[0] == 0:
-        return (rows.zero_() if clear else rows), dw
+        return (rows.zero_() if wanted and clear else rows), dw
     with _launch(tokens, "map_expand"):
         _lib.check(
             _L.fmoe_map_expand(tokens.data_ptr(), _ptr(given), _ptr(weight), token_off.data_ptr(),
                                pairs.data_ptr(), seg_off[-1:].data_ptr() if clear else None,
-                               rows.data_ptr(), _ptr(dw), tokens.shape[0], tokens.shape[1],
+                               _ptr(rows), _ptr(dw), tokens.shape[0], tokens.shape[1],
                                seg_off.numel() - 1, pairs.shape[0], _dt(tokens, "tokens"),
                                0 if weight is None else _dt(weight, "weight"), _stream(tokens)),
             "map_expand")
@@ -1127,23 +1130,26 @@ def map_expand(tokens: torch.Tensor, weight: Optional[torch.Tensor], seg_off: to
 
 def map_reduce(rows: torch.Tensor, weight: Optional[torch.Tensor], seg_off: torch.Tensor,
                token_off: torch.Tensor, pairs: torch.Tensor,
-               given: Optional[torch.Tensor] = None
-               ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """(tokens [T, d]: the sum of weight[t, e] * rows[row] over a token's pairs; with `given` tokens
-    also the weights' gradient <given[t], rows[row]>)."""
+               given: Optional[torch.Tensor] = None, wanted: bool = True
+               ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(tokens [T, d]: the sum of weight[t, e] * rows[row] over a token's pairs, unless they are not
+    `wanted`; with `given` tokens also the weights' gradient <given[t], rows[row]>)."""
     _map_check(rows, "rows", pairs.shape[0], weight, seg_off, token_off, pairs)
     if given is not None:
         _map_check(given, "tokens", token_off.numel() - 1, weight, seg_off, token_off, pairs)
         _need(weight is not None and given.shape[1] == rows.shape[1] and given.dtype == rows.dtype,
               "a gradient of weights needs them, and tokens like the rows")
-    tokens = rows.new_empty((token_off.numel() - 1, rows.shape[1]))
+    _need(wanted or given is not None,
+          "nothing to do without tokens and without a gradient of weights")
+    t = token_off.numel() - 1
+    tokens = rows.new_empty((t, rows.shape[1])) if wanted else None
     dw = None if given is None else torch.empty_like(weight)
-    if tokens.shape[0] == 0:
+    if t == 0:
         return tokens, dw
     with _launch(rows, "map_reduce"):
         _lib.check(
             _L.fmoe_map_reduce(rows.data_ptr(), _ptr(given), _ptr(weight), token_off.data_ptr(),
-                               pairs.data_ptr(), tokens.data_ptr(), _ptr(dw), tokens.shape[0],
+                               pairs.data_ptr(), _ptr(tokens), _ptr(dw), t,
                                rows.shape[1], seg_off.numel() - 1, pairs.shape[0],
                                _dt(rows, "rows"), 0 if weight is None else _dt(weight, "weight"),
                                _stream(rows)),

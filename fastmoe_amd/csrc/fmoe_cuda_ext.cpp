@@ -837,9 +837,10 @@ PYBIND11_MODULE(fmoe_cuda, m) {
   m.def("map_plan", &map_plan, py::arg("routing_map"), py::arg("max_rows"));
   m.def("map_expand", &map_expand, py::arg("tokens"), py::arg("weight"), py::arg("seg_off"),
         py::arg("token_off"), py::arg("pairs"), py::arg("given") = py::none(),
-        py::arg("clear") = false);
+        py::arg("clear") = false, py::arg("wanted") = true);
   m.def("map_reduce", &map_reduce, py::arg("rows"), py::arg("weight"), py::arg("seg_off"),
-        py::arg("token_off"), py::arg("pairs"), py::arg("given") = py::none());
+        py::arg("token_off"), py::arg("pairs"), py::arg("given") = py::none(),
+        py::arg("wanted") = true);
   m.def("sort_tokens", &sort_tokens);
   m.def("unsort_tokens", &unsort_tokens);
   m.def("gelu_fwd", &gelu_fwd, py::arg("x"), py::arg("n_rows_dev") = py::none());

@@ -272,7 +272,7 @@ struct MapMoveArgs {
 };
 
 // EXPAND: out[r] = w one[t] for a token's rows; else out[t] = sum of w many[r].  DOT: also
-// dweight[t][e] = <one[t], many[r]>, zero where the token has no row.
+// dweight[t][e] = <one[t], many[r]>, zero where the token has no row; out may be null then.
 //
 // A lane holds 8 values of a piece of a row, and U rows are under way at a time.  Without DOT a wave takes 512
 // values of a token's rows, whatever their length; with it a block of G threads takes a token,
@@ -298,6 +298,7 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
   const T* const many = (const T*)a.many;
   const W* const weight = (const W*)a.weight;
   T* const out = (T*)a.out;
+  const bool wanted = !DOT || out != nullptr;
   const int p0 = a.token_off[t], p1 = a.token_off[t + 1];
   float* const dot = s_dot + wave * a.n_expert;
   if constexpr (DOT)
@@ -361,6 +362,7 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
 #pragma unroll
           for (int h = 0; h < H; ++h) {
             if constexpr (EXPAND) {
+              if (!wanted) continue;
               float v[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(DOT ? G : 256) void map_move_kernel(MapMoveArgs a, 
         }
       }
     }
-    if constexpr (!EXPAND) {
+    if (!EXPAND && wanted) {
 #pragma unroll
       for (int h = 0; h < H; ++h) Eight<T>::store(out + t * a.d, k0 + h * kSpan + at, a.d, sum[h], kGap);
     }
@@ -449,7 +451,8 @@ static int move(const MapMoveArgs& a, int dtype, int weight_dtype, const int32_t
   if (a.n_tokens == 0) return FMOE_OK;
   // (rows of a plan without any may be null)
   FMOE_REQUIRE(a.token_off && (a.pairs || max_rows == 0) &&
-                   (EXPAND ? a.one && (a.out || max_rows == 0) : (a.many || max_rows == 0) && a.out),
+                   (EXPAND ? a.one && (a.out || a.dweight || max_rows == 0)
+                           : (a.many || max_rows == 0) && (a.out || a.dweight)),
                FMOE_ERR_INVALID, "%s: null pointer", name);
   FMOE_REQUIRE(!a.dweight || (a.weight && a.one && (a.many || max_rows == 0)), FMOE_ERR_INVALID,
                "%s: a gradient of weights needs them, the tokens and the rows", name);

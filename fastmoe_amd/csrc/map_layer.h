@@ -76,10 +76,11 @@ int weight_dtype(const OptTensor& weight) {
 }
 const Tensor* defined(const OptTensor& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
 
-// (rows [max_rows, d], the weights' gradient if `given` rows are handed over)
+// (rows [max_rows, d], unless they are not `wanted`, the weights' gradient if `given` rows are handed
+// over)
 std::tuple<Tensor, OptTensor> map_expand(Tensor tokens, OptTensor weight, Tensor seg_off,
-                                         Tensor token_off, Tensor pairs, OptTensor given,
-                                         bool clear) {
+                                         Tensor token_off, Tensor pairs, OptTensor given, bool clear,
+                                         bool wanted = true) {
   map_check(tokens, "tokens", token_off.numel() - 1, weight, seg_off, token_off, pairs);
   OptTensor dw;
   if (const Tensor* g = defined(given)) {
@@ -88,25 +89,28 @@ std::tuple<Tensor, OptTensor> map_expand(Tensor tokens, OptTensor weight, Tensor
          "a gradient of weights needs them, and rows like the tokens");
   }
   c10::DeviceGuard guard(tokens.device());
-  Tensor rows = torch::empty({pairs.size(0), tokens.size(1)}, tokens.options());
+  need(wanted || defined(given), "nothing to do without rows and without a gradient of weights");
+  Tensor rows;
+  if (wanted) rows = torch::empty({pairs.size(0), tokens.size(1)}, tokens.options());
   if (defined(given)) dw = torch::empty_like(*weight);
   if (tokens.size(0) == 0) {
-    if (clear) rows.zero_();
+    if (wanted && clear) rows.zero_();
     return {rows, dw};
   }
   check(fmoe_map_expand(tokens.data_ptr(), ptr(given), ptr(weight), token_off.data_ptr<int32_t>(),
                         pairs.data_ptr<int32_t>(),
                         clear ? seg_off.data_ptr<int32_t>() + seg_off.numel() - 1 : nullptr,
-                        rows.data_ptr(), ptr(dw), tokens.size(0), tokens.size(1),
+                        wanted ? rows.data_ptr() : nullptr, ptr(dw), tokens.size(0), tokens.size(1),
                         (int32_t)(seg_off.numel() - 1), pairs.size(0), dt(tokens, "tokens"),
                         weight_dtype(weight), stream_of(tokens)),
         "map_expand");
   return {rows, dw};
 }
 
-// (tokens [T, d], the weights' gradient if `given` tokens are handed over)
+// (tokens [T, d], unless they are not `wanted`, the weights' gradient if `given` tokens are handed over)
 std::tuple<Tensor, OptTensor> map_reduce(Tensor rows, OptTensor weight, Tensor seg_off,
-                                         Tensor token_off, Tensor pairs, OptTensor given) {
+                                         Tensor token_off, Tensor pairs, OptTensor given,
+                                         bool wanted = true) {
   map_check(rows, "rows", pairs.size(0), weight, seg_off, token_off, pairs);
   if (const Tensor* g = defined(given)) {
     map_check(*g, "tokens", token_off.numel() - 1, weight, seg_off, token_off, pairs);
@@ -114,12 +118,15 @@ std::tuple<Tensor, OptTensor> map_reduce(Tensor rows, OptTensor weight, Tensor s
          "a gradient of weights needs them, and tokens like the rows");
   }
   c10::DeviceGuard guard(rows.device());
+  need(wanted || defined(given), "nothing to do without tokens and without a gradient of weights");
+  const int64_t t = token_off.numel() - 1;
   OptTensor dw;
-  Tensor tokens = torch::empty({token_off.numel() - 1, rows.size(1)}, rows.options());
+  Tensor tokens;
+  if (wanted) tokens = torch::empty({t, rows.size(1)}, rows.options());
   if (defined(given)) dw = torch::empty_like(*weight);
-  if (tokens.size(0) == 0) return {tokens, dw};
+  if (t == 0) return {tokens, dw};
   check(fmoe_map_reduce(rows.data_ptr(), ptr(given), ptr(weight), token_off.data_ptr<int32_t>(),
-                        pairs.data_ptr<int32_t>(), tokens.data_ptr(), ptr(dw), tokens.size(0),
+                        pairs.data_ptr<int32_t>(), wanted ? tokens.data_ptr() : nullptr, ptr(dw), t,
                         rows.size(1), (int32_t)(seg_off.numel() - 1), pairs.size(0),
                         dt(rows, "rows"), weight_dtype(weight), stream_of(rows)),
         "map_reduce");
@@ -149,8 +156,12 @@ template <bool EXPAND> struct MapNode : public torch::autograd::Function<MapNode
     c10::DeviceGuard guard(v[0].device());
     const Tensor g = only_once(grads[0], EXPAND ? "sort_tokens" : "unsort_tokens");
     auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-    auto r = EXPAND ? map_reduce(g, opt(v[3]), v[0], v[1], v[2], opt(v[4]))
-                    : map_expand(g, opt(v[3]), v[0], v[1], v[2], opt(v[4]), true);
+    const bool wanted = ctx->needs_input_grad(0);
+    // (an absent weight is no input of the node; v[4] is there for one that has a gradient alone)
+    const OptTensor dot = v[4].defined() && ctx->needs_input_grad(4) ? OptTensor(v[4]) : OptTensor();
+    if (!wanted && !dot.has_value()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    auto r = EXPAND ? map_reduce(g, opt(v[3]), v[0], v[1], v[2], dot, wanted)
+                    : map_expand(g, opt(v[3]), v[0], v[1], v[2], dot, true, wanted);
     const OptTensor& dw = std::get<1>(r);
     return {std::get<0>(r), Tensor(), Tensor(), Tensor(), dw.has_value() ? *dw : Tensor()};
   }

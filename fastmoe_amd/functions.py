@@ -274,7 +274,9 @@ class _MapExpand(Function):
     @once_differentiable
     def backward(ctx, grad):
         x, weight, *plan = ctx.saved_tensors
-        dx, dw = fmoe_cuda.map_reduce(grad.contiguous(), weight, *plan, x)
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        dx, dw = fmoe_cuda.map_reduce(grad.contiguous(), weight, *plan, x if need_dw else None,
+                                      need_dx)
         return dx, dw, None, None, None
 
 
@@ -292,7 +294,9 @@ class _MapReduce(Function):
     @once_differentiable
     def backward(ctx, grad):
         rows, weight, *plan = ctx.saved_tensors
-        drows, dw = fmoe_cuda.map_expand(grad.contiguous(), weight, *plan, rows, True)
+        need_drows, need_dw = ctx.needs_input_grad[:2]
+        drows, dw = fmoe_cuda.map_expand(grad.contiguous(), weight, *plan,
+                                         rows if need_dw else None, True, need_drows)
         return drows, dw, None, None, None
 
 

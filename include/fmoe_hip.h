@@ -571,7 +571,8 @@ int fmoe_mx_linear_fwd(const void* x_codes, const void* x_scales, const void* w_
  *            seg_off[n_expert]) the rows from there to max_rows are cleared; without, left as they are.
  *   _reduce  tokens[t] = sum over the pairs (r, e) of t of weight[t][e] rows[r], 0 without any;
  *            dweight (if not NULL) [t][e] = <given[t], rows[r]>, 0 without a row.
- * (With n_tokens 0 neither does anything.)
+ * (With n_tokens 0 neither does anything.  With dweight, rows of _expand and tokens of _reduce may be
+ * NULL: they are left out.)
  * Each is the other's gradient.  weight and dweight [n_tokens, n_expert] of weight_dtype, which is
  * f32 or dtype; weight NULL: ones (and no dweight).  Sums in f32, in the order of the experts.
  * dtype: f32, f16 or bf16.  n_expert <= FMOE_MAP_MAX_EXPERTS, n_tokens <= 2^23 and
