@@ -225,3 +225,25 @@ def test_many_rows_captured_and_on_another_stream(dtype):
         got = [gradient(dy, [t], w) for _ in range(2)]
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_many_rows_beyond_32_bits(dtype):
+    """dy of 5.2 GB, its parts of as much or twice that; weights of 4.3 GB in f16."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("not enough memory")
+    g = torch.Generator("cuda").manual_seed(1)
+    for rows, e, n, k in ((40000, 1, 65536, 64), (8 * 600, 8, 16384, 16384)):
+        # (random codes in place of quantised weights: less memory)
+        codes = torch.randint(-127, 128, (e, n, -(-k // 128) * 128), dtype=torch.int8, device="cuda",
+                              generator=g)
+        codes[..., k:] = 0
+        w = i8.I8Tensor(codes, torch.rand(e, n, device="cuda", generator=g) * 1e-3, k)
+        dy = torch.randn(rows, n, device="cuda", generator=g, dtype=dtype)
+        each = rows // e
+        got = gradient(dy, [each] * e, w)
+        for i in {0, e - 1}:
+            one = i8.I8Tensor(codes[i:i + 1], w.scales[i:i + 1], k)
+            for r in {i * each, (i + 1) * each - 40}:
+                check(got[r:r + 40], dy[r:r + 40], [40], one)
+        del codes, w, dy, got

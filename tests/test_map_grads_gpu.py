@@ -78,3 +78,91 @@ def test_calls_for_nothing_are_refused(binding):
     v.grad = None
     functions.unsort_tokens(torch.zeros(4, 16, device="cuda"), none, v).sum().backward()
     assert v.grad.shape == (0, 3)
+
+
+@pytest.mark.parametrize("d", [8, 77, 1024])
+def test_rows_behind_the_last_are_left_as_they_were(d):
+    """On a buffer of the caller's own: without n_rows_dev nothing is written there, with it zeros."""
+    from fastmoe_amd import _lib
+
+    _, plan, x, w, _ = make("sort", 50, 6, d, torch.bfloat16, torch.float32)
+    live = plan.n_rows_dev.item()
+    assert live == plan.max_rows - 7
+    seg, off, pairs = plan._tensors()
+    want = functions.sort_tokens(x, plan, w)[:live]
+    for end in (None, seg[-1:].data_ptr()):
+        rows = torch.full((plan.max_rows, d), 5.0, dtype=torch.bfloat16, device="cuda")
+        rc = _lib.load().fmoe_map_expand(x.data_ptr(), None, w.data_ptr(), off.data_ptr(),
+                                         pairs.data_ptr(), end, rows.data_ptr(), None, 50, d, 6,
+                                         plan.max_rows, 3, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        assert torch.equal(rows[:live], want) and (rows[live:] == (5 if end is None else 0)).all()
+
+
+def test_gradients_beyond_32_bits():
+    """2.2 M rows of 1024 features in bf16: byte offsets of rows past 2^32 in either direction."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("not enough memory")
+    g = torch.Generator("cuda").manual_seed(1)
+    t, e, d = 1 << 20, 4, 1024
+    m = torch.rand(t, e, device="cuda", generator=g) < 0.52
+    plan = functions.MapPlan(m)
+    n = plan.max_rows
+    assert n * d * 2 > 1 << 32
+    expert, token = m.t().nonzero(as_tuple=True)
+    x = torch.randn(t, d, device="cuda", dtype=torch.bfloat16, generator=g)
+    rows = torch.randn(n, d, device="cuda", dtype=torch.bfloat16, generator=g)
+    w = torch.rand(t, e, device="cuda", generator=g)
+    places = [slice(a, a + 3000) for a in (0, t // 2, t - 3000)]
+    row_of = torch.full((t, e), -1, dtype=torch.long, device="cuda")
+    row_of[token, expert] = torch.arange(n, device="cuda")
+
+    def bound(want, size, dtype, terms):
+        return torch.finfo(dtype).eps / 2 * want.abs() * (1 + 1e-6) + (terms + 1) * 2.0 ** -24 * size
+
+    def check_weights(got):
+        assert (got[~m] == 0).all()
+        for p in places:
+            a, b = x[p].double()[:, None], rows[row_of[p].clamp(min=0)].double()
+            want, size = (a * b).sum(-1) * m[p], (a * b).abs().sum(-1)
+            assert ((got[p] - want).abs() <= bound(want, size, torch.float32, d)).all()
+
+    def check_tokens(got):
+        for p in places:
+            term = rows[row_of[p].clamp(min=0)].double() * (w[p] * m[p]).double()[..., None]
+            want, size = term.sum(1), term.abs().sum(1)
+            assert ((got[p] - want).abs() <= bound(want, size, torch.bfloat16, e)).all()
+
+    def check_rows(got):
+        for a in (0, n // 2, n - 3000):
+            p = slice(a, a + 3000)
+            want = x[token[p]].double() * w[token[p], expert[p]].double()[:, None]
+            assert ((got[p] - want).abs() <= bound(want, want.abs(), torch.bfloat16, 1)).all()
+
+    for f, have, grad, check in ((functions.sort_tokens, x, rows, check_tokens),
+                                 (functions.unsort_tokens, rows, x, check_rows)):
+        have, weight = have.detach().requires_grad_(), w.clone().requires_grad_()
+        f(have, plan, weight).backward(grad)
+        check(have.grad)
+        check_weights(weight.grad)
+        have.grad = None
+
+
+def test_the_most_tokens():
+    """2^23 tokens: a block each with the weights' gradient, 2^23 waves without."""
+    t, e, d = 1 << 23, 2, 8
+    m = torch.zeros(t, e, dtype=torch.bool, device="cuda")
+    at = torch.tensor([0, 1, 4095, 1 << 22, t - 1], device="cuda")
+    m[at, 1] = True
+    plan = functions.MapPlan(m)
+    x = torch.arange(t, device="cuda", dtype=torch.float32)[:, None].expand(t, d).contiguous()
+    x.requires_grad_()
+    w = torch.full((t, e), 2.0, device="cuda", requires_grad=True)
+    rows = functions.sort_tokens(x, plan, w)
+    assert torch.equal(rows[:, 0], 2.0 * at)
+    y = functions.unsort_tokens(rows, plan)
+    assert torch.equal(y[at, 3], 2.0 * at) and y.count_nonzero() == 4 * d
+    y.backward(torch.ones_like(y))
+    assert torch.equal(x.grad[at, 0], torch.full((5,), 2.0, device="cuda"))
+    assert x.grad.count_nonzero() == 5 * d
+    assert torch.equal(w.grad[at, 1], 8.0 * at) and w.grad.count_nonzero() == 4
