@@ -94,8 +94,9 @@ __global__ __launch_bounds__(256, (QuantTile<true, TN, TM>::kGroups)) void i8_ti
 constexpr int kCus = 256;
 
 // Which kernel: by the mean number of rows per expert, the features and the number of tiles this
-// makes.  Measured with several sets of operands in turn (us, bf16), with even loads and, behind the
-// slash, with half of all rows on one expert:
+// makes.  Measured with several sets of operands in turn (us, bf16), with even loads, which fill the
+// tiles (a routed batch's do not: 71.1 below is 95 there, 86.5 is 100), and, behind the slash, with half
+// of all rows on one expert:
 //   rows  experts  in -> out      stream       128x64       128x128      256x256
 //     64   16    1024 -> 4096   16.6 / 17.0  16.5 / 16.2  17.0 / 16.9  21.8 / 21.0
 //    128   16    4096 -> 1024   17.5 / 20.5  27.7 / 27.7  28.4 / 28.5  41.4 / 41.6
