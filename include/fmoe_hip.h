@@ -652,8 +652,9 @@ int fmoe_i8_linear_fwd(const void* x_codes, const float* x_scales, const void* w
  * rows, straight from the codes, and zeros in the rows at or behind seg_off[n_expert].  For any
  * number of rows, but made for few per expert (each 32 or 64 of them read its codes once) and for f32.
  * _dx_many: the same for many rows of f16 or bf16, by the products of fmoe_grouped_linear_bwd, to the
- * same precision: dx is off by at most 1.03 times its own rounding.  fmoe_i8_few_rows: 1 where
- * _dx is the faster of the two for so many rows, or the only one, else 0.  dy [n_rows, out_feat] and
+ * same precision: the norm of dx's error is at most 1.03 times that of its own rounding.
+ * fmoe_i8_few_rows: 1 where _dx is the faster of the two for so many rows, or the only one, else 0.
+ * dy [n_rows, out_feat] and
  * dx [n_rows, in_feat] of dtype (f32, f16 or bf16).  The workspaces are 16-byte aligned
  * (fmoe_i8_dx_workspace_bytes, none where that is 0; fmoe_i8_dx_many_workspace_bytes, n_expert <=
  * 65535).
